@@ -1,0 +1,161 @@
+"""A key/value cache in 4 or 8 bits: its format, what writing, reading and attending refuse, and a cached decoder, all on plain statements."""
+import pytest
+import torch
+
+from torchtune_b200 import ops
+from torchtune_b200.ops import QuantizedRows, reference
+from torchtune_b200.ops.mask import AttentionMask
+
+
+def _rows(b, slots, h, d, bits):
+    return QuantizedRows.zeros(b, slots, h, d, bits), QuantizedRows.zeros(b, slots, h, d, bits)
+
+
+def _value(codes, scales, bits, d, c):
+    """Channel ``c`` of one row, from the words of the format."""
+    code = int(codes[c]) if bits == 8 else (int(codes[c // 2]) >> (4 * (c % 2))) & 15
+    return (code - 2 ** (bits - 1)) * float(scales[(c % (d // 4)) // 8])
+
+
+@pytest.mark.parametrize("d", [32, 96, 128])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_row_stands_for_its_nearest_codes(bits, d):
+    x = torch.randn(2, 3, 2, d, generator=torch.Generator().manual_seed(d)).to(torch.bfloat16)
+    k_rows, v_rows = _rows(2, 7, 2, d, bits)
+    ops.quantized_append(x, -x, k_rows, v_rows, torch.arange(2, 5))
+    k, v = ops.quantized_read(k_rows, v_rows, 2, 5, torch.float32)
+    half = 2 ** (bits - 1)
+    for b, i, h in ((0, 0, 0), (1, 2, 1)):
+        row = x[b, i, h].double()
+        for c in range(d):
+            assert float(k[b, i, h, c]) == _value(k_rows.codes[b, h, 2 + i], k_rows.scales[b, h, 2 + i], bits, d, c)
+        for j in range(d // 32):
+            at = [c for c in range(d) if (c % (d // 4)) // 8 == j]
+            top = max(at, key=lambda c: (abs(float(row[c])), -c))
+            step = float(row[top]) / -half  # exact for bf16
+            assert float(k_rows.scales[b, h, 2 + i, j]) == step
+            for c in at:
+                error = abs(float(k[b, i, h, c]) - float(row[c]))
+                # the nearest code, but for +h, which does not exist
+                assert error <= abs(step) / 2 or (float(row[c]) / step > half - 1 and float(k[b, i, h, c]) == (half - 1) * step)
+    # the opposite values have opposite scales and the same codes
+    assert torch.equal(k_rows.codes, v_rows.codes) and torch.equal(k_rows.scales, -v_rows.scales) and torch.equal(k, -v)
+    untouched = [0, 1, 5, 6]
+    assert not k_rows.codes[:, :, untouched].any() and not k_rows.scales[:, :, untouched].any()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_groups_of_zeros_ties_and_non_finite_values(bits):
+    x = torch.randn(1, 5, 1, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    group = [c for c in range(64) if (c % 16) // 8 == 1]
+    x[0, 0, 0, group] = 0.0
+    x[0, 1, 0, group] = torch.linspace(-1, 1, 32).to(torch.bfloat16)  # -1 and 1 are equally large: the first counts
+    x[0, 2, 0, group[3]] = float("inf")
+    x[0, 3, 0, group[3]] = float("nan")
+    x[0, 4, 0, group] = 1e-40  # its scale underflows or is coarse: nothing turns into NaN
+    k_rows, v_rows = _rows(1, 5, 1, 64, bits)
+    ops.quantized_append(x, x, k_rows, v_rows, torch.arange(5))
+    k, _ = ops.quantized_read(k_rows, v_rows, dtype=torch.float32)
+    others = [c for c in range(64) if c not in group]
+    assert not k[0, 0, 0, group].any()
+    assert float(k[0, 1, 0, group[0]]) == -1.0 and float(k_rows.scales[0, 0, 1, 1]) == 1.0 / 2 ** (bits - 1)
+    assert float(k[0, 1, 0, group[-1]]) == 1.0 - 1.0 / 2 ** (bits - 1)
+    assert k[0, 2, 0, group].isnan().all() and k[0, 3, 0, group].isnan().all()
+    assert k[0, :, 0, others].isfinite().all() and k[0, 4].isfinite().all()
+
+
+def test_rows_are_views_with_their_own_sizes():
+    rows = QuantizedRows.zeros(3, 13, 2, 64, 4)
+    assert rows.codes.shape == (3, 2, 13, 32) and rows.scales.shape == (3, 2, 13, 2) and rows.bits == 4 and rows.head_dim == 64 and rows.slots == 13
+    part = rows.batch(2).first(5)
+    assert part.codes.shape == (2, 2, 5, 32) and part.codes.data_ptr() == rows.codes.data_ptr()
+    assert QuantizedRows.zeros(1, 3, 1, 32, 8).bits == 8
+    for bits, d in ((2, 64), (4, 48), (8, 0)):
+        with pytest.raises(ValueError):
+            QuantizedRows.zeros(1, 4, 1, d, bits)
+
+
+def test_writing_refuses_what_does_not_fit():
+    k_rows, v_rows = _rows(2, 8, 2, 64, 4)
+    x = torch.zeros(2, 3, 2, 64)
+    at = torch.arange(3)
+    for slots in (torch.arange(6, 9), torch.tensor([-1, 0, 1]), torch.tensor([1, 1, 1]), torch.tensor([0, 2, 4]), torch.arange(2), torch.arange(3, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            ops.quantized_append(x, x, k_rows, v_rows, slots)
+    assert not k_rows.codes.any()
+    for k, v in ((x[:1], x[:1]), (x[..., :32], x[..., :32]), (x[:, :, :1], x[:, :, :1]), (x, x[:, :2]), (x, x.half()), (x.int(), x.int()), (x.double(), x.double())):
+        with pytest.raises(ValueError):
+            ops.quantized_append(k, v, k_rows, v_rows, at)
+    with pytest.raises(ValueError):
+        ops.quantized_append(x, x, k_rows, QuantizedRows.zeros(2, 8, 2, 64, 8), at)
+    with pytest.raises(ValueError):
+        ops.quantized_append(x, x, k_rows, QuantizedRows(v_rows.codes, v_rows.scales.float()), at)
+    ops.quantized_append(x[:, :0], x[:, :0], k_rows, v_rows, at[:0])
+    for start, stop in ((-1, 2), (3, 2), (0, 9)):
+        with pytest.raises(ValueError):
+            ops.quantized_read(k_rows, v_rows, start, stop)
+    with pytest.raises(ValueError):
+        ops.quantized_read(k_rows, v_rows, dtype=torch.int32)
+    assert ops.quantized_read(k_rows, v_rows, 4, 4)[0].shape == (2, 0, 2, 64)
+
+
+def _filled(b, n, h, d, bits, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    k_rows, v_rows = _rows(b, n, h, d, bits)
+    ops.quantized_append(torch.randn(b, n, h, d, generator=g), torch.randn(b, n, h, d, generator=g), k_rows, v_rows, torch.arange(n))
+    return k_rows, v_rows
+
+
+def test_attention_refuses_what_does_not_fit():
+    k_rows, v_rows = _filled(2, 8, 2, 64, 4)
+    q = torch.randn(2, 3, 4, 64)
+    for x in (q[:1], q[..., :32], q[:, :, :3], q[0]):
+        with pytest.raises(ValueError):
+            ops.quantized_attention(x, k_rows, v_rows)
+    masks = [AttentionMask(causal=False, window=4), AttentionMask(doc_ids=torch.zeros(2, 8, dtype=torch.int32)), AttentionMask(chunk=4), AttentionMask(bool_mask=torch.ones(2, 3, 7, dtype=torch.bool)),
+             AttentionMask(bool_mask=torch.ones(2, 4, 3, 8, dtype=torch.bool)), AttentionMask(key_start=torch.zeros(2, dtype=torch.int32), query_start=6),
+             AttentionMask(key_start=torch.zeros(3, dtype=torch.int32)), AttentionMask(key_start=torch.zeros(2, dtype=torch.int32), window=3)]
+    for mask in masks:
+        with pytest.raises(ValueError):
+            ops.quantized_attention(q, k_rows, v_rows, mask)
+    with pytest.raises(ValueError):
+        ops.quantized_attention(torch.randn(2, 9, 4, 64), k_rows, v_rows, AttentionMask())
+    assert not ops.quantized_attention(q, k_rows.first(0), v_rows.first(0)).any()
+    assert ops.quantized_attention(q[:, :0], k_rows, v_rows).shape == (2, 0, 4, 64)
+
+
+@pytest.mark.parametrize("mask", [AttentionMask(causal=False), AttentionMask(), AttentionMask(window=3, sinks=2), AttentionMask(window=1), "bool", "start"])
+def test_attention_is_that_of_the_values_the_cache_stands_for(mask):
+    k_rows, v_rows = _filled(2, 11, 2, 64, 8)
+    q = torch.randn(2, 2, 6, 64, generator=torch.Generator().manual_seed(3))
+    i, j = torch.arange(2)[:, None] + 9, torch.arange(11)[None, :]
+    if mask == "bool":
+        dense = torch.rand(2, 2, 11, generator=torch.Generator().manual_seed(4)) < 0.5
+        dense[1, 0] = False  # a query that sees nothing
+        mask = AttentionMask(causal=False, bool_mask=dense)
+    elif mask == "start":
+        mask = AttentionMask(key_start=torch.tensor([0, 4], dtype=torch.int32), query_start=5)
+        dense = (j <= i - 4) & (j >= torch.tensor([0, 4])[:, None, None])
+    else:
+        dense = torch.ones(2, 2, 11, dtype=torch.bool)
+        if mask.causal:
+            dense = dense & (j <= i)
+        if mask.window:
+            dense = dense & ((i - j < mask.window) | (j < mask.sinks))
+    got = ops.quantized_attention(q, k_rows, v_rows, mask, scale=0.3)
+    k, v = (t.double() for t in ops.quantized_read(k_rows, v_rows, dtype=torch.float32))
+    score = torch.einsum("bqgnd,bkgd->bgnqk", q.double().view(2, 2, 2, 3, 64), k) * 0.3
+    p = torch.softmax(score.masked_fill(~dense[:, None, None], float("-inf")), -1).nan_to_num()
+    want = torch.einsum("bgnqk,bkgd->bqgnd", p, v).reshape(2, 2, 6, 64)
+    # fp32 sums of at most 64 products of size 10 and 11 terms: 2^-24 x 100
+    assert (got.double() - want).abs().max() <= 1e-5
+
+
+def test_gradients_reach_the_queries():
+    k_rows, v_rows = _filled(1, 5, 1, 32, 8)
+    q = torch.randn(1, 2, 2, 32, generator=torch.Generator().manual_seed(5), dtype=torch.float64).float().requires_grad_()
+    out = ops.quantized_attention(q, k_rows, v_rows, AttentionMask())
+    (grad,) = torch.autograd.grad(out.sum(), q)
+    k, v = ops.quantized_read(k_rows, v_rows, dtype=torch.float32)
+    (want,) = torch.autograd.grad(reference.attention(q, k, v, causal=True).sum(), q)
+    assert torch.equal(grad, want)

@@ -20,6 +20,7 @@ import torch.nn.functional as F
 
 from . import reference
 from .mask import AttentionMask
+from .quantized import QuantizedRows
 
 __all__ = [
     "grouped_matmul",
@@ -44,6 +45,10 @@ __all__ = [
     "rope_append",
     "swiglu",
     "attention",
+    "QuantizedRows",
+    "quantized_append",
+    "quantized_read",
+    "quantized_attention",
     "linear_cross_entropy",
     "linear_cross_entropy_mean",
     "token_logprobs",
@@ -423,7 +428,91 @@ def attention(
         scale=scale,
         softcap=softcap,
         dropout_p=dropout_p,
+        sinks=mask.sinks,
     )
+
+
+def quantized_append(k: torch.Tensor, v: torch.Tensor, k_rows: QuantizedRows, v_rows: QuantizedRows, slots: torch.Tensor) -> None:
+    """Writes keys and values ``[b, s, heads, d]`` (bf16, fp16 or fp32) in 4 or 8 bits to the slots ``slots`` (int64 ``[s]``, consecutive) of the rows of a cache with as many batch rows.
+    No gradient flows through a cache in few bits.  On a CUDA device, where the slots are not known to the host, a token whose slot lies outside the cache or does not follow the one
+    before is not written and counted as an index violation; elsewhere it is an error."""
+    from . import quantized
+
+    quantized.validate_pair(k_rows, v_rows)
+    b, h, n = k_rows.codes.shape[:3]
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != b or k.shape[2] != h or k.shape[3] != k_rows.head_dim:
+        raise ValueError(f"keys {tuple(k.shape)} and values {tuple(v.shape)} are not [{b}, tokens, {h}, {k_rows.head_dim}]")
+    if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"keys and values are bf16, fp16 or fp32, not {k.dtype} and {v.dtype}")
+    if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != k.shape[1] or not slots.is_contiguous():
+        raise ValueError(f"slots are contiguous int64 of [{k.shape[1]}], not {slots.dtype} of {tuple(slots.shape)}")
+    if not (k.device == v.device == slots.device == k_rows.codes.device):
+        raise ValueError("keys, values, slots and the cache are on one device")
+    if k.numel() == 0:
+        return
+    if cuda_ops_enabled(k) and _has_memory(k, v, slots, *k_rows, *v_rows):
+        quantized.append(k, v, k_rows, v_rows, slots)
+        return
+    first = int(slots[0])
+    if first < 0 or first + slots.shape[0] > n or not torch.equal(slots, torch.arange(first, first + slots.shape[0], device=slots.device)):
+        raise ValueError(f"slots are consecutive and within the {n} of the cache")
+    for x, rows in ((k, k_rows), (v, v_rows)):
+        codes, scales = reference.quantize_rows(x.detach().transpose(1, 2), rows.bits)
+        rows.codes[:, :, first : first + slots.shape[0]] = codes
+        rows.scales[:, :, first : first + slots.shape[0]] = scales
+
+
+def quantized_read(k_rows: QuantizedRows, v_rows: QuantizedRows, start: int = 0, stop: Optional[int] = None, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What slots ``start`` ... ``stop - 1`` of a quantised cache stand for: keys and values ``[b, stop - start, heads, d]``."""
+    from . import quantized
+
+    quantized.validate_pair(k_rows, v_rows)
+    stop = k_rows.slots if stop is None else stop
+    if not 0 <= start <= stop <= k_rows.slots:
+        raise ValueError(f"slots {start} to {stop} of a cache of {k_rows.slots}")
+    if not dtype.is_floating_point:
+        raise ValueError(f"a cache is read as floating-point numbers, not {dtype}")
+    if cuda_ops_enabled(k_rows.codes) and _has_memory(*k_rows, *v_rows):
+        k, v = quantized.read(k_rows, v_rows, start, stop, torch.bfloat16 if dtype == torch.bfloat16 else torch.float32)
+        return k.to(dtype), v.to(dtype)
+    k, v = (reference.dequantize_rows(r.codes[:, :, start:stop], r.scales[:, :, start:stop], dtype).transpose(1, 2).contiguous() for r in (k_rows, v_rows))
+    return k, v
+
+
+def quantized_attention(q: torch.Tensor, k_rows: QuantizedRows, v_rows: QuantizedRows, mask: Optional[AttentionMask] = None, *, scale: Optional[float] = None, softcap: float = 0.0,
+                        dropout_p: float = 0.0) -> torch.Tensor:
+    """:func:`attention` of ``q`` ``[b, s, h, d]`` over all slots of a quantised cache (``k_rows.first(n)`` for the first ``n``).  Up to 16 query rows per key head (tokens times heads that share it; 8
+    of 256 channels) attend to the codes as they are; more of them, and calls that need gradients, read the cache back in ``q``'s type first.  Masks are those of :func:`attention`
+    with other numbers of queries than of keys: causal ones put the queries into the last slots; documents and chunks have no meaning here."""
+    from . import quantized
+
+    mask = mask if mask is not None else AttentionMask(causal=False)
+    quantized.validate_pair(k_rows, v_rows)
+    b, h, n = k_rows.codes.shape[:3]
+    if q.dim() != 4 or q.shape[0] != b or q.shape[3] != k_rows.head_dim or h == 0 or q.shape[2] % h:
+        raise ValueError(f"queries {tuple(q.shape)} do not fit a cache of {b} rows and {h} heads of {k_rows.head_dim} channels")
+    if q.device != k_rows.codes.device:
+        raise ValueError(f"queries are on {q.device}, the cache on {k_rows.codes.device}")
+    s = q.shape[1]
+    if mask.bool_mask is not None:
+        m = mask.bool_mask
+        if m.dim() not in (3, 4) or m.shape[-1] != n or m.shape[-2] not in (1, s) or m.shape[0] not in (1, b) or (m.dim() == 4 and m.shape[1] != 1):
+            raise ValueError(f"a mask {tuple(m.shape)} does not fit {b} rows of {s} queries and {n} slots")
+    elif mask.doc_ids is not None or mask.chunk > 0:
+        raise ValueError("documents and chunks have no meaning over a cache")
+    elif mask.key_start is not None:
+        if mask.window > 0 or mask.key_start.numel() != b or mask.query_start < 0 or mask.query_start + s > n:
+            raise ValueError("key_start / query_start do not fit the queries and slots, or come with a window")
+    elif mask.window > 0 and not mask.causal:
+        raise ValueError("a window needs a causal mask")
+    elif mask.causal and s > n:
+        raise ValueError(f"{s} causal queries in {n} slots")
+    if q.numel() == 0 or n == 0:
+        return torch.zeros_like(q)
+    if (_native(q) and softcap <= 0.0 and dropout_p == 0.0 and not _differentiated(q) and _has_memory(q, *k_rows, *v_rows) and quantized.attends(s, q.shape[2], k_rows, v_rows)):
+        return quantized.attention(q, k_rows, v_rows, mask, scale)
+    k, v = quantized_read(k_rows, v_rows, dtype=q.dtype)
+    return attention(q, k, v, mask, scale=scale, softcap=softcap, dropout_p=dropout_p)
 
 
 def linear_cross_entropy(

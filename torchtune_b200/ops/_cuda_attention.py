@@ -169,6 +169,8 @@ def unsupported_reason(q: torch.Tensor, k: torch.Tensor, mask: AttentionMask) ->
         return "structured mask with different query and key lengths"
     if mask.bool_mask is not None and mask.bool_mask.dim() == 4 and mask.bool_mask.shape[1] != 1:
         return "per-head boolean mask"
+    if mask.bool_mask is None and mask.window > 0 and mask.sinks > 0:
+        return "first tokens that a window leaves visible"
     return None
 
 

@@ -21,6 +21,7 @@ class AttentionMask:
     doc_ids: Optional[torch.Tensor] = None  # [b, s] int32, equal ids may attend
     chunk: int = 0  # >0: positions attend only inside the same chunk of this size
     window: int = 0  # >0: key must be within this many positions before the query
+    sinks: int = 0  # >0, with a window: the first tokens of the sequence (of each document, where there are some) stay visible to all later ones
     bool_mask: Optional[torch.Tensor] = None  # dense [b, sq, skv], True = attend
     # Cached decoding of left-padded rows: query i sits in cache slot query_start + i and sees the slots key_start[b] ... its own.
     key_start: Optional[torch.Tensor] = None  # [b] int32
@@ -50,7 +51,7 @@ class AttentionMask:
             if self.doc_ids is not None or self.chunk > 0 or self.window > 0:
                 raise ValueError("key_start does not combine with document ids, chunks or windows")
             return m.expand(b, sq, skv)
-        m = dense_mask(b, sq, skv, device, self.causal, self.doc_ids, self.chunk, self.window)
+        m = dense_mask(b, sq, skv, device, self.causal, self.doc_ids, self.chunk, self.window, sinks=self.sinks)
         return None if m is None else m.squeeze(1)
 
     @staticmethod

@@ -159,8 +159,9 @@ def dense_mask(
     chunk: int = 0,
     window: int = 0,
     q_offset: int = 0,
+    sinks: int = 0,
 ) -> Optional[torch.Tensor]:
-    """Boolean ``[b, 1, sq, skv]`` mask (True = attend) for the structured mask kinds."""
+    """Boolean ``[b, 1, sq, skv]`` mask (True = attend) for the structured mask kinds; ``sinks``: first tokens (of each document) that a window leaves visible."""
     if not causal and doc_ids is None and chunk <= 0 and window <= 0:
         return None
     qi = torch.arange(sq, device=device).view(1, sq, 1) + q_offset
@@ -170,7 +171,13 @@ def dense_mask(
         m = m & (ki <= qi)
     if chunk > 0:
         m = m & ((qi // chunk) == (ki // chunk))
-    if window > 0:
+    if window > 0 and sinks > 0:
+        first = torch.zeros_like(ki)
+        if doc_ids is not None:
+            new = F.pad(doc_ids[:, 1:] != doc_ids[:, :-1], (1, 0))
+            first = torch.where(new, torch.arange(skv, device=device), 0).cummax(1).values.view(b, 1, skv)
+        m = m & (((qi - ki) < window) | ((ki - first) < sinks))
+    elif window > 0:
         m = m & ((qi - ki) < window)
     if doc_ids is not None:
         m = m & (doc_ids.view(b, sq, 1) == doc_ids.view(b, 1, skv))
@@ -190,6 +197,7 @@ def attention(
     scale: Optional[float] = None,
     softcap: float = 0.0,
     dropout_p: float = 0.0,
+    sinks: int = 0,
 ) -> torch.Tensor:
     """``softmax(q k^T * scale + mask) v`` on ``[b, s, h, d]`` tensors with grouped
     KV heads: query head ``h`` reads KV head ``h // (hq / hkv)``
@@ -208,7 +216,7 @@ def attention(
     if bool_mask is not None:
         m = bool_mask if bool_mask.dim() == 4 else bool_mask.unsqueeze(1)
     else:
-        m = dense_mask(b, sq, skv, q.device, causal, doc_ids, chunk, window, q_offset=skv - sq if causal else 0)
+        m = dense_mask(b, sq, skv, q.device, causal, doc_ids, chunk, window, q_offset=skv - sq if causal else 0, sinks=sinks)
     if m is not None:
         s = s.masked_fill(~m.unsqueeze(2), float("-inf"))
     p = torch.softmax(s, dim=-1)
@@ -441,3 +449,27 @@ def mx_dequantize(q: torch.Tensor, e_byte: torch.Tensor) -> torch.Tensor:
 def mx_roundtrip(x: torch.Tensor, transpose: bool = False) -> torch.Tensor:
     """Quantise and dequantise (fp32 result, shape of the operand)."""
     return mx_dequantize(*mx_quantize(x, transpose))
+
+
+# --------------------------------------------------------------------------- key/value caches in 4 or 8 bits
+def quantize_rows(x: torch.Tensor, bits: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Codes (uint8, packed) and bf16 scales of the rows ``x`` ``[..., d]``, as :class:`~torchtune_b200.ops.quantized.QuantizedRows` describes them: a group's scale is its value of largest
+    magnitude (the first of equals) over ``-2^(bits - 1)``, codes are the nearest.  Groups that hold an infinity or a NaN read as NaN."""
+    half = 2 ** (bits - 1)
+    g = x.float().unflatten(-1, (4, x.shape[-1] // 32, 8)).transpose(-3, -2).flatten(-2)
+    size = torch.where(g.isnan(), float("inf"), g.abs())
+    size = torch.where(g.isnan().any(-1, keepdim=True) & ~g.isnan(), 0.0, size)  # a NaN comes before an infinity
+    scale = (g.gather(-1, size.argmax(-1, keepdim=True)) / -half).to(torch.bfloat16)
+    s = scale.float()
+    code = torch.where((s != 0) & s.isfinite(), g / s, 0.0).round().clamp(-half, half - 1) + half
+    code = code.unflatten(-1, (4, 8)).transpose(-3, -2).reshape(x.shape).to(torch.uint8)
+    return (code if bits == 8 else code[..., 0::2] | code[..., 1::2] << 4), scale.squeeze(-1)
+
+
+def dequantize_rows(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """What :func:`quantize_rows` stands for, formed in fp32 and rounded to ``dtype``."""
+    groups = scales.shape[-1]
+    wide = codes.shape[-1] == groups * 32
+    code = codes if wide else torch.stack([codes & 15, codes >> 4], -1).flatten(-2)
+    x = (code.float() - (128 if wide else 8)).unflatten(-1, (4, groups, 8)) * scales.float()[..., None, :, None]
+    return x.flatten(-3).to(dtype)
