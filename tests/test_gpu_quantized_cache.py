@@ -214,14 +214,13 @@ def test_slots_behind_the_last_are_not_read():
 
 def test_views_and_odd_strides():
     k_rows, v_rows = _filled(6, 100, 4, 128, 4)
-    part = [QuantizedRows(r.codes[1::2, 1:3], r.scales[1::2, 1:3]) for r in (k_rows, v_rows)]
+    part = [QuantizedRows(r.codes[1::2, 1:3], r.scales[1::2, 1:3], 100) for r in (k_rows, v_rows)]
     seen = torch.ones(3, 1, 100, dtype=torch.bool, device="cuda")
     got = _check(_queries(3, 1, 8, 128), *part, AttentionMask(), seen)
     q = torch.randn(3, 1, 8, 257, generator=_gen(9), device="cuda").to(torch.bfloat16)
     _check(q[..., 1:129], *part, AttentionMask(), seen)
     # rows that do not start on 16 bytes are read back first
-    loose = [QuantizedRows(r.codes.contiguous(), r.scales[:, :, :99].contiguous()) for r in part]
-    loose = [QuantizedRows(r.codes[:, :, :99].contiguous(), r.scales) for r in loose]
+    loose = [QuantizedRows(r.codes[:, :, :99].contiguous(), r.scales[:, :, :99].contiguous()) for r in part]
     near = ops.quantized_attention(_queries(3, 1, 8, 128), *loose, AttentionMask())
     assert torch.allclose(near.float(), ops.quantized_attention(_queries(3, 1, 8, 128), part[0].first(99), part[1].first(99), AttentionMask()).float(), atol=2.0**-6)
     assert got.shape == (3, 1, 8, 128)

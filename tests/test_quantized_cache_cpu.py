@@ -66,10 +66,17 @@ def test_groups_of_zeros_ties_and_non_finite_values(bits):
 
 def test_rows_are_views_with_their_own_sizes():
     rows = QuantizedRows.zeros(3, 13, 2, 64, 4)
-    assert rows.codes.shape == (3, 2, 13, 32) and rows.scales.shape == (3, 2, 13, 2) and rows.bits == 4 and rows.head_dim == 64 and rows.slots == 13
+    assert rows.codes.shape == (3, 2, 16, 32) and rows.scales.shape == (3, 2, 16, 2) and rows.bits == 4 and rows.head_dim == 64 and rows.slots == 13
     part = rows.batch(2).first(5)
-    assert part.codes.shape == (2, 2, 5, 32) and part.codes.data_ptr() == rows.codes.data_ptr()
+    assert part.codes.shape[0] == 2 and part.slots == 5 and part.codes.data_ptr() == rows.codes.data_ptr()
+    for slots in (-1, 6):
+        with pytest.raises(ValueError):
+            part.first(slots)
     assert QuantizedRows.zeros(1, 3, 1, 32, 8).bits == 8
+    with pytest.raises(ValueError):
+        ops.quantized_read(rows, rows.first(3))
+    with pytest.raises(ValueError):
+        ops.quantized_read(*(QuantizedRows(rows.codes, rows.scales, 17) for _ in "kv"))
     for bits, d in ((2, 64), (4, 48), (8, 0)):
         with pytest.raises(ValueError):
             QuantizedRows.zeros(1, 4, 1, d, bits)

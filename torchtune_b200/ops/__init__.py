@@ -438,42 +438,42 @@ def quantized_append(k: torch.Tensor, v: torch.Tensor, k_rows: QuantizedRows, v_
     before is not written and counted as an index violation; elsewhere it is an error."""
     from . import quantized
 
-    quantized.validate_pair(k_rows, v_rows)
-    b, h, n = k_rows.codes.shape[:3]
-    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != b or k.shape[2] != h or k.shape[3] != k_rows.head_dim:
-        raise ValueError(f"keys {tuple(k.shape)} and values {tuple(v.shape)} are not [{b}, tokens, {h}, {k_rows.head_dim}]")
+    b, h, n, d, bits = quantized.sizes(k_rows, v_rows)
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or shape[0] != b or shape[2] != h or shape[3] != d:
+        raise ValueError(f"keys {tuple(k.shape)} and values {tuple(v.shape)} are not [{b}, tokens, {h}, {d}]")
     if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError(f"keys and values are bf16, fp16 or fp32, not {k.dtype} and {v.dtype}")
-    if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != k.shape[1] or not slots.is_contiguous():
-        raise ValueError(f"slots are contiguous int64 of [{k.shape[1]}], not {slots.dtype} of {tuple(slots.shape)}")
+    if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != shape[1] or not slots.is_contiguous():
+        raise ValueError(f"slots are contiguous int64 of [{shape[1]}], not {slots.dtype} of {tuple(slots.shape)}")
     if not (k.device == v.device == slots.device == k_rows.codes.device):
         raise ValueError("keys, values, slots and the cache are on one device")
-    if k.numel() == 0:
+    if b == 0 or h == 0 or shape[1] == 0:
         return
-    if cuda_ops_enabled(k) and _has_memory(k, v, slots, *k_rows, *v_rows):
-        quantized.append(k, v, k_rows, v_rows, slots)
+    if cuda_ops_enabled(k) and _has_memory(k, v, slots) and quantized.plain(k_rows, v_rows):
+        quantized.append(k, v, k_rows, v_rows, slots, bits)
         return
     first = int(slots[0])
-    if first < 0 or first + slots.shape[0] > n or not torch.equal(slots, torch.arange(first, first + slots.shape[0], device=slots.device)):
+    if first < 0 or first + shape[1] > n or not torch.equal(slots, torch.arange(first, first + shape[1], device=slots.device)):
         raise ValueError(f"slots are consecutive and within the {n} of the cache")
     for x, rows in ((k, k_rows), (v, v_rows)):
-        codes, scales = reference.quantize_rows(x.detach().transpose(1, 2), rows.bits)
-        rows.codes[:, :, first : first + slots.shape[0]] = codes
-        rows.scales[:, :, first : first + slots.shape[0]] = scales
+        codes, scales = reference.quantize_rows(x.detach().transpose(1, 2), bits)
+        rows.codes[:, :, first : first + shape[1]] = codes
+        rows.scales[:, :, first : first + shape[1]] = scales
 
 
 def quantized_read(k_rows: QuantizedRows, v_rows: QuantizedRows, start: int = 0, stop: Optional[int] = None, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """What slots ``start`` ... ``stop - 1`` of a quantised cache stand for: keys and values ``[b, stop - start, heads, d]``."""
     from . import quantized
 
-    quantized.validate_pair(k_rows, v_rows)
-    stop = k_rows.slots if stop is None else stop
-    if not 0 <= start <= stop <= k_rows.slots:
-        raise ValueError(f"slots {start} to {stop} of a cache of {k_rows.slots}")
+    size = quantized.sizes(k_rows, v_rows)
+    stop = size[2] if stop is None else stop
+    if not 0 <= start <= stop <= size[2]:
+        raise ValueError(f"slots {start} to {stop} of a cache of {size[2]}")
     if not dtype.is_floating_point:
         raise ValueError(f"a cache is read as floating-point numbers, not {dtype}")
-    if cuda_ops_enabled(k_rows.codes) and _has_memory(*k_rows, *v_rows):
-        k, v = quantized.read(k_rows, v_rows, start, stop, torch.bfloat16 if dtype == torch.bfloat16 else torch.float32)
+    if cuda_ops_enabled(k_rows.codes) and quantized.plain(k_rows, v_rows):
+        k, v = quantized.read(k_rows, v_rows, start, stop, torch.bfloat16 if dtype == torch.bfloat16 else torch.float32, size)
         return k.to(dtype), v.to(dtype)
     k, v = (reference.dequantize_rows(r.codes[:, :, start:stop], r.scales[:, :, start:stop], dtype).transpose(1, 2).contiguous() for r in (k_rows, v_rows))
     return k, v
@@ -487,17 +487,17 @@ def quantized_attention(q: torch.Tensor, k_rows: QuantizedRows, v_rows: Quantize
     from . import quantized
 
     mask = mask if mask is not None else AttentionMask(causal=False)
-    quantized.validate_pair(k_rows, v_rows)
-    b, h, n = k_rows.codes.shape[:3]
-    if q.dim() != 4 or q.shape[0] != b or q.shape[3] != k_rows.head_dim or h == 0 or q.shape[2] % h:
-        raise ValueError(f"queries {tuple(q.shape)} do not fit a cache of {b} rows and {h} heads of {k_rows.head_dim} channels")
+    size = b, h, n, d, _ = quantized.sizes(k_rows, v_rows)
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != b or shape[3] != d or h == 0 or shape[2] % h:
+        raise ValueError(f"queries {tuple(q.shape)} do not fit a cache of {b} rows and {h} heads of {d} channels")
     if q.device != k_rows.codes.device:
         raise ValueError(f"queries are on {q.device}, the cache on {k_rows.codes.device}")
-    s = q.shape[1]
+    s = shape[1]
     if mask.bool_mask is not None:
-        m = mask.bool_mask
-        if m.dim() not in (3, 4) or m.shape[-1] != n or m.shape[-2] not in (1, s) or m.shape[0] not in (1, b) or (m.dim() == 4 and m.shape[1] != 1):
-            raise ValueError(f"a mask {tuple(m.shape)} does not fit {b} rows of {s} queries and {n} slots")
+        m = mask.bool_mask.shape
+        if len(m) not in (3, 4) or m[-1] != n or m[-2] not in (1, s) or m[0] not in (1, b) or (len(m) == 4 and m[1] != 1):
+            raise ValueError(f"a mask {tuple(m)} does not fit {b} rows of {s} queries and {n} slots")
     elif mask.doc_ids is not None or mask.chunk > 0:
         raise ValueError("documents and chunks have no meaning over a cache")
     elif mask.key_start is not None:
@@ -507,10 +507,12 @@ def quantized_attention(q: torch.Tensor, k_rows: QuantizedRows, v_rows: Quantize
         raise ValueError("a window needs a causal mask")
     elif mask.causal and s > n:
         raise ValueError(f"{s} causal queries in {n} slots")
-    if q.numel() == 0 or n == 0:
+    if b == 0 or s == 0 or n == 0:
         return torch.zeros_like(q)
-    if (_native(q) and softcap <= 0.0 and dropout_p == 0.0 and not _differentiated(q) and _has_memory(q, *k_rows, *v_rows) and quantized.attends(s, q.shape[2], k_rows, v_rows)):
-        return quantized.attention(q, k_rows, v_rows, mask, scale)
+    if _native(q) and softcap <= 0.0 and dropout_p == 0.0 and not _differentiated(q) and _has_memory(q) and quantized.plain(k_rows, v_rows):
+        steps = quantized.layout(s, shape[2], k_rows, v_rows, size)
+        if steps is not None:
+            return quantized.attention(q, k_rows, v_rows, mask, scale, size, steps)
     k, v = quantized_read(k_rows, v_rows, dtype=q.dtype)
     return attention(q, k, v, mask, scale=scale, softcap=softcap, dropout_p=dropout_p)
 

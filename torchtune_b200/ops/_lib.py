@@ -173,7 +173,7 @@ def _declare(L: ctypes.CDLL) -> None:
     L.ttb_quantized_append.restype = i32
     L.ttb_quantized_read.argtypes = [vp] * 4 + [c.POINTER(i64), vp, vp] + [i32] * 7 + [vp]
     L.ttb_quantized_read.restype = i32
-    L.ttb_quantized_attention.argtypes = [vp] * 5 + [c.POINTER(i64), vp, vp, i64, i64, vp] + [i32] * 10 + [f32, vp]
+    L.ttb_quantized_attention.argtypes = [vp] * 5 + [c.POINTER(i64), vp, vp, i64, i64, vp] + [i32] * 10 + [f32, vp, i64, vp]
     L.ttb_quantized_attention.restype = i32
     for fn in (L.ttb_span_decode_tile, L.ttb_span_prepare, L.ttb_span_prefill, L.ttb_span_decode, L.ttb_stream_step, L.ttb_embed_positions, L.ttb_clamped_glu, L.ttb_lightning_recurrent,
                L.ttb_lightning_chunks, L.ttb_silu_rows, L.ttb_gated_norm):

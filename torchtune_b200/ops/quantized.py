@@ -18,22 +18,24 @@ class QuantizedRows(NamedTuple):
     """The keys (or the values) of a cache: one row of codes and scales per batch row, head and slot.
 
     ``codes`` uint8 ``[batch, heads, slots, d * bits / 8]``, ``scales`` bf16 ``[batch, heads, slots, d / 32]``; ``d`` is a multiple of 32, ``bits`` 4 or 8.  Seen as ``[4, d / 32, 8]``, a row's channels
-    with the same middle index are a group; channel ``c`` stands for ``scale[group] * (code[c] - 2^(bits - 1))``.  Of 4 bits two codes share a byte, the even channel in the low half."""
+    with the same middle index are a group; channel ``c`` stands for ``scale[group] * (code[c] - 2^(bits - 1))``.  Of 4 bits two codes share a byte, the even channel in the low half.
+    ``count``: how many of the slots are meant (:meth:`first`), ``-1`` for all."""
 
     codes: torch.Tensor
     scales: torch.Tensor
+    count: int = -1
 
     @property
     def head_dim(self) -> int:
-        return self.scales.shape[-1] * 32
+        return self.scales.shape[3] * 32
 
     @property
     def bits(self) -> int:
-        return self.codes.shape[-1] * 8 // self.head_dim
+        return self.codes.shape[3] * 8 // self.head_dim
 
     @property
     def slots(self) -> int:
-        return self.codes.shape[2]
+        return self.codes.shape[2] if self.count < 0 else self.count
 
     @classmethod
     def zeros(cls, batch: int, slots: int, heads: int, head_dim: int, bits: int, device=None) -> "QuantizedRows":
@@ -45,129 +47,128 @@ class QuantizedRows(NamedTuple):
         held = -(-slots // 8) * 8
         codes = torch.zeros(batch, heads, held, head_dim * bits // 8, dtype=torch.uint8, device=device)
         scales = torch.zeros(batch, heads, held, head_dim // 32, dtype=torch.bfloat16, device=device)
-        return cls(codes[:, :, :slots], scales[:, :, :slots])
+        return cls(codes, scales, slots)
 
     def first(self, slots: int) -> "QuantizedRows":
-        """The first ``slots`` slots (a view)."""
-        return QuantizedRows(self.codes[:, :, :slots], self.scales[:, :, :slots])
+        """The first ``slots`` slots."""
+        if not 0 <= slots <= self.slots:
+            raise ValueError(f"{slots} of {self.slots} slots")
+        return QuantizedRows(self.codes, self.scales, slots)
 
     def batch(self, rows: int) -> "QuantizedRows":
         """The first ``rows`` batch rows (a view)."""
-        return QuantizedRows(self.codes[:rows], self.scales[:rows])
+        return QuantizedRows(self.codes[:rows], self.scales[:rows], self.count)
 
 
-def validate(rows: QuantizedRows, name: str) -> None:
-    codes, scales = rows
-    if codes.dim() != 4 or scales.dim() != 4 or codes.shape[:3] != scales.shape[:3]:
-        raise ValueError(f"{name}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not [batch, heads, slots, ...] of the same rows")
-    if codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16:
-        raise ValueError(f"{name}: codes are uint8 and scales bfloat16, not {codes.dtype} and {scales.dtype}")
-    if scales.shape[3] == 0 or codes.shape[3] not in (scales.shape[3] * 16, scales.shape[3] * 32):
-        raise ValueError(f"{name}: rows of {codes.shape[3]} bytes with {scales.shape[3]} scales are neither 4 nor 8 bits (32 channels share a scale)")
-    if codes.device != scales.device:
-        raise ValueError(f"{name}: codes and scales are on different devices")
+def sizes(k_rows: QuantizedRows, v_rows: QuantizedRows) -> Tuple[int, int, int, int, int]:
+    """``(batch, heads, slots, head_dim, bits)`` of the keys and values of a cache; an error if they are not a pair of rows."""
+    kc, ks, n = k_rows
+    vc, vs, vn = v_rows
+    a, g = kc.shape, ks.shape
+    if (len(a) == 4 and a == vc.shape and g == vs.shape and n == vn and len(g) == 4 and a[:3] == g[:3] and kc.dtype is torch.uint8 and vc.dtype is torch.uint8 and ks.dtype is torch.bfloat16
+            and vs.dtype is torch.bfloat16 and n <= a[2] and g[3] > 0 and (a[3] == g[3] * 16 or a[3] == g[3] * 32) and kc.device == vc.device == ks.device == vs.device):
+        return a[0], a[1], a[2] if n < 0 else n, g[3] * 32, a[3] // (g[3] * 4)
+    for name, (codes, scales, count) in (("k_rows", k_rows), ("v_rows", v_rows)):
+        if codes.dim() != 4 or scales.dim() != 4 or codes.shape[:3] != scales.shape[:3] or count > codes.shape[2]:
+            raise ValueError(f"{name}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not [batch, heads, slots, ...] of the same rows")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16:
+            raise ValueError(f"{name}: codes are uint8 and scales bfloat16, not {codes.dtype} and {scales.dtype}")
+        if scales.shape[3] == 0 or codes.shape[3] not in (scales.shape[3] * 16, scales.shape[3] * 32):
+            raise ValueError(f"{name}: rows of {codes.shape[3]} bytes with {scales.shape[3]} scales are neither 4 nor 8 bits (32 channels share a scale)")
+    raise ValueError(f"keys {tuple(kc.shape)} on {kc.device} and values {tuple(vc.shape)} on {vc.device} of a cache have the same shape, bits, slots and device")
 
 
-def validate_pair(k_rows: QuantizedRows, v_rows: QuantizedRows) -> None:
-    validate(k_rows, "k_rows")
-    validate(v_rows, "v_rows")
-    if k_rows.codes.shape != v_rows.codes.shape or k_rows.scales.shape != v_rows.scales.shape or k_rows.codes.device != v_rows.codes.device:
-        raise ValueError(f"keys {tuple(k_rows.codes.shape)} and values {tuple(v_rows.codes.shape)} of a cache have the same shape, bits and device")
+def plain(*rows: QuantizedRows) -> bool:
+    """Whether these are ordinary tensors, whose address a kernel can be given."""
+    return all(type(r.codes) is torch.Tensor and type(r.scales) is torch.Tensor for r in rows)
 
 
-def _here(t: torch.Tensor) -> "_OnDevice":
-    return _OnDevice(t.device.index)
+def _on(device: torch.device, call, *args) -> int:
+    """Calls a kernel with the device of its operands as the current one (kernels launch on the current device's stream)."""
+    if device.index == torch.cuda.current_device():
+        return call(*args, stream_ptr())
+    with torch.cuda.device(device):
+        return call(*args, stream_ptr())
 
 
-class _OnDevice:
-    """Makes the device of the operands the current one, if it is not (kernels launch on the current device's stream)."""
-
-    def __init__(self, index: int) -> None:
-        self.index, self.was = index, -1
-
-    def __enter__(self) -> None:
-        if self.index != torch.cuda.current_device():
-            self.was = torch.cuda.current_device()
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc) -> None:
-        if self.was >= 0:
-            torch.cuda.set_device(self.was)
+def _steps(rows: QuantizedRows) -> Tuple[int, ...]:
+    """Strides of batch, head and slot, of codes and of scales."""
+    codes, scales = rows.codes.stride(), rows.scales.stride()
+    if codes[3] != 1 or (scales[3] != 1 and rows.scales.shape[3] > 1):
+        raise ValueError("the codes and scales of a row have to lie one behind the other")
+    return codes[:3] + scales[:3]
 
 
-def _inner(rows: QuantizedRows) -> bool:
-    """Whether each row's codes and scales lie one behind the other."""
-    return rows.codes.stride(3) == 1 and (rows.scales.stride(3) == 1 or rows.scales.shape[3] == 1)
-
-
-def append(k: torch.Tensor, v: torch.Tensor, k_rows: QuantizedRows, v_rows: QuantizedRows, slots: torch.Tensor) -> None:
+def append(k: torch.Tensor, v: torch.Tensor, k_rows: QuantizedRows, v_rows: QuantizedRows, slots: torch.Tensor, bits: int) -> None:
     b, s, h, d = k.shape
     if k.stride(3) != 1:
         k = k.contiguous()
     if v.stride(3) != 1:
         v = v.contiguous()
-    if not (_inner(k_rows) and _inner(v_rows)):
-        raise ValueError("the codes and scales of a row have to lie one behind the other")
-    strides = (ctypes.c_longlong * 18)(*k.stride()[:3], *v.stride()[:3], *k_rows.codes.stride()[:3], *k_rows.scales.stride()[:3], *v_rows.codes.stride()[:3], *v_rows.scales.stride()[:3])
-    with _here(k):
-        check(lib().ttb_quantized_append(k.data_ptr(), v.data_ptr(), k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides,
-                                         slots.data_ptr(), _TYPES[k.dtype], b, s, h, d, k_rows.bits, k_rows.slots, stream_ptr()), "quantised append")
+    strides = (ctypes.c_longlong * 18)(*k.stride()[:3], *v.stride()[:3], *_steps(k_rows), *_steps(v_rows))
+    check(_on(k.device, lib().ttb_quantized_append, k.data_ptr(), v.data_ptr(), k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides,
+              slots.data_ptr(), _TYPES[k.dtype], b, s, h, d, bits, k_rows.slots), "quantised append")
 
 
-def read(k_rows: QuantizedRows, v_rows: QuantizedRows, start: int, stop: int, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
-    b, h = k_rows.codes.shape[:2]
-    n, d = stop - start, k_rows.head_dim
-    k = torch.empty(b, n, h, d, dtype=dtype, device=k_rows.codes.device)
+def read(k_rows: QuantizedRows, v_rows: QuantizedRows, start: int, stop: int, dtype: torch.dtype, size: Tuple[int, int, int, int, int]) -> Tuple[torch.Tensor, torch.Tensor]:
+    b, h, _, d, bits = size
+    n = stop - start
+    codes = k_rows.codes
+    k = torch.empty(b, n, h, d, dtype=dtype, device=codes.device)
     v = torch.empty_like(k)
-    if k.numel() == 0:
-        return k, v
-    if not (_inner(k_rows) and _inner(v_rows)):
-        raise ValueError("the codes and scales of a row have to lie one behind the other")
-    strides = (ctypes.c_longlong * 12)(*k_rows.codes.stride()[:3], *k_rows.scales.stride()[:3], *v_rows.codes.stride()[:3], *v_rows.scales.stride()[:3])
-    with _here(k):
-        check(lib().ttb_quantized_read(k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides, k.data_ptr(), v.data_ptr(), b, start, n, h, d,
-                                       k_rows.bits, int(dtype == torch.float32), stream_ptr()), "quantised read")
+    if b and n and h:
+        strides = (ctypes.c_longlong * 12)(*_steps(k_rows), *_steps(v_rows))
+        check(_on(codes.device, lib().ttb_quantized_read, codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides, k.data_ptr(), v.data_ptr(), b, start,
+                  n, h, d, bits, int(dtype == torch.float32)), "quantised read")
     return k, v
 
 
-def attends(s: int, hq: int, k_rows: QuantizedRows, v_rows: QuantizedRows) -> bool:
-    """Whether the kernel for few queries takes these rows; the visibility words of a cluster of 16 CTAs bound the number of slots."""
-    d, group = k_rows.head_dim, hq // k_rows.codes.shape[1]
-    if d not in HEAD_DIMS or s * group > (8 if d == 256 else 16) or -(-k_rows.slots // 512) * (s + 1) * 4 > 16384:
-        return False
-    for rows in (k_rows, v_rows):
-        codes, scales = rows
-        if not _inner(rows) or codes.stride(2) != codes.shape[3] or scales.stride(2) != scales.shape[3]:
-            return False
-        if (codes.data_ptr() | scales.data_ptr() | codes.stride(0) | codes.stride(1) | 2 * scales.stride(0) | 2 * scales.stride(1)) & 15:
-            return False
-    return True
+def layout(s: int, hq: int, k_rows: QuantizedRows, v_rows: QuantizedRows, size: Tuple[int, int, int, int, int]) -> Optional[Tuple[int, ...]]:
+    """Batch and head strides of codes and scales for the kernel of few queries, or ``None`` where it does not take these rows; the visibility words of a cluster of 8 CTAs bound the number of slots."""
+    _, h, n, d, bits = size
+    if d not in HEAD_DIMS or s * (hq // h) > (8 if d == 256 else 16) or (-(-n // 256) * (s + 2) + 1) * 4 > 16384:
+        return None
+    row, groups = d * bits // 8, d // 32
+    steps: Tuple[int, ...] = ()
+    for codes, scales, _ in (k_rows, v_rows):
+        c, g = codes.stride(), scales.stride()
+        if c[3] != 1 or g[3] != 1 or c[2] != row or g[2] != groups or (c[0] | c[1] | 2 * g[0] | 2 * g[1] | codes.data_ptr() | scales.data_ptr()) & 15:
+            return None
+        steps += (c[0], c[1], g[0], g[1])
+    return steps
 
 
-def attention(q: torch.Tensor, k_rows: QuantizedRows, v_rows: QuantizedRows, mask: AttentionMask, scale: Optional[float]) -> torch.Tensor:
+def attention(q: torch.Tensor, k_rows: QuantizedRows, v_rows: QuantizedRows, mask: AttentionMask, scale: Optional[float], size: Tuple[int, int, int, int, int], steps: Tuple[int, ...]) -> torch.Tensor:
     b, s, hq, d = q.shape
-    hkv, n = k_rows.codes.shape[1], k_rows.slots
+    _, hkv, n, _, bits = size
     q = q.contiguous()
-    if q.data_ptr() % 16:
+    if q.data_ptr() & 15:
         q = q.clone()
     o = torch.empty_like(q)
-    seen, start, offset, window, sinks = None, None, -1, 0, 0
-    if mask.bool_mask is not None:
-        seen = mask.bool_mask if mask.bool_mask.dim() == 3 else mask.bool_mask[:, 0]
-        if seen.dtype != torch.bool or not seen.device == q.device:
-            seen = seen.to(device=q.device, dtype=torch.bool)
-        seen = seen.expand(b, s, n)
-        if seen.stride(2) != 1 and n > 1:
-            seen = seen.contiguous()
+    seen, seen_b, seen_r, start, offset, window, sinks = None, 0, 0, None, -1, 0, 0
+    m = mask.bool_mask
+    if m is not None:
+        m = m if m.dim() == 3 else m[:, 0]
+        if m.dtype is not torch.bool or m.device != q.device:
+            m = m.to(device=q.device, dtype=torch.bool)
+        if m.shape[0] != b or m.shape[1] != s:
+            m = m.expand(b, s, n)
+        seen_b, seen_r, unit = m.stride()
+        if unit != 1 and n > 1:
+            m = m.contiguous()
+            seen_b, seen_r, _ = m.stride()
+        seen = m.data_ptr()
     elif mask.key_start is not None:
         start = mask.key_start.to(device=q.device, dtype=torch.int32).contiguous()
         offset = mask.query_start
     elif mask.causal:
-        offset, window, sinks = n - s, mask.window, mask.sinks if mask.window else 0
-    strides = (ctypes.c_longlong * 8)(*k_rows.codes.stride()[:2], *k_rows.scales.stride()[:2], *v_rows.codes.stride()[:2], *v_rows.scales.stride()[:2])
-    with _here(q):
-        check(lib().ttb_quantized_attention(q.data_ptr(), k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides, o.data_ptr(),
-                                            None if seen is None else seen.data_ptr(), 0 if seen is None else seen.stride(0), 0 if seen is None else seen.stride(1),
-                                            None if start is None else start.data_ptr(), offset, window, sinks, b, s, n, hq, hkv, d, k_rows.bits,
-                                            1.0 / math.sqrt(d) if scale is None else float(scale), stream_ptr()), "attention over a quantised cache")
+        offset, window = n - s, max(mask.window, 0)
+        sinks = max(mask.sinks, 0) if window else 0
+    work, floats = None, 0
+    if n >= 2048 and b * hkv * 8 < 592:  # few and long rows are split further than a cluster reaches
+        floats = 128 * b * s * hq * (d + 4)
+        work = torch.empty(floats, dtype=torch.float32, device=q.device)
+    check(_on(q.device, lib().ttb_quantized_attention, q.data_ptr(), k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(),
+              (ctypes.c_longlong * 8)(*steps), o.data_ptr(), seen, seen_b, seen_r, None if start is None else start.data_ptr(), offset, window, sinks, b, s, n, hq, hkv, d, bits,
+              1.0 / math.sqrt(d) if scale is None else float(scale), None if work is None else work.data_ptr(), floats), "attention over a quantised cache")
     return o
