@@ -5,7 +5,7 @@
 
 Parity: recipes/generate.py:29-220 of the reference — same config keys (``prompt.system`` /
 ``prompt.user``, ``max_new_tokens``, ``temperature``, ``top_k``, ``enable_kv_cache``,
-``quantizer``).  Decoding uses the package's KV-cache attention path; the time to first token
+``quantizer``), and ``kv_cache_bits`` (4 or 8) for caches in few bits.  Decoding uses the package's KV-cache attention path; the time to first token
 and tokens/s are logged.
 """
 import itertools
@@ -72,7 +72,8 @@ class InferenceRecipe:
         total_len = prompt.numel() + cfg.max_new_tokens
         if cfg.get("enable_kv_cache", True):
             with self._device:
-                self._model.setup_caches(batch_size=1, dtype=self._dtype, decoder_max_seq_len=total_len)
+                bits = cfg.get("kv_cache_bits")
+                self._model.setup_caches(batch_size=1, dtype=self._dtype, decoder_max_seq_len=total_len, **({} if bits is None else {"kv_cache_bits": bits}))
         t0 = time.perf_counter()
         generated, _ = generation.generate(
             model=self._model,

@@ -295,3 +295,59 @@ def test_recorded_and_replayed():
         graph, out = graphs[i % 2]
         graph.replay()
         assert torch.equal(out, step(plain_k, plain_v)), i
+
+
+# --------------------------------------------------------------------------------------------------------------------------------- decoders
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [256, 512])
+def test_generation_recorded_and_step_by_step(bits, dim, monkeypatch):
+    """Recorded decode steps on quantised caches give what the modules give, for left-padded prompts and on caches that are used again."""
+    from torchtune_b200 import generation
+    from torchtune_b200.generation._step_graph import StepGraph
+    from torchtune_b200.models.llama2 import llama2
+
+    torch.manual_seed(3)
+    with torch.device("cuda"):
+        model = llama2(vocab_size=304, num_layers=2, num_heads=4, num_kv_heads=2, embed_dim=dim, max_seq_len=128, intermediate_dim=512).to(torch.bfloat16).eval()
+        model.setup_caches(3, torch.bfloat16, decoder_max_seq_len=61, kv_cache_bits=bits)
+    prompt = torch.randint(1, 304, (3, 23), generator=_gen(1), device="cuda")
+    prompt[1, :7] = 0
+    recorded = []
+    real = StepGraph._record
+    monkeypatch.setattr(StepGraph, "_record", lambda self, *a: (recorded.append(1), real(self, *a))[1])
+
+    def run():
+        model.reset_caches()
+        return generation.generate(model, prompt, max_generated_tokens=30, pad_id=0, temperature=0.8, top_k=20, rng=_gen(5))
+
+    tokens, logits = run()
+    assert recorded
+    again, logits_again = run()
+    with monkeypatch.context() as m:
+        m.setattr(StepGraph, "suits", staticmethod(lambda *a: False))
+        plain, plain_logits = run()
+    assert torch.equal(tokens, again) and torch.equal(logits, logits_again)
+    assert torch.equal(tokens, plain) and torch.equal(logits, plain_logits)
+
+
+def test_a_decode_step_attends_to_what_the_cache_stands_for():
+    from torchtune_b200.models.llama2 import llama2
+
+    torch.manual_seed(4)
+    with torch.device("cuda"):
+        model = llama2(vocab_size=304, num_layers=1, num_heads=8, num_kv_heads=2, embed_dim=512, max_seq_len=256, intermediate_dim=512).to(torch.bfloat16).eval()
+        model.setup_caches(2, torch.bfloat16, decoder_max_seq_len=200, kv_cache_bits=4)
+    attn = model.layers[0].attn
+    x = torch.randn(2, 150, 512, generator=_gen(2), device="cuda").to(torch.bfloat16)
+    causal = torch.ones(150, 200, dtype=torch.bool, device="cuda").tril().expand(2, 150, 200)
+    with torch.no_grad():
+        attn(x[:, :149], x[:, :149], mask=causal[:, :149], input_pos=torch.arange(149, device="cuda").expand(2, -1))
+        got = attn(x[:, 149:], x[:, 149:], mask=causal[:, 149:], input_pos=torch.full((2, 1), 149, device="cuda"))
+        k, v = ops.quantized_read(*attn.kv_cache.rows(2))
+        q = attn.pos_embeddings(attn.q_proj(x[:, 149:]).view(2, 1, 8, 64), input_pos=torch.full((2, 1), 149, device="cuda"))
+        want = attn.output_proj(ops.attention(q, k, v, AttentionMask(causal=False, bool_mask=causal[:, 149:])).reshape(2, 1, 512))
+    assert attn.kv_cache.size == 150 and not attn.kv_cache.k_scales[:, :, 150:].any()
+    # values rounded to bf16 on the way (2^-9 of each) and 150 of them averaged; the projection adds its own rounding to both sides
+    assert (got.float() - want.float()).norm() <= 2.0**-6 * want.float().norm()

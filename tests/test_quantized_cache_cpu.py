@@ -166,3 +166,106 @@ def test_gradients_reach_the_queries():
     k, v = ops.quantized_read(k_rows, v_rows, dtype=torch.float32)
     (want,) = torch.autograd.grad(reference.attention(q, k, v, causal=True).sum(), q)
     assert torch.equal(grad, want)
+
+
+# ------------------------------------------------------------------------------------------------------------------------- decoders
+
+
+def _decoder(**kwargs):
+    from torchtune_b200.models.llama2 import llama2
+
+    torch.manual_seed(7)
+    return llama2(**{**dict(vocab_size=50, num_layers=2, num_heads=4, num_kv_heads=2, embed_dim=128, max_seq_len=64, intermediate_dim=64), **kwargs}).eval()
+
+
+class _RoundTrip(torch.nn.Module):
+    """Stands for quantised values in an ordinary cache: rounds what it is given as the format does."""
+
+    def __init__(self, cache, bits):
+        super().__init__()
+        self.cache, self.bits = cache, bits
+
+    def __getattr__(self, name):
+        return super().__getattr__(name) if name in ("cache", "bits") else getattr(self.cache, name)
+
+    def update(self, k, v):
+        return self.cache.update(*(reference.dequantize_rows(*reference.quantize_rows(t, self.bits), torch.float32) for t in (k, v)))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_decoder_sees_what_its_quantised_caches_stand_for(bits):
+    from torchtune_b200.modules import QuantizedKVCache
+
+    model, plain = _decoder(), _decoder()
+    model.setup_caches(2, torch.float32, decoder_max_seq_len=20, kv_cache_bits=bits)
+    plain.setup_caches(2, torch.float32, decoder_max_seq_len=20)
+    for layer in plain.layers:
+        layer.attn.kv_cache = _RoundTrip(layer.attn.kv_cache, bits)
+    cache = model.layers[0].attn.kv_cache
+    assert type(cache) is QuantizedKVCache and cache.bits == bits and cache.k_codes.dtype == torch.uint8 and not any("codes" in k for k in model.state_dict())
+    tokens = torch.randint(0, 50, (2, 9), generator=torch.Generator().manual_seed(1))
+    mask = torch.tril(torch.ones(9, 20, dtype=torch.bool)).expand(2, 9, 20)
+    with torch.no_grad():
+        for a, z in ((0, 6), (6, 7), (7, 9)):
+            pos = torch.arange(a, z).expand(2, -1)
+            got, want = (m(tokens[:, a:z], input_pos=pos, mask=mask[:, a:z]) for m in (model, plain))
+            # both fp32; sums of up to 128 products in another order, two layers: a thousand roundings of 2^-24
+            assert (got - want).abs().max() <= 1e-4 * want.abs().max()
+        assert cache.size == 9
+        before = got
+        model.reset_caches()
+        assert cache.size == 0 and not cache.k_codes.any()
+        for a, z in ((0, 6), (6, 9)):
+            got = model(tokens[:, a:z], input_pos=torch.arange(a, z).expand(2, -1), mask=mask[:, a:z])
+        assert (got[:, -2:] - before).abs().max() <= 1e-4 * before.abs().max()
+        one = model.layers[0].attn.kv_cache
+        with pytest.raises(AssertionError):
+            one.append(torch.zeros(2, 12, 2, 32), torch.zeros(2, 12, 2, 32))
+        with pytest.raises(ValueError):
+            one.append(torch.zeros(3, 1, 2, 32), torch.zeros(3, 1, 2, 32))
+        k, v = one.update(torch.ones(1, 1, 2, 32), torch.ones(1, 1, 2, 32))
+        assert k.shape == (1, 20, 2, 32) and k.dtype == torch.float32 and torch.equal(k[:, 9], torch.ones(1, 2, 32))
+
+
+def test_caches_in_few_bits_are_refused_where_they_do_not_apply():
+    with pytest.raises(ValueError):
+        _decoder().setup_caches(1, torch.float32, decoder_max_seq_len=8, kv_cache_bits=3)
+    with pytest.raises(ValueError):
+        _decoder(num_heads=8).setup_caches(1, torch.float32, decoder_max_seq_len=8, kv_cache_bits=4)  # 16 channels per head
+    from torchtune_b200.models.llama3_2_vision import llama3_2_vision_decoder
+
+    fused = llama3_2_vision_decoder(vocab_size=50, num_layers=2, fusion_interval=2, num_special_tokens=2, num_heads=2, num_kv_heads=2, embed_dim=64, max_seq_len=16, encoder_max_seq_len=4,
+                                    intermediate_dim=32)
+    with pytest.raises(ValueError):
+        fused.setup_caches(1, torch.float32, encoder_max_seq_len=4, decoder_max_seq_len=8, kv_cache_bits=4)
+
+
+def test_generation_on_quantised_caches():
+    from torchtune_b200 import generation
+    from torchtune_b200.modules import delete_kv_caches, local_kv_cache
+
+    model = _decoder()
+    prompt = torch.tensor([[0, 0, 5, 6, 7], [3, 4, 5, 6, 7]])
+    with local_kv_cache(model, batch_size=2, device=torch.device("cpu"), dtype=torch.float32, decoder_max_seq_len=16, kv_cache_bits=8):
+        tokens, logits = generation.generate(model, prompt, max_generated_tokens=6, pad_id=0, top_k=1)
+    assert tokens.shape == (2, 11) and logits.isfinite().all()
+    model.setup_caches(2, torch.float32, decoder_max_seq_len=16)
+    plain, _ = generation.generate(model, prompt, max_generated_tokens=1, pad_id=0, top_k=1)
+    assert torch.equal(tokens[:, 5], plain[:, 5])  # logits of random weights lie further apart than 8 bits move them
+    delete_kv_caches(model)
+
+
+def test_generate_recipe_with_a_quantised_cache(tmp_path, tune_path, monkeypatch, caplog):
+    from helpers import run_tune, write_tiny_hf_checkpoint
+    from tokenizer_assets import write_sentencepiece_model
+    from torchtune_b200.models.llama2 import llama2
+
+    arch = dict(vocab_size=200, num_layers=1, num_heads=2, num_kv_heads=1, embed_dim=64, max_seq_len=128, intermediate_dim=64, norm_eps=1e-5)
+    write_tiny_hf_checkpoint(tmp_path / "ckpt", arch=arch, builder=llama2)
+    (tmp_path / "tok").mkdir()
+    sp = write_sentencepiece_model(tmp_path / "tok", vocab_size=200)
+    model = " ".join(f"model.{k}={v}" for k, v in arch.items())
+    run_tune(tune_path, f"run generate --config generation model._component_=torchtune_b200.models.llama2.llama2 {model} checkpointer.checkpoint_dir={tmp_path / 'ckpt'} "
+             f"checkpointer.checkpoint_files=[model-00001-of-00001.safetensors] device=cpu dtype=fp32 output_dir={tmp_path / 'out'} tokenizer.path={sp} max_new_tokens=6 prompt.user=hello "
+             "kv_cache_bits=4", monkeypatch)
+    assert "tokens/sec" in caplog.text

@@ -189,6 +189,10 @@ class SingleTurnGenerator:
             cache_kwargs = dict(batch_size=1, dtype=self._dtype, decoder_max_seq_len=total)
             if multimodal and isinstance(self.model, DeepFusionModel):
                 cache_kwargs["encoder_max_seq_len"] = self.model_transform.image_seq_len
+            if cfg.get("kv_cache_bits") is not None:
+                if self._tp is not None or isinstance(self.model, (DeepFusionModel, EarlyFusionModel)):
+                    raise ValueError("kv_cache_bits is for decoders on one GPU")
+                cache_kwargs["kv_cache_bits"] = cfg.kv_cache_bits
             self.model.setup_caches(**cache_kwargs)
         if multimodal:
             prompt, prefill_extras, step_extras = self._multimodal_extras(inputs, seq_len)

@@ -42,6 +42,8 @@ class NativeLayers:
             return None
         first, dim, eps = model.layers[0], emb.shape[1], model.norm.eps
         hq, hkv, D, scale, cache = first.attn.num_heads, first.attn.num_kv_heads, first.attn.head_dim, first.attn.scale, first.attn.kv_cache
+        if type(cache) is not KVCache:  # one in few bits is attended to by its modules
+            return None
         hidden = getattr(getattr(first.mlp, "w1", None), "out_features", 0)
         interleaved = getattr(first.attn.pos_embeddings, "interleaved", True)
         words: List[int] = []

@@ -11,14 +11,14 @@ from torch import nn
 from torch.utils._device import DeviceContext
 
 from .. import ops
-from ..modules import FeedForward, KVCache, MultiHeadAttention, RMSNorm, TransformerDecoder, TransformerSelfAttentionLayer
+from ..modules import FeedForward, KVCache, MultiHeadAttention, QuantizedKVCache, RMSNorm, TransformerDecoder, TransformerSelfAttentionLayer
 from ..modules.linear import Linear, has_hooks
 from ..modules.position_embeddings import RotaryPositionalEmbeddings
 from ..modules.tied_linear import TiedLinear
 from ._native_layers import NativeLayers
 
 # Modules whose forward pass of one token is the same sequence of launches in every step and needs no look at the device.
-_PLAIN = (TransformerDecoder, TransformerSelfAttentionLayer, MultiHeadAttention, FeedForward, KVCache, RMSNorm, Linear, nn.Linear, nn.Embedding, nn.ModuleList, nn.Identity,
+_PLAIN = (TransformerDecoder, TransformerSelfAttentionLayer, MultiHeadAttention, FeedForward, KVCache, QuantizedKVCache, RMSNorm, Linear, nn.Linear, nn.Embedding, nn.ModuleList, nn.Identity,
           nn.SiLU, nn.GELU, nn.ReLU)
 
 
@@ -72,7 +72,7 @@ class StepGraph:
             if type(layer) is not TransformerSelfAttentionLayer or layer.mask_mod is not None or type(layer.attn) is not MultiHeadAttention:
                 return False
             attn = layer.attn
-            if type(attn.kv_cache) is not KVCache or not attn.cache_enabled or attn.kv_cache.cache_pos.is_inference() or getattr(attn, "context_parallel", None) is not None:
+            if type(attn.kv_cache) not in (KVCache, QuantizedKVCache) or not attn.cache_enabled or attn.kv_cache.cache_pos.is_inference() or getattr(attn, "context_parallel", None) is not None:
                 return False
             if attn.training and attn.attn_dropout:
                 return False

@@ -12,7 +12,7 @@ from .embedding_utils import resize_token_embeddings
 from .cached_mixer import CachedMixer
 from .feed_forward import ClampedGLU, FeedForward
 from .hyper_connections import HyperConnection, LayerScale
-from .kv_cache import KVCache, PassCaches, RowCache, SpanKVCache, StateCache
+from .kv_cache import KVCache, PassCaches, QuantizedKVCache, RowCache, SpanKVCache, StateCache
 from .latent_attention import LatentAttention, LatentCache
 from .layer_norm import Fp32LayerNorm
 from .linear import Linear
@@ -58,6 +58,7 @@ __all__ = [
     "HyperConnection",
     "HyperConnectionLayer",
     "KVCache",
+    "QuantizedKVCache",
     "LatentAttention",
     "LatentCache",
     "LayerScale",

@@ -9,7 +9,7 @@ from torch import nn
 
 from .. import ops
 from ..ops.mask import AttentionMask
-from .kv_cache import KVCache
+from .kv_cache import KVCache, QuantizedKVCache
 from .linear import Linear, has_hooks, is_plain_linear
 from .position_embeddings import RotaryPositionalEmbeddings
 
@@ -88,14 +88,18 @@ class MultiHeadAttention(nn.Module):
         self.qk_norm_before_rope = qk_norm_before_rope
         self.cache_enabled = False
 
-    def setup_cache(self, batch_size: int, dtype: torch.dtype, max_seq_len: int) -> None:
+    def setup_cache(self, batch_size: int, dtype: torch.dtype, max_seq_len: int, bits: Optional[int] = None) -> None:
+        """``bits``: 4 or 8 for a :class:`QuantizedKVCache` instead of one of ``dtype``."""
         if self.kv_cache is not None:
             logger.warning("Key value caches are already setup. You cannot call ``setup_caches()`` twice. Skipping.")
             return
-        self.kv_cache = KVCache(batch_size, max_seq_len, self.num_kv_heads, self.head_dim, dtype)
+        if bits is None:
+            self.kv_cache = KVCache(batch_size, max_seq_len, self.num_kv_heads, self.head_dim, dtype)
+        else:
+            self.kv_cache = QuantizedKVCache(batch_size, max_seq_len, self.num_kv_heads, self.head_dim, bits)
         # a cache created outside a device context lands on the CPU; it belongs where this module's weights are
         home = next((t.device for t in list(self.parameters()) + list(self.buffers()) if t.device.type != "meta"), None)
-        if home is not None and home.type != "cpu" and self.kv_cache.k_cache.device.type == "cpu":
+        if home is not None and home.type != "cpu" and self.kv_cache.cache_pos.device.type == "cpu":
             self.kv_cache.to(home)
         self.cache_enabled = True
 
@@ -140,6 +144,7 @@ class MultiHeadAttention(nn.Module):
             q = self.q_proj(x)
         q = q.view(b, s_x, self.num_heads, self.head_dim)
         rotated = None
+        quantized = self.cache_enabled and isinstance(self.kv_cache, QuantizedKVCache)
         if k is not None:
             k, v = (t.view(b, s_x, self.num_kv_heads, self.head_dim) for t in (k, v))
             rotated = self._rotate_into_cache(q, k, v, input_pos)
@@ -155,7 +160,8 @@ class MultiHeadAttention(nn.Module):
             if y is None:
                 if self.kv_cache is None or not self.cache_enabled:
                     raise ValueError("Must provide y input or use kv_cache to enable streaming decoding")
-                k, v = self.kv_cache.k_cache[:b], self.kv_cache.v_cache[:b]
+                if not quantized:
+                    k, v = self.kv_cache.k_cache[:b], self.kv_cache.v_cache[:b]
             else:
                 s_y = y.shape[1]
                 if k is None:
@@ -167,7 +173,9 @@ class MultiHeadAttention(nn.Module):
                     k = self.pos_embeddings(k, input_pos=input_pos)
                 if self.k_norm is not None and not self.qk_norm_before_rope:
                     k = self.k_norm(k)
-                if self.kv_cache is not None and self.cache_enabled:
+                if quantized:
+                    self.kv_cache.append(k, v)
+                elif self.kv_cache is not None and self.cache_enabled:
                     k, v = self.kv_cache.update(k, v)
 
         plain = self.kv_cache is None or not self.cache_enabled
@@ -175,15 +183,8 @@ class MultiHeadAttention(nn.Module):
         cp = getattr(self, "context_parallel", None)
         if cp is not None and plain:  # sequence-sharded activations: whole sequences for a subset of heads inside attention
             q, k, v = cp.seq_to_heads(q), cp.seq_to_heads(k), cp.seq_to_heads(v)
-        out = ops.attention(
-            q,
-            k,
-            v,
-            attn_mask,
-            scale=self.scale,
-            softcap=self.softcap,
-            dropout_p=self.attn_dropout if self.training else 0.0,
-        )
+        how = dict(scale=self.scale, softcap=self.softcap, dropout_p=self.attn_dropout if self.training else 0.0)
+        out = self.kv_cache.attend(q, attn_mask, **how) if quantized else ops.attention(q, k, v, attn_mask, **how)
         if cp is not None and plain:
             out = cp.heads_to_seq(out)
         out = out.reshape(b, s_x, self.num_heads * self.head_dim)

@@ -94,12 +94,14 @@ def local_kv_cache(
     dtype: torch.dtype,
     encoder_max_seq_len: Optional[int] = None,
     decoder_max_seq_len: Optional[int] = None,
+    kv_cache_bits: Optional[int] = None,
 ) -> Generator[None, None, None]:
-    """Create KV caches for the duration of the block and delete them afterwards."""
+    """Create KV caches (with ``kv_cache_bits`` in 4 or 8 bits) for the duration of the block and delete them afterwards."""
     if model.caches_are_setup():
         raise ValueError("Model caches must be not setup prior to entering this context manager! Please use delete_kv_caches(model) to delete existing caches.")
     with device:
-        model.setup_caches(batch_size, dtype, encoder_max_seq_len=encoder_max_seq_len, decoder_max_seq_len=decoder_max_seq_len)
+        model.setup_caches(batch_size, dtype, encoder_max_seq_len=encoder_max_seq_len, decoder_max_seq_len=decoder_max_seq_len,
+                           **({} if kv_cache_bits is None else {"kv_cache_bits": kv_cache_bits}))
     try:
         yield
     finally:

@@ -12,7 +12,7 @@ from ..ops.mask import AttentionMask
 from .attention import MaskLike, MultiHeadAttention
 from .cached_mixer import CachedMixer
 from .hyper_connections import HyperConnection, LayerScale, StreamEntry
-from .kv_cache import KVCache, counted_appends
+from .kv_cache import KVCache, QuantizedKVCache, counted_appends
 from .linear import Linear, is_plain_linear
 from .rms_norm import StreamLayerNorm, StreamRMSNorm
 
@@ -43,8 +43,11 @@ class TransformerSelfAttentionLayer(nn.Module):
         self.mlp_scale = mlp_scale or nn.Identity()
         self.mask_mod = mask_mod
 
-    def setup_caches(self, batch_size: int, dtype: torch.dtype, *, encoder_max_seq_len: int, decoder_max_seq_len: int) -> None:
-        self.attn.setup_cache(batch_size, dtype, max_seq_len=decoder_max_seq_len)
+    def setup_caches(self, batch_size: int, dtype: torch.dtype, *, encoder_max_seq_len: int, decoder_max_seq_len: int, kv_cache_bits: Optional[int] = None) -> None:
+        if kv_cache_bits is None:
+            self.attn.setup_cache(batch_size, dtype, max_seq_len=decoder_max_seq_len)
+        else:
+            self.attn.setup_cache(batch_size, dtype, max_seq_len=decoder_max_seq_len, bits=kv_cache_bits)
 
     def caches_are_setup(self) -> bool:
         return self.attn.kv_cache is not None
@@ -318,7 +321,16 @@ class TransformerDecoder(nn.Module):
         *,
         encoder_max_seq_len: Optional[int] = None,
         decoder_max_seq_len: Optional[int] = None,
+        kv_cache_bits: Optional[int] = None,
     ) -> None:
+        """``kv_cache_bits``: 4 or 8 for caches that are quantised as they are written (:class:`QuantizedKVCache`), in decoders of plain self-attention layers."""
+        if kv_cache_bits is not None:
+            for layer in self.layers:
+                attn = getattr(layer, "attn", None)
+                if not isinstance(attn, MultiHeadAttention) or type(attn).setup_cache is not MultiHeadAttention.setup_cache or isinstance(layer, TransformerCrossAttentionLayer):
+                    raise ValueError("caches in few bits are for decoders whose layers are plain self-attention (kv_cache_bits)")
+                if kv_cache_bits not in (4, 8) or attn.head_dim % 32:
+                    raise ValueError(f"kv_cache_bits is 4 or 8, not {kv_cache_bits}, and head dimensions are multiples of 32, not {attn.head_dim}")
         kinds = [getattr(m, "inner_cls", type(m)) for m in self.modules()]  # sees through checkpoint wrappers
         has_enc = any(issubclass(k, TransformerCrossAttentionLayer) for k in kinds)
         has_dec = any(issubclass(k, TransformerSelfAttentionLayer) for k in kinds)
@@ -332,6 +344,7 @@ class TransformerDecoder(nn.Module):
                 dtype,
                 encoder_max_seq_len=self.encoder_max_cache_seq_len,
                 decoder_max_seq_len=self.decoder_max_cache_seq_len,
+                **({} if kv_cache_bits is None else {"kv_cache_bits": kv_cache_bits}),
             )
 
     def caches_are_setup(self) -> bool:
@@ -348,7 +361,7 @@ class TransformerDecoder(nn.Module):
         for layer in self.layers:
             attn = getattr(layer, "attn", None)
             cache = getattr(attn, "kv_cache", None)
-            if type(cache) is KVCache and getattr(attn, "cache_enabled", False):
+            if type(cache) in (KVCache, QuantizedKVCache) and getattr(attn, "cache_enabled", False):
                 if cache.counted and not caches:
                     return []
                 caches.append(cache)

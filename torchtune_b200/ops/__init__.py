@@ -474,7 +474,7 @@ def quantized_read(k_rows: QuantizedRows, v_rows: QuantizedRows, start: int = 0,
         raise ValueError(f"a cache is read as floating-point numbers, not {dtype}")
     if cuda_ops_enabled(k_rows.codes) and quantized.plain(k_rows, v_rows):
         k, v = quantized.read(k_rows, v_rows, start, stop, torch.bfloat16 if dtype == torch.bfloat16 else torch.float32, size)
-        return k.to(dtype), v.to(dtype)
+        return (k, v) if k.dtype == dtype else (k.to(dtype), v.to(dtype))
     k, v = (reference.dequantize_rows(r.codes[:, :, start:stop], r.scales[:, :, start:stop], dtype).transpose(1, 2).contiguous() for r in (k_rows, v_rows))
     return k, v
 

@@ -64,10 +64,13 @@ def sizes(k_rows: QuantizedRows, v_rows: QuantizedRows) -> Tuple[int, int, int, 
     """``(batch, heads, slots, head_dim, bits)`` of the keys and values of a cache; an error if they are not a pair of rows."""
     kc, ks, n = k_rows
     vc, vs, vn = v_rows
-    a, g = kc.shape, ks.shape
-    if (len(a) == 4 and a == vc.shape and g == vs.shape and n == vn and len(g) == 4 and a[:3] == g[:3] and kc.dtype is torch.uint8 and vc.dtype is torch.uint8 and ks.dtype is torch.bfloat16
-            and vs.dtype is torch.bfloat16 and n <= a[2] and g[3] > 0 and (a[3] == g[3] * 16 or a[3] == g[3] * 32) and kc.device == vc.device == ks.device == vs.device):
-        return a[0], a[1], a[2] if n < 0 else n, g[3] * 32, a[3] // (g[3] * 4)
+    a, g, device = kc.shape, ks.shape, kc.device
+    if len(a) == 4 and len(g) == 4 and a == vc.shape and g == vs.shape and n == vn and kc.dtype is vc.dtype is torch.uint8 and ks.dtype is vs.dtype is torch.bfloat16:
+        b, h, held, row = a
+        groups = g[3]
+        if (g[0] == b and g[1] == h and g[2] == held and n <= held and groups > 0 and (row == groups * 16 or row == groups * 32)
+                and device == vc.device and device == ks.device and device == vs.device):
+            return b, h, held if n < 0 else n, groups * 32, row // (groups * 4)
     for name, (codes, scales, count) in (("k_rows", k_rows), ("v_rows", v_rows)):
         if codes.dim() != 4 or scales.dim() != 4 or codes.shape[:3] != scales.shape[:3] or count > codes.shape[2]:
             raise ValueError(f"{name}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not [batch, heads, slots, ...] of the same rows")
@@ -83,11 +86,11 @@ def plain(*rows: QuantizedRows) -> bool:
     return all(type(r.codes) is torch.Tensor and type(r.scales) is torch.Tensor for r in rows)
 
 
-def _on(device: torch.device, call, *args) -> int:
+def _on(t: torch.Tensor, call, *args) -> int:
     """Calls a kernel with the device of its operands as the current one (kernels launch on the current device's stream)."""
-    if device.index == torch.cuda.current_device():
+    if t.get_device() == torch._C._cuda_getDevice():
         return call(*args, stream_ptr())
-    with torch.cuda.device(device):
+    with torch.cuda.device(t.device):
         return call(*args, stream_ptr())
 
 
@@ -106,7 +109,7 @@ def append(k: torch.Tensor, v: torch.Tensor, k_rows: QuantizedRows, v_rows: Quan
     if v.stride(3) != 1:
         v = v.contiguous()
     strides = (ctypes.c_longlong * 18)(*k.stride()[:3], *v.stride()[:3], *_steps(k_rows), *_steps(v_rows))
-    check(_on(k.device, lib().ttb_quantized_append, k.data_ptr(), v.data_ptr(), k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides,
+    check(_on(k, lib().ttb_quantized_append, k.data_ptr(), v.data_ptr(), k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides,
               slots.data_ptr(), _TYPES[k.dtype], b, s, h, d, bits, k_rows.slots), "quantised append")
 
 
@@ -114,11 +117,11 @@ def read(k_rows: QuantizedRows, v_rows: QuantizedRows, start: int, stop: int, dt
     b, h, _, d, bits = size
     n = stop - start
     codes = k_rows.codes
-    k = torch.empty(b, n, h, d, dtype=dtype, device=codes.device)
+    k = codes.new_empty((b, n, h, d), dtype=dtype)
     v = torch.empty_like(k)
     if b and n and h:
         strides = (ctypes.c_longlong * 12)(*_steps(k_rows), *_steps(v_rows))
-        check(_on(codes.device, lib().ttb_quantized_read, codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides, k.data_ptr(), v.data_ptr(), b, start,
+        check(_on(codes, lib().ttb_quantized_read, codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides, k.data_ptr(), v.data_ptr(), b, start,
                   n, h, d, bits, int(dtype == torch.float32)), "quantised read")
     return k, v
 
@@ -168,7 +171,7 @@ def attention(q: torch.Tensor, k_rows: QuantizedRows, v_rows: QuantizedRows, mas
     if n >= 2048 and b * hkv * 8 < 592:  # few and long rows are split further than a cluster reaches
         floats = 128 * b * s * hq * (d + 4)
         work = torch.empty(floats, dtype=torch.float32, device=q.device)
-    check(_on(q.device, lib().ttb_quantized_attention, q.data_ptr(), k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(),
+    check(_on(q, lib().ttb_quantized_attention, q.data_ptr(), k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(),
               (ctypes.c_longlong * 8)(*steps), o.data_ptr(), seen, seen_b, seen_r, None if start is None else start.data_ptr(), offset, window, sinks, b, s, n, hq, hkv, d, bits,
               1.0 / math.sqrt(d) if scale is None else float(scale), None if work is None else work.data_ptr(), floats), "attention over a quantised cache")
     return o
