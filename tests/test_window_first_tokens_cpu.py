@@ -1,0 +1,111 @@
+"""Masks of a sliding window beside which the first tokens stay visible: their dense form, the plain statement's gradients, models that use them."""
+import pytest
+import torch
+
+from torchtune_b200 import ops
+from torchtune_b200.ops import reference
+from torchtune_b200.ops.mask import AttentionMask
+
+
+def _visible(sq, sk, window, sinks, docs=None):
+    """By the words of the definition, pair by pair."""
+    b = 1 if docs is None else docs.shape[0]
+    m = torch.zeros(b, sq, sk, dtype=torch.bool)
+    for r in range(b):
+        for i in range(sq):
+            at = i + sk - sq
+            for j in range(at + 1):
+                first = 0
+                if docs is not None:
+                    if docs[r, at] != docs[r, j]:
+                        continue
+                    first = int((docs[r] == docs[r, at]).nonzero()[0])
+                m[r, i, j] = at - j < window or j - first < sinks
+    return m
+
+
+DOCS = torch.tensor([[0] * 5 + [1] * 1 + [2] * 9, [4] * 15], dtype=torch.int32)
+
+
+@pytest.mark.parametrize("window, sinks", [(1, 0), (1, 1), (3, 2), (4, 20), (20, 3)])
+def test_dense_masks(window, sinks):
+    mask = AttentionMask(window=window, sinks=sinks)
+    assert torch.equal(mask.dense(1, 15, 15, "cpu"), _visible(15, 15, window, sinks))
+    packed = AttentionMask(window=window, sinks=sinks, doc_ids=DOCS)
+    assert torch.equal(packed.dense(2, 15, 15, "cpu"), _visible(15, 15, window, sinks, DOCS))
+    assert torch.equal(packed.to("cpu").dense(2, 15, 15, "cpu"), packed.dense(2, 15, 15, "cpu"))
+    assert torch.equal(AttentionMask(window=window).dense(1, 9, 9, "cpu"), _visible(9, 9, window, 0))
+
+
+@pytest.mark.parametrize("sq", [1, 4, 11])
+@pytest.mark.parametrize("docs", [False, True])
+def test_plain_attention_and_its_gradients(sq, docs):
+    if docs and sq < 11:
+        return  # documents go with whole sequences
+    g = torch.Generator().manual_seed(sq)
+    ids = torch.tensor([[0] * 4 + [1] * 7], dtype=torch.int32) if docs else None
+    q, k, v, d_o, u = (torch.randn(1, n, h, 8, generator=g, dtype=torch.float64) for n, h in ((sq, 4), (11, 2), (11, 2), (sq, 4), (sq, 4)))
+    mask = AttentionMask(window=3, sinks=2, doc_ids=ids)
+    seen = _visible(sq, 11, 3, 2, ids)
+
+    def formula(q, k, v):
+        score = torch.einsum("bqgnd,bkgd->bgnqk", q.view(1, sq, 2, 2, 8), k) * 8**-0.5
+        return torch.einsum("bgnqk,bkgd->bqgnd", torch.softmax(score.masked_fill(~seen[:, None, None], float("-inf")), -1), v).reshape(1, sq, 4, 8)
+
+    leaves = [t.float().requires_grad_() for t in (q, k, v)]
+    out = ops.attention(*leaves, mask)
+    wide = [t.requires_grad_() for t in (q, k, v)]
+    want = formula(*wide)
+    assert (out.double() - want).abs().max() <= 1e-5  # fp32 sums of at most 11 terms of size 10
+    grads, wants = torch.autograd.grad(out, leaves, d_o.float()), torch.autograd.grad(want, wide, d_o)
+    for a, w in zip(grads, wants):
+        assert (a.double() - w).abs().max() <= 1e-4
+    step = 1e-5
+    with torch.no_grad():
+        slope = ((formula(q + step * u, k, v) - formula(q - step * u, k, v)) * d_o).sum() / (2 * step)
+    assert abs(float((grads[0].double() * u).sum() - slope)) <= 1e-4
+
+
+def test_a_decoder_with_windows_and_first_tokens():
+    """Whole sequences by the structured mask and cached steps by boolean ones see the same tokens."""
+    from torchtune_b200.models.mistral import mistral
+
+    arch = dict(vocab_size=60, num_layers=2, num_heads=4, num_kv_heads=2, embed_dim=64, intermediate_dim=64, max_seq_len=64)
+    torch.manual_seed(5)
+    model = mistral(**arch, sliding_window_size=6, attention_sinks=2).eval()
+    torch.manual_seed(5)
+    full = mistral(**arch).eval()
+    tokens = torch.randint(0, 60, (2, 20), generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():
+        want = model(tokens)
+        assert not torch.allclose(want, full(tokens))
+        dense = _visible(20, 20, 6, 2).expand(2, 20, 20)
+        assert (full(tokens, mask=dense) - want).abs().max() <= 1e-4
+        docs = torch.tensor([[0] * 8 + [1] * 12, [0] * 20], dtype=torch.int32)
+        packed = model(tokens, mask=AttentionMask(doc_ids=docs))
+        assert (full(tokens, mask=_visible(20, 20, 6, 2, docs)) - packed).abs().max() <= 1e-4
+        model.setup_caches(2, torch.float32, decoder_max_seq_len=24)
+        causal = torch.ones(24, 24, dtype=torch.bool).tril().expand(2, 24, 24)
+        got = [model(tokens[:, a:z], input_pos=torch.arange(a, z).expand(2, -1), mask=causal[:, a:z]) for a, z in ((0, 11), (11, 12), (12, 20))]
+        assert (torch.cat(got, 1) - want).abs().max() <= 1e-4
+    with pytest.raises(ValueError):
+        mistral(**arch, attention_sinks=2)
+
+
+def test_windows_over_a_quantised_cache_and_left_padded_rows():
+    from torchtune_b200 import generation
+    from torchtune_b200.models.mistral import mistral
+
+    torch.manual_seed(6)
+    model = mistral(vocab_size=60, num_layers=2, num_heads=4, num_kv_heads=2, embed_dim=128, intermediate_dim=64, max_seq_len=64, sliding_window_size=5, attention_sinks=2).eval()
+    prompt = torch.randint(1, 60, (1, 9), generator=torch.Generator().manual_seed(2))
+    padded = torch.cat([torch.zeros(1, 4, dtype=torch.long), prompt], 1)
+    both = torch.cat([padded, torch.randint(1, 60, (1, 13), generator=torch.Generator().manual_seed(3))])
+    results = []
+    for p, n in ((prompt, 1), (both, 2)):
+        model.setup_caches(n, torch.float32, decoder_max_seq_len=24, kv_cache_bits=8)
+        results.append(generation.generate(model, p, max_generated_tokens=8, pad_id=0, top_k=1)[1][0])
+        for layer in model.layers:
+            layer.attn.kv_cache, layer.attn.cache_enabled = None, False
+    # padding changes neither positions nor what is seen: the same sums in another order
+    assert (results[0] - results[1]).abs().max() <= 1e-3 * results[0].abs().max()

@@ -91,6 +91,7 @@ class DecoderArch:
     logit_softcap: float = 0.0  # cap·tanh(logits/cap) on the output logits (Gemma-2)
     attn_scale: Optional[float] = None
     sliding_window: Optional[Callable[[int], int]] = None  # layer index -> window (0 = global)
+    attention_sinks: Optional[int] = None  # first tokens that a window leaves visible; a number (0 too) counts windows of dense masks from each query's own key
     # per-layer overrides (Llama-4): feed-forward module, whether the layer rotates/normalises q and k,
     # and an extra mask hook
     mlp_factory: Optional[Callable[[int, "AdapterSpec"], nn.Module]] = None
@@ -162,6 +163,27 @@ def _window_mask_mod(window: int):
     return mod
 
 
+def _window_first_mask_mod(window: int, sinks: int):
+    """Per-layer mask hook adding a sliding window, beside which the first tokens stay visible, to whatever mask the batch carries.  Rows of a dense mask are taken to be causal, so
+    their first and last visible keys are the first token of the query's document (or of its left-padded row) and the query's own, wherever in a cache they lie."""
+    from dataclasses import replace
+
+    from ..ops.mask import AttentionMask
+
+    def mod(mask, bsz, seq_len):
+        if mask is None:
+            return AttentionMask(causal=True, window=window, sinks=sinks)
+        if isinstance(mask, AttentionMask) and mask.bool_mask is None:
+            return replace(mask, window=window, sinks=sinks)
+        dense = mask.bool_mask if isinstance(mask, AttentionMask) else mask
+        k = torch.arange(dense.shape[-1], device=dense.device)
+        own = torch.where(dense, k, -1).amax(-1, keepdim=True)
+        first = torch.where(dense, k, dense.shape[-1]).amin(-1, keepdim=True)
+        return dense & ((own - k < window) | (k - first < sinks))
+
+    return mod
+
+
 def build_mlp(dim: int, hidden: int, ad: AdapterSpec, activation: Optional[nn.Module] = None, bias: bool = False) -> FeedForward:
     return FeedForward(
         gate_proj=ad.make(dim, hidden, ad.apply_to_mlp, bias),
@@ -179,7 +201,9 @@ def build_decoder(arch: DecoderArch, adapter: Optional[AdapterSpec] = None) -> T
     for idx in range(arch.num_layers):
         window = arch.sliding_window(idx) if arch.sliding_window else 0
         positional = arch.layer_uses_rope(idx) if arch.layer_uses_rope else True
-        mask_mod = _window_mask_mod(window) if window else None
+        mask_mod = None
+        if window:
+            mask_mod = _window_mask_mod(window) if arch.attention_sinks is None else _window_first_mask_mod(window, arch.attention_sinks)
         if arch.layer_mask_mod is not None and mask_mod is None:
             mask_mod = arch.layer_mask_mod(idx)
         mlp = arch.mlp_factory(idx, ad) if arch.mlp_factory else build_mlp(arch.embed_dim, arch.resolved_hidden(), ad, arch.activation(), arch.mlp_bias)

@@ -7,11 +7,15 @@ from .._family import lora_preset, preset, qlora_preset
 from .._generic import classifier_builders, component_builders, layer_builders
 
 
-def _arch(vocab_size: int, num_layers: int, num_heads: int, num_kv_heads: int, embed_dim: int, intermediate_dim: int, max_seq_len: int, attn_dropout: float = 0.0, norm_eps: float = 1e-5, rope_base: int = 10_000) -> DecoderArch:
-    return DecoderArch(vocab_size=vocab_size, num_layers=num_layers, num_heads=num_heads, num_kv_heads=num_kv_heads, embed_dim=embed_dim, max_seq_len=max_seq_len, intermediate_dim=intermediate_dim, attn_dropout=attn_dropout, norm_eps=norm_eps, rope=lambda hd, msl: RotaryPositionalEmbeddings(dim=hd, max_seq_len=msl, base=rope_base))
+def _arch(vocab_size: int, num_layers: int, num_heads: int, num_kv_heads: int, embed_dim: int, intermediate_dim: int, max_seq_len: int, attn_dropout: float = 0.0, norm_eps: float = 1e-5, rope_base: int = 10_000, sliding_window_size: Optional[int] = None, attention_sinks: int = 0) -> DecoderArch:
+    if attention_sinks and not sliding_window_size:
+        raise ValueError("attention_sinks are the first tokens that a window leaves visible: they need a sliding_window_size")
+    return DecoderArch(vocab_size=vocab_size, num_layers=num_layers, num_heads=num_heads, num_kv_heads=num_kv_heads, embed_dim=embed_dim, max_seq_len=max_seq_len, intermediate_dim=intermediate_dim, attn_dropout=attn_dropout, norm_eps=norm_eps, rope=lambda hd, msl: RotaryPositionalEmbeddings(dim=hd, max_seq_len=msl, base=rope_base),
+                       sliding_window=(lambda idx: sliding_window_size) if sliding_window_size else None, attention_sinks=attention_sinks)
 
 
-mistral, lora_mistral = component_builders("mistral", _arch, "Mistral decoder: GQA, SwiGLU, RMSNorm, interleaved RoPE (the sliding window of the original is not applied).")
+mistral, lora_mistral = component_builders("mistral", _arch, "Mistral decoder: GQA, SwiGLU, RMSNorm, interleaved RoPE.  The sliding window of the original is applied only where ``sliding_window_size`` "
+                                             "asks for it; ``attention_sinks`` first tokens then stay visible.")
 mistral_mlp, lora_mistral_self_attention, lora_mistral_mlp = layer_builders(_arch)
 mistral_classifier, lora_mistral_classifier = classifier_builders("mistral", _arch, "Mistral decoder.")
 

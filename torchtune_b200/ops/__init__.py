@@ -410,7 +410,7 @@ def attention(
         elif q.shape[-1] not in (64, 128):
             why = f"head_dim {q.shape[-1]}"
         else:
-            why = _cuda_attention.unsupported_reason(q, k, mask)
+            why = _cuda_attention.unsupported_reason(q, k, mask, softcap)
         if why is None:
             return _cuda_attention.attention(q, k, v, mask, scale, softcap)
         _fallback("attention", why, q)

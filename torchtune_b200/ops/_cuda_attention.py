@@ -157,20 +157,78 @@ class _FlashAttention(torch.autograd.Function):
         return dq_acc.to(q.dtype), dk, dv, None, None, None, None, None, None, None, None
 
 
-def unsupported_reason(q: torch.Tensor, k: torch.Tensor, mask: AttentionMask) -> Optional[str]:
+class _WindowAttention(torch.autograd.Function):
+    """A causal window (query i at position ``sk - s + i``) beside which the first ``sinks`` positions stay visible; documents keep their own first positions."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, doc_ids, window, sinks, scale):
+        b, s, hq, d = q.shape
+        sk, hkv = k.shape[1], k.shape[2]
+        q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q.contiguous(), k.contiguous(), v.contiguous()))
+        o = torch.empty_like(q)
+        grads = any(ctx.needs_input_grad)
+        with torch.cuda.device(q.device):
+            if not grads and doc_ids is None and decodes(s, sk, hq, hkv):
+                check(lib().ttb_attn_decode_first(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), window, sinks, b, s, sk, hq, hkv, d, float(scale), stream_ptr()),
+                      "attention of few queries (window)")
+                return o
+            start = last = None
+            if doc_ids is not None:
+                ids = doc_ids.to(device=q.device, dtype=torch.int32).contiguous()
+                start = torch.empty(b, s, dtype=torch.int32, device=q.device)
+                last = torch.empty_like(start)
+                check(lib().ttb_document_bounds(ids.data_ptr(), b, s, window, sinks, start.data_ptr(), last.data_ptr(), stream_ptr()), "document bounds")
+            lse = torch.empty(b, hq, s, dtype=torch.float32, device=q.device)
+            # the kernel takes the largest score before it is scaled: another sign of the scale (or 0) goes into the queries, which is exact
+            queries, positive = (q, scale) if scale > 0 else (-q, -scale) if scale < 0 else (q * 0.0, 1.0)
+            check(lib().ttb_attn_fwd2_first(queries.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), _p(start), window, sinks, b, s, sk, hq, hkv, d, float(positive),
+                                            err_word(q.device).data_ptr(), stream_ptr()), "attention forward (window)")
+        if grads:
+            ctx.save_for_backward(q, k, v, o, lse, last)
+            ctx.meta = (window, sinks, scale)
+        return o
+
+    @staticmethod
+    def backward(ctx, d_o):
+        q, k, v, o, lse, last = ctx.saved_tensors
+        window, sinks, scale = ctx.meta
+        b, s, hq, d = q.shape
+        sk, hkv = k.shape[1], k.shape[2]
+        d_o = d_o.contiguous()
+        q, k, v, o, d_o = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q, k, v, o, d_o))  # handed back by a saved-tensor hook, or a view
+        with torch.cuda.device(q.device):
+            delta = torch.empty(b, hq, s, dtype=torch.float32, device=q.device)
+            dq = torch.zeros(b, s, hq, d, dtype=torch.float32, device=q.device)
+            dk, dv = torch.empty_like(k), torch.empty_like(v)
+            floats = lib().ttb_attn_bwd_first_workspace(window, sinks, int(last is not None), b, s, sk, hkv, d)
+            work = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+            check(lib().ttb_attn_bwd_first(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), d_o.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                           _p(last), window, sinks, _p(work), floats, b, s, sk, hq, hkv, d, float(scale), err_word(q.device).data_ptr(), stream_ptr()), "attention backward (window)")
+        return dq.to(q.dtype), dk, dv, None, None, None, None
+
+
+def _first_positions(s: int, sk: int, mask: AttentionMask) -> bool:
+    """Whether a mask is a causal window that the kernels with first positions take: with such positions, or with other numbers of queries than of keys."""
+    return (mask.bool_mask is None and mask.key_start is None and mask.causal and mask.window > 0 and mask.chunk <= 0 and (mask.sinks > 0 or s != sk) and s <= sk
+            and (mask.doc_ids is None or s == sk))
+
+
+def unsupported_reason(q: torch.Tensor, k: torch.Tensor, mask: AttentionMask, softcap: float = 0.0) -> Optional[str]:
     """Why a bf16 CUDA call cannot run on the kernels (``None`` = it can)."""
     s, sk = q.shape[1], k.shape[1]
     structured = mask.doc_ids is not None or mask.chunk > 0 or mask.window > 0
     if q.shape[2] % k.shape[2]:
         return "query heads not a multiple of key heads"
+    if softcap <= 0.0 and _first_positions(s, sk, mask):
+        return None
+    if mask.bool_mask is None and mask.window > 0 and mask.sinks > 0 and mask.causal:
+        return "first tokens beside a window together with chunks, soft-capped scores or fewer keys than queries"
     if mask.bool_mask is None and structured and not mask.causal:
         return "structured mask without causality"
     if mask.bool_mask is None and structured and s != sk:
         return "structured mask with different query and key lengths"
     if mask.bool_mask is not None and mask.bool_mask.dim() == 4 and mask.bool_mask.shape[1] != 1:
         return "per-head boolean mask"
-    if mask.bool_mask is None and mask.window > 0 and mask.sinks > 0:
-        return "first tokens that a window leaves visible"
     return None
 
 
@@ -181,6 +239,8 @@ def attention(q, k, v, mask: AttentionMask, scale: Optional[float], softcap: flo
     sk = k.shape[1]
     scale = (1.0 / math.sqrt(d)) if scale is None else scale
     softcap = max(0.0, float(softcap or 0.0))  # 0 and below: no cap
+    if softcap == 0.0 and _first_positions(s, sk, mask):
+        return _WindowAttention.apply(q, k, v, mask.doc_ids, min(mask.window, sk), min(max(mask.sinks, 0), sk), float(scale))
     lo = hi = kmask = dense = None
     monotone, causal = 1, bool(mask.causal)
     if mask.key_start is not None:

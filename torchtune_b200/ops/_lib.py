@@ -169,6 +169,16 @@ def _declare(L: ctypes.CDLL) -> None:
     L.ttb_lightning_chunks.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, i32, vp, vp]
     L.ttb_silu_rows.argtypes = [vp, i64, i64, i32, vp]
     L.ttb_gated_norm.argtypes = [vp, i32, vp, vp, i64, vp, i64, i32, f32, i32, vp]
+    L.ttb_attn_fwd2_first.argtypes = [vp] * 6 + [i32] * 8 + [f32, vp, vp]
+    L.ttb_attn_fwd2_first.restype = i32
+    L.ttb_attn_decode_first.argtypes = [vp] * 4 + [i32] * 8 + [f32, vp]
+    L.ttb_attn_decode_first.restype = i32
+    L.ttb_attn_bwd_first.argtypes = [vp] * 11 + [i32, i32, vp, i64] + [i32] * 6 + [f32, vp, vp]
+    L.ttb_attn_bwd_first.restype = i32
+    L.ttb_attn_bwd_first_workspace.argtypes = [i32] * 8
+    L.ttb_attn_bwd_first_workspace.restype = i64
+    L.ttb_document_bounds.argtypes = [vp, i32, i32, i32, i32, vp, vp, vp]
+    L.ttb_document_bounds.restype = i32
     L.ttb_quantized_append.argtypes = [vp] * 6 + [c.POINTER(i64), vp] + [i32] * 7 + [vp]
     L.ttb_quantized_append.restype = i32
     L.ttb_quantized_read.argtypes = [vp] * 4 + [c.POINTER(i64), vp, vp] + [i32] * 7 + [vp]

@@ -777,6 +777,22 @@ extern "C" int ttb_attn_fwd(const void* q, const void* k, const void* v, void* o
   return d == 128 ? launch_fwd<128>(q, k, v, p, st) : launch_fwd<64>(q, k, v, p, st);
 }
 
+// delta of the backward pass: rowsum(dO o O) per token and head
+static int launch_delta(const void* o, const void* d_o, float* delta, int b, int s, int hq, int d, cudaStream_t st) {
+  const long long tokens = static_cast<long long>(b) * s;
+  if ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(d_o)) & 15) return kErrBadShape;  // both are read 16 bytes at a time
+  int log_per = 3;
+  static_assert(kDeltaTokens == 1 << 3, "eight tokens, halved below");
+  while (log_per > 0 && (tokens >> log_per) < sm_count()) --log_per;
+  const int per = 1 << log_per;
+  const bool staged = hq <= 48 * 1024 / (per * 4);
+  const int smem = staged ? hq * per * 4 : 0;
+  TTB_COUNT_LAUNCH(1);
+  auto delta_kernel = d == 128 ? attn_delta_kernel<128> : attn_delta_kernel<64>;
+  delta_kernel<<<static_cast<unsigned>((tokens + per - 1) / per), 256, smem, st>>>(static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(d_o), delta, tokens, s, hq, log_per, staged);
+  return kOk;
+}
+
 // attention_bwd2.cu
 int ttb_attn_bwd2(const void* q, const void* k, const void* v, const void* d_o, const float* lse, const float* delta, float* dq, void* dk, void* dv, const int* lo, const int* hi,
                   int monotone, int b, int s, int sk, int hq, int hkv, int d, float scale, int causal, int* err, cudaStream_t stream);
@@ -789,17 +805,8 @@ extern "C" int ttb_attn_bwd(const void* q, const void* k, const void* v, const v
   if ((d != 64 && d != 128) || hq % hkv || s <= 0 || sk <= 0) return kErrBadShape;
   if (causal && hi == nullptr && s != sk) return kErrBadShape;
   auto st = static_cast<cudaStream_t>(stream);
-  const long long tokens = static_cast<long long>(b) * s;
-  if ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(d_o)) & 15) return kErrBadShape;  // both are read 16 bytes at a time
-  int log_per = 3;
-  static_assert(kDeltaTokens == 1 << 3, "eight tokens, halved below");
-  while (log_per > 0 && (tokens >> log_per) < sm_count()) --log_per;
-  const int per = 1 << log_per;
-  const bool staged = hq <= 48 * 1024 / (per * 4);
-  const int smem = staged ? hq * per * 4 : 0;
-  TTB_COUNT_LAUNCH(1);
-  auto delta_kernel = d == 128 ? attn_delta_kernel<128> : attn_delta_kernel<64>;
-  delta_kernel<<<static_cast<unsigned>((tokens + per - 1) / per), 256, smem, st>>>(static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(d_o), delta, tokens, s, hq, log_per, staged);
+  const int rc = launch_delta(o, d_o, delta, b, s, hq, d, st);
+  if (rc != kOk) return rc;
   AttnParams p{};
   p.b = b, p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.d = d, p.scale = scale, p.causal = causal, p.lo = lo, p.hi = hi;
   p.kmask = static_cast<const uint8_t*>(kmask), p.monotone = monotone, p.softcap = softcap;
@@ -807,4 +814,16 @@ extern "C" int ttb_attn_bwd(const void* q, const void* k, const void* v, const v
   p.dk = static_cast<__nv_bfloat16*>(dk), p.dv = static_cast<__nv_bfloat16*>(dv), p.err = err;
   if (!(softcap > 0.f) && kmask == nullptr) return ttb_attn_bwd2(q, k, v, d_o, lse, delta, dq_accum, dk, dv, lo, hi, monotone, b, s, sk, hq, hkv, d, scale, causal, err, st);
   return d == 128 ? launch_bwd<128>(q, k, v, d_o, p, st) : launch_bwd<64>(q, k, v, d_o, p, st);
+}
+
+int ttb_attn_bwd2_first(const void* q, const void* k, const void* v, const void* d_o, const float* lse, const float* delta, float* dq, void* dk, void* dv, const int* last, int window, int sinks,
+                        float* work, long long work_floats, int b, int s, int sk, int hq, int hkv, int d, float scale, int* err, cudaStream_t stream);
+
+// Backward of ttb_attn_fwd2_first: tensors as in ttb_attn_bwd; last (with documents, else nullptr) as ttb_document_bounds gives it; work: as many fp32 numbers as ttb_attn_bwd_first_workspace says.
+extern "C" int ttb_attn_bwd_first(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse, float* delta, float* dq_accum, void* dk, void* dv, const int* last,
+                                  int window, int sinks, float* work, long long work_floats, int b, int s, int sk, int hq, int hkv, int d, float scale, int* err, void* stream) {
+  if ((d != 64 && d != 128) || hkv <= 0 || hq % hkv || s <= 0 || sk < s || b <= 0 || window <= 0 || sinks < 0 || (last != nullptr && s != sk) || sk > (1 << 30)) return kErrBadShape;
+  auto st = static_cast<cudaStream_t>(stream);
+  const int rc = launch_delta(o, d_o, delta, b, s, hq, d, st);
+  return rc != kOk ? rc : ttb_attn_bwd2_first(q, k, v, d_o, lse, delta, dq_accum, dk, dv, last, window, sinks, work, work_floats, b, s, sk, hq, hkv, d, scale, err, st);
 }

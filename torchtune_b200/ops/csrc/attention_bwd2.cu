@@ -16,6 +16,8 @@
 // 4 x 2048 of 128 937 -> 588 us, in documents of 512 394 -> 296 us.  With dQ added by 16-byte atomics instead of TMA reductions the first took 13 300 us.  What bounds it:
 // at head dim 128 the chain dS -> dQ -> dP -> dS beside 2560 cycles of products per block, at head dim 64 the exponentials.
 //
+// FIRST: a causal window beside which the first positions (of the sequence, or of each document) stay visible.  A key is seen by one run of queries, so the mask of a thread is two numbers.
+//
 // Structured masks as in attention.cu (bounds lo / hi per query); soft-capped scores and boolean masks stay on the first form.  Every wait is bounded.
 #include <type_traits>
 
@@ -42,6 +44,13 @@ struct Params {
   __nv_bfloat16* dk;   // [b, sk, hkv, D]
   __nv_bfloat16* dv;
   int* err;
+  // FIRST: a causal window (query i at position sk - s + i) beside which the first `sinks` positions stay visible
+  int window, sinks;
+  const int* last;     // [b, sk] last query that sees a key of packed documents (s == sk), or nullptr
+  // The first positions are seen by all later queries.  Without documents the queries beyond the window of a block that holds some are cut into `pieces` runs of `piece` query blocks, each a
+  // CTA of its own, so that no CTA walks the whole sequence; their gradients and those of the block's own CTA meet in `partial` [b * hkv][blocks][1 + pieces][rows][dk, dv][D].
+  int blocks, pieces, piece, rows;
+  float* partial;
 };
 
 template <int D>
@@ -59,7 +68,7 @@ __device__ __forceinline__ uint32_t swizzled(int row, int col) {  // byte offset
   return (col >> 6) * kPanelBytes + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4);
 }
 
-template <int D>
+template <int D, bool FIRST>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
                  const __grid_constant__ CUtensorMap tmdQ, Params p) {
@@ -97,7 +106,11 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hk = blockIdx.y, bi = blockIdx.z;
   const int group = p.hq / p.hkv;
-  const int kv0 = blockIdx.x * kBlk;
+  const int key_blocks = (p.sk + kBlk - 1) / kBlk;
+  const bool far = FIRST && static_cast<int>(blockIdx.x) >= key_blocks;  // queries beyond the window of a block with first positions
+  const int far_index = static_cast<int>(blockIdx.x) - key_blocks;
+  const int kv0 = (far ? far_index / max(p.pieces, 1) : static_cast<int>(blockIdx.x)) * kBlk;
+  const int shift = p.sk - p.s;
   const int row_base = bi * p.s, krow_base = bi * p.sk;
   const int nq_blocks = (p.s + kBlk - 1) / kBlk;
   int qb_begin = (p.hi == nullptr && p.causal) ? static_cast<int>(blockIdx.x) : 0;
@@ -111,6 +124,21 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           qb_end = qb;
           break;
         }
+  }
+  if constexpr (FIRST) {
+    qb_begin = max(0, kv0 - shift) / kBlk;
+    if (p.last != nullptr) {
+      int end = -1;
+      for (int x = threadIdx.x & 31; x < kBlk && kv0 + x < p.sk; x += 32) end = max(end, p.last[krow_base + kv0 + x]);
+      qb_end = __reduce_max_sync(0xffffffffu, end) / kBlk + 1;
+    } else {
+      const int beyond = min(nq_blocks, max(0, min(p.sk - 1, kv0 + kBlk - 1) - shift + p.window - 1) / kBlk + 1);  // of the window of the last key
+      qb_end = kv0 < p.sinks && p.pieces == 0 ? nq_blocks : beyond;
+      if (far) {
+        qb_begin = beyond + far_index % p.pieces * p.piece;
+        qb_end = min(nq_blocks, qb_begin + p.piece);
+      }
+    }
   }
   const int per_head = max(qb_end - qb_begin, 0);
   const int n = per_head * group;
@@ -150,11 +178,17 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   if (warp < 4) {
     if (warp == 0) {
       // -------------------------------------------------------------- TMA producer
+      auto load_rows = [&](uint8_t* to, const CUtensorMap* m, uint64_t* bar, int col, int base, int row) {
+        if constexpr (FIRST)
+          tma_load_3d(to, m, bar, col, row, bi);  // rows behind the last one are zeros, not the next batch row's
+        else
+          tma_load_2d(to, m, bar, col, base + row);
+      };
       if (n > 0 && lane == 0) {
         mbar_arrive_expect_tx(kv_full, 2 * L::kTile);
         for (int j = 0; j < kPanels; ++j) {
-          tma_load_2d(sK + j * kPanelBytes, &tmK, kv_full, hk * D + j * 64, krow_base + kv0);
-          tma_load_2d(sV + j * kPanelBytes, &tmV, kv_full, hk * D + j * 64, krow_base + kv0);
+          load_rows(sK + j * kPanelBytes, &tmK, kv_full, hk * D + j * 64, krow_base, kv0);
+          load_rows(sV + j * kPanelBytes, &tmV, kv_full, hk * D + j * 64, krow_base, kv0);
         }
       }
       for (int i = 0; i < n && !stopped(); ++i) {
@@ -166,7 +200,7 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
         if (lane == 0) {
           mbar_arrive_expect_tx(&q_full[st], L::kTile);
-          for (int j = 0; j < kPanels; ++j) tma_load_2d(sQ + st * L::kTile + j * kPanelBytes, &tmQ, &q_full[st], h * D + j * 64, row_base + q0);
+          for (int j = 0; j < kPanels; ++j) load_rows(sQ + st * L::kTile + j * kPanelBytes, &tmQ, &q_full[st], h * D + j * 64, row_base, q0);
         }
         if (!wait(do_empty, (i & 1) ^ 1)) {
           fail(abort_flag, p.err, 316);
@@ -174,7 +208,7 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
         if (lane == 0) {
           mbar_arrive_expect_tx(do_full, L::kTile);
-          for (int j = 0; j < kPanels; ++j) tma_load_2d(sdO + j * kPanelBytes, &tmdO, do_full, h * D + j * 64, row_base + q0);
+          for (int j = 0; j < kPanels; ++j) load_rows(sdO + j * kPanelBytes, &tmdO, do_full, h * D + j * 64, row_base, q0);
         }
         __syncwarp();
       }
@@ -278,12 +312,15 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
     const float c = p.scale * kLog2e;
     const uint64_t c2 = pack_f32x2(c, c), sc2 = pack_f32x2(p.scale, p.scale);
+    const int last_doc = FIRST && p.last != nullptr && key < p.sk ? p.last[krow_base + key] : -1;
     bool ok = true;
     for (int i = 0; i < n && !stopped(); ++i) {
       const int st = i & 1;
       const int q0 = (qb_begin + i % per_head) * kBlk;
-      bool interior = (p.monotone || (p.lo == nullptr && p.hi == nullptr)) && q0 + kBlk <= p.s && kv0 + kBlk <= p.sk;
-      if (interior) {
+      // FIRST: the queries that see this thread's key
+      const int from_q = key - shift, last_q = !FIRST || key >= p.sk ? -1 : p.last != nullptr ? last_doc : key < p.sinks ? p.s - 1 : min(p.s - 1, from_q + p.window - 1);
+      bool interior = FIRST ? __all_sync(0xffffffffu, from_q <= q0 && last_q >= q0 + kBlk - 1) : (p.monotone || (p.lo == nullptr && p.hi == nullptr)) && q0 + kBlk <= p.s && kv0 + kBlk <= p.sk;
+      if (!FIRST && interior) {
         const int lo_max = p.lo != nullptr ? p.lo[row_base + q0 + kBlk - 1] : 0;
         const int hi_min = p.hi != nullptr ? p.hi[row_base + q0] : (p.causal ? q0 : p.sk - 1);
         interior = lo_max <= kv0 && hi_min >= kv0 + kBlk - 1;
@@ -300,7 +337,10 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
           uint32_t seen = 0xffffffffu;  // queries of the chunk that see this thread's key
-          if constexpr (masked.value) {
+          if constexpr (masked.value && FIRST) {
+            const int first = q0 + half * 64 + ch * 32, a = max(from_q - first, 0), z = min(last_q - first, 31);
+            seen = z >= a ? (0xffffffffu << a) & (0xffffffffu >> (31 - z)) : 0u;
+          } else if constexpr (masked.value) {
             const int first = q0 + half * 64 + ch * 32, q = min(first + lane, p.s - 1);
             const int lo = p.lo != nullptr ? __ldg(p.lo + row_base + q) : 0;
             const int hi = p.hi != nullptr ? __ldg(p.hi + row_base + q) : (p.causal ? q : p.sk - 1);
@@ -388,6 +428,10 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       // the first half's warps write dK, the second half's dV
       const uint32_t from = half == 0 ? tdK : tdV;
       __nv_bfloat16* to = (half == 0 ? p.dk : p.dv) + (static_cast<long long>(krow_base + key) * p.hkv + hk) * D;
+      const bool shared = FIRST && p.pieces > 0 && kv0 < p.sinks;  // others have parts of the gradients of the first positions
+      float* part = nullptr;
+      if (shared && r < p.rows && key < p.sinks)
+        part = p.partial + ((((static_cast<long long>(bi) * p.hkv + hk) * p.blocks + kv0 / kBlk) * (1 + p.pieces) + (far ? 1 + far_index % p.pieces : 0)) * p.rows + r) * 2 * D + half * D;
 #pragma unroll 1
       for (int ch = 0; ch < D / 32; ++ch) {
         uint32_t a[32];
@@ -398,7 +442,11 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
           for (int j = 0; j < 32; ++j) a[j] = 0;
         }
-        if (key < p.sk) {
+        if (FIRST && part != nullptr) {
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            *reinterpret_cast<uint4*>(part + ch * 32 + g * 4) = make_uint4(a[g * 4], a[g * 4 + 1], a[g * 4 + 2], a[g * 4 + 3]);
+        } else if (key < p.sk && !far) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             uint4 u;
@@ -460,10 +508,27 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   if (warp == 2) tmem_dealloc(tmem_base, 512);
 }
 
+// Gradients of the first positions: the parts of the CTAs in their order.  Grid (rows, blocks, batch times key heads), 2D threads.
 template <int D>
+__global__ void __launch_bounds__(2 * D)
+first_rows_kernel(Params p) {
+  const int r = blockIdx.x, block = blockIdx.y, bi = blockIdx.z / p.hkv, hk = blockIdx.z % p.hkv;
+  const int key = block * kBlk + r;
+  if (key >= p.sinks || key >= p.sk) return;
+  const float* from = p.partial + ((static_cast<long long>(blockIdx.z) * p.blocks + block) * (1 + p.pieces) * p.rows + r) * 2 * D + threadIdx.x;
+  float sum = 0.f;
+#pragma unroll 4
+  for (int x = 0; x <= p.pieces; ++x) sum += from[static_cast<long long>(x) * p.rows * 2 * D];
+  const int d = threadIdx.x % D;
+  (threadIdx.x < D ? p.dk : p.dv)[(static_cast<long long>(bi * p.sk + key) * p.hkv + hk) * D + d] = __float2bfloat16_rn(sum);
+}
+
+template <int D, bool FIRST = false>
 static int launch(const void* q, const void* k, const void* v, const void* d_o, float* dq, int b, const Params& p, cudaStream_t st) {
   CUtensorMap tq, tk, tv, tdo, tdq;
   auto map = [&](CUtensorMap* m, const void* base, int s, int heads) {
+    const uint64_t pitch = static_cast<uint64_t>(heads) * D * 2;
+    if (FIRST) return make_tmap_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<uint64_t>(heads) * D, s, b, pitch, pitch * s, 64, kBlk, 1, CU_TENSOR_MAP_SWIZZLE_128B);
     return make_tmap_2d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, static_cast<uint64_t>(b) * s, static_cast<uint64_t>(heads) * D, static_cast<uint64_t>(heads) * D, kBlk, 64,
                         CU_TENSOR_MAP_SWIZZLE_128B);
   };
@@ -471,14 +536,18 @@ static int launch(const void* q, const void* k, const void* v, const void* d_o, 
   if ((rc = map(&tq, q, p.s, p.hq)) != kOk || (rc = map(&tk, k, p.sk, p.hkv)) != kOk || (rc = map(&tv, v, p.sk, p.hkv)) != kOk || (rc = map(&tdo, d_o, p.s, p.hq)) != kOk) return rc;
   const uint64_t width = static_cast<uint64_t>(p.hq) * D;
   if ((rc = make_tmap_3d(&tdq, dq, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, width, p.s, b, width * 4, width * 4 * p.s, 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_128B)) != kOk) return rc;
-  auto kern = attn_bwd2_kernel<D>;
+  auto kern = attn_bwd2_kernel<D, FIRST>;
   static bool attr = false;
   if (!attr) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kDynamic) != cudaSuccess) return kErrDriver;
     attr = true;
   }
   TTB_COUNT_LAUNCH(1);
-  kern<<<dim3((p.sk + kBlk - 1) / kBlk, p.hkv, b), kThreads, Layout<D>::kDynamic, st>>>(tq, tk, tv, tdo, tdq, p);
+  kern<<<dim3((p.sk + kBlk - 1) / kBlk + (FIRST ? p.blocks * p.pieces : 0), p.hkv, b), kThreads, Layout<D>::kDynamic, st>>>(tq, tk, tv, tdo, tdq, p);
+  if (FIRST && p.pieces > 0) {
+    TTB_COUNT_LAUNCH(1);
+    first_rows_kernel<D><<<dim3(p.rows, p.blocks, b * p.hkv), 2 * D, 0, st>>>(p);
+  }
   return cudaGetLastError() == cudaSuccess ? kOk : kErrDriver;
 }
 
@@ -493,4 +562,50 @@ int ttb_attn_bwd2(const void* q, const void* k, const void* v, const void* d_o, 
   p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.scale = scale, p.causal = causal, p.lo = lo, p.hi = hi, p.monotone = monotone;
   p.lse = lse, p.delta = delta, p.dk = static_cast<__nv_bfloat16*>(dk), p.dv = static_cast<__nv_bfloat16*>(dv), p.err = err;
   return d == 128 ? fb2::launch<128>(q, k, v, d_o, dq, b, p, stream) : fb2::launch<64>(q, k, v, d_o, dq, b, p, stream);
+}
+
+namespace ttb {
+namespace fb2 {
+
+// How the queries beyond the window of the blocks with first positions are cut: runs as long as what a block's own CTA walks, at most 32 of them and 2^24 fp32 numbers of partial gradients.
+static void cut(Params& p, int b, int d, bool documents) {
+  const int nq = (p.s + kBlk - 1) / kBlk, shift = p.sk - p.s;
+  p.blocks = (p.sinks + kBlk - 1) / kBlk, p.rows = p.sinks < kBlk ? p.sinks : kBlk, p.pieces = 0, p.piece = 0;
+  if (documents || p.sinks == 0) return;
+  const int last = kBlk - 1 < p.sk - 1 ? kBlk - 1 : p.sk - 1;
+  const int beyond = (last - shift + p.window - 1 > 0 ? last - shift + p.window - 1 : 0) / kBlk + 1;  // as in the kernel, for the first block: the others have fewer
+  const int left = nq - beyond;
+  if (left <= 0) return;
+  const int own = p.window / kBlk + 2;
+  const long long one = static_cast<long long>(b) * p.hkv * p.blocks * p.rows * 2 * d, most = (1ll << 24) / one - 1;
+  long long pieces = (left + own - 1) / own;
+  if (pieces > 32) pieces = 32;
+  if (pieces > most) pieces = most;
+  if (pieces < 1) return;
+  p.piece = static_cast<int>((left + pieces - 1) / pieces);
+  p.pieces = (left + p.piece - 1) / p.piece;
+}
+
+}  // namespace fb2
+}  // namespace ttb
+
+// fp32 numbers of workspace that ttb_attn_bwd_first wants.
+extern "C" long long ttb_attn_bwd_first_workspace(int window, int sinks, int documents, int b, int s, int sk, int hkv, int d) {
+  using namespace ttb;
+  fb2::Params p{};
+  p.s = s, p.sk = sk, p.hkv = hkv, p.window = window < sk ? window : sk, p.sinks = sinks < sk ? sinks : sk;
+  fb2::cut(p, b, d, documents != 0);
+  return p.pieces == 0 ? 0 : static_cast<long long>(b) * hkv * p.blocks * (1 + p.pieces) * p.rows * 2 * d;
+}
+
+// Backward of ttb_attn_fwd2_first; delta [b, hq, s] as attn_delta_kernel leaves it, dq fp32 zeros.  last (nullable, with documents) int32 [b, sk]: last query that sees a key.
+int ttb_attn_bwd2_first(const void* q, const void* k, const void* v, const void* d_o, const float* lse, const float* delta, float* dq, void* dk, void* dv, const int* last, int window, int sinks,
+                        float* work, long long work_floats, int b, int s, int sk, int hq, int hkv, int d, float scale, int* err, cudaStream_t stream) {
+  using namespace ttb;
+  fb2::Params p{};
+  p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.scale = scale, p.causal = 1, p.window = window < sk ? window : sk, p.sinks = sinks < sk ? sinks : sk, p.last = last;
+  p.lse = lse, p.delta = delta, p.dk = static_cast<__nv_bfloat16*>(dk), p.dv = static_cast<__nv_bfloat16*>(dv), p.err = err, p.partial = work;
+  fb2::cut(p, b, d, last != nullptr);
+  if (p.pieces > 0 && (work == nullptr || work_floats < ttb_attn_bwd_first_workspace(window, sinks, 0, b, s, sk, hkv, d) || (reinterpret_cast<uintptr_t>(work) & 15))) return kErrBadShape;
+  return d == 128 ? fb2::launch<128, true>(q, k, v, d_o, dq, b, p, stream) : fb2::launch<64, true>(q, k, v, d_o, dq, b, p, stream);
 }

@@ -43,6 +43,7 @@ struct Params {
   long long mask_b, mask_r;
   const int* lo;           // [b, s] first / last visible key, or nullptr (0 / sk - 1)
   const int* hi;
+  int window, sinks;       // window > 0: query i is position sk - s + i and sees the last `window` positions up to its own and the first `sinks`
   int s, sk, hq, hkv;
   float scale;
   // APPEND: one query per row; q is still to be rotated, and the new key (to be rotated as well) and value go to slot slots[0] of the caches k and v first
@@ -108,6 +109,10 @@ decode_kernel(Params p) {
     for (int x = 0; x < 2; ++x) {
       const int j = j0 + x * 32 + lane;
       bool seen = j < p.sk && j >= lo && j <= hi;
+      if (p.window > 0) {
+        const int at = p.sk - p.s + qi;
+        seen = seen && j <= at && (at - j < p.window || j < p.sinks);
+      }
       if (seen && p.mask != nullptr) seen = p.mask[bi * p.mask_b + qi * p.mask_r + j] != 0;
       half[x] = __ballot_sync(0xffffffffu, seen);
     }
@@ -409,6 +414,44 @@ mask_bounds_kernel(const uint8_t* __restrict__ mask, long long stride_b, long lo
   }
 }
 
+// Where each token's document (a run of equal ids) begins, and the last query that sees it as a key under a causal window beside which the first `sinks` tokens of a document stay visible: the
+// document's last token for those, else the last one in the window.  One CTA per row; a thread has a run of tokens, and two scans over the threads carry the borders across the runs.
+static constexpr int kDocThreads = 1024;
+__global__ void __launch_bounds__(kDocThreads)
+document_bounds_kernel(const int* __restrict__ ids, int s, int window, int sinks, int* __restrict__ start, int* __restrict__ last) {
+  __shared__ int before[kDocThreads], behind[kDocThreads];
+  const int* row = ids + static_cast<long long>(blockIdx.x) * s;
+  const int per = (s + kDocThreads - 1) / kDocThreads, i0 = threadIdx.x * per, i1 = min(s, i0 + per);
+  int newest = 0, next = s;  // last border in the run (0 holds for all), first border in it
+  for (int i = i0; i < i1; ++i)
+    if (i > 0 && row[i] != row[i - 1]) {
+      newest = i;
+      if (next == s) next = i;
+    }
+  before[threadIdx.x] = newest, behind[threadIdx.x] = next;
+  __syncthreads();
+  for (int o = 1; o < kDocThreads; o *= 2) {
+    const int t = threadIdx.x;
+    const int x = t >= o ? before[t - o] : 0, y = t + o < kDocThreads ? behind[t + o] : s;
+    __syncthreads();
+    before[t] = max(before[t], x), behind[t] = min(behind[t], y);
+    __syncthreads();
+  }
+  int from = threadIdx.x > 0 ? before[threadIdx.x - 1] : 0, to = i0;  // the document of the token at hand: its first token, and the border behind it (found when it is passed)
+  const int after = threadIdx.x + 1 < kDocThreads ? behind[threadIdx.x + 1] : s;
+  for (int i = i0; i < i1; ++i) {
+    if (i > 0 && row[i] != row[i - 1]) from = i;
+    if (to <= i) {
+      to = i + 1;
+      while (to < i1 && row[to] == row[to - 1]) ++to;
+      if (to == i1 && (to == s || row[to] == row[to - 1])) to = after;
+    }
+    const long long at = static_cast<long long>(blockIdx.x) * s + i;
+    start[at] = from;
+    last[at] = i - from < sinks ? to - 1 : min(to - 1, i + window - 1);
+  }
+}
+
 }  // namespace dec
 }  // namespace ttb
 
@@ -425,6 +468,19 @@ extern "C" int ttb_attn_decode(const void* q, const void* k, const void* v, void
   p.q = static_cast<const __nv_bfloat16*>(q), p.k = static_cast<const __nv_bfloat16*>(k), p.v = static_cast<const __nv_bfloat16*>(v), p.o = static_cast<__nv_bfloat16*>(o);
   p.mask = static_cast<const uint8_t*>(mask), p.mask_b = mask_b, p.mask_r = mask_r, p.lo = lo, p.hi = hi;
   p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.scale = scale;
+  auto st = static_cast<cudaStream_t>(stream);
+  return d == 128 ? dec::launch<128, false>(p, b, st) : dec::launch<64, false>(p, b, st);
+}
+
+// The same under the mask of ttb_attn_fwd2_first without documents.
+extern "C" int ttb_attn_decode_first(const void* q, const void* k, const void* v, void* o, int window, int sinks, int b, int s, int sk, int hq, int hkv, int d, float scale, void* stream) {
+  using namespace ttb;
+  if ((d != 64 && d != 128) || b <= 0 || s <= 0 || sk < s || hkv <= 0 || hq % hkv || s * (hq / hkv) > dec::kMaxRows || b > 65535 || hkv > 65535 || window <= 0 || sinks < 0) return kErrBadShape;
+  for (const void* t : {q, k, v, static_cast<const void*>(o)})
+    if (reinterpret_cast<uintptr_t>(t) & 15) return kErrBadShape;
+  dec::Params p{};
+  p.q = static_cast<const __nv_bfloat16*>(q), p.k = static_cast<const __nv_bfloat16*>(k), p.v = static_cast<const __nv_bfloat16*>(v), p.o = static_cast<__nv_bfloat16*>(o);
+  p.window = window, p.sinks = sinks, p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.scale = scale;
   auto st = static_cast<cudaStream_t>(stream);
   return d == 128 ? dec::launch<128, false>(p, b, st) : dec::launch<64, false>(p, b, st);
 }
@@ -455,5 +511,14 @@ extern "C" int ttb_mask_bounds(const void* mask, long long stride_b, long long s
   TTB_COUNT_LAUNCH(1);
   dec::mask_bounds_kernel<<<static_cast<unsigned>((warps + 7) / 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(
       static_cast<const uint8_t*>(mask), stride_b, stride_r, b, s, sk, lo, hi, static_cast<uint8_t*>(solid));
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrDriver;
+}
+
+// start, last int32 [b, s] of document ids int32 [b, s], contiguous (see document_bounds_kernel).
+extern "C" int ttb_document_bounds(const int* ids, int b, int s, int window, int sinks, int* start, int* last, void* stream) {
+  using namespace ttb;
+  if (b <= 0 || s <= 0 || s > (1 << 30) || window <= 0 || sinks < 0) return kErrBadShape;
+  TTB_COUNT_LAUNCH(1);
+  dec::document_bounds_kernel<<<b, dec::kDocThreads, 0, static_cast<cudaStream_t>(stream)>>>(ids, s, window < s ? window : s, sinks, start, last);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrDriver;
 }

@@ -12,6 +12,7 @@
 // none; each tile visits only its own range of key blocks.  A boolean mask comes with the bounds of its rows in any order (the MASKED
 // form takes a tile's range from all its rows) and a flag per row that says whether everything between its bounds is visible: then the
 // bounds are the whole mask, as for the causal masks of cached generation, and only the other rows read mask bytes.
+// FIRST: a causal window beside which the first positions stay visible; both tiles visit the blocks of the first positions and then those of the window.
 // Causal forward, head dim 64 (one-tile kernel before): 8 x 2048 tokens 788 -> 374 us, 1 x 16384 tokens 5079 -> 2042 us; exponentials bound it.
 // Soft-capped scores stay on the one-tile kernel in attention.cu.  Every wait is bounded and reports through the error word.
 #include "common/attn_math.cuh"
@@ -40,12 +41,21 @@ struct Params {
   const uint8_t* solid;
   const uint8_t* mask;
   long long mask_b, mask_r;
+  // FIRST: a causal window of `window` positions, query i at position sk - s + i, beside which the first `sinks` positions of the sequence, or of the query's document, stay visible
+  int window, sinks;
+  const int* start;  // [b, s] first position of each query's document (s == sk), or nullptr
   __nv_bfloat16* o;
   float* lse;
   int* err;
 };
 
-template <int D, bool MASKED>
+// Bits of the keys first ... last among the 32 from k0 on.
+__device__ __forceinline__ uint32_t keys_between(int k0, int first, int last) {
+  const int a = max(first - k0, 0), b = min(last - k0, 31);
+  return b >= a ? (0xffffffffu << a) & (0xffffffffu >> (31 - b)) : 0u;
+}
+
+template <int D, bool MASKED, bool FIRST>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, Params p) {
   constexpr int kTileBytes = kTileBytesOf<D>, kPanels = D / 64;
@@ -94,9 +104,39 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
   // Key-block range of each tile: [begin, begin + count).  The bounds are monotone, so first and last row give them.
   int begin[2], count[2];
+  // FIRST: blocks are numbered along what the two tiles visit: `heads` blocks of first positions, from the first one of the first row's document on and as wide as needed, then those from block
+  // `tail0` of the keys on, where the window of the first row begins (a document that begins later has its first positions there).  The second tile leaves out `skip` blocks of the latter.
+  int heads = 0, head_key = 0, head_end = 0, tail0 = 0, skip = 0;
+  const int shift = p.sk - p.s;
+  if constexpr (FIRST) {
+    head_key = p.start != nullptr ? p.start[row_base + q0] : 0;
+    tail0 = max(head_key, q0 + shift - p.window + 1) / kBlk;
+    head_end = min(head_key + p.sinks, tail0 * kBlk);
+    heads = head_end > head_key ? (head_end - head_key + kBlk - 1) / kBlk : 0;
+    if (const int qb = q0 + kBlk; qb < p.s) {
+      const int start = p.start != nullptr ? p.start[row_base + qb] : 0, lo = max(start, qb + shift - p.window + 1);
+      if (start == lo || start + p.sinks <= tail0 * kBlk) skip = lo / kBlk - tail0;
+    }
+  }
+  auto block_key = [&](int i) {  // first key of block i
+    if constexpr (FIRST) return i < heads ? head_key + i * kBlk : (tail0 + i - heads) * kBlk;
+    return i * kBlk;
+  };
+  auto chunks = [&](int i) {  // of 32 keys in block i
+    if constexpr (FIRST) return i < heads ? min(4, (head_end - head_key - i * kBlk + 31) >> 5) : 4;
+    return 4;
+  };
+  auto skipped = [&](int x) { return FIRST && x == 1 ? skip : 0; };
+  auto resume = [&](int x) { return heads + skipped(x); };  // the first of the window's blocks that tile x visits
+  auto local = [&](int x, int i) { return FIRST && i >= heads ? i - skipped(x) : i; };  // FIRST: count of the blocks of tile x in front of block i
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const int qa = q0 + x * kBlk;
+    if constexpr (FIRST) {
+      begin[x] = 0;
+      count[x] = qa < p.s ? heads + (min(qa + kBlk, p.s) - 1 + shift) / kBlk + 1 - tail0 - skipped(x) : 0;
+      continue;
+    }
     if (qa >= p.s) {
       begin[x] = 0, count[x] = 0;
       continue;
@@ -114,7 +154,9 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (begin[late] > end) count[late] += begin[late] - end, begin[late] = end;
   }
   int u_begin, u_end;  // union of the two ranges
-  if (count[0] > 0 && count[1] > 0) {
+  if constexpr (FIRST) {
+    u_begin = 0, u_end = max(count[0], count[1] > 0 ? count[1] + skip : 0);
+  } else if (count[0] > 0 && count[1] > 0) {
     u_begin = min(begin[0], begin[1]);
     u_end = max(begin[0] + count[0], begin[1] + count[1]);
   } else if (count[0] > 0) {
@@ -156,17 +198,23 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       for (int x = 0; x < 2; ++x)
         for (int j = 0; j < kPanels; ++j) tma_load_2d(sQ[x] + j * kPanelBytes, &tmQ, q_full, h * D + j * 64, row_base + q0 + x * kBlk);
     }
+    auto load_rows = [&](uint8_t* to, const CUtensorMap* m, uint64_t* bar, int col, int key) {
+      if constexpr (FIRST)
+        tma_load_3d(to, m, bar, col, key, bi);  // keys behind the last one are zeros, not the next batch row's
+      else
+        tma_load_2d(to, m, bar, col, krow_base + key);
+    };
     uint32_t phase = 0;
     for (int i = 0; i < n_union && !*abort_flag; ++i) {
       const int st = i & 1;
-      const int kv0 = (u_begin + i) * kBlk;
+      const int kv0 = block_key(u_begin + i);
       if (!mbar_wait(&k_empty[st], phase ^ 1)) {
         fail(abort_flag, p.err, 211);
         break;
       }
       if (lane == 0) {
         mbar_arrive_expect_tx(&k_full[st], kTileBytes);
-        for (int j = 0; j < kPanels; ++j) tma_load_2d(sK[st] + j * kPanelBytes, &tmK, &k_full[st], hk * D + j * 64, krow_base + kv0);
+        for (int j = 0; j < kPanels; ++j) load_rows(sK[st] + j * kPanelBytes, &tmK, &k_full[st], hk * D + j * 64, kv0);
       }
       __syncwarp();
       if (!mbar_wait(&v_empty[st], phase ^ 1)) {
@@ -175,7 +223,7 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       if (lane == 0) {
         mbar_arrive_expect_tx(&v_full[st], kTileBytes);
-        for (int j = 0; j < kPanels; ++j) tma_load_2d(sV[st] + j * kPanelBytes, &tmV, &v_full[st], hk * D + j * 64, krow_base + kv0);
+        for (int j = 0; j < kPanels; ++j) load_rows(sV[st] + j * kPanelBytes, &tmV, &v_full[st], hk * D + j * 64, kv0);
       }
       __syncwarp();
       if (st == 1) phase ^= 1;
@@ -190,7 +238,15 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     bool ok = n_union == 0 || mbar_wait(q_full, 0);
     int k_ready = u_begin - 1;  // highest block whose K tile has been waited for
     int v_ready = u_begin - 1;
-    auto active = [&](int x, int j) { return count[x] > 0 && j >= begin[x] && j < begin[x] + count[x]; };
+    auto active = [&](int x, int j) {
+      if constexpr (FIRST) return count[x] > 0 && (j < heads || j >= resume(x)) && j < count[x] + skipped(x);
+      return count[x] > 0 && j >= begin[x] && j < begin[x] + count[x];
+    };
+    // FIRST: scores are issued one block ahead, but over a gap when its end is reached: the first tile, which has no gap, hands the stage of K on to the second
+    auto starts = [&](int x, int j) {
+      if constexpr (FIRST) return (j == 0 && heads > 0) || (j == resume(x) && (heads == 0 || skipped(x) > 0));
+      return j == begin[x];
+    };
     // S_x(j) = Q_x · K_jᵀ; the K stage is handed back after the last tile that reads it
     auto issue_s = [&](int x, int j) -> bool {
       const int i = j - u_begin, st = i & 1;
@@ -201,7 +257,7 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       tc_fence_after();
       if (lane == 0) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) umma_f16(tS[x], desc_kmajor(aQ[x], k), desc_kmajor(aK[st], k), idesc_s, k != 0);
+        for (int k = 0; k < D / 16; ++k) umma_f16(tS[x], desc_kmajor(aQ[x], k), desc_kmajor(aK[st], k), FIRST ? make_idesc_bf16(128, 32 * chunks(j), false, false) : idesc_s, k != 0);
         umma_commit(&s_full[x]);
         const bool other_later = (x == 0) && active(1, j);  // tile 1 issues its S(j) after tile 0's
         if (!other_later) umma_commit(&k_empty[st]);
@@ -211,10 +267,10 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     };
     for (int j = u_begin; j < u_end && ok && !*abort_flag; ++j) {
       for (int x = 0; x < 2 && ok; ++x)
-        if (active(x, j) && j == begin[x]) ok = issue_s(x, j);  // first block of a tile
+        if (active(x, j) && starts(x, j)) ok = issue_s(x, j);  // first block of a tile
       for (int x = 0; x < 2 && ok; ++x) {
         if (!active(x, j)) continue;
-        const int n = j - begin[x];  // tile-local block counter
+        const int n = FIRST ? local(x, j) : j - begin[x];  // tile-local block counter
         const int i = j - u_begin, st = i & 1;
         if (!mbar_wait(&p_full[x], n & 1)) {
           ok = false;
@@ -230,13 +286,19 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         tc_fence_after();
         if (lane == 0) {
 #pragma unroll
-          for (int k = 0; k < kBlk / 16; ++k) umma_f16_ts(tO[x], tS[x] + k * 8, desc_mnmajor(aV[st], k), idesc_o, (n | k) != 0);
+          for (int k = 0; k < kBlk / 16; ++k)
+            if (!FIRST || k < 2 * chunks(j)) umma_f16_ts(tO[x], tS[x] + k * 8, desc_mnmajor(aV[st], k), idesc_o, (n | k) != 0);
           const bool other_later = (x == 0) && active(1, j);
           if (!other_later) umma_commit(&v_empty[st]);
           if (n + 1 == count[x]) umma_commit(&o_done[x]);
         }
         __syncwarp();
-        if (n + 1 < count[x]) ok = issue_s(x, j + 1);
+        if constexpr (FIRST) {
+          const int next = j + 1 == heads ? resume(x) : j + 1;
+          if (n + 1 < count[x] && !starts(x, next)) ok = issue_s(x, next);
+        } else {
+          if (n + 1 < count[x]) ok = issue_s(x, j + 1);
+        }
       }
     }
     if (!ok) fail(abort_flag, p.err, 213);
@@ -251,10 +313,12 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
     const bool row_valid = q_idx < p.s;
     const bool tile_valid = qa < p.s;
-    const int lo_row = (p.lo != nullptr && row_valid) ? p.lo[bound_base + q_idx] : 0;
-    const int hi_row = (p.hi != nullptr) ? (row_valid ? p.hi[bound_base + q_idx] : -1) : (p.causal ? (row_valid ? q_idx : -1) : (row_valid ? p.sk - 1 : -1));
-    const int lo_max = (p.lo == nullptr || !tile_valid) ? 0 : (MASKED ? ranges[5 * x + 1] : p.lo[row_base + q_last]);
-    const int hi_min = !tile_valid ? -1 : (MASKED ? ranges[5 * x + 2] : ((p.hi != nullptr) ? p.hi[row_base + qa] : (p.causal ? qa : p.sk - 1)));
+    const int start_row = FIRST && p.start != nullptr ? p.start[row_base + min(q_idx, p.s - 1)] : 0, kept_end = start_row + p.sinks;
+    const int lo_row = FIRST ? max(start_row, q_idx + shift - p.window + 1) : (p.lo != nullptr && row_valid) ? p.lo[bound_base + q_idx] : 0;
+    const int hi_row = FIRST ? (row_valid ? q_idx + shift : -1)
+                             : (p.hi != nullptr) ? (row_valid ? p.hi[bound_base + q_idx] : -1) : (p.causal ? (row_valid ? q_idx : -1) : (row_valid ? p.sk - 1 : -1));
+    const int lo_max = FIRST ? (tile_valid ? max(p.start != nullptr ? p.start[row_base + q_last] : 0, q_last + shift - p.window + 1) : 0) : (p.lo == nullptr || !tile_valid) ? 0 : (MASKED ? ranges[5 * x + 1] : p.lo[row_base + q_last]);
+    const int hi_min = !tile_valid ? -1 : FIRST ? qa + shift : (MASKED ? ranges[5 * x + 2] : ((p.hi != nullptr) ? p.hi[row_base + qa] : (p.causal ? qa : p.sk - 1)));
     const bool bytes = MASKED && ranges[5 * x + 4] != 0;  // the same for all rows of the tile
     const uint8_t* mrow = (bytes && row_valid && !p.solid[bound_base + q_idx]) ? p.mask + bi * p.mask_b + q_idx * p.mask_r : nullptr;
     const bool ragged_rows = qa + kBlk > p.s;  // rows past the end of the sequence must be masked in every block
@@ -262,7 +326,7 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     for (int n = 0; n < count[x] && !*abort_flag; ++n) {
-      const int kv0 = (begin[x] + n) * kBlk;
+      const int block = FIRST && n >= heads ? n + skipped(x) : begin[x] + n, kv0 = block_key(block);
       if (!mbar_wait(&s_full[x], n & 1)) {
         ok = false;
         break;
@@ -276,7 +340,23 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       // Raw scores stay in registers; the softmax scale is folded into the exponent (exp2(s·c − m·c)) and, c being positive, the row
       // maximum is taken on the raw values.  Three-input max and two-wide fp32 arithmetic halve the instruction count of the two
       // passes over the row.
-      if (need_mask) {
+      if constexpr (FIRST) {
+        // One bit per key; chunks that all rows of the warp see whole, most of a diagonal block's, are left alone.  Of a narrow block of first positions the columns behind its end hold what was there
+        // before; no row sees them.
+        if (need_mask) {
+          const bool head = block < heads;
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) {
+            const int k0 = kv0 + ch * 32;
+            uint32_t seen = keys_between(k0, start_row, min(min(kept_end, head ? head_end : 0x7fffffff) - 1, hi_row));
+            if (!head) seen |= keys_between(k0, lo_row, hi_row);
+            if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) sv[ch][i] = (seen >> i) & 1u ? sv[ch][i] : 0xff800000u;  // -inf
+            }
+          }
+        }
+      } else if (need_mask) {
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) {
 #pragma unroll
@@ -400,21 +480,27 @@ static int make_head_map(CUtensorMap* m, const void* base, int b, int s, int hea
                       static_cast<uint64_t>(heads) * D, kBlk, 64, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int D, bool MASKED>
+template <int D>
+static int make_rows_map(CUtensorMap* m, const void* base, int b, int s, int heads) {
+  const uint64_t pitch = static_cast<uint64_t>(heads) * D * 2;
+  return make_tmap_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<uint64_t>(heads) * D, s, b, pitch, pitch * s, 64, kBlk, 1, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int D, bool MASKED, bool FIRST = false>
 static int launch(const void* q, const void* k, const void* v, const Params& p, cudaStream_t st) {
   CUtensorMap tq, tk, tv;
   int rc;
   if ((rc = make_head_map<D>(&tq, q, p.b, p.s, p.hq)) != kOk) return rc;
-  if ((rc = make_head_map<D>(&tk, k, p.b, p.sk, p.hkv)) != kOk) return rc;
-  if ((rc = make_head_map<D>(&tv, v, p.b, p.sk, p.hkv)) != kOk) return rc;
+  if ((rc = FIRST ? make_rows_map<D>(&tk, k, p.b, p.sk, p.hkv) : make_head_map<D>(&tk, k, p.b, p.sk, p.hkv)) != kOk) return rc;
+  if ((rc = FIRST ? make_rows_map<D>(&tv, v, p.b, p.sk, p.hkv) : make_head_map<D>(&tv, v, p.b, p.sk, p.hkv)) != kOk) return rc;
   static bool attr = false;
   if (!attr) {
-    if (cudaFuncSetAttribute(attn_fwd2_kernel<D, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<D>) != cudaSuccess) return kErrDriver;
+    if (cudaFuncSetAttribute(attn_fwd2_kernel<D, MASKED, FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<D>) != cudaSuccess) return kErrDriver;
     attr = true;
   }
   dim3 grid((p.s + 2 * kBlk - 1) / (2 * kBlk), p.hq, p.b);
   TTB_COUNT_LAUNCH(1);
-  attn_fwd2_kernel<D, MASKED><<<grid, kThreads, kSmemBytes<D>, st>>>(tq, tk, tv, p);
+  attn_fwd2_kernel<D, MASKED, FIRST><<<grid, kThreads, kSmemBytes<D>, st>>>(tq, tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrDriver;
 }
 
@@ -433,6 +519,19 @@ extern "C" int ttb_attn_fwd2(const void* q, const void* k, const void* v, void* 
   p.o = static_cast<__nv_bfloat16*>(o), p.lse = lse, p.err = err;
   auto st = static_cast<cudaStream_t>(stream);
   return d == 128 ? fa2::launch<128, false>(q, k, v, p, st) : fa2::launch<64, false>(q, k, v, p, st);
+}
+
+// The same under a causal window of `window` positions (query i at position sk - s + i), beside which the first `sinks` positions stay visible: of the sequence, or (start int32 [b, s], needs
+// s == sk) of the query's document, which begins at its `start`.
+extern "C" int ttb_attn_fwd2_first(const void* q, const void* k, const void* v, void* o, float* lse, const int* start, int window, int sinks, int b, int s, int sk, int hq, int hkv, int d,
+                                   float scale, int* err, void* stream) {
+  using namespace ttb;
+  if ((d != 64 && d != 128) || hkv <= 0 || hq % hkv || s <= 0 || sk < s || b <= 0 || window <= 0 || sinks < 0 || (start != nullptr && s != sk) || sk > (1 << 30)) return kErrBadShape;
+  fa2::Params p{};
+  p.b = b, p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.scale = scale, p.causal = 1, p.window = window < sk ? window : sk, p.sinks = sinks < sk ? sinks : sk, p.start = start;
+  p.o = static_cast<__nv_bfloat16*>(o), p.lse = lse, p.err = err;
+  auto st = static_cast<cudaStream_t>(stream);
+  return d == 128 ? fa2::launch<128, false, true>(q, k, v, p, st) : fa2::launch<64, false, true>(q, k, v, p, st);
 }
 
 // The same under a boolean mask: lo, hi, solid as ttb_mask_bounds gives them (bound_b elements per batch row, 0 = one set for all), the mask as there.
