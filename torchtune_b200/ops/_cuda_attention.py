@@ -179,30 +179,31 @@ class _WindowAttention(torch.autograd.Function):
                 last = torch.empty_like(start)
                 check(lib().ttb_document_bounds(ids.data_ptr(), b, s, window, sinks, start.data_ptr(), last.data_ptr(), stream_ptr()), "document bounds")
             lse = torch.empty(b, hq, s, dtype=torch.float32, device=q.device)
+            rest = torch.empty_like(o) if grads else None  # what rounding the output left over: delta of the backward pass is formed from both
             # the kernel takes the largest score before it is scaled: another sign of the scale (or 0) goes into the queries, which is exact
             queries, positive = (q, scale) if scale > 0 else (-q, -scale) if scale < 0 else (q * 0.0, 1.0)
-            check(lib().ttb_attn_fwd2_first(queries.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), _p(start), window, sinks, b, s, sk, hq, hkv, d, float(positive),
+            check(lib().ttb_attn_fwd2_first(queries.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _p(rest), lse.data_ptr(), _p(start), window, sinks, b, s, sk, hq, hkv, d, float(positive),
                                             err_word(q.device).data_ptr(), stream_ptr()), "attention forward (window)")
         if grads:
-            ctx.save_for_backward(q, k, v, o, lse, last)
+            ctx.save_for_backward(q, k, v, o, rest, lse, last)
             ctx.meta = (window, sinks, scale)
         return o
 
     @staticmethod
     def backward(ctx, d_o):
-        q, k, v, o, lse, last = ctx.saved_tensors
+        q, k, v, o, rest, lse, last = ctx.saved_tensors
         window, sinks, scale = ctx.meta
         b, s, hq, d = q.shape
         sk, hkv = k.shape[1], k.shape[2]
         d_o = d_o.contiguous()
-        q, k, v, o, d_o = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q, k, v, o, d_o))  # handed back by a saved-tensor hook, or a view
+        q, k, v, o, rest, d_o = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q, k, v, o, rest, d_o))  # handed back by a saved-tensor hook, or a view
         with torch.cuda.device(q.device):
             delta = torch.empty(b, hq, s, dtype=torch.float32, device=q.device)
             dq = torch.zeros(b, s, hq, d, dtype=torch.float32, device=q.device)
             dk, dv = torch.empty_like(k), torch.empty_like(v)
             floats = lib().ttb_attn_bwd_first_workspace(window, sinks, int(last is not None), b, s, sk, hkv, d)
             work = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-            check(lib().ttb_attn_bwd_first(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), d_o.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            check(lib().ttb_attn_bwd_first(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.data_ptr(), d_o.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                            _p(last), window, sinks, _p(work), floats, b, s, sk, hq, hkv, d, float(scale), err_word(q.device).data_ptr(), stream_ptr()), "attention backward (window)")
         return dq.to(q.dtype), dk, dv, None, None, None, None
 

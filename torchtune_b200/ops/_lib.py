@@ -169,11 +169,11 @@ def _declare(L: ctypes.CDLL) -> None:
     L.ttb_lightning_chunks.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, i32, vp, vp]
     L.ttb_silu_rows.argtypes = [vp, i64, i64, i32, vp]
     L.ttb_gated_norm.argtypes = [vp, i32, vp, vp, i64, vp, i64, i32, f32, i32, vp]
-    L.ttb_attn_fwd2_first.argtypes = [vp] * 6 + [i32] * 8 + [f32, vp, vp]
+    L.ttb_attn_fwd2_first.argtypes = [vp] * 7 + [i32] * 8 + [f32, vp, vp]
     L.ttb_attn_fwd2_first.restype = i32
     L.ttb_attn_decode_first.argtypes = [vp] * 4 + [i32] * 8 + [f32, vp]
     L.ttb_attn_decode_first.restype = i32
-    L.ttb_attn_bwd_first.argtypes = [vp] * 11 + [i32, i32, vp, i64] + [i32] * 6 + [f32, vp, vp]
+    L.ttb_attn_bwd_first.argtypes = [vp] * 12 + [i32, i32, vp, i64] + [i32] * 6 + [f32, vp, vp]
     L.ttb_attn_bwd_first.restype = i32
     L.ttb_attn_bwd_first_workspace.argtypes = [i32] * 8
     L.ttb_attn_bwd_first_workspace.restype = i64

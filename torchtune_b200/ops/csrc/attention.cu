@@ -374,9 +374,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 // at head dim 128 and 125 us at 64, here 59 and 34 us.  Fewer tokens to a CTA where eight would leave SMs without one (the launcher's rule): a backward pass of 128 tokens, 32 heads of 128, took 38.0 us with
 // eight and takes 33.9 us, one of 512 69.8 and 65.7 us.
 static constexpr int kDeltaTokens = 8;
-template <int D>
+// REST: o comes in two bf16 numbers, the second what the rounding to the first left over.  dS = P (dP - delta) is small beside its two terms where a query sees few keys, and the rounding of o then is
+// what limits the gradients of queries and keys (relative errors at windows of 200 tokens of 64 channels: 0.0026 without it, 0.0024 with it).
+template <int D, bool REST>
 __global__ void __launch_bounds__(256)
-attn_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ d_o, float* __restrict__ delta, long long tokens, int s, int hq, int log_per, bool staged) {
+attn_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ rest, const __nv_bfloat16* __restrict__ d_o, float* __restrict__ delta, long long tokens, int s, int hq, int log_per, bool staged) {
   extern __shared__ float sums[];  // [hq][2^log_per], a column for each token; without `staged`, for more heads than fit, results leave one by one
   constexpr int kLanes = D / 8, kItems = 256 / kLanes;
   const int per = 1 << log_per;
@@ -385,13 +387,15 @@ attn_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __re
   const int lane = threadIdx.x % kLanes;
   const uint4* po = reinterpret_cast<const uint4*>(o + tok0 * hq * D) + lane;
   const uint4* pd = reinterpret_cast<const uint4*>(d_o + tok0 * hq * D) + lane;
+  const uint4* pr = REST ? reinterpret_cast<const uint4*>(rest + tok0 * hq * D) + lane : nullptr;
   for (int first = threadIdx.x / kLanes; first < (count + 4 * kItems - 1) / (4 * kItems) * (4 * kItems); first += 4 * kItems) {
-    uint4 a[4], g[4];
+    uint4 a[4], g[4], r[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int item = first + j * kItems;
       a[j] = item < count ? __ldg(po + item * kLanes) : make_uint4(0, 0, 0, 0);
       g[j] = item < count ? __ldg(pd + item * kLanes) : make_uint4(0, 0, 0, 0);
+      if (REST) r[j] = item < count ? __ldg(pr + item * kLanes) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -400,7 +404,12 @@ attn_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __re
       float acc = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 u = __bfloat1622float2(x[i]), v = __bfloat1622float2(y[i]);
+        float2 u = __bfloat1622float2(x[i]);
+        const float2 v = __bfloat1622float2(y[i]);
+        if (REST) {
+          const float2 w = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&r[j])[i]);
+          u.x += w.x, u.y += w.y;
+        }
         acc += u.x * v.x + u.y * v.y;
       }
 #pragma unroll
@@ -778,9 +787,9 @@ extern "C" int ttb_attn_fwd(const void* q, const void* k, const void* v, void* o
 }
 
 // delta of the backward pass: rowsum(dO o O) per token and head
-static int launch_delta(const void* o, const void* d_o, float* delta, int b, int s, int hq, int d, cudaStream_t st) {
+static int launch_delta(const void* o, const void* rest, const void* d_o, float* delta, int b, int s, int hq, int d, cudaStream_t st) {
   const long long tokens = static_cast<long long>(b) * s;
-  if ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(d_o)) & 15) return kErrBadShape;  // both are read 16 bytes at a time
+  if ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(rest) | reinterpret_cast<uintptr_t>(d_o)) & 15) return kErrBadShape;  // they are read 16 bytes at a time
   int log_per = 3;
   static_assert(kDeltaTokens == 1 << 3, "eight tokens, halved below");
   while (log_per > 0 && (tokens >> log_per) < sm_count()) --log_per;
@@ -788,8 +797,9 @@ static int launch_delta(const void* o, const void* d_o, float* delta, int b, int
   const bool staged = hq <= 48 * 1024 / (per * 4);
   const int smem = staged ? hq * per * 4 : 0;
   TTB_COUNT_LAUNCH(1);
-  auto delta_kernel = d == 128 ? attn_delta_kernel<128> : attn_delta_kernel<64>;
-  delta_kernel<<<static_cast<unsigned>((tokens + per - 1) / per), 256, smem, st>>>(static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(d_o), delta, tokens, s, hq, log_per, staged);
+  auto delta_kernel = rest != nullptr ? (d == 128 ? attn_delta_kernel<128, true> : attn_delta_kernel<64, true>) : (d == 128 ? attn_delta_kernel<128, false> : attn_delta_kernel<64, false>);
+  delta_kernel<<<static_cast<unsigned>((tokens + per - 1) / per), 256, smem, st>>>(static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(rest),
+                                                                                             static_cast<const __nv_bfloat16*>(d_o), delta, tokens, s, hq, log_per, staged);
   return kOk;
 }
 
@@ -805,7 +815,7 @@ extern "C" int ttb_attn_bwd(const void* q, const void* k, const void* v, const v
   if ((d != 64 && d != 128) || hq % hkv || s <= 0 || sk <= 0) return kErrBadShape;
   if (causal && hi == nullptr && s != sk) return kErrBadShape;
   auto st = static_cast<cudaStream_t>(stream);
-  const int rc = launch_delta(o, d_o, delta, b, s, hq, d, st);
+  const int rc = launch_delta(o, nullptr, d_o, delta, b, s, hq, d, st);
   if (rc != kOk) return rc;
   AttnParams p{};
   p.b = b, p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.d = d, p.scale = scale, p.causal = causal, p.lo = lo, p.hi = hi;
@@ -820,10 +830,10 @@ int ttb_attn_bwd2_first(const void* q, const void* k, const void* v, const void*
                         float* work, long long work_floats, int b, int s, int sk, int hq, int hkv, int d, float scale, int* err, cudaStream_t stream);
 
 // Backward of ttb_attn_fwd2_first: tensors as in ttb_attn_bwd; last (with documents, else nullptr) as ttb_document_bounds gives it; work: as many fp32 numbers as ttb_attn_bwd_first_workspace says.
-extern "C" int ttb_attn_bwd_first(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse, float* delta, float* dq_accum, void* dk, void* dv, const int* last,
+extern "C" int ttb_attn_bwd_first(const void* q, const void* k, const void* v, const void* o, const void* rest, const void* d_o, const float* lse, float* delta, float* dq_accum, void* dk, void* dv, const int* last,
                                   int window, int sinks, float* work, long long work_floats, int b, int s, int sk, int hq, int hkv, int d, float scale, int* err, void* stream) {
   if ((d != 64 && d != 128) || hkv <= 0 || hq % hkv || s <= 0 || sk < s || b <= 0 || window <= 0 || sinks < 0 || (last != nullptr && s != sk) || sk > (1 << 30)) return kErrBadShape;
   auto st = static_cast<cudaStream_t>(stream);
-  const int rc = launch_delta(o, d_o, delta, b, s, hq, d, st);
+  const int rc = launch_delta(o, rest, d_o, delta, b, s, hq, d, st);
   return rc != kOk ? rc : ttb_attn_bwd2_first(q, k, v, d_o, lse, delta, dq_accum, dk, dv, last, window, sinks, work, work_floats, b, s, sk, hq, hkv, d, scale, err, st);
 }

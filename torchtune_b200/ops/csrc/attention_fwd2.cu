@@ -44,6 +44,7 @@ struct Params {
   // FIRST: a causal window of `window` positions, query i at position sk - s + i, beside which the first `sinks` positions of the sequence, or of the query's document, stay visible
   int window, sinks;
   const int* start;  // [b, s] first position of each query's document (s == sk), or nullptr
+  __nv_bfloat16* rest;  // like o, or nullptr: what rounding o to bf16 left over, for the backward pass
   __nv_bfloat16* o;
   float* lse;
   int* err;
@@ -461,6 +462,14 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             u.z = pack_bf16x2(__uint_as_float(v[g * 8 + 4]) * inv_l, __uint_as_float(v[g * 8 + 5]) * inv_l);
             u.w = pack_bf16x2(__uint_as_float(v[g * 8 + 6]) * inv_l, __uint_as_float(v[g * 8 + 7]) * inv_l);
             *reinterpret_cast<uint4*>(orow + ch * 32 + g * 8) = u;
+            if constexpr (FIRST) {
+              if (p.rest != nullptr) {
+                auto left = [&](uint32_t w, int i) {
+                  return pack_bf16x2(__uint_as_float(v[i]) * inv_l - __uint_as_float(w << 16), __uint_as_float(v[i + 1]) * inv_l - __uint_as_float(w & 0xffff0000u));
+                };
+                *reinterpret_cast<uint4*>(p.rest + (orow - p.o) + ch * 32 + g * 8) = make_uint4(left(u.x, g * 8), left(u.y, g * 8 + 2), left(u.z, g * 8 + 4), left(u.w, g * 8 + 6));
+              }
+            }
           }
         }
       }
@@ -522,13 +531,14 @@ extern "C" int ttb_attn_fwd2(const void* q, const void* k, const void* v, void* 
 }
 
 // The same under a causal window of `window` positions (query i at position sk - s + i), beside which the first `sinks` positions stay visible: of the sequence, or (start int32 [b, s], needs
-// s == sk) of the query's document, which begins at its `start`.
-extern "C" int ttb_attn_fwd2_first(const void* q, const void* k, const void* v, void* o, float* lse, const int* start, int window, int sinks, int b, int s, int sk, int hq, int hkv, int d,
+// s == sk) of the query's document, which begins at its `start`.  rest (nullable): like o, what its rounding left over.
+extern "C" int ttb_attn_fwd2_first(const void* q, const void* k, const void* v, void* o, void* rest, float* lse, const int* start, int window, int sinks, int b, int s, int sk, int hq, int hkv, int d,
                                    float scale, int* err, void* stream) {
   using namespace ttb;
   if ((d != 64 && d != 128) || hkv <= 0 || hq % hkv || s <= 0 || sk < s || b <= 0 || window <= 0 || sinks < 0 || (start != nullptr && s != sk) || sk > (1 << 30)) return kErrBadShape;
   fa2::Params p{};
   p.b = b, p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.scale = scale, p.causal = 1, p.window = window < sk ? window : sk, p.sinks = sinks < sk ? sinks : sk, p.start = start;
+  p.rest = static_cast<__nv_bfloat16*>(rest);
   p.o = static_cast<__nv_bfloat16*>(o), p.lse = lse, p.err = err;
   auto st = static_cast<cudaStream_t>(stream);
   return d == 128 ? fa2::launch<128, false, true>(q, k, v, p, st) : fa2::launch<64, false, true>(q, k, v, p, st);
