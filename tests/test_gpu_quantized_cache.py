@@ -351,3 +351,29 @@ def test_a_decode_step_attends_to_what_the_cache_stands_for():
     assert attn.kv_cache.size == 150 and not attn.kv_cache.k_scales[:, :, 150:].any()
     # values rounded to bf16 on the way (2^-9 of each) and 150 of them averaged; the projection adds its own rounding to both sides
     assert (got.float() - want.float()).norm() <= 2.0**-6 * want.float().norm()
+
+
+def test_every_quotient_of_two_bf16_numbers():
+    """All pairs of significands, at several exponents apart: the codes are those of exact division, ties included."""
+    sig = torch.arange(128, 256, device="cuda", dtype=torch.float64)
+    for bits in (4, 8):
+        half = 2 ** (bits - 1)
+        for shift in range(0, bits + 2):
+            # a group per divisor: the largest value, then 31 dividends at a time
+            largest = sig * 2.0**-3
+            for sign in (1.0, -1.0):
+                rows = []
+                for start in range(0, 128, 31):
+                    part = sig[start : start + 31] * 2.0 ** (-3 - shift)
+                    part = torch.nn.functional.pad(part, (0, 31 - part.shape[0]))
+                    group = torch.cat([largest[:, None] * sign, part[None, :].expand(128, -1)], 1)
+                    group[group.abs() > group[:, :1].abs()] = 0.0  # the first one has to be the largest
+                    rows.append(group)
+                x = torch.cat(rows)[None, :, None, :].to(torch.bfloat16)
+                cache = _zeros(1, x.shape[1], 1, 32, bits)
+                ops.quantized_append(x, x, *cache, torch.arange(x.shape[1], device="cuda"))
+                got = ops.quantized_read(*cache, dtype=torch.float32)[0][0, :, 0].double()
+                wide = x[0, :, 0].double()
+                step = wide[:, :1] / -half
+                want = (wide / step).round().clamp(-half, half - 1) * step
+                assert torch.equal(got, want)

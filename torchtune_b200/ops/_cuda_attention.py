@@ -168,7 +168,7 @@ class _WindowAttention(torch.autograd.Function):
         o = torch.empty_like(q)
         grads = any(ctx.needs_input_grad)
         with torch.cuda.device(q.device):
-            if not grads and doc_ids is None and decodes(s, sk, hq, hkv):
+            if not grads and doc_ids is None and decodes(s, min(sk, window + sinks + s + 192), hq, hkv):  # what it visits, and the rest of its blocks
                 check(lib().ttb_attn_decode_first(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), window, sinks, b, s, sk, hq, hkv, d, float(scale), stream_ptr()),
                       "attention of few queries (window)")
                 return o

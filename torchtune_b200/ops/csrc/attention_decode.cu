@@ -43,7 +43,8 @@ struct Params {
   long long mask_b, mask_r;
   const int* lo;           // [b, s] first / last visible key, or nullptr (0 / sk - 1)
   const int* hi;
-  int window, sinks;       // window > 0: query i is position sk - s + i and sees the last `window` positions up to its own and the first `sinks`
+  // FIRST: query i is position sk - s + i and sees the last `window` positions up to its own and the first `sinks`; blocks skip_from ... skip_from + skipped - 1 lie between the two
+  int window, sinks, skip_from, skipped;
   int s, sk, hq, hkv;
   float scale;
   // APPEND: one query per row; q is still to be rotated, and the new key (to be rotated as well) and value go to slot slots[0] of the caches k and v first
@@ -84,7 +85,7 @@ struct Layout {
 // grid (splits = cluster, key heads, batch)
 // With APPEND the step between the projections and the cache, a launch of 2 - 5 us that moved a few KB, happens here: the queries are rotated into shared memory, and the CTA whose
 // blocks hold the new slot writes the cache before it reads.
-template <int D, bool APPEND>
+template <int D, bool APPEND, bool FIRST>
 __global__ void __launch_bounds__(kWarps * 32)
 decode_kernel(Params p) {
   using L = Layout<D>;
@@ -94,14 +95,18 @@ decode_kernel(Params p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x, splits = gridDim.x, hk = blockIdx.y, bi = blockIdx.z;
   const int group = p.hq / p.hkv, rows = p.s * group;
-  const int blocks = (p.sk + kKeys - 1) / kKeys;
+  const int blocks = (p.sk + kKeys - 1) / kKeys - (FIRST ? p.skipped : 0);
+  auto first_key = [&](int i) {  // of own block i
+    const int block = split + i * splits;
+    return (FIRST && block >= p.skip_from ? block + p.skipped : block) * kKeys;
+  };
   const int own = blocks > split ? (blocks - split + splits - 1) / splits : 0;
   const int words = p.s + 1;
 
   // Which keys of the own blocks each query sees, one bit per key.
   for (int w = warp; w < own * p.s; w += kWarps) {
     const int i = w / p.s, qi = w % p.s;
-    const int j0 = (split + i * splits) * kKeys;
+    const int j0 = first_key(i);
     const long long row = static_cast<long long>(bi) * p.s + qi;
     const int lo = p.lo != nullptr ? p.lo[row] : 0, hi = p.hi != nullptr ? p.hi[row] : p.sk - 1;
     uint32_t half[2];
@@ -109,7 +114,7 @@ decode_kernel(Params p) {
     for (int x = 0; x < 2; ++x) {
       const int j = j0 + x * 32 + lane;
       bool seen = j < p.sk && j >= lo && j <= hi;
-      if (p.window > 0) {
+      if constexpr (FIRST) {
         const int at = p.sk - p.s + qi;
         seen = seen && j <= at && (at - j < p.window || j < p.sinks);
       }
@@ -189,7 +194,7 @@ decode_kernel(Params p) {
   constexpr int kChunks = D / 8;  // 16-byte chunks of a key
   auto load = [&](int i, int stage) {
     if (i < own) {
-      const int j0 = (split + i * splits) * kKeys + shift;
+      const int j0 = first_key(i) + shift;
       const uint32_t any = static_cast<uint32_t>(bits[i * words + p.s] >> shift) & 0xffffu;
 #pragma unroll
       for (int c = lane; c < 16 * kChunks; c += 32) {
@@ -341,9 +346,9 @@ decode_kernel(Params p) {
   cluster.sync();  // no CTA leaves while another reads its shared memory
 }
 
-template <int D, bool APPEND>
+template <int D, bool APPEND, bool FIRST = false>
 static int launch(const Params& p, int b, cudaStream_t st) {
-  const int blocks = (p.sk + kKeys - 1) / kKeys;
+  const int blocks = (p.sk + kKeys - 1) / kKeys - (FIRST ? p.skipped : 0);
   int splits = 1;  // fill the SMs twice over as long as every CTA has a block of its own
   while (splits < kMaxSplit && static_cast<long long>(b) * p.hkv * splits < 2ll * sm_count() && blocks >= 2 * splits) splits *= 2;
   const int own = (blocks + splits - 1) / splits;
@@ -353,7 +358,7 @@ static int launch(const Params& p, int b, cudaStream_t st) {
   const int smem = fixed + static_cast<int>(bit_bytes);
   static bool attr = false;
   if (!attr) {
-    if (cudaFuncSetAttribute(decode_kernel<D, APPEND>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + kMaxBitBytes) != cudaSuccess) return kErrDriver;
+    if (cudaFuncSetAttribute(decode_kernel<D, APPEND, FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + kMaxBitBytes) != cudaSuccess) return kErrDriver;
     attr = true;
   }
   cudaLaunchConfig_t cfg = {};
@@ -366,7 +371,7 @@ static int launch(const Params& p, int b, cudaStream_t st) {
   at[0].val.clusterDim.x = splits, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
   cfg.attrs = at, cfg.numAttrs = 1;
   TTB_COUNT_LAUNCH(1);
-  return cudaLaunchKernelEx(&cfg, decode_kernel<D, APPEND>, p) == cudaSuccess ? kOk : kErrDriver;
+  return cudaLaunchKernelEx(&cfg, decode_kernel<D, APPEND, FIRST>, p) == cudaSuccess ? kOk : kErrDriver;
 }
 
 // First and last visible key of every mask row and whether all keys between them are visible; one warp per row, 16 bytes per lane and
@@ -480,9 +485,12 @@ extern "C" int ttb_attn_decode_first(const void* q, const void* k, const void* v
     if (reinterpret_cast<uintptr_t>(t) & 15) return kErrBadShape;
   dec::Params p{};
   p.q = static_cast<const __nv_bfloat16*>(q), p.k = static_cast<const __nv_bfloat16*>(k), p.v = static_cast<const __nv_bfloat16*>(v), p.o = static_cast<__nv_bfloat16*>(o);
-  p.window = window, p.sinks = sinks, p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.scale = scale;
+  p.window = window < sk ? window : sk, p.sinks = sinks < sk ? sinks : sk, p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.scale = scale;
+  const int from = (p.sinks + dec::kKeys - 1) / dec::kKeys, to = (sk - s - p.window + 1 > 0 ? sk - s - p.window + 1 : 0) / dec::kKeys;  // the first query's window begins first
+  p.skip_from = 0x7fffffff;
+  if (to > from) p.skip_from = from, p.skipped = to - from;
   auto st = static_cast<cudaStream_t>(stream);
-  return d == 128 ? dec::launch<128, false>(p, b, st) : dec::launch<64, false>(p, b, st);
+  return d == 128 ? dec::launch<128, false, true>(p, b, st) : dec::launch<64, false, true>(p, b, st);
 }
 
 // ttb_rope_append for one token per row followed by ttb_attn_decode on the caches, in one launch and with the same values: q, o [b, hq, d], k, v [b, hkv, d] before the rotation, caches [b, max_seq,

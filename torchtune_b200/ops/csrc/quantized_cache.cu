@@ -47,108 +47,186 @@ struct ReadParams {
 __device__ __forceinline__ float widened(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float widened(__half x) { return __half2float(x); }
 __device__ __forceinline__ float widened(float x) { return x; }
+template <typename T>
+static constexpr bool kHalfPrecision = false;
+template <>
+constexpr bool kHalfPrecision<__half> = true;
 
-// grid (units / 256, batch, keys and values), 4 threads per group: thread t has run t of it.
-template <int BITS, typename T, bool WIDE>
-__global__ void __launch_bounds__(kThreads) append_kernel(AppendParams p, int groups) {
-  constexpr int kHalf = 1 << (BITS - 1);
-  const int which = blockIdx.z, bi = blockIdx.y;
-  const long long unit = static_cast<long long>(blockIdx.x) * (kThreads / 4) + (threadIdx.x >> 2);
-  const int t = threadIdx.x & 3;
-  const bool live = unit < static_cast<long long>(p.s) * p.h * groups;
-  const long long at = live ? unit : 0;
-  const int j = static_cast<int>(at % groups);
-  const long long row = at / groups;
-  const int head = static_cast<int>(row % p.h), i = static_cast<int>(row / p.h);
-  const int run = t * groups + j;  // runs of eight channels
-  const T* x = static_cast<const T*>(p.x[which]) + bi * p.x_b[which] + i * p.x_s[which] + head * p.x_h[which] + run * 8;
-  T from[8];
-  if (WIDE) {
-#pragma unroll
-    for (int e = 0; e < static_cast<int>(sizeof(T)) / 2; ++e) reinterpret_cast<uint4*>(from)[e] = reinterpret_cast<const uint4*>(x)[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) from[e] = x[e];
-  }
-  float v[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = widened(from[e]);
-  // The value of largest magnitude (its bits; NaN is above infinity), then the first channel that has it, with its sign.
-  uint32_t top = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  uint32_t place = 0xffffffffu;
-#pragma unroll
-  for (int e = 7; e >= 0; --e)
-    if ((__float_as_uint(v[e]) & 0x7fffffffu) == top) place = static_cast<uint32_t>(t * 8 + e) << 1 | __float_as_uint(v[e]) >> 31;
-  place = min(place, __shfl_xor_sync(0xffffffffu, place, 1));
-  place = min(place, __shfl_xor_sync(0xffffffffu, place, 2));
-  const float m = __uint_as_float(top | place << 31);
-  const __nv_bfloat16 scale = __float2bfloat16_rn(m * (-1.f / kHalf));
-  const float s = __bfloat162float(scale);
-  const bool usable = s != 0.f && fabsf(s) <= 3.4e38f;
-  uint32_t code[2] = {0u, 0u};  // 4 bits: one word; 8 bits: two
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    int c = usable ? __float2int_rn(__fdiv_rn(v[e], s)) : 0;
-    c = min(max(c, -kHalf), kHalf - 1) + kHalf;
-    if (BITS == 4)
-      code[0] |= static_cast<uint32_t>(c) << (4 * e);
-    else
-      code[e >> 2] |= static_cast<uint32_t>(c) << (8 * (e & 3));
-  }
-  if (!live) return;
-  // Tokens take consecutive slots, so that no two of them meet in one: anything else, and what does not fit, is counted and not written.
-  const long long slot = p.slots[0] + i;
-  if (slot < 0 || slot >= p.slot_count || p.slots[i] != slot) {
-    if (t == 0 && j == 0 && head == 0 && which == 0) TTB_NOTE_VIOLATION(quantized);
-    return;
-  }
-  const Rows& to = p.to[which];
-  uint8_t* codes = to.codes + bi * to.codes_b + head * to.codes_h + slot * to.codes_s + run * BITS;
-  if (BITS == 4)
-    *reinterpret_cast<uint32_t*>(codes) = code[0];
-  else
-    *reinterpret_cast<uint2*>(codes) = make_uint2(code[0], code[1]);
-  if (t == 0) *reinterpret_cast<__nv_bfloat16*>(to.scales + bi * to.scales_b + head * to.scales_h + slot * to.scales_s + j * 2) = scale;
+// How a CTA's threads lie over the rows of a token and several tokens: `lanes` units (a quad of threads for a group when writing, a thread for eight channels when reading) have one token each, `sub`
+// tokens at a time; a thread goes through kRun tokens, `sub` apart, with its addresses moving by constants.  grid (runs of tokens, parts of a token, 2 * batch: keys and values)
+static constexpr int kRun = 4;
+struct Spread {
+  int units, lanes, sub;
+};
+static Spread spread_of(long long units, int per_cta) {
+  Spread sp;
+  sp.units = static_cast<int>(units), sp.lanes = static_cast<int>(units < per_cta ? units : per_cta), sp.sub = per_cta / sp.lanes;
+  return sp;
 }
 
-// grid (units / 256, batch, keys and values); a thread has eight channels of one row.  bf16 results are rounded once, fp32 ones are exact.
-template <int BITS, typename T>
-__global__ void __launch_bounds__(kThreads) read_kernel(ReadParams p, int groups) {
+// The largest and the smallest of three; a NaN stays.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// A quad of threads per group: thread t has run t of it.
+template <int BITS, typename T, bool WIDE, int GROUPS>
+__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendParams p, const __grid_constant__ Spread sp, int some_groups) {
   constexpr int kHalf = 1 << (BITS - 1);
-  const int which = blockIdx.z, bi = blockIdx.y;
-  const int runs = 4 * groups;
-  const long long unit = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
-  if (unit >= static_cast<long long>(p.n) * p.h * runs) return;
-  const int run = static_cast<int>(unit % runs);
-  const long long row = unit / runs;
-  const int head = static_cast<int>(row % p.h), i = static_cast<int>(row / p.h);
-  const Rows& from = p.from[which];
-  const long long slot = p.first + i;
-  const uint8_t* codes = from.codes + bi * from.codes_b + head * from.codes_h + slot * from.codes_s + run * BITS;
-  const float s = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(from.scales + bi * from.scales_b + head * from.scales_h + slot * from.scales_s + (run % groups) * 2));
-  uint32_t w[2];
-  if (BITS == 4) {
-    w[0] = *reinterpret_cast<const uint32_t*>(codes);
-  } else {
-    const uint2 u = *reinterpret_cast<const uint2*>(codes);
-    w[0] = u.x, w[1] = u.y;
-  }
-  float v[8];
+  const int groups = GROUPS > 0 ? GROUPS : some_groups;
+  const int which = blockIdx.z & 1, bi = blockIdx.z >> 1;
+  const int lane = threadIdx.x & 31, t = lane & 3, quad = threadIdx.x >> 2;
+  const int sub = quad / sp.lanes, unit = blockIdx.y * sp.lanes + (quad - sub * sp.lanes);
+  const bool live = sub < sp.sub && unit < sp.units;
+  const int head = live ? unit / groups : 0, j = live ? unit - head * groups : 0;
+  const int run = t * groups + j;  // runs of eight channels
+  const int i0 = blockIdx.x * (kRun * sp.sub) + sub;
+  const long long first = p.slots[0];
+  const T* row = static_cast<const T*>(p.x[which]) + bi * p.x_b[which] + head * p.x_h[which] + run * 8 + (live && i0 < p.s ? i0 : 0) * p.x_s[which];
+  const long long step = sp.sub * p.x_s[which];
+  T from[kRun][8];
+  bool ours[kRun];  // whether a token takes the slot behind the one before it
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t c = BITS == 4 ? w[0] >> (4 * e) & 15u : w[e >> 2] >> (8 * (e & 3)) & 255u;
-    v[e] = static_cast<float>(static_cast<int>(c) - kHalf) * s;
+  for (int k = 0; k < kRun; ++k) {
+    const int i = i0 + k * sp.sub;
+    const bool there = live && i < p.s;
+    ours[k] = there && p.slots[i] == first + i && first + i >= 0 && first + i < p.slot_count;
+    if (k > 0 && there) row += step;
+    if (WIDE) {
+#pragma unroll
+      for (int e = 0; e < static_cast<int>(sizeof(T)) / 2; ++e) reinterpret_cast<uint4*>(from[k])[e] = reinterpret_cast<const uint4*>(row)[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) from[k][e] = row[e];
+    }
   }
-  T* y = static_cast<T*>(p.y[which]) + ((static_cast<long long>(bi) * p.n + i) * p.h + head) * (runs * 8) + run * 8;
-  if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<uint4*>(y) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-  } else {
-    *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(y + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  const Rows& to = p.to[which];
+  uint8_t* codes = to.codes + bi * to.codes_b + head * to.codes_h + run * BITS + (first + i0) * to.codes_s;
+  uint8_t* scales = to.scales + bi * to.scales_b + head * to.scales_h + j * 2 + (first + i0) * to.scales_s;
+  const long long codes_step = sp.sub * to.codes_s, scales_step = sp.sub * to.scales_s;
+#pragma unroll
+  for (int k = 0; k < kRun; ++k) {
+    if (static_cast<int>(blockIdx.x) * (kRun * sp.sub) + k * sp.sub >= p.s) break;  // for the whole CTA
+    const int i = i0 + k * sp.sub;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = widened(from[k][e]);
+    // The value of largest magnitude: the largest or the smallest one, and where they are opposites the one that comes first.
+    float high = max3_nan(max3_nan(v[0], v[1], v[2]), max3_nan(v[3], v[4], v[5]), v[6]), low = min3_nan(min3_nan(v[0], v[1], v[2]), min3_nan(v[3], v[4], v[5]), v[6]);
+    high = max3_nan(high, v[7], v[7]), low = min3_nan(low, v[7], v[7]);
+    const float h1 = __shfl_xor_sync(0xffffffffu, high, 1), l1 = __shfl_xor_sync(0xffffffffu, low, 1);
+    high = max3_nan(high, h1, h1), low = min3_nan(low, l1, l1);
+    const float h2 = __shfl_xor_sync(0xffffffffu, high, 2), l2 = __shfl_xor_sync(0xffffffffu, low, 2);
+    high = max3_nan(high, h2, h2), low = min3_nan(low, l2, l2);
+    float m = high > -low ? high : low;
+    if (__any_sync(0xffffffffu, high == -low)) {
+      float own = 0.f;  // the first of this thread's channels that has the magnitude
+      bool has = false;
+#pragma unroll
+      for (int e = 7; e >= 0; --e)
+        if (fabsf(v[e]) == high) own = v[e], has = true;
+      const uint32_t with = __ballot_sync(0xffffffffu, has) >> (lane & 28) & 15u;
+      own = __shfl_sync(0xffffffffu, own, (lane & 28) + (with != 0u ? __ffs(with) - 1 : 0));
+      if (high == -low) m = own;
+    }
+    const __nv_bfloat16 scale = __float2bfloat16_rn(m * (-1.f / kHalf));
+    const float s = __bfloat162float(scale);
+    const bool usable = s != 0.f && fabsf(s) <= 3.4e38f;
+    uint32_t code[2] = {0u, 0u};  // 4 bits: one word; 8 bits: two
+    auto put = [&](int e, uint32_t c) {
+      constexpr int kPer = 32 / BITS;
+      asm("mad.lo.u32 %0, %1, %2, %0;" : "+r"(code[e / kPer]) : "r"(c), "r"(1u << (BITS * (e % kPer))));  // the integer unit is what bounds this kernel; this is not on it
+    };
+    if (sizeof(T) == 2 && !kHalfPrecision<T> && fabsf(s) >= 1e-30f && usable) {
+      // bf16: a quotient is a tie or at least 2^-9 away from one (see above).  The product with the reciprocal (off by at most 2^-22 of itself) is off by at most 2^-15, so that on a grid of 2^-10 it lies on the same side, and a tie
+      // on itself; the last sum rounds it to a whole number, ties to even, and leaves that in the low bits.  A tenth of the instructions of a division.
+      float inv;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float grid = __fadd_rn(__fmaf_rn(v[e], inv, 12288.f), -12288.f);  // 1.5 x 2^13
+        const uint32_t c = __float_as_uint(__fadd_rn(grid, 12582912.f + kHalf)) - 0x4b400000u;  // 1.5 x 2^23
+        put(e, min(c, 2u * kHalf - 1u));  // no quotient is below -h: m itself gives that
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = usable ? __float2int_rn(__fdiv_rn(v[e], s)) : 0;
+        put(e, static_cast<uint32_t>(min(max(c, -kHalf), kHalf - 1) + kHalf));
+      }
+    }
+    // Tokens take consecutive slots, so that no two of them meet in one: anything else, and what does not fit, is counted and not written.
+    if (ours[k]) {
+      if (BITS == 4)
+        *reinterpret_cast<uint32_t*>(codes) = code[0];
+      else
+        *reinterpret_cast<uint2*>(codes) = make_uint2(code[0], code[1]);
+      if (t == 0) *reinterpret_cast<__nv_bfloat16*>(scales) = scale;
+    } else if (live && i < p.s && t == 0 && unit == 0 && which == 0) {
+      TTB_NOTE_VIOLATION(quantized);
+    }
+    codes += codes_step, scales += scales_step;
+  }
+}
+
+// A thread has eight channels of a row.  bf16 results are rounded once, fp32 ones are exact.
+template <int BITS, typename T, int GROUPS>
+__global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadParams p, const __grid_constant__ Spread sp, int some_groups) {
+  constexpr float kHalf = 1 << (BITS - 1);
+  const int groups = GROUPS > 0 ? GROUPS : some_groups;
+  const int which = blockIdx.z & 1, bi = blockIdx.z >> 1;
+  const int sub = threadIdx.x / sp.lanes, unit = blockIdx.y * sp.lanes + (threadIdx.x - sub * sp.lanes);
+  if (sub >= sp.sub || unit >= sp.units) return;
+  const int runs = 4 * groups, head = unit / runs, run = unit - head * runs;
+  const int i0 = blockIdx.x * (kRun * sp.sub) + sub;
+  const Rows& from = p.from[which];
+  const uint8_t* codes = from.codes + bi * from.codes_b + head * from.codes_h + run * BITS + static_cast<long long>(p.first) * from.codes_s;
+  const uint8_t* scales = from.scales + bi * from.scales_b + head * from.scales_h + (run % groups) * 2 + static_cast<long long>(p.first) * from.scales_s;
+  uint32_t w[kRun][2];
+  float s[kRun];
+#pragma unroll
+  for (int k = 0; k < kRun; ++k) {
+    const long long i = min(i0 + k * sp.sub, p.n - 1);
+    const uint8_t* at = codes + i * from.codes_s;
+    if (BITS == 4) {
+      w[k][0] = *reinterpret_cast<const uint32_t*>(at);
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(at);
+      w[k][0] = u.x, w[k][1] = u.y;
+    }
+    s[k] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(scales + i * from.scales_s));
+  }
+  T* y = static_cast<T*>(p.y[which]) + static_cast<long long>(bi) * p.n * sp.units * 8 + unit * 8;
+#pragma unroll
+  for (int k = 0; k < kRun; ++k) {
+    const int i = i0 + k * sp.sub;
+    if (i >= p.n) return;
+    float v[8];
+    // 2^23 + (code << n) is exact, and so is the sum that leaves code - h of it
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (BITS == 4) {
+        const uint32_t part = e < 4 ? w[k][0] : w[k][0] >> 16;
+        const int n = 4 * (e & 3);
+        v[e] = fmaf(__uint_as_float(0x4b000000u | (part & (15u << n))), 1.f / (1 << n), -(8388608.f / (1 << n) + kHalf)) * s[k];
+      } else {
+        v[e] = (__uint_as_float(0x4b000000u | (w[k][e >> 2] >> (8 * (e & 3)) & 255u)) - (8388608.f + kHalf)) * s[k];
+      }
+    }
+    T* to = y + static_cast<long long>(i) * sp.units * 8;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    } else {
+      *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    }
   }
 }
 
@@ -163,14 +241,37 @@ static bool aligned(const Rows& r) {  // eight codes are one access
   return ((reinterpret_cast<uintptr_t>(r.codes) | r.codes_b | r.codes_h | r.codes_s) & 7) == 0 && (reinterpret_cast<uintptr_t>(r.scales) & 1) == 0;
 }
 
+// Tokens and parts of a token as a grid; 0 CTAs where a dimension is too large.
+static dim3 grid_of(const Spread& sp, long long tokens, int b) {
+  const long long runs = (tokens + kRun * sp.sub - 1) / (kRun * sp.sub), parts = (sp.units + sp.lanes - 1) / sp.lanes;
+  return runs > 0x7fffffff - kRun || parts > 65535 || 2ll * b > 65535 ? dim3(0) : dim3(static_cast<unsigned>(runs), static_cast<unsigned>(parts), 2u * b);
+}
+
+template <typename T, int GROUPS>
+static void append_of(const AppendParams& p, const Spread& sp, bool wide, dim3 grid, int groups, int bits, cudaStream_t st) {
+  auto kern = bits == 4 ? (wide ? append_kernel<4, T, true, GROUPS> : append_kernel<4, T, false, GROUPS>) : (wide ? append_kernel<8, T, true, GROUPS> : append_kernel<8, T, false, GROUPS>);
+  kern<<<grid, kThreads, 0, st>>>(p, sp, groups);
+}
+
 template <typename T>
 static int launch_append(const AppendParams& p, bool wide, int b, int groups, int bits, cudaStream_t st) {
-  const long long blocks = (static_cast<long long>(p.s) * p.h * groups + kThreads / 4 - 1) / (kThreads / 4);
-  if (blocks > 0x7fffffff) return kErrTooLarge;
-  auto kern = bits == 4 ? (wide ? append_kernel<4, T, true> : append_kernel<4, T, false>) : (wide ? append_kernel<8, T, true> : append_kernel<8, T, false>);
+  const Spread sp = spread_of(static_cast<long long>(p.h) * groups, kThreads / 4);
+  const dim3 grid = grid_of(sp, p.s, b);
+  if (grid.x == 0) return kErrTooLarge;
   TTB_COUNT_LAUNCH(1);
-  kern<<<dim3(static_cast<unsigned>(blocks), b, 2), kThreads, 0, st>>>(p, groups);
+  if (groups == 4)
+    append_of<T, 4>(p, sp, wide, grid, groups, bits, st);
+  else if (groups == 2)
+    append_of<T, 2>(p, sp, wide, grid, groups, bits, st);
+  else
+    append_of<T, 0>(p, sp, wide, grid, groups, bits, st);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrDriver;
+}
+
+template <int GROUPS>
+static void read_of(const ReadParams& p, const Spread& sp, dim3 grid, int groups, int bits, int wide, cudaStream_t st) {
+  auto kern = bits == 4 ? (wide ? read_kernel<4, float, GROUPS> : read_kernel<4, __nv_bfloat16, GROUPS>) : (wide ? read_kernel<8, float, GROUPS> : read_kernel<8, __nv_bfloat16, GROUPS>);
+  kern<<<grid, kThreads, 0, st>>>(p, sp, groups);
 }
 
 }  // namespace qkv
@@ -181,7 +282,8 @@ static int launch_append(const AppendParams& p, bool wide, int b, int groups, in
 extern "C" int ttb_quantized_append(const void* k, const void* v, void* k_codes, void* k_scales, void* v_codes, void* v_scales, const long long* strides, const long long* slots, int type, int b,
                                     int s, int h, int d, int bits, int slot_count, void* stream) {
   using namespace ttb;
-  if (b <= 0 || b > 65535 || s <= 0 || h <= 0 || d <= 0 || d % 32 || (bits != 4 && bits != 8) || slot_count <= 0) return kErrBadShape;
+  if (b <= 0 || s <= 0 || s > 0x7fffffff - qkv::kRun * qkv::kThreads || h <= 0 || d <= 0 || d % 32 || static_cast<long long>(h) * d > 0x7fffffff || (bits != 4 && bits != 8) || slot_count <= 0)
+    return kErrBadShape;
   qkv::AppendParams p;
   p.x[0] = k, p.x[1] = v;
   const int per = type == 2 ? 3 : 7;  // elements of 16 bytes, less one
@@ -206,7 +308,7 @@ extern "C" int ttb_quantized_append(const void* k, const void* v, void* k_codes,
 extern "C" int ttb_quantized_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, const long long* strides, void* k, void* v, int b, int first, int n, int h,
                                   int d, int bits, int wide, void* stream) {
   using namespace ttb;
-  if (b <= 0 || b > 65535 || first < 0 || n <= 0 || h <= 0 || d <= 0 || d % 32 || (bits != 4 && bits != 8)) return kErrBadShape;
+  if (b <= 0 || first < 0 || n <= 0 || h <= 0 || d <= 0 || d % 32 || static_cast<long long>(h) * d > 0x7fffffff || (bits != 4 && bits != 8)) return kErrBadShape;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return kErrBadShape;
   qkv::ReadParams p;
   p.from[0] = qkv::rows_of(const_cast<void*>(k_codes), const_cast<void*>(k_scales), strides);
@@ -214,11 +316,16 @@ extern "C" int ttb_quantized_read(const void* k_codes, const void* k_scales, con
   if (!qkv::aligned(p.from[0]) || !qkv::aligned(p.from[1])) return kErrBadShape;
   p.y[0] = k, p.y[1] = v, p.first = first, p.n = n, p.h = h;
   const int groups = d / 32;
-  const long long blocks = (static_cast<long long>(n) * h * groups * 4 + qkv::kThreads - 1) / qkv::kThreads;
-  if (blocks > 0x7fffffff) return kErrTooLarge;
-  const dim3 grid(static_cast<unsigned>(blocks), b, 2);
-  auto kern = bits == 4 ? (wide ? qkv::read_kernel<4, float> : qkv::read_kernel<4, __nv_bfloat16>) : (wide ? qkv::read_kernel<8, float> : qkv::read_kernel<8, __nv_bfloat16>);
+  const qkv::Spread sp = qkv::spread_of(static_cast<long long>(h) * groups * 4, qkv::kThreads);
+  const dim3 grid = qkv::grid_of(sp, n, b);
+  if (grid.x == 0 || n > 0x7fffffff - qkv::kRun * qkv::kThreads) return kErrTooLarge;
+  auto st = static_cast<cudaStream_t>(stream);
   TTB_COUNT_LAUNCH(1);
-  kern<<<grid, qkv::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, groups);
+  if (groups == 4)
+    qkv::read_of<4>(p, sp, grid, groups, bits, wide, st);
+  else if (groups == 2)
+    qkv::read_of<2>(p, sp, grid, groups, bits, wide, st);
+  else
+    qkv::read_of<0>(p, sp, grid, groups, bits, wide, st);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrDriver;
 }
