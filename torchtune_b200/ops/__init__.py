@@ -20,6 +20,7 @@ import torch.nn.functional as F
 
 from . import reference
 from .mask import AttentionMask
+from . import quantized
 from .quantized import QuantizedRows
 
 __all__ = [
@@ -436,8 +437,6 @@ def quantized_append(k: torch.Tensor, v: torch.Tensor, k_rows: QuantizedRows, v_
     """Writes keys and values ``[b, s, heads, d]`` (bf16, fp16 or fp32) in 4 or 8 bits to the slots ``slots`` (int64 ``[s]``, consecutive) of the rows of a cache with as many batch rows.
     No gradient flows through a cache in few bits.  On a CUDA device, where the slots are not known to the host, a token whose slot lies outside the cache or does not follow the one
     before is not written and counted as an index violation; elsewhere it is an error."""
-    from . import quantized
-
     b, h, n, d, bits = quantized.sizes(k_rows, v_rows)
     shape = k.shape
     if len(shape) != 4 or shape != v.shape or shape[0] != b or shape[2] != h or shape[3] != d:
@@ -464,8 +463,6 @@ def quantized_append(k: torch.Tensor, v: torch.Tensor, k_rows: QuantizedRows, v_
 
 def quantized_read(k_rows: QuantizedRows, v_rows: QuantizedRows, start: int = 0, stop: Optional[int] = None, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """What slots ``start`` ... ``stop - 1`` of a quantised cache stand for: keys and values ``[b, stop - start, heads, d]``."""
-    from . import quantized
-
     size = quantized.sizes(k_rows, v_rows)
     stop = size[2] if stop is None else stop
     if not 0 <= start <= stop <= size[2]:
@@ -484,8 +481,6 @@ def quantized_attention(q: torch.Tensor, k_rows: QuantizedRows, v_rows: Quantize
     """:func:`attention` of ``q`` ``[b, s, h, d]`` over all slots of a quantised cache (``k_rows.first(n)`` for the first ``n``).  Up to 16 query rows per key head (tokens times heads that share it; 8
     of 256 channels) attend to the codes as they are; more of them, and calls that need gradients, read the cache back in ``q``'s type first.  Masks are those of :func:`attention`
     with other numbers of queries than of keys: causal ones put the queries into the last slots; documents and chunks have no meaning here."""
-    from . import quantized
-
     mask = mask if mask is not None else AttentionMask(causal=False)
     size = b, h, n, d, _ = quantized.sizes(k_rows, v_rows)
     shape = q.shape
@@ -512,7 +507,7 @@ def quantized_attention(q: torch.Tensor, k_rows: QuantizedRows, v_rows: Quantize
     if _native(q) and softcap <= 0.0 and dropout_p == 0.0 and not _differentiated(q) and _has_memory(q) and quantized.plain(k_rows, v_rows):
         steps = quantized.layout(s, shape[2], k_rows, v_rows, size)
         if steps is not None:
-            return quantized.attention(q, k_rows, v_rows, mask, scale, size, steps)
+            return quantized.attention(q, mask, scale, size, steps)
     k, v = quantized_read(k_rows, v_rows, dtype=q.dtype)
     return attention(q, k, v, mask, scale=scale, softcap=softcap, dropout_p=dropout_p)
 

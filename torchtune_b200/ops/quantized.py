@@ -11,6 +11,7 @@ from ._lib import check, lib, stream_ptr
 from .mask import AttentionMask
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # of rows that are written
+_Eight, _Twelve, _Eighteen = (ctypes.c_longlong * n for n in (8, 12, 18))  # strides of a call
 HEAD_DIMS = (64, 96, 128, 256)  # that the attention kernel has
 
 
@@ -108,7 +109,7 @@ def append(k: torch.Tensor, v: torch.Tensor, k_rows: QuantizedRows, v_rows: Quan
         k = k.contiguous()
     if v.stride(3) != 1:
         v = v.contiguous()
-    strides = (ctypes.c_longlong * 18)(*k.stride()[:3], *v.stride()[:3], *_steps(k_rows), *_steps(v_rows))
+    strides = _Eighteen(*k.stride()[:3], *v.stride()[:3], *_steps(k_rows), *_steps(v_rows))
     check(_on(k, lib().ttb_quantized_append, k.data_ptr(), v.data_ptr(), k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides,
               slots.data_ptr(), _TYPES[k.dtype], b, s, h, d, bits, k_rows.slots), "quantised append")
 
@@ -120,28 +121,33 @@ def read(k_rows: QuantizedRows, v_rows: QuantizedRows, start: int, stop: int, dt
     k = codes.new_empty((b, n, h, d), dtype=dtype)
     v = torch.empty_like(k)
     if b and n and h:
-        strides = (ctypes.c_longlong * 12)(*_steps(k_rows), *_steps(v_rows))
+        strides = _Twelve(*_steps(k_rows), *_steps(v_rows))
         check(_on(codes, lib().ttb_quantized_read, codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides, k.data_ptr(), v.data_ptr(), b, start,
                   n, h, d, bits, int(dtype == torch.float32)), "quantised read")
     return k, v
 
 
 def layout(s: int, hq: int, k_rows: QuantizedRows, v_rows: QuantizedRows, size: Tuple[int, int, int, int, int]) -> Optional[Tuple[int, ...]]:
-    """Batch and head strides of codes and scales for the kernel of few queries, or ``None`` where it does not take these rows; the visibility words of a cluster of 8 CTAs bound the number of slots."""
+    """Addresses, and batch and head strides, of codes and scales for the kernel of few queries, or ``None`` where it does not take these rows; the visibility words of a cluster of 8 CTAs bound the number of slots."""
     _, h, n, d, bits = size
     if d not in HEAD_DIMS or s * (hq // h) > (8 if d == 256 else 16) or (-(-n // 256) * (s + 2) + 1) * 4 > 16384:
         return None
     row, groups = d * bits // 8, d // 32
-    steps: Tuple[int, ...] = ()
-    for codes, scales, _ in (k_rows, v_rows):
-        c, g = codes.stride(), scales.stride()
-        if c[3] != 1 or g[3] != 1 or c[2] != row or g[2] != groups or (c[0] | c[1] | 2 * g[0] | 2 * g[1] | codes.data_ptr() | scales.data_ptr()) & 15:
-            return None
-        steps += (c[0], c[1], g[0], g[1])
-    return steps
+    kc, ks, _ = k_rows
+    vc, vs, _ = v_rows
+    c0, c1, c2, c3 = kc.stride()
+    g0, g1, g2, g3 = ks.stride()
+    d0, d1, d2, d3 = vc.stride()
+    h0, h1, h2, h3 = vs.stride()
+    if not (c2 == d2 == row and g2 == h2 == groups and c3 == g3 == d3 == h3 == 1) or (c0 | c1 | d0 | d1 | 2 * (g0 | g1 | h0 | h1)) & 15:
+        return None
+    at = kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()
+    if (at[0] | at[1] | at[2] | at[3]) & 15:
+        return None
+    return (*at, c0, c1, g0, g1, d0, d1, h0, h1)
 
 
-def attention(q: torch.Tensor, k_rows: QuantizedRows, v_rows: QuantizedRows, mask: AttentionMask, scale: Optional[float], size: Tuple[int, int, int, int, int], steps: Tuple[int, ...]) -> torch.Tensor:
+def attention(q: torch.Tensor, mask: AttentionMask, scale: Optional[float], size: Tuple[int, int, int, int, int], steps: Tuple[int, ...]) -> torch.Tensor:
     b, s, hq, d = q.shape
     _, hkv, n, _, bits = size
     q = q.contiguous()
@@ -171,7 +177,6 @@ def attention(q: torch.Tensor, k_rows: QuantizedRows, v_rows: QuantizedRows, mas
     if n >= 2048 and b * hkv * 8 < 592:  # few and long rows are split further than a cluster reaches
         floats = 128 * b * s * hq * (d + 4)
         work = torch.empty(floats, dtype=torch.float32, device=q.device)
-    check(_on(q, lib().ttb_quantized_attention, q.data_ptr(), k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(),
-              (ctypes.c_longlong * 8)(*steps), o.data_ptr(), seen, seen_b, seen_r, None if start is None else start.data_ptr(), offset, window, sinks, b, s, n, hq, hkv, d, bits,
+    check(_on(q, lib().ttb_quantized_attention, q.data_ptr(), *steps[:4], _Eight(*steps[4:]), o.data_ptr(), seen, seen_b, seen_r, None if start is None else start.data_ptr(), offset, window, sinks, b, s, n, hq, hkv, d, bits,
               1.0 / math.sqrt(d) if scale is None else float(scale), None if work is None else work.data_ptr(), floats), "attention over a quantised cache")
     return o
