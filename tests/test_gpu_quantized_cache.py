@@ -106,7 +106,7 @@ def test_slots_outside_the_cache_or_out_of_order_are_not_written():
 # ---------------------------------------------------------------------------------------------------------------------------------- attention
 
 
-def _check(q, k_rows, v_rows, mask, dense, scale=None):
+def _check(q, k_rows, v_rows, mask, dense, scale=None, spread=False):
     with torch.no_grad():
         got = ops.quantized_attention(q, k_rows, v_rows, mask, scale=scale)
     b, s, hq, d = q.shape
@@ -118,6 +118,11 @@ def _check(q, k_rows, v_rows, mask, dense, scale=None):
     # The result is rounded to 8 bits (at most 2^-9 of it; twice that here); so is every weight times its scale: errors of at most 2^-9 of the terms, without a common sign, so eight times 2^-9 of the
     # terms' root of squares bounds their sum (14 standard deviations).  Scores: fp32 sums whose terms are at most 136 |q| |scale|: at these sizes 1e-4, a twentieth of a weight's rounding.
     bound = 2.0**-8 * want.abs() + 2.0**-6 * square.sqrt()
+    if spread:
+        # Values of very different sizes: where the largest have the code 0, the small ones are what is left.  The kernel's fp32 sums hold codes (below 2^bits) and take 2^(bits - 1) off, so they pass
+        # through numbers of sum p |scale| 2^bits; at most 2^5 steps of a warp and joins, each off by at most 2^-23 of that.
+        size = torch.where(dense.any(1)[:, None, :, None], v_rows.scales[:, :, : v_rows.slots].double(), 0.0).abs().amax(-1)
+        bound = bound + 2.0 ** (v_rows.bits - 18) * torch.einsum("bgnqk,bgk->bqgn", p, size).reshape(b, s, hq, 1)
     assert ((got.double() - want).abs() <= bound).all(), float(((got.double() - want).abs() - bound).max())
     return got
 
@@ -377,3 +382,70 @@ def test_every_quotient_of_two_bf16_numbers():
                 step = wide[:, :1] / -half
                 want = (wide / step).round().clamp(-half, half - 1) * step
                 assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("power", [-70, -30, 20, 40, 60, 100])
+def test_large_and_small_values(power, bits):
+    """Values, and keys against queries, far from 1: the powers of two that the kernel works with stay within fp32."""
+    k_rows, v_rows = _filled(2, 300, 2, 64, bits, seed=2)
+    q = _queries(2, 1, 8, 64)
+    seen = torch.ones(2, 1, 300, dtype=torch.bool, device="cuda")
+    v_rows.scales.mul_(2.0**power)
+    got = _check(q, k_rows, v_rows, AttentionMask(), seen)
+    assert got.any()
+    k_rows.scales.mul_(2.0**-power)
+    assert torch.equal(got, _check((q.float() * 2.0**power).to(torch.bfloat16), k_rows, v_rows, AttentionMask(), seen))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_values_of_very_different_sizes(bits):
+    """Scales that grow along the slots: every warp moves to a smaller power of two on the way; a row whose largest scales lie in slots that it does not see."""
+    k_rows, v_rows = _filled(3, 700, 1, 128, bits, seed=2)
+    v_rows.scales[:, :, :700] *= (2.0 ** torch.linspace(-6, 40, 700, device="cuda"))[:, None].to(torch.bfloat16)
+    dense = torch.ones(3, 1, 700, dtype=torch.bool, device="cuda")
+    dense[1, :, 300:] = False
+    v_rows.scales[1, :, 300:] = 3e38
+    dense[2, :, 600:] = torch.rand(100, generator=_gen(4), device="cuda") < 0.5
+    _check(_queries(3, 1, 4, 128), k_rows, v_rows, AttentionMask(causal=False, bool_mask=dense), dense, spread=True)
+    _check(_queries(3, 1, 4, 128), k_rows, v_rows, AttentionMask(causal=False, bool_mask=dense), dense, scale=2.0, spread=True)
+
+
+def test_a_query_that_is_not_finite_spoils_its_own_rows_only():
+    k_rows, v_rows = _filled(2, 100, 2, 64, 4)
+    q = _queries(2, 2, 8, 64)
+    clean = ops.quantized_attention(q, k_rows, v_rows, AttentionMask())
+    spoilt = q.clone()
+    spoilt[0, 1, 3, 5], spoilt[1, 0, 7, 0] = float("nan"), float("inf")
+    got = ops.quantized_attention(spoilt, k_rows, v_rows, AttentionMask())
+    assert got[0, 1, 3].isnan().all() and got[1, 0, 7].isnan().all()
+    same = torch.ones(2, 2, 8, dtype=torch.bool, device="cuda")
+    same[0, 1, 3] = same[1, 0, 7] = False
+    assert torch.equal(got[same], clean[same])
+
+
+def test_few_long_rows_recorded():
+    """The split that meets in a workspace, in two recordings at once."""
+    k_rows, v_rows = _filled(1, 20000, 2, 64, 4)
+    q = [_queries(1, 1, 8, 64, seed=i) for i in (1, 2)]
+    want = [ops.quantized_attention(x, k_rows, v_rows) for x in q]
+    static, graphs = [x.clone() for x in q], []
+    for x in static:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.quantized_attention(x, k_rows, v_rows)
+        graphs.append((graph, out))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(4):
+        for i, (x, (graph, _), stream) in enumerate(zip(static, graphs, streams)):
+            x.copy_(q[(i + turn) % 2])
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                graph.replay()
+        for stream in streams:
+            torch.cuda.current_stream().wait_stream(stream)
+        for i, (_, out) in enumerate(graphs):
+            assert torch.equal(out, want[(i + turn) % 2])
+    dense = torch.rand(1, 1, 20000, generator=_gen(3), device="cuda") < 0.4
+    _check(q[0], k_rows, v_rows, AttentionMask(causal=False, bool_mask=dense), dense)
+    assert not ops.quantized_attention(q[0], k_rows, v_rows, AttentionMask(causal=False, bool_mask=torch.zeros_like(dense))).any()

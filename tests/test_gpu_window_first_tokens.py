@@ -306,3 +306,22 @@ def test_a_model_is_tuned_and_generates_with_windows():
         model.setup_caches(2, torch.bfloat16, decoder_max_seq_len=320, kv_cache_bits=4)
     out, _ = generation.generate(model, tokens[:, :200], max_generated_tokens=10, pad_id=0, top_k=1)
     assert out.shape == (2, 210)
+
+
+def test_no_queries_and_what_does_not_fit():
+    mask = AttentionMask(window=4, sinks=1)
+    k = _randn(2, 5, 2, 64, seed=1).requires_grad_()
+    q = k[:, :0].detach().requires_grad_()
+    out = ops.attention(q, k, k, mask)
+    assert out.shape == (2, 0, 2, 64)
+    assert not torch.autograd.grad(out.sum(), k)[0].any()
+    x = _randn(2, 9, 2, 64, seed=2)
+    for q, k, v, m in ((x, x[:1], x[:1], mask), (x, x, x[:, :8], mask), (x, x.float(), x, mask), (x, x[..., :32], x[..., :32], mask), (x, x, x, AttentionMask(window=4, sinks=1, doc_ids=_docs(2, 8, 3)))):
+        with pytest.raises(ValueError):
+            ops.attention(q, k, v, m)
+    one = _docs(1, 9, 3)
+    assert torch.equal(ops.attention(x, x, x, AttentionMask(window=4, sinks=1, doc_ids=one)), ops.attention(x, x, x, AttentionMask(window=4, sinks=1, doc_ids=one.expand(2, 9))))
+    y = x.clone().requires_grad_()
+    (grad,) = torch.autograd.grad(ops.attention(y, y, y, mask).float().square().sum(), y, create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.float().sum().backward()

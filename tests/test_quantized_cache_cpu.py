@@ -269,3 +269,13 @@ def test_generate_recipe_with_a_quantised_cache(tmp_path, tune_path, monkeypatch
              f"checkpointer.checkpoint_files=[model-00001-of-00001.safetensors] device=cpu dtype=fp32 output_dir={tmp_path / 'out'} tokenizer.path={sp} max_new_tokens=6 prompt.user=hello "
              "kv_cache_bits=4", monkeypatch)
     assert "tokens/sec" in caplog.text
+
+
+def test_a_cache_keeps_its_types_when_a_model_changes_its_own():
+    model = _decoder()
+    model.setup_caches(1, torch.float32, decoder_max_seq_len=8, kv_cache_bits=4)
+    cache = model.layers[0].attn.kv_cache
+    cache.append(torch.randn(1, 3, 2, 32), torch.randn(1, 3, 2, 32))
+    scales = cache.k_scales.clone()
+    model.to(torch.bfloat16).float()
+    assert cache.k_scales.dtype == torch.bfloat16 and torch.equal(cache.k_scales, scales) and cache.k_codes.dtype == torch.uint8 and cache.cache_pos.dtype == torch.int64

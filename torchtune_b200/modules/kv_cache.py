@@ -93,6 +93,11 @@ class QuantizedKVCache(KVCache):
         self.max_seq_len = max_seq_len
         self.bits = bits
 
+    def _apply(self, fn, recurse: bool = True):
+        super()._apply(fn, recurse)  # moves to a device apply to all; the format's types stay
+        self.k_scales, self.v_scales = self.k_scales.to(torch.bfloat16), self.v_scales.to(torch.bfloat16)
+        return self
+
     def rows(self, batch: int) -> Tuple[ops.QuantizedRows, ops.QuantizedRows]:
         """Keys and values of the first ``batch`` batch rows."""
         k, v = ops.QuantizedRows(self.k_codes, self.k_scales, self.max_seq_len), ops.QuantizedRows(self.v_codes, self.v_scales, self.max_seq_len)

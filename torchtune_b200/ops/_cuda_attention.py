@@ -5,6 +5,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import check, err_word, lib, stream_ptr
 from .mask import AttentionMask
@@ -167,6 +168,9 @@ class _WindowAttention(torch.autograd.Function):
         q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q.contiguous(), k.contiguous(), v.contiguous()))
         o = torch.empty_like(q)
         grads = any(ctx.needs_input_grad)
+        if q.numel() == 0:
+            ctx.save_for_backward(q, k, v)
+            return o
         with torch.cuda.device(q.device):
             if not grads and doc_ids is None and decodes(s, min(sk, window + sinks + s + 192), hq, hkv):  # what it visits, and the rest of its blocks
                 check(lib().ttb_attn_decode_first(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), window, sinks, b, s, sk, hq, hkv, d, float(scale), stream_ptr()),
@@ -174,7 +178,7 @@ class _WindowAttention(torch.autograd.Function):
                 return o
             start = last = None
             if doc_ids is not None:
-                ids = doc_ids.to(device=q.device, dtype=torch.int32).contiguous()
+                ids = doc_ids.to(device=q.device, dtype=torch.int32).expand(b, s).contiguous()
                 start = torch.empty(b, s, dtype=torch.int32, device=q.device)
                 last = torch.empty_like(start)
                 check(lib().ttb_document_bounds(ids.data_ptr(), b, s, window, sinks, start.data_ptr(), last.data_ptr(), stream_ptr()), "document bounds")
@@ -190,7 +194,10 @@ class _WindowAttention(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_o):
+        if len(ctx.saved_tensors) == 3:  # no queries
+            return (*(torch.zeros_like(t) for t in ctx.saved_tensors), None, None, None, None)
         q, k, v, o, rest, lse, last = ctx.saved_tensors
         window, sinks, scale = ctx.meta
         b, s, hq, d = q.shape
@@ -241,6 +248,10 @@ def attention(q, k, v, mask: AttentionMask, scale: Optional[float], softcap: flo
     scale = (1.0 / math.sqrt(d)) if scale is None else scale
     softcap = max(0.0, float(softcap or 0.0))  # 0 and below: no cap
     if softcap == 0.0 and _first_positions(s, sk, mask):
+        if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d or not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device):
+            raise ValueError(f"queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not fit one another, or differ in type or device")
+        if mask.doc_ids is not None and tuple(mask.doc_ids.shape) not in ((b, s), (1, s)):
+            raise ValueError(f"document ids {tuple(mask.doc_ids.shape)} are not those of {b} rows of {s} tokens")
         return _WindowAttention.apply(q, k, v, mask.doc_ids, min(mask.window, sk), min(max(mask.sinks, 0), sk), float(scale))
     lo = hi = kmask = dense = None
     monotone, causal = 1, bool(mask.causal)

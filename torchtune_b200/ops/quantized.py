@@ -171,8 +171,8 @@ def attention(q: torch.Tensor, mask: AttentionMask, scale: Optional[float], size
         start = mask.key_start.to(device=q.device, dtype=torch.int32).contiguous()
         offset = mask.query_start
     elif mask.causal:
-        offset, window = n - s, max(mask.window, 0)
-        sinks = max(mask.sinks, 0) if window else 0
+        offset, window = n - s, min(max(mask.window, 0), n)
+        sinks = min(max(mask.sinks, 0), n) if window else 0
     work, floats = None, 0
     if n >= 2048 and b * hkv * 8 < 592:  # few and long rows are split further than a cluster reaches
         floats = 128 * b * s * hq * (d + 4)
