@@ -10,6 +10,7 @@
     python -m torchtune_b200.ops.microbench latent --heads 16 --rank 512       (latent attention beside grouped-query attention)
     python -m torchtune_b200.ops.microbench ragenex --heads 16 --streams 4     (lightning and span attention, stream steps)
     python -m torchtune_b200.ops.microbench decode --shapes 4096x4096 6144x4096 --tokens 1 16 32   (few tokens: products, attention, sampling)
+    python -m torchtune_b200.ops.microbench contexts    (caches in 4 and 8 bits, windows beside which the first tokens stay visible)
     python -m torchtune_b200.ops.microbench joined      (epilogues that take a pass along, sums of input gradients, grouped products)
     python -m torchtune_b200.ops.microbench suite --tokens 8192      (norm, RoPE, SwiGLU, loss, embedding, LoRA, grouped GEMM, NF4, offload copies)
 
@@ -292,6 +293,87 @@ def bench_decode(args, flush):
             logits, q = torch.randn(b, 128256, device="cuda"), torch.rand(b, 128256, device="cuda") + 1e-3
             emit("sample, top 300", _time_captured(lambda i: lambda: _cuda.sample(logits, q, 0.6, 300), args.iters, 8.0 * logits.numel()), rows=b, vocabulary=128256)
     return {"op": "decode", "rows": len(rows)}
+
+
+def bench_contexts(args, flush):
+    """Caches in 4 and 8 bits (written, read back, attended to by one token per row, beside the bf16 cache) and windows beside which the first tokens stay visible (forward, backward, one token per
+    row): 32 query and 8 key heads.  Times of one launch inside a CUDA graph over inputs larger than L2, of training passes between flushes."""
+    from . import QuantizedRows, attention, quantized_append, quantized_attention, quantized_read
+    from .mask import AttentionMask
+
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+
+    def emit(op, ms, nbytes=0.0, flops=0.0, **kw):
+        row = {"op": op, **kw, "us": round(ms * 1e3, 1)}
+        if nbytes:
+            row["gbs"] = round(nbytes / ms / 1e6)
+        if flops:
+            row["tflops"] = round(flops / ms / 1e9)
+        print(json.dumps(row), flush=True)
+        return row
+
+    rows = []
+    with torch.no_grad():
+        for shape in args.caches:
+            b, n, d = (int(x) for x in shape.split("x"))
+            for bits in (4, 8):
+                size = bits / 8 + 1 / 16
+                nbytes = 2 * b * n * 8 * d * size
+
+                def filled(i):
+                    caches = [QuantizedRows.zeros(b, n, 8, d, bits, device="cuda") for _ in range(2)]
+                    for c in caches:
+                        c.codes.random_(0, 256)
+                        c.scales.normal_(0, 0.1)
+                    return caches
+
+                def attend(i):
+                    caches, q = filled(i), torch.randn(b, 1, 32, d, **bf)
+                    return lambda: quantized_attention(q, *caches, AttentionMask())
+
+                rows.append(emit("attend", _time_captured(attend, args.iters, nbytes), nbytes, rows=b, slots=n, head_dim=d, bits=bits))
+                moved = 2 * b * n * 8 * d * (2 + size)
+
+                def append(i):
+                    caches, kv, at = filled(i), torch.randn(b, n, 16, d, **bf), torch.arange(n, device="cuda")
+                    return lambda: quantized_append(kv[:, :, :8], kv[:, :, 8:], *caches, at)
+
+                def read(i):
+                    caches = filled(i)
+                    return lambda: quantized_read(*caches)
+
+                if moved < 1 << 30:
+                    rows.append(emit("append", _time_captured(append, args.iters, moved), moved, rows=b, tokens=n, head_dim=d, bits=bits))
+                    rows.append(emit("read", _time_captured(read, args.iters, moved), moved, rows=b, tokens=n, head_dim=d, bits=bits))
+
+            def plain(i):
+                k, v, q = torch.randn(b, n, 8, d, **bf), torch.randn(b, n, 8, d, **bf), torch.randn(b, 1, 32, d, **bf)
+                return lambda: attention(q, k, v, AttentionMask())
+
+            nbytes = 4 * b * n * 8 * d
+            rows.append(emit("attend", _time_captured(plain, args.iters, nbytes), nbytes, rows=b, slots=n, head_dim=d, bits=16))
+            torch.cuda.empty_cache()
+        for b, n, d, window, sinks in ((8, 8012, 128, 2048, 4), (16, 8012, 64, 2048, 4)):
+
+            def windowed(i):
+                k, v, q = torch.randn(b, n, 8, d, **bf), torch.randn(b, n, 8, d, **bf), torch.randn(b, 1, 32, d, **bf)
+                return lambda: attention(q, k, v, AttentionMask(window=window, sinks=sinks))
+
+            nbytes = 4 * b * (window + sinks) * 8 * d
+            rows.append(emit("window token", _time_captured(windowed, args.iters, nbytes), nbytes, rows=b, slots=n, head_dim=d, window=window, sinks=sinks))
+    for b, s, d, window, sinks in ((1, 6000, 128, 1024, 4), (4, 4096, 128, 1024, 4), (1, 16384, 128, 4096, 4), (4, 4096, 64, 512, 4)):
+        q, k, v = (torch.randn(b, s, h, d, requires_grad=True, **bf) for h in (32, 8, 8))
+        mask = AttentionMask(window=window, sinks=sinks)
+        pairs = sum(min(i + 1, window + min(sinks, max(0, i + 1 - window))) for i in range(s))
+        flops = 4.0 * b * 32 * d * pairs
+        with torch.no_grad():
+            t = _time(lambda: attention(q, k, v, mask), args.iters, args.warmup, flush)
+        rows.append(emit("window forward", t, flops=flops, rows=b, tokens=s, head_dim=d, window=window, sinks=sinks))
+        out = attention(q, k, v, mask)
+        go = torch.randn_like(out)
+        t = _time(lambda: torch.autograd.grad(out, (q, k, v), go, retain_graph=True), args.iters, args.warmup, flush)
+        rows.append(emit("window backward", t, flops=2.5 * flops, rows=b, tokens=s, head_dim=d, window=window, sinks=sinks))
+    return {"op": "contexts", "kernels": len(rows)}
 
 
 def bench_joined(args, flush):
@@ -819,13 +901,15 @@ def main() -> None:
     rx.add_argument("--streams", type=int, default=4)
     rx.add_argument("--seq", type=int, default=8192)
     sub.add_parser("joined")
+    cx = sub.add_parser("contexts")
+    cx.add_argument("--caches", nargs="*", default=["1x61x64", "16x732x128", "2x8000x128", "1x65000x128", "32x4096x64", "64x4096x128"], help="rows x slots x head dim")
     su = sub.add_parser("suite")
     su.add_argument("--tokens", type=int, default=8192)
     args = ap.parse_args()
     from ._lib import check_device_errors
 
     flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
-    fn = {"gemm": bench_gemm, "gemm_fp8": bench_gemm_fp8, "gemm_mxfp8": bench_gemm_mxfp8, "attention": bench_attention, "rmsnorm": bench_rmsnorm, "adamw": bench_adamw, "adamw8bit": bench_adamw8bit, "gate_up": bench_gate_up, "comm": bench_comm, "decode": bench_decode, "joined": bench_joined, "latent": bench_latent, "ragenex": bench_ragenex, "suite": bench_suite}[args.op]
+    fn = {"gemm": bench_gemm, "gemm_fp8": bench_gemm_fp8, "gemm_mxfp8": bench_gemm_mxfp8, "attention": bench_attention, "rmsnorm": bench_rmsnorm, "adamw": bench_adamw, "adamw8bit": bench_adamw8bit, "gate_up": bench_gate_up, "comm": bench_comm, "decode": bench_decode, "joined": bench_joined, "contexts": bench_contexts, "latent": bench_latent, "ragenex": bench_ragenex, "suite": bench_suite}[args.op]
     res = fn(args, flush)
     check_device_errors()
     print(json.dumps(res), flush=True)
