@@ -79,9 +79,10 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   int* ranges = reinterpret_cast<int*>(tmem_slot + 2);  // MASKED, per tile: smallest lo, largest lo, smallest hi, largest hi, rows that read mask bytes
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y, bi = blockIdx.z;
+  // FIRST: grid (heads, batch, tiles), the last tiles first, so that those which see less than a window end the launch
+  const int h = FIRST ? blockIdx.x : blockIdx.y, bi = FIRST ? blockIdx.y : blockIdx.z;
   const int hk = h / (p.hq / p.hkv);
-  const int q0 = blockIdx.x * 2 * kBlk;
+  const int q0 = (FIRST ? gridDim.z - 1 - blockIdx.z : blockIdx.x) * 2 * kBlk;
   const int row_base = bi * p.s;
   const int krow_base = bi * p.sk;
   const long long bound_base = MASKED ? bi * p.bound_b : row_base;
@@ -507,7 +508,8 @@ static int launch(const void* q, const void* k, const void* v, const Params& p, 
     if (cudaFuncSetAttribute(attn_fwd2_kernel<D, MASKED, FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<D>) != cudaSuccess) return kErrDriver;
     attr = true;
   }
-  dim3 grid((p.s + 2 * kBlk - 1) / (2 * kBlk), p.hq, p.b);
+  const unsigned tiles = (p.s + 2 * kBlk - 1) / (2 * kBlk);
+  const dim3 grid = FIRST ? dim3(p.hq, p.b, tiles) : dim3(tiles, p.hq, p.b);
   TTB_COUNT_LAUNCH(1);
   attn_fwd2_kernel<D, MASKED, FIRST><<<grid, kThreads, kSmemBytes<D>, st>>>(tq, tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrDriver;

@@ -711,7 +711,7 @@ static long long bit_bytes(int tiles, int s, int splits) { return (static_cast<l
 static int splits_of(long long pairs, int tiles, int s, int per_sm, bool spread, bool more) {
   int best = 0;
   long long least = 0, least_waves = 0;
-  for (int n = 1; n <= (spread ? kMaxSpread : kMaxCluster); n += n < kMaxCluster ? n : 8) {  // clusters of 3, 5 or 7 are placed worse
+  for (int n = 1; n <= (spread ? kMaxSpread : kMaxCluster); n += n < kMaxCluster ? n : 1) {  // clusters of 3, 5 or 7 are placed worse
     if (bit_bytes(tiles, s, n) > kMaxBitBytes) continue;
     const long long ctas = (pairs * n + sm_count() - 1) / sm_count(), waves = (ctas + per_sm - 1) / per_sm, rounds = (tiles + n * kWarps - 1) / (n * kWarps);
     const long long cost = max(10 * ctas * rounds, 14 * waves * rounds) + 80 * waves + (n > kMaxCluster ? 80 : 0);
