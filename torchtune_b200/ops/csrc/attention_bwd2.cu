@@ -50,6 +50,9 @@ struct Params {
   // The first positions are seen by all later queries.  Without documents the queries beyond the window of a block that holds some are cut into `pieces` runs of `piece` query blocks, each a
   // CTA of its own, so that no CTA walks the whole sequence; their gradients and those of the block's own CTA meet in `partial` [b * hkv][blocks][1 + pieces][rows][dk, dv][D].
   int blocks, pieces, piece, rows;
+  // Launches of up to four waves go through pieces and key blocks with all heads at a time, so that the last key blocks, which fewer queries than a window see, end them (1 x 6000 tokens, window
+  // 1024, forward and backward 620 -> 606 us; 4 x 1413 packed 283 -> 267); larger ones a head at a time, whose neighbouring blocks share queries (4 x 4096 backward 961 us, the other way 985).
+  int by_length;
   float* partial;
 };
 
@@ -104,12 +107,13 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hk = blockIdx.y, bi = blockIdx.z;
+  const bool across = FIRST && p.by_length;  // grid (key heads, batch, pieces and key blocks) instead of (pieces and key blocks, key heads, batch)
+  const int hk = across ? blockIdx.x : blockIdx.y, bi = across ? blockIdx.y : blockIdx.z;
   const int group = p.hq / p.hkv;
-  const int key_blocks = (p.sk + kBlk - 1) / kBlk;
-  const bool far = FIRST && static_cast<int>(blockIdx.x) >= key_blocks;  // queries beyond the window of a block with first positions
-  const int far_index = static_cast<int>(blockIdx.x) - key_blocks;
-  const int kv0 = (far ? far_index / max(p.pieces, 1) : static_cast<int>(blockIdx.x)) * kBlk;
+  const int index = static_cast<int>(across ? blockIdx.z : blockIdx.x), far_count = FIRST ? p.blocks * p.pieces : 0;
+  const bool far = FIRST && index < far_count;  // queries beyond the window of a block with first positions
+  const int far_index = index;
+  const int kv0 = (far ? far_index / max(p.pieces, 1) : index - far_count) * kBlk;
   const int shift = p.sk - p.s;
   const int row_base = bi * p.s, krow_base = bi * p.sk;
   const int nq_blocks = (p.s + kBlk - 1) / kBlk;
@@ -543,7 +547,9 @@ static int launch(const void* q, const void* k, const void* v, const void* d_o, 
     attr = true;
   }
   TTB_COUNT_LAUNCH(1);
-  kern<<<dim3((p.sk + kBlk - 1) / kBlk + (FIRST ? p.blocks * p.pieces : 0), p.hkv, b), kThreads, Layout<D>::kDynamic, st>>>(tq, tk, tv, tdo, tdq, p);
+  const unsigned parts = (p.sk + kBlk - 1) / kBlk + (FIRST ? p.blocks * p.pieces : 0);
+  const dim3 grid = FIRST && p.by_length ? dim3(p.hkv, b, parts) : dim3(parts, p.hkv, b);
+  kern<<<grid, kThreads, Layout<D>::kDynamic, st>>>(tq, tk, tv, tdo, tdq, p);
   if (FIRST && p.pieces > 0) {
     TTB_COUNT_LAUNCH(1);
     first_rows_kernel<D><<<dim3(p.rows, p.blocks, b * p.hkv), 2 * D, 0, st>>>(p);
@@ -606,6 +612,7 @@ int ttb_attn_bwd2_first(const void* q, const void* k, const void* v, const void*
   p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.scale = scale, p.causal = 1, p.window = window < sk ? window : sk, p.sinks = sinks < sk ? sinks : sk, p.last = last;
   p.lse = lse, p.delta = delta, p.dk = static_cast<__nv_bfloat16*>(dk), p.dv = static_cast<__nv_bfloat16*>(dv), p.err = err, p.partial = work;
   fb2::cut(p, b, d, last != nullptr);
+  p.by_length = static_cast<long long>((sk + attn::kBlk - 1) / attn::kBlk + p.blocks * p.pieces) * hkv * b <= 4ll * sm_count();
   if (p.pieces > 0 && (work == nullptr || work_floats < ttb_attn_bwd_first_workspace(window, sinks, 0, b, s, sk, hkv, d) || (reinterpret_cast<uintptr_t>(work) & 15))) return kErrBadShape;
   return d == 128 ? fb2::launch<128, true>(q, k, v, d_o, dq, b, p, stream) : fb2::launch<64, true>(q, k, v, d_o, dq, b, p, stream);
 }
