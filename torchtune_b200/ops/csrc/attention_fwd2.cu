@@ -327,7 +327,43 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const float c = p.scale * kLog2e;
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int n = 0; n < count[x] && !*abort_flag; ++n) {
+    int n_first = 0;
+    if constexpr (FIRST) {
+      // Up to 32 first positions are the whole first block: a quarter of a block's columns, and nothing is there to be rescaled (4 x 4096 tokens of 64 channels, window 512, 366 -> 345 us).
+      if (heads == 1 && chunks(0) == 1 && count[x] > 0 && !*abort_flag) {
+        n_first = 1;
+        ok = mbar_wait(&s_full[x], 0);
+        if (!ok) {
+          n_first = count[x];
+        } else {
+          tc_fence_after();
+          uint32_t sv[32], pk[16];
+          tmem_ld_32x32(tS[x] + lane_sel, sv);
+          tmem_ld_wait();
+          const uint32_t seen = keys_between(head_key, start_row, min(min(kept_end, head_end) - 1, hi_row));
+          float mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            sv[i] = (seen >> i) & 1u ? sv[i] : 0xff800000u;  // -inf
+            mx = fmaxf(mx, __uint_as_float(sv[i]));
+          }
+          m_used = mx * c;
+          const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float e0 = fast_exp2(fmaf(__uint_as_float(sv[i]), c, neg_m)), e1 = fast_exp2(fmaf(__uint_as_float(sv[i + 1]), c, neg_m));
+            l += e0 + e1;
+            pk[i >> 1] = pack_bf16x2(e0, e1);
+          }
+          tmem_st_32x16(tS[x] + lane_sel, pk);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[x]);
+        }
+      }
+    }
+    for (int n = n_first; n < count[x] && !*abort_flag; ++n) {
       const int block = FIRST && n >= heads ? n + skipped(x) : begin[x] + n, kv0 = block_key(block);
       if (!mbar_wait(&s_full[x], n & 1)) {
         ok = false;
