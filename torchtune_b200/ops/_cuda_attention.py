@@ -215,20 +215,19 @@ class _WindowAttention(torch.autograd.Function):
         return dq.to(q.dtype), dk, dv, None, None, None, None
 
 
-def _first_positions(s: int, sk: int, mask: AttentionMask) -> bool:
-    """Whether a mask is a causal window that the kernels with first positions take: with such positions, or with other numbers of queries than of keys."""
+def takes_window(q: torch.Tensor, k: torch.Tensor, mask: AttentionMask, softcap: float) -> bool:
+    """Whether a call is a causal window of the kernels with first positions: with such positions, or with other numbers of queries than of keys."""
+    s, sk = q.shape[1], k.shape[1]
     return (mask.bool_mask is None and mask.key_start is None and mask.causal and mask.window > 0 and mask.chunk <= 0 and (mask.sinks > 0 or s != sk) and s <= sk
-            and (mask.doc_ids is None or s == sk))
+            and (mask.doc_ids is None or s == sk) and (softcap or 0.0) <= 0.0 and q.shape[2] % k.shape[2] == 0)
 
 
-def unsupported_reason(q: torch.Tensor, k: torch.Tensor, mask: AttentionMask, softcap: float = 0.0) -> Optional[str]:
-    """Why a bf16 CUDA call cannot run on the kernels (``None`` = it can)."""
+def unsupported_reason(q: torch.Tensor, k: torch.Tensor, mask: AttentionMask) -> Optional[str]:
+    """Why a bf16 CUDA call that is not one of ``takes_window`` cannot run on the kernels (``None`` = it can)."""
     s, sk = q.shape[1], k.shape[1]
     structured = mask.doc_ids is not None or mask.chunk > 0 or mask.window > 0
     if q.shape[2] % k.shape[2]:
         return "query heads not a multiple of key heads"
-    if softcap <= 0.0 and _first_positions(s, sk, mask):
-        return None
     if mask.bool_mask is None and mask.window > 0 and mask.sinks > 0 and mask.causal:
         return "first tokens beside a window together with chunks, soft-capped scores or fewer keys than queries"
     if mask.bool_mask is None and structured and not mask.causal:
@@ -247,7 +246,7 @@ def attention(q, k, v, mask: AttentionMask, scale: Optional[float], softcap: flo
     sk = k.shape[1]
     scale = (1.0 / math.sqrt(d)) if scale is None else scale
     softcap = max(0.0, float(softcap or 0.0))  # 0 and below: no cap
-    if softcap == 0.0 and _first_positions(s, sk, mask):
+    if takes_window(q, k, mask, softcap):
         if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d or not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device):
             raise ValueError(f"queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not fit one another, or differ in type or device")
         if mask.doc_ids is not None and tuple(mask.doc_ids.shape) not in ((b, s), (1, s)):
