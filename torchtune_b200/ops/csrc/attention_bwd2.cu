@@ -541,10 +541,12 @@ static int launch(const void* q, const void* k, const void* v, const void* d_o, 
   const uint64_t width = static_cast<uint64_t>(p.hq) * D;
   if ((rc = make_tmap_3d(&tdq, dq, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, width, p.s, b, width * 4, width * 4 * p.s, 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_128B)) != kOk) return rc;
   auto kern = attn_bwd2_kernel<D, FIRST>;
-  static bool attr = false;
-  if (!attr) {
+  static bool attr[64] = {};  // an attribute of the kernel on one device
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return kErrDriver;
+  if (!attr[device]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kDynamic) != cudaSuccess) return kErrDriver;
-    attr = true;
+    attr[device] = true;
   }
   TTB_COUNT_LAUNCH(1);
   const unsigned parts = (p.sk + kBlk - 1) / kBlk + (FIRST ? p.blocks * p.pieces : 0);

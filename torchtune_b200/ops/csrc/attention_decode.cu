@@ -358,10 +358,12 @@ static int launch(const Params& p, int b, cudaStream_t st) {
   if (bit_bytes > kMaxBitBytes) return kErrTooLarge;
   constexpr int fixed = Layout<D>::kRing + Layout<D>::kStats + (APPEND ? Layout<D>::kQueries : 0);
   const int smem = fixed + static_cast<int>(bit_bytes);
-  static bool attr = false;
-  if (!attr) {
+  static bool attr[64] = {};  // an attribute of the kernel on one device
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return kErrDriver;
+  if (!attr[device]) {
     if (cudaFuncSetAttribute(decode_kernel<D, APPEND, FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + kMaxBitBytes) != cudaSuccess) return kErrDriver;
-    attr = true;
+    attr[device] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(splits, p.hkv, b);

@@ -539,10 +539,12 @@ static int launch(const void* q, const void* k, const void* v, const Params& p, 
   if ((rc = make_head_map<D>(&tq, q, p.b, p.s, p.hq)) != kOk) return rc;
   if ((rc = FIRST ? make_rows_map<D>(&tk, k, p.b, p.sk, p.hkv) : make_head_map<D>(&tk, k, p.b, p.sk, p.hkv)) != kOk) return rc;
   if ((rc = FIRST ? make_rows_map<D>(&tv, v, p.b, p.sk, p.hkv) : make_head_map<D>(&tv, v, p.b, p.sk, p.hkv)) != kOk) return rc;
-  static bool attr = false;
-  if (!attr) {
+  static bool attr[64] = {};  // an attribute of the kernel on one device
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return kErrDriver;
+  if (!attr[device]) {
     if (cudaFuncSetAttribute(attn_fwd2_kernel<D, MASKED, FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<D>) != cudaSuccess) return kErrDriver;
-    attr = true;
+    attr[device] = true;
   }
   const unsigned tiles = (p.s + 2 * kBlk - 1) / (2 * kBlk);
   const dim3 grid = FIRST ? dim3(p.hq, p.b, tiles) : dim3(tiles, p.hq, p.b);

@@ -14,8 +14,9 @@
 // integer unit.  So keys (and channels) are the 16 rows of an m16n8k16 tile and a key head's query rows its 8 columns: no code is turned twice, and few rows do not pay for 16.  A lane holds a
 // quarter of a row of keys (with eight channels of every group) and, for the second product, half a word of every group of four rows of values, whose nibbles meet in one register as
 // the pairs of keys that the operand wants.
-// Measured (4 bits, 32 query on 8 key heads of 128 channels, cold L2, launch included): 64 x 4096 slots 74 us (4.1 TB/s), in 8 bits 119 us (4.8 TB/s); 16 x 732 12 us; 1 x 65 003 31 us.  The large ones
-// issue 590 instructions per tile at 0.55 per cycle and scheduler: 16 warps per SM (128 registers each) do not hide the latency of the chains from load to product; the small ones are latency.
+// Measured (4 bits, 32 query on 8 key heads of 128 channels, cold L2, replayed from a graph): 64 x 4096 slots 66 us (4.5 TB/s), in 8 bits 102 us (5.6 TB/s); 16 x 732 9.3 us; 1 x 65 000 25 us.  The same
+// from bf16 rows: 176, 29 and 117 us.  The large ones issue 590 instructions per tile at 0.58 per cycle and scheduler (integer unit 54 % busy, tensor cores 37 %): 16 warps per SM (128
+// registers each) do not hide the latency of the chains from load to product, and with 12, 20 or 24 it is no better.  The small ones are latency.
 //
 // A warp takes tiles of 32 keys through a cp.async ring of its own, with its own running maximum (moved only when a score exceeds it by 2^8), sum and output.  Tiles are dealt round-robin to
 // the warps of a CTA and the CTAs of a cluster, which meet once at the end in distributed shared memory in a fixed order; of few and long rows to more CTAs, which meet in a workspace, also in a

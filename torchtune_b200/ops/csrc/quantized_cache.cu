@@ -10,7 +10,10 @@
 //
 // Rows come as bf16, fp16 or fp32 (the scale of the latter two is rounded, and codes are those of the scale that is stored).
 //
-// Both kernels are bound by bytes: 8 channels per thread, 16-byte accesses on the wide side.  Rows lie [batch, head, slot]: a head's rows are one stream for the attention kernel.
+// Rows lie [batch, head, slot]: a head's rows are one stream for the attention kernel.  A thread has 8 channels, 16 bytes of bf16.  Measured (4 bits, 8 heads of 128 channels, cold L2): 2 x 8000
+// tokens 26.5 us written, 17.3 us read (83.5 MB: 3.2 and 4.8 TB/s); 1 x 65 000 tokens 95.7 and 61.1 us (3.5 and 5.6); one token of 16 rows 4 and 3.3 us, a launch.  Reading is bound by its bytes; writing
+// by issue: 165 instructions per 8 channels (unpacking, the two extrema, codes and their packing), at 0.79 of the rate.  With one token to a thread and
+// divisions instead of products with the reciprocal the first took 55 and 34 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
       asm("mad.lo.u32 %0, %1, %2, %0;" : "+r"(code[e / kPer]) : "r"(c), "r"(1u << (BITS * (e % kPer))));  // the integer unit is what bounds this kernel; this is not on it
     };
     if (sizeof(T) == 2 && !kHalfPrecision<T> && fabsf(s) >= 1e-30f && usable) {
-      // bf16: a quotient is a tie or at least 2^-9 away from one (see above).  The product with the reciprocal (off by at most 2^-22 of itself) is off by at most 2^-15, so that on a grid of 2^-10 it lies on the same side, and a tie
+      // bf16: a quotient is a tie or at least 2^-10 away from one (see above).  The product with the reciprocal (off by at most 2^-22 of itself) is off by at most 2^-15, so that on a grid of 2^-10 it lies on the same side, and a tie
       // on itself; the last sum rounds it to a whole number, ties to even, and leaves that in the low bits.  A tenth of the instructions of a division.
       float inv;
       asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));

@@ -21,11 +21,11 @@ class AttentionMask:
     doc_ids: Optional[torch.Tensor] = None  # [b, s] int32, equal ids may attend
     chunk: int = 0  # >0: positions attend only inside the same chunk of this size
     window: int = 0  # >0: key must be within this many positions before the query
-    sinks: int = 0  # >0, with a window: the first tokens of the sequence (of each document, where there are some) stay visible to all later ones
     bool_mask: Optional[torch.Tensor] = None  # dense [b, sq, skv], True = attend
     # Cached decoding of left-padded rows: query i sits in cache slot query_start + i and sees the slots key_start[b] ... its own.
     key_start: Optional[torch.Tensor] = None  # [b] int32
     query_start: int = 0
+    sinks: int = 0  # >0, with a window: the first tokens of the sequence (of each document, where there are some) stay visible to all later ones
 
     def to(self, device, non_blocking: bool = False) -> "AttentionMask":
         return replace(
