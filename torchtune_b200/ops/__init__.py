@@ -106,12 +106,19 @@ def _native(t: torch.Tensor, dtypes=(torch.bfloat16,)) -> bool:
 
 def _differentiated(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether a call on these tensors may have to be differentiated, in either mode; kernels without an autograd function then don't apply."""
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or torch.autograd.forward_ad._current_level >= 0
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return torch.autograd.forward_ad._current_level >= 0
 
 
 def _has_memory(*tensors: torch.Tensor) -> bool:
     """Whether these are ordinary tensors, whose address a kernel can be given: not fake ones of a trace, batched ones of vmap or of autograd, or other subclasses."""
-    return all(type(t) in (torch.Tensor, torch.nn.Parameter) and torch._C._has_storage(t) for t in tensors)
+    for t in tensors:
+        if type(t) not in (torch.Tensor, torch.nn.Parameter) or not torch._C._has_storage(t):
+            return False
+    return True
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -179,11 +179,11 @@ def _declare(L: ctypes.CDLL) -> None:
     L.ttb_attn_bwd_first_workspace.restype = i64
     L.ttb_document_bounds.argtypes = [vp, i32, i32, i32, i32, vp, vp, vp]
     L.ttb_document_bounds.restype = i32
-    L.ttb_quantized_append.argtypes = [vp] * 6 + [c.POINTER(i64), vp] + [i32] * 7 + [vp]
+    L.ttb_quantized_append.argtypes = [c.c_char_p, vp]  # the arguments packed, and the stream
     L.ttb_quantized_append.restype = i32
-    L.ttb_quantized_read.argtypes = [vp] * 4 + [c.POINTER(i64), vp, vp] + [i32] * 7 + [vp]
+    L.ttb_quantized_read.argtypes = [c.c_char_p, vp]
     L.ttb_quantized_read.restype = i32
-    L.ttb_quantized_attention.argtypes = [vp] * 5 + [c.POINTER(i64), vp, vp, i64, i64, vp] + [i32] * 10 + [f32, vp, i64, vp]
+    L.ttb_quantized_attention.argtypes = [c.c_char_p, f32, vp]
     L.ttb_quantized_attention.restype = i32
     for fn in (L.ttb_span_decode_tile, L.ttb_span_prepare, L.ttb_span_prefill, L.ttb_span_decode, L.ttb_stream_step, L.ttb_embed_positions, L.ttb_clamped_glu, L.ttb_lightning_recurrent,
                L.ttb_lightning_chunks, L.ttb_silu_rows, L.ttb_gated_norm):

@@ -778,30 +778,47 @@ static int by_rows(const Params& p, int b, long long work_floats, cudaStream_t s
 }  // namespace qattn
 }  // namespace ttb
 
+// A call's arguments, 8 bytes each: handed over as one piece, which takes the caller less time than as many arguments.
+struct QuantizedAttentionCall {
+  const void *q, *k_codes, *k_scales, *v_codes, *v_scales;
+  long long strides[8];
+  void* o;
+  const void* mask;
+  long long mask_b, mask_r;
+  const int* key_start;
+  long long offset, window, sinks, b, s, sk, hq, hkv, d, bits;
+  void* work;
+  long long work_floats;
+};
+
 // Attention of s queries over the first sk slots of a quantised cache: q, o [b, s, hq, d] contiguous, s * (hq / hkv) <= 16 (d 256: 8) query rows per key head, d 64, 96, 128 or 256, bits 4 or 8.
 // Rows as ttb_quantized_append writes them, those of one head one behind the other; strides[0..1]: batch and head of k's codes (bytes), [2..3] of its scales (elements), [4..7] of v's; all starts on
 // 16 bytes.  mask (nullable): nonzero byte = visible, row (b, i) at mask + b * mask_b + i * mask_r.  key_start (nullable) int32 [b]: first visible slot.  offset >= 0: query i sits in slot
 // offset + i and sees no later one, with window > 0 only the last `window` of them and the first `sinks`.  A query that sees nothing gives 0.
 // work (nullable): work_floats fp32 numbers, used where few and long rows are split further than a cluster reaches, if they are at least 128 * b * hq * s * (d + 4).
-extern "C" int ttb_quantized_attention(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, const long long* strides, void* o, const void* mask,
-                                       long long mask_b, long long mask_r, const int* key_start, int offset, int window, int sinks, int b, int s, int sk, int hq, int hkv, int d, int bits,
-                                       float scale, void* work, long long work_floats, void* stream) {
+extern "C" int ttb_quantized_attention(const QuantizedAttentionCall* call, float scale, void* stream) {
   using namespace ttb;
-  if (b <= 0 || b > 65535 || s <= 0 || sk <= 0 || hkv <= 0 || hkv > 65535 || hq <= 0 || hq % hkv || s > 16 || hq / hkv > 16 || s * (hq / hkv) > (d == 256 ? 8 : 16)) return kErrBadShape;
-  if (sk > 0x7fffffff - 64 || offset > 0x7fffffff - 64 || window < 0 || sinks < 0 || (window > 0 && offset < 0)) return kErrBadShape;
+  const QuantizedAttentionCall& x = *call;
+  const long long most = 0x7fffffff - 64;
+  if (x.b <= 0 || x.b > 65535 || x.s <= 0 || x.s > 16 || x.sk <= 0 || x.sk > most || x.hkv <= 0 || x.hkv > 65535 || x.hq <= 0 || x.hq % x.hkv || x.hq / x.hkv > 16 ||
+      x.s * (x.hq / x.hkv) > (x.d == 256 ? 8 : 16) || x.d > 256)
+    return kErrBadShape;
+  if (x.offset > most || x.window < 0 || x.window > most || x.sinks < 0 || x.sinks > most || (x.window > 0 && x.offset < 0)) return kErrBadShape;
   qattn::Params p{};
-  p.q = static_cast<const __nv_bfloat16*>(q), p.o = static_cast<__nv_bfloat16*>(o);
-  p.kc = static_cast<const uint8_t*>(k_codes), p.vc = static_cast<const uint8_t*>(v_codes);
-  p.ks = static_cast<const uint8_t*>(k_scales), p.vs = static_cast<const uint8_t*>(v_scales);
-  p.kc_b = strides[0], p.kc_h = strides[1], p.ks_b = strides[2] * 2, p.ks_h = strides[3] * 2;
-  p.vc_b = strides[4], p.vc_h = strides[5], p.vs_b = strides[6] * 2, p.vs_h = strides[7] * 2;
-  for (const void* x : {q, k_codes, k_scales, v_codes, v_scales, static_cast<const void*>(o)})
-    if (reinterpret_cast<uintptr_t>(x) & 15) return kErrBadShape;
-  if (reinterpret_cast<uintptr_t>(work) & 15) return kErrBadShape;
+  p.q = static_cast<const __nv_bfloat16*>(x.q), p.o = static_cast<__nv_bfloat16*>(x.o);
+  p.kc = static_cast<const uint8_t*>(x.k_codes), p.vc = static_cast<const uint8_t*>(x.v_codes);
+  p.ks = static_cast<const uint8_t*>(x.k_scales), p.vs = static_cast<const uint8_t*>(x.v_scales);
+  p.kc_b = x.strides[0], p.kc_h = x.strides[1], p.ks_b = x.strides[2] * 2, p.ks_h = x.strides[3] * 2;
+  p.vc_b = x.strides[4], p.vc_h = x.strides[5], p.vs_b = x.strides[6] * 2, p.vs_h = x.strides[7] * 2;
+  for (const void* t : {x.q, x.k_codes, x.k_scales, x.v_codes, x.v_scales, static_cast<const void*>(x.o), static_cast<const void*>(x.work)})
+    if (reinterpret_cast<uintptr_t>(t) & 15) return kErrBadShape;
   if ((p.kc_b | p.kc_h | p.ks_b | p.ks_h | p.vc_b | p.vc_h | p.vs_b | p.vs_h) & 15) return kErrBadShape;
-  p.mask = static_cast<const uint8_t*>(mask), p.mask_b = mask_b, p.mask_r = mask_r, p.key_start = key_start;
+  const int b = static_cast<int>(x.b), s = static_cast<int>(x.s), sk = static_cast<int>(x.sk), hq = static_cast<int>(x.hq), hkv = static_cast<int>(x.hkv);
+  const int offset = x.offset < 0 ? -1 : static_cast<int>(x.offset), window = static_cast<int>(x.window), sinks = static_cast<int>(x.sinks);
+  const long long work_floats = x.work != nullptr ? x.work_floats : 0;
+  p.mask = static_cast<const uint8_t*>(x.mask), p.mask_b = x.mask_b, p.mask_r = x.mask_r, p.key_start = x.key_start;
   p.offset = offset, p.window = window, p.sinks = sinks;
-  p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.scale = scale, p.work = static_cast<float*>(work);
+  p.s = s, p.sk = sk, p.hq = hq, p.hkv = hkv, p.scale = scale, p.work = static_cast<float*>(x.work);
   p.group = hq / hkv, p.per_query = 65536 / p.group + 1;
   p.skip_from = 0x7fffffff;
   if (window > 0) {  // the first query's window begins first
@@ -811,7 +828,7 @@ extern "C" int ttb_quantized_attention(const void* q, const void* k_codes, const
   }
   p.tiles = (sk + qattn::kTileKeys - 1) / qattn::kTileKeys - p.skipped;
   auto st = static_cast<cudaStream_t>(stream);
-  switch (d * 16 + bits) {
+  switch (x.d * 16 + x.bits) {
     case 64 * 16 + 4: return qattn::by_rows<64, 4>(p, b, work_floats, st);
     case 64 * 16 + 8: return qattn::by_rows<64, 8>(p, b, work_floats, st);
     case 96 * 16 + 4: return qattn::by_rows<96, 4>(p, b, work_floats, st);

@@ -1,8 +1,8 @@
 """A key/value cache in 4 or 8 bits: its rows, and the kernels that write, read and attend over them (``csrc/quantized_cache.cu``, ``csrc/quantized_attention.cu``)."""
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -11,7 +11,7 @@ from ._lib import check, lib, stream_ptr
 from .mask import AttentionMask
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # of rows that are written
-_Eight, _Twelve, _Eighteen = (ctypes.c_longlong * n for n in (8, 12, 18))  # strides of a call
+_pack_append, _pack_read, _pack_attention = (struct.Struct(f"={n}q").pack for n in (32, 25, 30))  # arguments of a call, as its struct in the kernel's source has them
 HEAD_DIMS = (64, 96, 128, 256)  # that the attention kernel has
 
 
@@ -84,7 +84,10 @@ def sizes(k_rows: QuantizedRows, v_rows: QuantizedRows) -> Tuple[int, int, int, 
 
 def plain(*rows: QuantizedRows) -> bool:
     """Whether these are ordinary tensors, whose address a kernel can be given."""
-    return all(type(r.codes) is torch.Tensor and type(r.scales) is torch.Tensor for r in rows)
+    for codes, scales, _ in rows:
+        if type(codes) is not torch.Tensor or type(scales) is not torch.Tensor:
+            return False
+    return True
 
 
 def _on(t: torch.Tensor, call, *args) -> int:
@@ -109,9 +112,9 @@ def append(k: torch.Tensor, v: torch.Tensor, k_rows: QuantizedRows, v_rows: Quan
         k = k.contiguous()
     if v.stride(3) != 1:
         v = v.contiguous()
-    strides = _Eighteen(*k.stride()[:3], *v.stride()[:3], *_steps(k_rows), *_steps(v_rows))
-    check(_on(k, lib().ttb_quantized_append, k.data_ptr(), v.data_ptr(), k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides,
-              slots.data_ptr(), _TYPES[k.dtype], b, s, h, d, bits, k_rows.slots), "quantised append")
+    call = _pack_append(k.data_ptr(), v.data_ptr(), k_rows.codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), *k.stride()[:3], *v.stride()[:3],
+                        *_steps(k_rows), *_steps(v_rows), slots.data_ptr(), _TYPES[k.dtype], b, s, h, d, bits, k_rows.slots)
+    check(_on(k, lib().ttb_quantized_append, call), "quantised append")
 
 
 def read(k_rows: QuantizedRows, v_rows: QuantizedRows, start: int, stop: int, dtype: torch.dtype, size: Tuple[int, int, int, int, int]) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -121,9 +124,9 @@ def read(k_rows: QuantizedRows, v_rows: QuantizedRows, start: int, stop: int, dt
     k = codes.new_empty((b, n, h, d), dtype=dtype)
     v = torch.empty_like(k)
     if b and n and h:
-        strides = _Twelve(*_steps(k_rows), *_steps(v_rows))
-        check(_on(codes, lib().ttb_quantized_read, codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), strides, k.data_ptr(), v.data_ptr(), b, start,
-                  n, h, d, bits, int(dtype == torch.float32)), "quantised read")
+        call = _pack_read(codes.data_ptr(), k_rows.scales.data_ptr(), v_rows.codes.data_ptr(), v_rows.scales.data_ptr(), *_steps(k_rows), *_steps(v_rows), k.data_ptr(), v.data_ptr(), b, start,
+                          n, h, d, bits, dtype == torch.float32)
+        check(_on(codes, lib().ttb_quantized_read, call), "quantised read")
     return k, v
 
 
@@ -154,7 +157,7 @@ def attention(q: torch.Tensor, mask: AttentionMask, scale: Optional[float], size
     if q.data_ptr() & 15:
         q = q.clone()
     o = torch.empty_like(q)
-    seen, seen_b, seen_r, start, offset, window, sinks = None, 0, 0, None, -1, 0, 0
+    seen, seen_b, seen_r, start, offset, window, sinks = 0, 0, 0, None, -1, 0, 0
     m = mask.bool_mask
     if m is not None:
         m = m if m.dim() == 3 else m[:, 0]
@@ -177,6 +180,7 @@ def attention(q: torch.Tensor, mask: AttentionMask, scale: Optional[float], size
     if n >= 2048 and b * hkv * 8 < 592:  # few and long rows are split further than a cluster reaches
         floats = 128 * b * s * hq * (d + 4)
         work = torch.empty(floats, dtype=torch.float32, device=q.device)
-    check(_on(q, lib().ttb_quantized_attention, q.data_ptr(), *steps[:4], _Eight(*steps[4:]), o.data_ptr(), seen, seen_b, seen_r, None if start is None else start.data_ptr(), offset, window, sinks, b, s, n, hq, hkv, d, bits,
-              1.0 / math.sqrt(d) if scale is None else float(scale), None if work is None else work.data_ptr(), floats), "attention over a quantised cache")
+    call = _pack_attention(q.data_ptr(), *steps, o.data_ptr(), seen, seen_b, seen_r, 0 if start is None else start.data_ptr(), offset, window, sinks, b, s, n, hq, hkv, d, bits,
+                           0 if work is None else work.data_ptr(), floats)
+    check(_on(q, lib().ttb_quantized_attention, call, 1.0 / math.sqrt(d) if scale is None else float(scale)), "attention over a quantised cache")
     return o
