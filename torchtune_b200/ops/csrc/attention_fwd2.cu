@@ -12,7 +12,10 @@
 // none; each tile visits only its own range of key blocks.  A boolean mask comes with the bounds of its rows in any order (the MASKED
 // form takes a tile's range from all its rows) and a flag per row that says whether everything between its bounds is visible: then the
 // bounds are the whole mask, as for the causal masks of cached generation, and only the other rows read mask bytes.
-// FIRST: a causal window beside which the first positions stay visible; both tiles visit the blocks of the first positions and then those of the window.
+// FIRST: a causal window beside which the first positions stay visible; a tile visits the blocks of the first positions and then those of its window.  These visits are short, and what a CTA does in
+// front of them and behind them counts: one tile per CTA, and two CTAs per SM that hide it from one another (for 128 channels with one stage of K and V each).  Against two tiles per CTA, 32 / 8 heads,
+// 4 first positions: 1 x 6000 tokens of 128 channels, window 1024, 206 -> 184 us; 4 x 4096, window 512, 393 -> 342; 1 x 16384, window 4096, 1276 -> 1139; 4 x 1413 of 64, window 200, 103 -> 84 us.
+// With 64 channels the exponentials bound it (twice those of the visible pairs are taken at a window of 200), with 128 they and the products, which take turns within a tile.
 // Causal forward, head dim 64 (one-tile kernel before): 8 x 2048 tokens 788 -> 374 us, 1 x 16384 tokens 5079 -> 2042 us; exponentials bound it.
 // Soft-capped scores stay on the one-tile kernel in attention.cu.  Every wait is bounded and reports through the error word.
 #include "common/attn_math.cuh"
@@ -28,6 +31,11 @@ template <int D>
 static constexpr int kTileBytesOf = kBlk * D * 2;
 template <int D>
 static constexpr int kSmemBytes = 6 * kTileBytesOf<D> + 1024 + 256;
+static constexpr int kThreadsOne = 192;  // FIRST: one query tile
+template <int D>
+static constexpr int kStagesOne = D == 64 ? 2 : 1;  // of keys and of values: two CTAs share an SM
+template <int D>
+static constexpr int kSmemBytesOne = (1 + 2 * kStagesOne<D>) * kTileBytesOf<D> + 1024 + 256;
 
 struct Params {
   int b, s, sk, hq, hkv;
@@ -57,15 +65,18 @@ __device__ __forceinline__ uint32_t keys_between(int k0, int first, int last) {
 }
 
 template <int D, bool MASKED, bool FIRST>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(FIRST ? kThreadsOne : kThreads, FIRST ? 2 : 1)
 attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, Params p) {
   constexpr int kTileBytes = kTileBytesOf<D>, kPanels = D / 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ[2] = {smem, smem + kTileBytes};
-  uint8_t* sK[2] = {smem + 2 * kTileBytes, smem + 3 * kTileBytes};
-  uint8_t* sV[2] = {smem + 4 * kTileBytes, smem + 5 * kTileBytes};
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * kTileBytes);
+  constexpr int kTiles = FIRST ? 1 : 2;  // of queries
+  constexpr uint32_t kColumns = FIRST ? 256 : 512;
+  uint8_t* sQ[2] = {smem, smem + (kTiles - 1) * kTileBytes};
+  constexpr int kStages = FIRST ? kStagesOne<D> : 2;
+  uint8_t* sK[2] = {smem + kTiles * kTileBytes, smem + (kTiles + kStages - 1) * kTileBytes};
+  uint8_t* sV[2] = {smem + (kTiles + kStages) * kTileBytes, smem + (kTiles + 2 * kStages - 1) * kTileBytes};
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (kTiles + 2 * kStages) * kTileBytes);
   uint64_t* q_full = bars;        // both query tiles
   uint64_t* k_full = bars + 1;    // [2]
   uint64_t* k_empty = bars + 3;   // [2]
@@ -82,7 +93,7 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   // FIRST: grid (heads, batch, tiles), the last tiles first, so that those which see less than a window end the launch
   const int h = FIRST ? blockIdx.x : blockIdx.y, bi = FIRST ? blockIdx.y : blockIdx.z;
   const int hk = h / (p.hq / p.hkv);
-  const int q0 = (FIRST ? gridDim.z - 1 - blockIdx.z : blockIdx.x) * 2 * kBlk;
+  const int q0 = (FIRST ? gridDim.z - 1 - blockIdx.z : blockIdx.x) * kTiles * kBlk;
   const int row_base = bi * p.s;
   const int krow_base = bi * p.sk;
   const long long bound_base = MASKED ? bi * p.bound_b : row_base;
@@ -106,19 +117,15 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
   // Key-block range of each tile: [begin, begin + count).  The bounds are monotone, so first and last row give them.
   int begin[2], count[2];
-  // FIRST: blocks are numbered along what the two tiles visit: `heads` blocks of first positions, from the first one of the first row's document on and as wide as needed, then those from block
-  // `tail0` of the keys on, where the window of the first row begins (a document that begins later has its first positions there).  The second tile leaves out `skip` blocks of the latter.
-  int heads = 0, head_key = 0, head_end = 0, tail0 = 0, skip = 0;
+  // FIRST: blocks are numbered along what the tile visits: `heads` blocks of first positions, from the first one of the first row's document on and as wide as needed, then those from block
+  // `tail0` of the keys on, where the window of the first row begins (a document that begins later has its first positions there).
+  int heads = 0, head_key = 0, head_end = 0, tail0 = 0;
   const int shift = p.sk - p.s;
   if constexpr (FIRST) {
     head_key = p.start != nullptr ? p.start[row_base + q0] : 0;
     tail0 = max(head_key, q0 + shift - p.window + 1) / kBlk;
     head_end = min(head_key + p.sinks, tail0 * kBlk);
     heads = head_end > head_key ? (head_end - head_key + kBlk - 1) / kBlk : 0;
-    if (const int qb = q0 + kBlk; qb < p.s) {
-      const int start = p.start != nullptr ? p.start[row_base + qb] : 0, lo = max(start, qb + shift - p.window + 1);
-      if (start == lo || start + p.sinks <= tail0 * kBlk) skip = lo / kBlk - tail0;
-    }
   }
   auto block_key = [&](int i) {  // first key of block i
     if constexpr (FIRST) return i < heads ? head_key + i * kBlk : (tail0 + i - heads) * kBlk;
@@ -128,15 +135,12 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if constexpr (FIRST) return i < heads ? min(4, (head_end - head_key - i * kBlk + 31) >> 5) : 4;
     return 4;
   };
-  auto skipped = [&](int x) { return FIRST && x == 1 ? skip : 0; };
-  auto resume = [&](int x) { return heads + skipped(x); };  // the first of the window's blocks that tile x visits
-  auto local = [&](int x, int i) { return FIRST && i >= heads ? i - skipped(x) : i; };  // FIRST: count of the blocks of tile x in front of block i
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const int qa = q0 + x * kBlk;
     if constexpr (FIRST) {
       begin[x] = 0;
-      count[x] = qa < p.s ? heads + (min(qa + kBlk, p.s) - 1 + shift) / kBlk + 1 - tail0 - skipped(x) : 0;
+      count[x] = x < kTiles ? heads + (min(qa + kBlk, p.s) - 1 + shift) / kBlk + 1 - tail0 : 0;
       continue;
     }
     if (qa >= p.s) {
@@ -156,9 +160,7 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (begin[late] > end) count[late] += begin[late] - end, begin[late] = end;
   }
   int u_begin, u_end;  // union of the two ranges
-  if constexpr (FIRST) {
-    u_begin = 0, u_end = max(count[0], count[1] > 0 ? count[1] + skip : 0);
-  } else if (count[0] > 0 && count[1] > 0) {
+  if (count[0] > 0 && count[1] > 0) {
     u_begin = min(begin[0], begin[1]);
     u_end = max(begin[0] + count[0], begin[1] + count[1]);
   } else if (count[0] > 0) {
@@ -182,8 +184,9 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 2) {
-    tmem_alloc(tmem_slot, 512);
+  constexpr int kHolder = FIRST ? 1 : 2;
+  if (warp == kHolder) {
+    tmem_alloc(tmem_slot, kColumns);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -191,13 +194,13 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t tS[2] = {tmem_base, tmem_base + 128};
-  const uint32_t tO[2] = {tmem_base + 256, tmem_base + 384};
+  const uint32_t tO[2] = {tmem_base + kTiles * 128, tmem_base + 384};
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
     if (lane == 0 && n_union > 0) {
-      mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
-      for (int x = 0; x < 2; ++x)
+      mbar_arrive_expect_tx(q_full, kTiles * kTileBytes);
+      for (int x = 0; x < kTiles; ++x)
         for (int j = 0; j < kPanels; ++j) tma_load_2d(sQ[x] + j * kPanelBytes, &tmQ, q_full, h * D + j * 64, row_base + q0 + x * kBlk);
     }
     auto load_rows = [&](uint8_t* to, const CUtensorMap* m, uint64_t* bar, int col, int key) {
@@ -208,7 +211,7 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     };
     uint32_t phase = 0;
     for (int i = 0; i < n_union && !*abort_flag; ++i) {
-      const int st = i & 1;
+      const int st = i & (kStages - 1);
       const int kv0 = block_key(u_begin + i);
       if (!mbar_wait(&k_empty[st], phase ^ 1)) {
         fail(abort_flag, p.err, 211);
@@ -228,7 +231,7 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         for (int j = 0; j < kPanels; ++j) load_rows(sV[st] + j * kPanelBytes, &tmV, &v_full[st], hk * D + j * 64, kv0);
       }
       __syncwarp();
-      if (st == 1) phase ^= 1;
+      if (st == kStages - 1) phase ^= 1;
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
@@ -240,20 +243,12 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     bool ok = n_union == 0 || mbar_wait(q_full, 0);
     int k_ready = u_begin - 1;  // highest block whose K tile has been waited for
     int v_ready = u_begin - 1;
-    auto active = [&](int x, int j) {
-      if constexpr (FIRST) return count[x] > 0 && (j < heads || j >= resume(x)) && j < count[x] + skipped(x);
-      return count[x] > 0 && j >= begin[x] && j < begin[x] + count[x];
-    };
-    // FIRST: scores are issued one block ahead, but over a gap when its end is reached: the first tile, which has no gap, hands the stage of K on to the second
-    auto starts = [&](int x, int j) {
-      if constexpr (FIRST) return (j == 0 && heads > 0) || (j == resume(x) && (heads == 0 || skipped(x) > 0));
-      return j == begin[x];
-    };
+    auto active = [&](int x, int j) { return count[x] > 0 && j >= begin[x] && j < begin[x] + count[x]; };
     // S_x(j) = Q_x · K_jᵀ; the K stage is handed back after the last tile that reads it
     auto issue_s = [&](int x, int j) -> bool {
-      const int i = j - u_begin, st = i & 1;
+      const int i = j - u_begin, st = i & (kStages - 1);
       if (j > k_ready) {
-        if (!mbar_wait(&k_full[st], (i >> 1) & 1)) return false;
+        if (!mbar_wait(&k_full[st], (i / kStages) & 1)) return false;
         k_ready = j;
       }
       tc_fence_after();
@@ -269,17 +264,17 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     };
     for (int j = u_begin; j < u_end && ok && !*abort_flag; ++j) {
       for (int x = 0; x < 2 && ok; ++x)
-        if (active(x, j) && starts(x, j)) ok = issue_s(x, j);  // first block of a tile
+        if (active(x, j) && j == begin[x]) ok = issue_s(x, j);  // first block of a tile
       for (int x = 0; x < 2 && ok; ++x) {
         if (!active(x, j)) continue;
-        const int n = FIRST ? local(x, j) : j - begin[x];  // tile-local block counter
-        const int i = j - u_begin, st = i & 1;
+        const int n = j - begin[x];  // tile-local block counter
+        const int i = j - u_begin, st = i & (kStages - 1);
         if (!mbar_wait(&p_full[x], n & 1)) {
           ok = false;
           break;
         }
         if (j > v_ready) {
-          if (!mbar_wait(&v_full[st], (i >> 1) & 1)) {
+          if (!mbar_wait(&v_full[st], (i / kStages) & 1)) {
             ok = false;
             break;
           }
@@ -295,18 +290,13 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           if (n + 1 == count[x]) umma_commit(&o_done[x]);
         }
         __syncwarp();
-        if constexpr (FIRST) {
-          const int next = j + 1 == heads ? resume(x) : j + 1;
-          if (n + 1 < count[x] && !starts(x, next)) ok = issue_s(x, next);
-        } else {
-          if (n + 1 < count[x]) ok = issue_s(x, j + 1);
-        }
+        if (n + 1 < count[x]) ok = issue_s(x, j + 1);
       }
     }
     if (!ok) fail(abort_flag, p.err, 213);
-  } else if (warp >= 4) {
+  } else if (warp >= (FIRST ? 2 : 4)) {
     // ---------------------------------------------------------------- softmax / correction / epilogue, one warpgroup per tile
-    const int x = (warp - 4) >> 2;
+    const int x = FIRST ? 0 : (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const int qa = q0 + x * kBlk;
@@ -364,7 +354,7 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
     }
     for (int n = n_first; n < count[x] && !*abort_flag; ++n) {
-      const int block = FIRST && n >= heads ? n + skipped(x) : begin[x] + n, kv0 = block_key(block);
+      const int block = begin[x] + n, kv0 = block_key(block);
       if (!mbar_wait(&s_full[x], n & 1)) {
         ok = false;
         break;
@@ -517,7 +507,7 @@ attn_fwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 2) tmem_dealloc(tmem_base, 512);
+  if (warp == kHolder) tmem_dealloc(tmem_base, kColumns);
 }
 
 template <int D>
@@ -539,17 +529,19 @@ static int launch(const void* q, const void* k, const void* v, const Params& p, 
   if ((rc = make_head_map<D>(&tq, q, p.b, p.s, p.hq)) != kOk) return rc;
   if ((rc = FIRST ? make_rows_map<D>(&tk, k, p.b, p.sk, p.hkv) : make_head_map<D>(&tk, k, p.b, p.sk, p.hkv)) != kOk) return rc;
   if ((rc = FIRST ? make_rows_map<D>(&tv, v, p.b, p.sk, p.hkv) : make_head_map<D>(&tv, v, p.b, p.sk, p.hkv)) != kOk) return rc;
+  constexpr int smem = FIRST ? kSmemBytesOne<D> : kSmemBytes<D>;
   static bool attr[64] = {};  // an attribute of the kernel on one device
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return kErrDriver;
   if (!attr[device]) {
-    if (cudaFuncSetAttribute(attn_fwd2_kernel<D, MASKED, FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<D>) != cudaSuccess) return kErrDriver;
+    if (cudaFuncSetAttribute(attn_fwd2_kernel<D, MASKED, FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return kErrDriver;
     attr[device] = true;
   }
-  const unsigned tiles = (p.s + 2 * kBlk - 1) / (2 * kBlk);
+  constexpr int kRows = (FIRST ? 1 : 2) * kBlk;
+  const unsigned tiles = (p.s + kRows - 1) / kRows;
   const dim3 grid = FIRST ? dim3(p.hq, p.b, tiles) : dim3(tiles, p.hq, p.b);
   TTB_COUNT_LAUNCH(1);
-  attn_fwd2_kernel<D, MASKED, FIRST><<<grid, kThreads, kSmemBytes<D>, st>>>(tq, tk, tv, p);
+  attn_fwd2_kernel<D, MASKED, FIRST><<<grid, FIRST ? kThreadsOne : kThreads, smem, st>>>(tq, tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrDriver;
 }
 
