@@ -50,8 +50,8 @@ struct Params {
   // The first positions are seen by all later queries.  Without documents the queries beyond the window of a block that holds some are cut into `pieces` runs of `piece` query blocks, each a
   // CTA of its own, so that no CTA walks the whole sequence; their gradients and those of the block's own CTA meet in `partial` [b * hkv][blocks][1 + pieces][rows][dk, dv][D].
   int blocks, pieces, piece, rows;
-  // Launches of up to four waves go through pieces and key blocks with all heads at a time, so that the last key blocks, which fewer queries than a window see, end them (1 x 6000 tokens, window
-  // 1024, forward and backward 620 -> 615 us; 4 x 1413 packed 283 -> 267); larger ones a head at a time, whose neighbouring blocks share queries (4 x 4096 backward 961 us, the other way 985).
+  // Launches of up to four waves go through pieces and key blocks with all heads at a time, so that the last key blocks, which fewer queries than a window see, end them (5 us of
+  // 350 less at 1 x 6000 tokens, window 1024, 16 of 130 at 4 x 1413 packed); larger ones a head at a time, whose neighbouring blocks share queries (4 x 4096 backward 961 us, the other way 985).
   int by_length;
   float* partial;
 };

@@ -707,7 +707,7 @@ static long long bit_bytes(int tiles, int s, int splits) { return (static_cast<l
 
 // Splits of a key head's tiles, by a model of the time in units of what an SM needs for one round of tiles of a CTA's warps when it is full (0.57 us at 4 bits and 128 channels): an SM works off
 // its share of the CTAs in waves of those that it holds, a wave costs 8 units of latency in front of and behind its tiles and at least 1.4 per round, and a join in the workspace another 8.
-// Measured and modelled us (4 bits, 128 channels): 64 x 4096 slots, 1 split 74 / 73, 2 74 / 73, 8 96 / 96; 16 x 732, 1 11 / 9, 8 17 / 18; 1 x 65 003, 8 54 / 56, 32 in the workspace 30 / 30.
+// Measured (without a graph) and modelled us (4 bits, 128 channels): 64 x 4096 slots, 1 split 74 / 73, 2 74 / 73, 8 96 / 96; 16 x 732, 1 11 / 9, 8 17 / 18; 1 x 65 003, 8 54 / 56, 32 in the workspace 30 / 30.
 // Of equal ones `more` takes the larger, where two stages of a tile hide less latency than a wave of more CTAs (32 x 4096 of 64 channels, 1 and 2 splits: 33 and 31 us in 4 bits, 39 and 43 in 8).
 static int splits_of(long long pairs, int tiles, int s, int per_sm, bool spread, bool more) {
   int best = 0;
