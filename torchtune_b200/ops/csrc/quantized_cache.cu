@@ -11,9 +11,9 @@
 // Rows come as bf16, fp16 or fp32 (the scale of the latter two is rounded, and codes are those of the scale that is stored).
 //
 // Rows lie [batch, head, slot]: a head's rows are one stream for the attention kernel.  A thread has 8 channels, 16 bytes of bf16.  Measured (4 bits, 8 heads of 128 channels, cold L2): 2 x 8000
-// tokens 26.5 us written, 17.3 us read (83.5 MB: 3.2 and 4.8 TB/s); 1 x 65 000 tokens 95.7 and 61.1 us (3.5 and 5.6); one token of 16 rows 4 and 3.3 us, a launch.  Reading is bound by its bytes; writing
-// by issue: 165 instructions per 8 channels (unpacking, the two extrema, codes and their packing), at 0.79 of the rate.  With one token to a thread and
-// divisions instead of products with the reciprocal the first took 55 and 34 us.
+// tokens 25 us written, 17.5 us read (83.5 MB: 3.4 and 4.8 TB/s); 1 x 65 000 tokens 88 and 60 us (3.9 and 5.7); one token of 16 rows 4 and 3.3 us, a launch.  Reading is bound by its bytes; writing
+// by issue: about 150 instructions per 8 channels (unpacking, the two extrema, codes and their packing), two fifths of them in the integer unit, which takes one every other cycle.  With one token to a
+// thread and divisions instead of products with the reciprocal the first took 55 and 34 us; with eight tokens to a thread it takes 27.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -60,10 +60,11 @@ constexpr bool kHalfPrecision<__half> = true;
 static constexpr int kRun = 4;
 struct Spread {
   int units, lanes, sub;
+  uint32_t per_lane;  // 2^20 / lanes, rounded up: a CTA's thread over `lanes` without a division
 };
 static Spread spread_of(long long units, int per_cta) {
   Spread sp;
-  sp.units = static_cast<int>(units), sp.lanes = static_cast<int>(units < per_cta ? units : per_cta), sp.sub = per_cta / sp.lanes;
+  sp.units = static_cast<int>(units), sp.lanes = static_cast<int>(units < per_cta ? units : per_cta), sp.sub = per_cta / sp.lanes, sp.per_lane = ((1u << 20) + sp.lanes - 1) / sp.lanes;
   return sp;
 }
 
@@ -86,12 +87,14 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
   const int groups = GROUPS > 0 ? GROUPS : some_groups;
   const int which = blockIdx.z & 1, bi = blockIdx.z >> 1;
   const int lane = threadIdx.x & 31, t = lane & 3, quad = threadIdx.x >> 2;
-  const int sub = quad / sp.lanes, unit = blockIdx.y * sp.lanes + (quad - sub * sp.lanes);
+  const int sub = static_cast<int>(quad * sp.per_lane >> 20), unit = blockIdx.y * sp.lanes + (quad - sub * sp.lanes);
   const bool live = sub < sp.sub && unit < sp.units;
   const int head = live ? unit / groups : 0, j = live ? unit - head * groups : 0;
   const int run = t * groups + j;  // runs of eight channels
   const int i0 = blockIdx.x * (kRun * sp.sub) + sub;
   const long long first = p.slots[0];
+  // tokens whose slot is in the cache
+  const int from_i = first >= 0 ? 0 : first <= -p.s ? p.s : static_cast<int>(-first), to_i = first >= p.slot_count ? 0 : first <= p.slot_count - p.s ? p.s : static_cast<int>(p.slot_count - first);
   const T* row = static_cast<const T*>(p.x[which]) + bi * p.x_b[which] + head * p.x_h[which] + run * 8 + (live && i0 < p.s ? i0 : 0) * p.x_s[which];
   const long long step = sp.sub * p.x_s[which];
   T from[kRun][8];
@@ -100,7 +103,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
   for (int k = 0; k < kRun; ++k) {
     const int i = i0 + k * sp.sub;
     const bool there = live && i < p.s;
-    ours[k] = there && p.slots[i] == first + i && first + i >= 0 && first + i < p.slot_count;
+    ours[k] = there && i >= from_i && i < to_i && p.slots[i] == first + i;
     if (k > 0 && there) row += step;
     if (WIDE) {
 #pragma unroll
@@ -143,20 +146,22 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     const float s = __bfloat162float(scale);
     const bool usable = s != 0.f && fabsf(s) <= 3.4e38f;
     uint32_t code[2] = {0u, 0u};  // 4 bits: one word; 8 bits: two
+    constexpr int kPer = 32 / BITS;
     auto put = [&](int e, uint32_t c) {
-      constexpr int kPer = 32 / BITS;
       asm("mad.lo.u32 %0, %1, %2, %0;" : "+r"(code[e / kPer]) : "r"(c), "r"(1u << (BITS * (e % kPer))));  // the integer unit is what bounds this kernel; this is not on it
     };
     if (sizeof(T) == 2 && !kHalfPrecision<T> && fabsf(s) >= 1e-30f && usable) {
       // bf16: a quotient is a tie or at least 2^-10 away from one (see above).  The product with the reciprocal (off by at most 2^-22 of itself) is off by at most 2^-15, so that on a grid of 2^-10 it lies on the same side, and a tie
-      // on itself; the last sum rounds it to a whole number, ties to even, and leaves that in the low bits.  A tenth of the instructions of a division.
+      // on itself: 1.5 x 2^13 + quotient has that grid.  The sum that brings it to 1.5 x 2^23 + h is rounded to a whole number, ties to even, whose low bits are the code; what the exponents add up to in a word of
+      // codes is taken off beforehand.  A tenth of the instructions of a division.
+      constexpr uint32_t kBase = 0x4b400000u;  // 1.5 x 2^23
+      code[0] = code[1] = 0u - kBase * (BITS == 4 ? 0x11111111u : 0x01010101u);
       float inv;
       asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float grid = __fadd_rn(__fmaf_rn(v[e], inv, 12288.f), -12288.f);  // 1.5 x 2^13
-        const uint32_t c = __float_as_uint(__fadd_rn(grid, 12582912.f + kHalf)) - 0x4b400000u;  // 1.5 x 2^23
-        put(e, min(c, 2u * kHalf - 1u));  // no quotient is below -h: m itself gives that
+        const uint32_t c = __float_as_uint(__fadd_rn(__fmaf_rn(v[e], inv, 12288.f), 12582912.f - 12288.f + kHalf));
+        put(e, min(c, kBase + 2u * kHalf - 1u));  // no quotient is below -h: m itself gives that
       }
     } else {
 #pragma unroll
@@ -185,7 +190,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
   constexpr float kHalf = 1 << (BITS - 1);
   const int groups = GROUPS > 0 ? GROUPS : some_groups;
   const int which = blockIdx.z & 1, bi = blockIdx.z >> 1;
-  const int sub = threadIdx.x / sp.lanes, unit = blockIdx.y * sp.lanes + (threadIdx.x - sub * sp.lanes);
+  const int sub = static_cast<int>(threadIdx.x * sp.per_lane >> 20), unit = blockIdx.y * sp.lanes + (threadIdx.x - sub * sp.lanes);
   if (sub >= sp.sub || unit >= sp.units) return;
   const int runs = 4 * groups, head = unit / runs, run = unit - head * runs;
   const int i0 = blockIdx.x * (kRun * sp.sub) + sub;
