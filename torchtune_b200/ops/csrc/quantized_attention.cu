@@ -112,7 +112,7 @@ struct Layout {
   static constexpr int kCodes = kTileKeys * kRow;
   static constexpr int kScales = kTileKeys * kGroups * 2;
   static constexpr int kStage = 2 * (kCodes + kScales);
-  static constexpr int kStages = BITS == 8 && D <= 128 ? 3 : 2;
+  static constexpr int kStages = 2;                   // a third takes room from other CTAs (8 bits, 16 x 4111 slots of 128 channels, 16 query rows: 47 us, with three 51; 1 x 65 000, one: 38.7 and 42.0)
   static constexpr int kWarpRing = kStages * kStage;
   // where 16-byte piece `piece` of key `key` lies: the four rows of values that a quarter of a warp reads at once (even keys) are spread over the banks
   __device__ static __forceinline__ int place(int key, int piece) {
@@ -708,15 +708,15 @@ static long long bit_bytes(int tiles, int s, int splits) { return (static_cast<l
 // Splits of a key head's tiles, by a model of the time in units of what an SM needs for one round of tiles of a CTA's warps when it is full (0.57 us at 4 bits and 128 channels): an SM works off
 // its share of the CTAs in waves of those that it holds, a wave costs 8 units of latency in front of and behind its tiles and at least 1.4 per round, and a join in the workspace another 8.
 // Measured (without a graph) and modelled us (4 bits, 128 channels): 64 x 4096 slots, 1 split 74 / 73, 2 74 / 73, 8 96 / 96; 16 x 732, 1 11 / 9, 8 17 / 18; 1 x 65 003, 8 54 / 56, 32 in the workspace 30 / 30.
-// Of equal ones `more` takes the larger, where two stages of a tile hide less latency than a wave of more CTAs (32 x 4096 of 64 channels, 1 and 2 splits: 33 and 31 us in 4 bits, 39 and 43 in 8).
-static int splits_of(long long pairs, int tiles, int s, int per_sm, bool spread, bool more) {
+// Of equal ones it takes the larger, since two stages of a tile hide less latency than a wave of more CTAs (32 x 4096 of 64 channels, 1 and 2 splits: 33 and 31 us in 4 bits, 41 and 37 in 8).
+static int splits_of(long long pairs, int tiles, int s, int per_sm, bool spread) {
   int best = 0;
   long long least = 0, least_waves = 0;
   for (int n = 1; n <= (spread ? kMaxSpread : kMaxCluster); n += n < kMaxCluster ? n : 1) {  // clusters of 3, 5 or 7 are placed worse
     if (bit_bytes(tiles, s, n) > kMaxBitBytes) continue;
     const long long ctas = (pairs * n + sm_count() - 1) / sm_count(), waves = (ctas + per_sm - 1) / per_sm, rounds = (tiles + n * kWarps - 1) / (n * kWarps);
     const long long cost = max(10 * ctas * rounds, 14 * waves * rounds) + 80 * waves + (n > kMaxCluster ? 80 : 0);
-    if (best == 0 || cost < least || (more && cost == least && waves == least_waves)) best = n, least = cost, least_waves = waves;
+    if (best == 0 || cost < least || (cost == least && waves == least_waves)) best = n, least = cost, least_waves = waves;
   }
   return best;
 }
@@ -738,7 +738,7 @@ static int launch(const Params& p, int b, long long work_floats, cudaStream_t st
   }
   const int rows = p.s * (p.hq / p.hkv);
   const long long pairs = static_cast<long long>(b) * p.hkv;
-  const int splits = splits_of(pairs, tiles, p.s, resident[device], work_floats >= kMaxSpread * pairs * rows * kPitch<D>, Layout<D, BITS>::kStages == 2);
+  const int splits = splits_of(pairs, tiles, p.s, resident[device], work_floats >= kMaxSpread * pairs * rows * kPitch<D>);
   if (splits == 0) return kErrTooLarge;
   const int spread = splits > kMaxCluster ? 1 : 0;
   cudaLaunchConfig_t cfg = {};
