@@ -708,15 +708,16 @@ static long long bit_bytes(int tiles, int s, int splits) { return (static_cast<l
 // Splits of a key head's tiles, by a model of the time in units of what an SM needs for one round of tiles of a CTA's warps when it is full (0.57 us at 4 bits and 128 channels): an SM works off
 // its share of the CTAs in waves of those that it holds, a wave costs 8 units of latency in front of and behind its tiles and at least 1.4 per round, and a join in the workspace another 8.
 // Measured (without a graph) and modelled us (4 bits, 128 channels): 64 x 4096 slots, 1 split 74 / 73, 2 74 / 73, 8 96 / 96; 16 x 732, 1 11 / 9, 8 17 / 18; 1 x 65 003, 8 54 / 56, 32 in the workspace 30 / 30.
-// Of equal ones it takes the larger, since two stages of a tile hide less latency than a wave of more CTAs (32 x 4096 of 64 channels, 1 and 2 splits: 33 and 31 us in 4 bits, 41 and 37 in 8).
+// Of equal ones it takes the larger if its CTAs have fewer rounds, since two stages of a tile hide less latency than a wave of more CTAs (32 x 4096 of 64 channels, 1 and 2 splits: 33 and 31 us in 4
+// bits, 41 and 37 in 8).
 static int splits_of(long long pairs, int tiles, int s, int per_sm, bool spread) {
   int best = 0;
-  long long least = 0, least_waves = 0;
+  long long least = 0, least_waves = 0, least_rounds = 0;
   for (int n = 1; n <= (spread ? kMaxSpread : kMaxCluster); n += n < kMaxCluster ? n : 1) {  // clusters of 3, 5 or 7 are placed worse
     if (bit_bytes(tiles, s, n) > kMaxBitBytes) continue;
     const long long ctas = (pairs * n + sm_count() - 1) / sm_count(), waves = (ctas + per_sm - 1) / per_sm, rounds = (tiles + n * kWarps - 1) / (n * kWarps);
     const long long cost = max(10 * ctas * rounds, 14 * waves * rounds) + 80 * waves + (n > kMaxCluster ? 80 : 0);
-    if (best == 0 || cost < least || (cost == least && waves == least_waves)) best = n, least = cost, least_waves = waves;
+    if (best == 0 || cost < least || (cost == least && waves == least_waves && rounds < least_rounds)) best = n, least = cost, least_waves = waves, least_rounds = rounds;
   }
   return best;
 }

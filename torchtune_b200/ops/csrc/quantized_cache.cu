@@ -11,8 +11,8 @@
 // Rows come as bf16, fp16 or fp32 (the scale of the latter two is rounded, and codes are those of the scale that is stored).
 //
 // Rows lie [batch, head, slot]: a head's rows are one stream for the attention kernel.  A thread has 8 channels, 16 bytes of bf16.  Measured (4 bits, 8 heads of 128 channels, cold L2): 2 x 8000
-// tokens 25 us written, 17.5 us read (83.5 MB: 3.4 and 4.8 TB/s); 1 x 65 000 tokens 88 and 60 us (3.9 and 5.7); one token of 16 rows 4 and 3.3 us, a launch.  Reading is bound by its bytes; writing
-// by issue: about 150 instructions per 8 channels (unpacking, the two extrema, codes and their packing), two fifths of them in the integer unit, which takes one every other cycle.  With one token to a
+// tokens 25 us written, 17.5 us read (83.5 MB: 3.4 and 4.8 TB/s); 1 x 65 000 tokens 86 and 60 us (4.0 and 5.7); one token of 16 rows 4 and 3.3 us, a launch.  Reading is bound by its bytes; writing
+// by issue: 151 instructions per 8 channels (unpacking, the two extrema, codes and their packing) at 0.74 of the rate, two fifths of them in the integer unit, which takes one every other cycle (59 %).  With one token to a
 // thread and divisions instead of products with the reciprocal the first took 55 and 34 us; with eight tokens to a thread it takes 27.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
