@@ -449,3 +449,12 @@ def test_few_long_rows_recorded():
     dense = torch.rand(1, 1, 20000, generator=_gen(3), device="cuda") < 0.4
     _check(q[0], k_rows, v_rows, AttentionMask(causal=False, bool_mask=dense), dense)
     assert not ops.quantized_attention(q[0], k_rows, v_rows, AttentionMask(causal=False, bool_mask=torch.zeros_like(dense))).any()
+
+
+@pytest.mark.parametrize("d, bits", [(64, 8), (128, 4), (256, 8)])
+@pytest.mark.parametrize("n, window", [(6143, 0), (6144, 0), (6271, 0), (6305, 0), (12345, 0), (30011, 0), (30011, 6139), (30011, 6140), (30011, 20000)])
+def test_lengths_where_few_rows_are_split_further(n, window, d, bits):
+    k_rows, v_rows = _filled(1, n, 1, d, bits, seed=n)
+    at = torch.arange(n, device="cuda")
+    dense = ((at > n - 1 - window) | (at < 4))[None, None] if window else torch.ones(1, 1, n, dtype=torch.bool, device="cuda")
+    _check(_queries(1, 1, 4, d), k_rows, v_rows, AttentionMask(causal=True, window=window, sinks=4 if window else 0), dense)

@@ -109,3 +109,24 @@ def test_windows_over_a_quantised_cache_and_left_padded_rows():
             layer.attn.kv_cache, layer.attn.cache_enabled = None, False
     # padding changes neither positions nor what is seen: the same sums in another order
     assert (results[0] - results[1]).abs().max() <= 1e-3 * results[0].abs().max()
+
+
+def test_which_calls_are_windows_of_the_kernels():
+    from torchtune_b200.ops._cuda_attention import takes_window, unsupported_reason
+
+    q, k = torch.zeros(1, 8, 4, 64), torch.zeros(1, 9, 2, 64)
+    ids = torch.zeros(1, 8, dtype=torch.int32)
+    takes = lambda q, k, softcap=0.0, **mask: takes_window(q, k, AttentionMask(**mask), softcap)  # noqa: E731
+    assert takes(q, q[:, :, :2], window=4, sinks=1) and takes(q, q[:, :, :2], window=4, sinks=1, doc_ids=ids) and takes(q, k, window=4) and takes(q, k, window=4, sinks=2, softcap=None)
+    for kind in (dict(window=4), dict(sinks=2), dict(window=4, sinks=2, causal=False), dict(window=4, sinks=2, chunk=4), dict(window=4, sinks=2, bool_mask=torch.ones(1, 8, 8, dtype=torch.bool))):
+        assert not takes(q, q[:, :, :2], **kind)
+    assert not takes(q, q[:, :, :2], window=4, sinks=2, softcap=30.0) and not takes(q, k, window=4, sinks=2, doc_ids=ids) and not takes(k, q[:, :, :1], window=4, sinks=2)
+    assert not takes(q, torch.zeros(1, 8, 3, 64), window=4, sinks=2)
+    assert "first tokens" in unsupported_reason(q, q[:, :, :2], AttentionMask(window=4, sinks=2, chunk=4))
+    assert unsupported_reason(q, q[:, :, :2], AttentionMask(window=4)) is None  # the general kernels
+
+
+def test_fields_of_a_mask_keep_their_places():
+    dense = torch.ones(1, 2, 2, dtype=torch.bool)
+    mask = AttentionMask(False, None, 0, 0, dense, None, 1)
+    assert mask.bool_mask is dense and mask.query_start == 1 and mask.sinks == 0
