@@ -196,9 +196,10 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_o):
-        if len(ctx.saved_tensors) == 3:  # no queries
-            return (*(torch.zeros_like(t) for t in ctx.saved_tensors), None, None, None, None)
-        q, k, v, o, rest, lse, last = ctx.saved_tensors
+        saved = ctx.saved_tensors  # asked for once: under activation checkpointing a second time is an error, with offloading a second copy
+        if len(saved) == 3:  # no queries
+            return (*(torch.zeros_like(t) for t in saved), None, None, None, None)
+        q, k, v, o, rest, lse, last = saved
         window, sinks, scale = ctx.meta
         b, s, hq, d = q.shape
         sk, hkv = k.shape[1], k.shape[2]
