@@ -361,3 +361,29 @@ def test_saved_tensors_are_asked_for_once():
     # the recomputed forward is the same bit for bit; dQ is summed by atomics, and where another order tips its rounding an element moves by 2^-8 of itself
     for a, b in zip(*grads):
         assert (a.float() - b.float()).norm() <= 2.0**-6 * a.float().norm()
+
+
+def test_attention_over_key_ranges_does_not_drop_first_tokens(monkeypatch):
+    """Latent and span attention take one range of keys per query: a window with first tokens beside it is refused, or computed by the statement."""
+    from torchtune_b200.modules import Linear, SpanAttention
+    from torchtune_b200.ops import KernelFallbackError
+
+    torch.manual_seed(1)
+    with torch.device("cuda"):
+        attn = SpanAttention(embed_dim=128, num_heads=4, num_kv_heads=2, key_dim=32, value_dim=32, scale=0.2, **{f"{n}_proj": Linear(128, w, bias=False) for n, w in (("q", 128), ("k", 64), ("v", 64), ("output", 128))})
+    attn = attn.to(torch.bfloat16)
+    x = _randn(2, 60, 128, seed=1)
+    for docs in (None, _docs(2, 60, 20)):
+        mask = AttentionMask(window=5, sinks=2, doc_ids=docs)
+        with torch.no_grad():
+            with pytest.raises(KernelFallbackError):
+                attn(x, mask=mask)
+            with monkeypatch.context() as m:
+                m.setenv("TTB_STRICT", "0")
+                m.setattr(ops, "fallback_counts", {})
+                with pytest.warns(RuntimeWarning):
+                    got = attn(x, mask=mask)
+            with ops.use_reference_ops():
+                want = attn(x, mask=_visible(60, 60, 5, 2, docs).expand(2, 60, 60))
+        # bf16 projections by two GEMMs and an attention that are rounded alike but for the order of fp32 sums
+        assert (got.float() - want.float()).norm() <= 2.0**-6 * want.float().norm()

@@ -130,3 +130,12 @@ def test_fields_of_a_mask_keep_their_places():
     dense = torch.ones(1, 2, 2, dtype=torch.bool)
     mask = AttentionMask(False, None, 0, 0, dense, None, 1)
     assert mask.bool_mask is dense and mask.query_start == 1 and mask.sinks == 0
+
+
+def test_one_range_of_keys_does_not_stand_for_a_window_and_first_tokens():
+    from torchtune_b200.modules._spans import make_bounds
+
+    assert make_bounds(AttentionMask(window=4, sinks=2), 2, 15, 0, "cpu") is None
+    assert make_bounds(AttentionMask(window=4, sinks=2, doc_ids=DOCS), 2, 15, 0, "cpu") is None
+    assert torch.equal(make_bounds(AttentionMask(window=4), 1, 6, 0, "cpu").lo, torch.tensor([[0, 0, 0, 0, 1, 2]], dtype=torch.int32))
+    assert make_bounds(AttentionMask(sinks=2), 1, 6, 0, "cpu").lo is None  # first tokens of no window: causal

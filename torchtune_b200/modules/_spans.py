@@ -78,7 +78,7 @@ def make_bounds(mask, b: int, s: int, first: int, device):
             if mask.key_start.numel() != b:
                 raise ValueError(f"key_start has {mask.key_start.numel()} rows, the batch has {b}")
             return Bounds(lo=mask.key_start.to(device=device, dtype=torch.int32).contiguous(), lo_row=1)
-        if not mask.causal:
+        if not mask.causal or (mask.window > 0 and mask.sinks > 0):  # a window and the first tokens beside it are two ranges
             return None
         lo = lower_bounds(mask, b, s, device)
         if lo is None:

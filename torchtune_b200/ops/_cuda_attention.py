@@ -14,7 +14,8 @@ from .mask import AttentionMask
 def lower_bounds(mask: AttentionMask, b: int, s: int, device) -> Optional[torch.Tensor]:
     """Per-query first visible key index ``lo[b, s]`` (int32) for the structured mask kinds,
     or ``None`` when every key from 0 is visible.  Documents must be contiguous runs of equal
-    ids (sample packing), which makes ``lo`` non-decreasing along the sequence."""
+    ids (sample packing), which makes ``lo`` non-decreasing along the sequence.  First tokens that a
+    window leaves visible are no part of such a range: callers take masks with them another way."""
     cached = getattr(mask, "_lo_cache", None)
     if cached is not None and cached[0] == (b, s, str(device)):
         return cached[1]
