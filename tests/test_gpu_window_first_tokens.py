@@ -1,4 +1,6 @@
 """Attention with a sliding window beside which the first tokens (of each document) stay visible: kernels against the definition in float64."""
+import warnings
+
 import pytest
 import torch
 
@@ -387,3 +389,54 @@ def test_attention_over_key_ranges_does_not_drop_first_tokens(monkeypatch):
                 want = attn(x, mask=_visible(60, 60, 5, 2, docs).expand(2, 60, 60))
         # bf16 projections by two GEMMs and an attention that are rounded alike but for the order of fp32 sums
         assert (got.float() - want.float()).norm() <= 2.0**-6 * want.float().norm()
+
+
+def test_windows_over_other_numbers_of_keys_can_do_what_the_statement_can(monkeypatch):
+    """Second derivatives, transforms of functions, mixed types and broadcasts of a window without first tokens: all of them the statement's."""
+    monkeypatch.setattr(ops, "fallback_counts", {})
+    base = _randn(2, 20, 2, 72, seed=2)
+    q, k, v, d_o = _randn(2, 6, 4, 64, seed=1), base[..., 3:67], base[..., 8:], _randn(2, 6, 4, 64, seed=4)  # strided keys, values at an odd address
+    mask = AttentionMask(window=5)
+
+    def twice():
+        leaves = [t.clone(memory_format=torch.preserve_format).requires_grad_() for t in (q, k, v)]
+        parts = [leaves[0], leaves[1].expand(2, -1, -1, -1), leaves[2].transpose(1, 2).contiguous().transpose(1, 2)]
+        first = torch.autograd.grad(ops.attention(*parts, mask), leaves, d_o, create_graph=True)
+        return [*first, *torch.autograd.grad(sum(t.float().square().sum() for t in first), leaves)]
+
+    def some():  # not all of them have gradients
+        x = k.clone().requires_grad_()
+        (first,) = torch.autograd.grad(ops.attention(q, x, v, mask), x, d_o, create_graph=True)
+        return torch.autograd.grad(first.float().square().sum(), x)
+
+    def tied():  # the same tensor as keys and values, and queries made of it
+        x = k.clone().requires_grad_()
+        (first,) = torch.autograd.grad(ops.attention(torch.cat([x, -x], 2)[:, :6] * 0.5, x, x, mask), x, d_o, create_graph=True)
+        return [first, *torch.autograd.grad(first.float().square().sum(), x)]
+
+    calls = [
+        twice,
+        some,
+        tied,
+        lambda: [torch.func.vmap(lambda t: ops.attention(t, k, v, mask))(torch.stack([q, -q]))],
+        lambda: [torch.func.grad(lambda t: ops.attention(q, t, v, mask).float().square().sum())(k)],
+        lambda: list(torch.func.jvp(lambda t: ops.attention(q, k, t, mask), (v,), (v,))),
+        lambda: [ops.attention(q, k.float(), v, mask)],
+        lambda: [ops.attention(q, k[:1], v[:1], mask), ops.attention(q, k, v[:, :, :1], mask)],
+        lambda: [ops.attention(q[:1, :1].expand(65536, 1, 4, 64), k[:1, :2].expand(65536, 2, 2, 64), v[:1, :2].expand(65536, 2, 2, 64), mask)],
+    ]
+    for call in calls:
+        with pytest.raises(ops.KernelFallbackError):
+            call()
+        with monkeypatch.context() as m:
+            m.setenv("TTB_STRICT", "0")
+            with warnings.catch_warnings():
+                warnings.simplefilter("ignore")
+                got = call()
+        with ops.use_reference_ops():
+            want = call()
+        for a, w in zip(got, want, strict=True):
+            assert a.dtype == w.dtype and torch.equal(a, w)
+    # one backward pass, whose gradients nobody differentiates, is the kernels'
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    torch.autograd.grad(ops.attention(*leaves, mask), leaves, d_o)

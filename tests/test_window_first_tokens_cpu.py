@@ -139,3 +139,22 @@ def test_one_range_of_keys_does_not_stand_for_a_window_and_first_tokens():
     assert make_bounds(AttentionMask(window=4, sinks=2, doc_ids=DOCS), 2, 15, 0, "cpu") is None
     assert torch.equal(make_bounds(AttentionMask(window=4), 1, 6, 0, "cpu").lo, torch.tensor([[0, 0, 0, 0, 1, 2]], dtype=torch.int32))
     assert make_bounds(AttentionMask(sinks=2), 1, 6, 0, "cpu").lo is None  # first tokens of no window: causal
+
+
+def test_windows_that_stay_with_the_statement():
+    """Transforms, and without first tokens what the statement broadcasts or converts; with them these calls are refused elsewhere."""
+    from torchtune_b200.ops._cuda_attention import window_reason
+
+    q, k = torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 9, 2, 64, dtype=torch.bfloat16)
+    plain, first = AttentionMask(window=4), AttentionMask(window=4, sinks=1)
+    assert window_reason(q, k, k, plain) is None and window_reason(q, k, k, first) is None
+    for keys, values in ((k.float(), k.float()), (k, k.float()), (k[:1], k[:1]), (k, k[:, :, :1]), (k[..., :32], k[..., :32])):
+        assert window_reason(q, keys, values, plain) is not None and window_reason(q, keys, values, first) is None
+    reasons = []
+    torch.func.vmap(lambda t: reasons.append(window_reason(t, k, k, first)) or t)(q[None])
+    torch.func.jvp(lambda t: reasons.append(window_reason(q, t, k, plain)) or t, (k,), (k,))
+    with torch.autograd.forward_ad.dual_level():
+        reasons.append(window_reason(q, k, k, plain))
+    assert len(reasons) == 3 and all(reasons)
+    many = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16)
+    assert window_reason(many.expand(65536, 1, 1, 64), many.expand(65536, 2, 1, 64), many.expand(65536, 2, 1, 64), plain) is not None

@@ -417,7 +417,9 @@ def attention(
             why = "key_start together with another mask kind"
         elif q.shape[-1] not in (64, 128):
             why = f"head_dim {q.shape[-1]}"
-        elif not _cuda_attention.takes_window(q, k, mask, softcap):
+        elif _cuda_attention.takes_window(q, k, mask, softcap):
+            why = _cuda_attention.window_reason(q, k, v, mask)
+        else:
             why = _cuda_attention.unsupported_reason(q, k, mask)
         if why is None:
             return _cuda_attention.attention(q, k, v, mask, scale, softcap)

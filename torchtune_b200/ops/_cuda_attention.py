@@ -160,15 +160,16 @@ class _FlashAttention(torch.autograd.Function):
 
 
 class _WindowAttention(torch.autograd.Function):
-    """A causal window (query i at position ``sk - s + i``) beside which the first ``sinks`` positions stay visible; documents keep their own first positions."""
+    """A causal window (query i at position ``sk - s + i``) beside which the first ``sinks`` positions stay visible; documents keep their own first positions.  ``q``, ``k`` and ``v`` are contiguous
+    and start on 16 bytes."""
 
     @staticmethod
     def forward(ctx, q, k, v, doc_ids, window, sinks, scale):
         b, s, hq, d = q.shape
         sk, hkv = k.shape[1], k.shape[2]
-        q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q.contiguous(), k.contiguous(), v.contiguous()))
         o = torch.empty_like(q)
         grads = any(ctx.needs_input_grad)
+        ctx.meta = (window, sinks, scale)
         if q.numel() == 0:
             ctx.save_for_backward(q, k, v)
             return o
@@ -191,7 +192,6 @@ class _WindowAttention(torch.autograd.Function):
                                             err_word(q.device).data_ptr(), stream_ptr()), "attention forward (window)")
         if grads:
             ctx.save_for_backward(q, k, v, o, rest, lse, last)
-            ctx.meta = (window, sinks, scale)
         return o
 
     @staticmethod
@@ -217,11 +217,47 @@ class _WindowAttention(torch.autograd.Function):
         return dq.to(q.dtype), dk, dv, None, None, None, None
 
 
+class _PlainWindowAttention(_WindowAttention):
+    """Without first positions, where the statement's gradients can be differentiated again: so can these.  A backward pass that is recorded for that goes through the statement."""
+
+    @staticmethod
+    def backward(ctx, d_o):
+        if not torch.is_grad_enabled():
+            return _WindowAttention.backward(ctx, d_o)
+        from . import _fallback, reference
+
+        leaves = [t.view_as(t) for t in ctx.saved_tensors[:3]]  # queries that come from the keys, or keys that are the values, have gradients of their own here
+        window, _, scale = ctx.meta
+        _fallback("attention", "a window's gradients that are to be differentiated", leaves[0])
+        out = reference.attention(*leaves, causal=True, window=window, scale=scale)
+        wanted = [t for t, need in zip(leaves, ctx.needs_input_grad) if need]
+        grads = iter(torch.autograd.grad(out, wanted, d_o, create_graph=True))
+        return (*(next(grads) if need else None for need in ctx.needs_input_grad[:3]), None, None, None, None)
+
+
 def takes_window(q: torch.Tensor, k: torch.Tensor, mask: AttentionMask, softcap: float) -> bool:
     """Whether a call is a causal window of the kernels with first positions: with such positions, or with other numbers of queries than of keys."""
     s, sk = q.shape[1], k.shape[1]
     return (mask.bool_mask is None and mask.key_start is None and mask.causal and mask.window > 0 and mask.chunk <= 0 and (mask.sinks > 0 or s != sk) and s <= sk
             and (mask.doc_ids is None or s == sk) and (softcap or 0.0) <= 0.0 and q.shape[2] % k.shape[2] == 0)
+
+
+def window_reason(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: AttentionMask) -> Optional[str]:
+    """Why a call of ``takes_window`` cannot run on the kernels (``None`` = it can).  Without first tokens the statement's broadcasts and mixed types stay with the statement; with them
+    :func:`attention` refuses what does not fit."""
+    from . import _has_memory
+
+    if torch.autograd.forward_ad._current_level >= 0 or not _has_memory(q, k, v):
+        return "forward-mode derivatives, transforms or traces of a window beside other numbers of keys, or of one with first tokens"
+    if mask.sinks <= 0 and not _fits(q, k, v):
+        return "a window over keys and values of other sizes or types than the queries'"
+    if q.shape[0] > 65535 or k.shape[2] > 65535:
+        return "more than 65535 batch rows or key heads"
+    return None
+
+
+def _fits(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bool:
+    return k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[3] == q.shape[3] and q.dtype == k.dtype == v.dtype and q.device == k.device == v.device
 
 
 def unsupported_reason(q: torch.Tensor, k: torch.Tensor, mask: AttentionMask) -> Optional[str]:
@@ -249,11 +285,13 @@ def attention(q, k, v, mask: AttentionMask, scale: Optional[float], softcap: flo
     scale = (1.0 / math.sqrt(d)) if scale is None else scale
     softcap = max(0.0, float(softcap or 0.0))  # 0 and below: no cap
     if takes_window(q, k, mask, softcap):
-        if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d or not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device):
+        if not _fits(q, k, v):
             raise ValueError(f"queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not fit one another, or differ in type or device")
         if mask.doc_ids is not None and tuple(mask.doc_ids.shape) not in ((b, s), (1, s)):
             raise ValueError(f"document ids {tuple(mask.doc_ids.shape)} are not those of {b} rows of {s} tokens")
-        return _WindowAttention.apply(q, k, v, mask.doc_ids, min(mask.window, sk), min(max(mask.sinks, 0), sk), float(scale))
+        q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q.contiguous(), k.contiguous(), v.contiguous()))
+        kernels = _WindowAttention if mask.sinks > 0 else _PlainWindowAttention
+        return kernels.apply(q, k, v, mask.doc_ids, min(mask.window, sk), min(max(mask.sinks, 0), sk), float(scale))
     lo = hi = kmask = dense = None
     monotone, causal = 1, bool(mask.causal)
     if mask.key_start is not None:
