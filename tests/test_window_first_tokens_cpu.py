@@ -158,3 +158,39 @@ def test_windows_that_stay_with_the_statement():
     assert len(reasons) == 3 and all(reasons)
     many = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16)
     assert window_reason(many.expand(65536, 1, 1, 64), many.expand(65536, 2, 1, 64), many.expand(65536, 2, 1, 64), plain) is not None
+
+
+class _Widest(torch.utils._python_dispatch.TorchDispatchMode):
+    """Notes the most bytes that a result of an operation has."""
+
+    most = 0
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        out = func(*args, **(kwargs or {}))
+        for t in out if isinstance(out, (tuple, list)) else (out,):
+            if isinstance(t, torch.Tensor):
+                self.most = max(self.most, t.numel() * t.element_size())
+        return out
+
+
+@pytest.mark.parametrize("sinks", [0, 3])
+def test_dense_masks_are_narrowed_without_wider_copies(sinks):
+    from torchtune_b200.models._factory import _window_first_mask_mod
+
+    mod = _window_first_mask_mod(5, sinks)
+    causal = torch.ones(40, 64, dtype=torch.bool).tril(11).expand(2, 40, 64)
+    with _Widest() as widest:
+        got = mod(causal, 2, 40)
+    assert widest.most <= causal.numel()
+    i, j = torch.arange(40)[:, None] + 11, torch.arange(64)
+    want = (j <= i) & ((i - j < 5) | (j < sinks))
+    assert torch.equal(got, want.expand(2, 40, 64))
+    # left-padded rows, a row that sees itself only, rows without a key, and a mask with a dimension of heads
+    start = torch.tensor([7, 0])[:, None, None]
+    padded = causal & (j >= start)
+    padded[0, 0], padded[1, 5] = False, False
+    padded[1, 6] = j == 17
+    want = padded & ((i - j < 5) | (j - start < sinks))
+    assert torch.equal(mod(padded, 2, 40), want) and torch.equal(mod(padded[:, None], 2, 40), want[:, None])
+    assert torch.equal(mod(AttentionMask(causal=False, bool_mask=padded), 2, 40), want)
+    assert mod(padded[:, :0], 2, 0).shape == (2, 0, 64)

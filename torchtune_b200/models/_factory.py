@@ -176,10 +176,16 @@ def _window_first_mask_mod(window: int, sinks: int):
         if isinstance(mask, AttentionMask) and mask.bool_mask is None:
             return replace(mask, window=window, sinks=sinks)
         dense = mask.bool_mask if isinstance(mask, AttentionMask) else mask
-        k = torch.arange(dense.shape[-1], device=dense.device)
-        own = torch.where(dense, k, -1).amax(-1, keepdim=True)
-        first = torch.where(dense, k, dense.shape[-1]).amin(-1, keepdim=True)
-        return dense & ((own - k < window) | (k - first < sinks))
+        n = dense.shape[-1]
+        if dense.numel() == 0:
+            return dense
+        k = torch.arange(n, device=dense.device)
+        seen = dense.to(torch.bool).view(torch.uint8)
+        # Borders are one number per row, so that nothing of the mask's size is wider than it.  A row without keys has any; it stays empty.
+        keep = k > n - 1 - window - seen.flip(-1).argmax(-1, keepdim=True)
+        if sinks > 0:
+            keep |= k < seen.argmax(-1, keepdim=True) + sinks
+        return dense & keep
 
     return mod
 
