@@ -279,3 +279,24 @@ def test_a_cache_keeps_its_types_when_a_model_changes_its_own():
     scales = cache.k_scales.clone()
     model.to(torch.bfloat16).float()
     assert cache.k_scales.dtype == torch.bfloat16 and torch.equal(cache.k_scales, scales) and cache.k_codes.dtype == torch.uint8 and cache.cache_pos.dtype == torch.int64
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_scales_do_not_pass_through_a_models_new_type(bits):
+    """Scales below the smallest number of fp16 and above its largest."""
+    model = _decoder()
+    model.setup_caches(1, torch.float32, decoder_max_seq_len=8, kv_cache_bits=bits)
+    cache = model.layers[1].attn.kv_cache
+    x = torch.randn(1, 6, 2, 32, generator=torch.Generator().manual_seed(1)) * torch.tensor([1e-30, 1e-6, 1e-3, 1.0, 1e8, 1e30])[:, None, None]
+    cache.append(x, -x)
+    want = [t.clone() for t in (cache.k_scales, cache.v_scales, cache.k_codes, cache.v_codes)]
+    for convert in (torch.nn.Module.half, torch.nn.Module.double, lambda m: m.to("cpu", torch.float16), lambda m: m.to(torch.bfloat16), torch.nn.Module.float):
+        convert(model)
+        assert all(torch.equal(a, b) for a, b in zip(want, (cache.k_scales, cache.v_scales, cache.k_codes, cache.v_codes)))
+        assert cache.k_scales.dtype == cache.v_scales.dtype == torch.bfloat16 and dict(cache.named_buffers())["k_scales"] is cache.k_scales
+    meta = _decoder()
+    meta.setup_caches(1, torch.float32, decoder_max_seq_len=8, kv_cache_bits=bits)
+    meta.to("meta").half()
+    assert meta.layers[0].attn.kv_cache.k_scales.dtype == torch.bfloat16 and meta.layers[0].attn.kv_cache.k_scales.device.type == "meta"
+    meta.to_empty(device="cpu")
+    assert meta.layers[0].attn.kv_cache.k_scales.dtype == torch.bfloat16 and meta.layers[0].attn.kv_cache.k_scales.device.type == "cpu"

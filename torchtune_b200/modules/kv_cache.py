@@ -94,8 +94,11 @@ class QuantizedKVCache(KVCache):
         self.bits = bits
 
     def _apply(self, fn, recurse: bool = True):
-        super()._apply(fn, recurse)  # moves to a device apply to all; the format's types stay
-        self.k_scales, self.v_scales = self.k_scales.to(torch.bfloat16), self.v_scales.to(torch.bfloat16)
+        before = self.k_scales, self.v_scales
+        super()._apply(fn, recurse)
+        for name, scales in zip(("k_scales", "v_scales"), before):  # moves to a device apply to all; the format's types stay, and values do not pass through another type
+            if getattr(self, name).dtype != torch.bfloat16:
+                setattr(self, name, scales.to(getattr(self, name).device))
         return self
 
     def rows(self, batch: int) -> Tuple[ops.QuantizedRows, ops.QuantizedRows]:
