@@ -300,3 +300,19 @@ def test_scales_do_not_pass_through_a_models_new_type(bits):
     assert meta.layers[0].attn.kv_cache.k_scales.dtype == torch.bfloat16 and meta.layers[0].attn.kv_cache.k_scales.device.type == "meta"
     meta.to_empty(device="cpu")
     assert meta.layers[0].attn.kv_cache.k_scales.dtype == torch.bfloat16 and meta.layers[0].attn.kv_cache.k_scales.device.type == "cpu"
+
+
+def test_a_cache_whose_buffers_were_exchanged_takes_as_many_rows_as_they_have():
+    from torchtune_b200.modules import KVCache, QuantizedKVCache
+
+    plain = KVCache(2, 8, 1, 32, torch.float32)
+    plain.k_cache, plain.v_cache = torch.zeros(3, 8, 1, 32), torch.zeros(3, 8, 1, 32)
+    x = torch.randn(3, 2, 1, 32, generator=torch.Generator().manual_seed(1))
+    assert torch.equal(plain.update(x, -x)[0][:, :2], x)
+    few = QuantizedKVCache(2, 8, 1, 32, 8)
+    for name, t in QuantizedKVCache(3, 8, 1, 32, 8).named_buffers():
+        setattr(few, name, t)
+    assert few.update(x, -x)[0].shape == (3, 8, 1, 32)
+    for cache in (plain, few):
+        with pytest.raises(ValueError, match="batch size of 3"):
+            cache.update(x.repeat(2, 1, 1, 1), x.repeat(2, 1, 1, 1))

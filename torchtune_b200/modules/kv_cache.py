@@ -46,11 +46,16 @@ class KVCache(nn.Module):
     def size(self) -> int:
         return int(self.cache_pos[0].item()) if self._level is None else self._level
 
+    @property
+    def held_rows(self) -> int:
+        """Batch rows of the buffers."""
+        return self.k_cache.shape[0]
+
     def reserve(self, bsz: int, seq_len: int) -> torch.Tensor:
         """Slots of the next ``seq_len`` tokens of ``bsz`` rows; :meth:`advance` follows once they are written."""
-        if bsz > self.batch_size:
+        if bsz > self.held_rows:
             raise ValueError(
-                f"The current cache has been setup with a batch size of {self.batch_size}"
+                f"The current cache has been setup with a batch size of {self.held_rows}"
                 f", but found new key tensors with batch size {bsz}!"
             )
         if not self.recording and self.size + seq_len > self.max_seq_len:
@@ -101,10 +106,14 @@ class QuantizedKVCache(KVCache):
                 setattr(self, name, scales.to(getattr(self, name).device))
         return self
 
+    @property
+    def held_rows(self) -> int:
+        return self.k_codes.shape[0]
+
     def rows(self, batch: int) -> Tuple[ops.QuantizedRows, ops.QuantizedRows]:
         """Keys and values of the first ``batch`` batch rows."""
         k, v = ops.QuantizedRows(self.k_codes, self.k_scales, self.max_seq_len), ops.QuantizedRows(self.v_codes, self.v_scales, self.max_seq_len)
-        return (k, v) if batch == self.batch_size else (k.batch(batch), v.batch(batch))
+        return (k, v) if batch == self.held_rows else (k.batch(batch), v.batch(batch))
 
     def reset(self) -> None:
         for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales):
