@@ -440,3 +440,20 @@ def test_windows_over_other_numbers_of_keys_can_do_what_the_statement_can(monkey
     # one backward pass, whose gradients nobody differentiates, is the kernels'
     leaves = [t.clone().requires_grad_() for t in (q, k, v)]
     torch.autograd.grad(ops.attention(*leaves, mask), leaves, d_o)
+
+
+def test_more_rows_and_key_heads_than_a_grid_dimension_has():
+    """Gradients of first positions that meet in a workspace, of 65 536 pairs of a batch row and a key head."""
+    b, s, h = 1024, 129, 64
+    q, k, v, d_o = (_randn(b, s, h, 64, seed=i) for i in range(4))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    mask = AttentionMask(window=1, sinks=1)
+    out = ops.attention(*leaves, mask)
+    grads = torch.autograd.grad(out, leaves, d_o)
+    at = [0, 511, 1023]
+    for got in (out, *grads):
+        assert got.isfinite().all()
+    parts = [t.detach()[at] for t in leaves]
+    want, square, *wants = _formula(*parts, d_o[at], _visible(s, s, 1, 1), 64**-0.5)
+    _near(out[at], want, square)
+    _check_gradients([g[at] for g in grads], wants, d_o[at], want, 64**-0.5)

@@ -512,14 +512,14 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   if (warp == 2) tmem_dealloc(tmem_base, 512);
 }
 
-// Gradients of the first positions: the parts of the CTAs in their order.  Grid (rows, blocks, batch times key heads), 2D threads.
+// Gradients of the first positions: the parts of the CTAs in their order.  Grid (batch times key heads, blocks, rows), 2D threads: only the first dimension may pass 65 535.
 template <int D>
 __global__ void __launch_bounds__(2 * D)
 first_rows_kernel(Params p) {
-  const int r = blockIdx.x, block = blockIdx.y, bi = blockIdx.z / p.hkv, hk = blockIdx.z % p.hkv;
+  const int r = blockIdx.z, block = blockIdx.y, bi = blockIdx.x / p.hkv, hk = blockIdx.x % p.hkv;
   const int key = block * kBlk + r;
   if (key >= p.sinks || key >= p.sk) return;
-  const float* from = p.partial + ((static_cast<long long>(blockIdx.z) * p.blocks + block) * (1 + p.pieces) * p.rows + r) * 2 * D + threadIdx.x;
+  const float* from = p.partial + ((static_cast<long long>(blockIdx.x) * p.blocks + block) * (1 + p.pieces) * p.rows + r) * 2 * D + threadIdx.x;
   float sum = 0.f;
 #pragma unroll 4
   for (int x = 0; x <= p.pieces; ++x) sum += from[static_cast<long long>(x) * p.rows * 2 * D];
@@ -554,7 +554,7 @@ static int launch(const void* q, const void* k, const void* v, const void* d_o, 
   kern<<<grid, kThreads, Layout<D>::kDynamic, st>>>(tq, tk, tv, tdo, tdq, p);
   if (FIRST && p.pieces > 0) {
     TTB_COUNT_LAUNCH(1);
-    first_rows_kernel<D><<<dim3(p.rows, p.blocks, b * p.hkv), 2 * D, 0, st>>>(p);
+    first_rows_kernel<D><<<dim3(b * p.hkv, p.blocks, p.rows), 2 * D, 0, st>>>(p);
   }
   return cudaGetLastError() == cudaSuccess ? kOk : kErrDriver;
 }
