@@ -458,3 +458,26 @@ def test_lengths_where_few_rows_are_split_further(n, window, d, bits):
     at = torch.arange(n, device="cuda")
     dense = ((at > n - 1 - window) | (at < 4))[None, None] if window else torch.ones(1, 1, n, dtype=torch.bool, device="cuda")
     _check(_queries(1, 1, 4, d), k_rows, v_rows, AttentionMask(causal=True, window=window, sinks=4 if window else 0), dense)
+
+
+@pytest.mark.parametrize("kind", ["all", "causal", "window", "bool"])
+@pytest.mark.parametrize("d, bits", [(64, 4), (96, 4), (96, 8), (128, 8), (256, 4)])
+@pytest.mark.parametrize("b, s, group", [(2, 1, 4), (1, 3, 4), (2, 4, 4), (1, 1, 5), (3, 16, 1), (1, 1, 16)])
+def test_several_rows_that_meet_in_a_workspace(b, s, group, d, bits, kind):
+    """One and two tiles of query rows, several queries, batch rows and key heads, whose slots are split further than a cluster reaches."""
+    if d == 256 and s * group > 8:
+        pytest.skip("read back instead; the other attention has no kernel for 256 channels")
+    n, h = 20011, 2
+    k_rows, v_rows = _filled(b, n, h, d, bits, seed=s * group)
+    j, i = torch.arange(n, device="cuda"), torch.arange(s, device="cuda")[:, None] + n - s
+    dense, mask = {
+        "all": (torch.ones(b, s, n, dtype=torch.bool, device="cuda"), AttentionMask(causal=False)),
+        "causal": ((j <= i).expand(b, s, n), AttentionMask()),
+        "window": (((j <= i) & ((i - j < 15000) | (j < 77))).expand(b, s, n), AttentionMask(window=15000, sinks=77)),
+        "bool": (torch.rand(b, s, n, generator=_gen(6), device="cuda") < 0.3, None),
+    }[kind]
+    if mask is None:
+        dense[-1, -1] = False  # the last query sees nothing
+        mask = AttentionMask(causal=False, bool_mask=dense)
+    got = _check(_queries(b, s, h * group, d), k_rows, v_rows, mask, dense)
+    assert kind != "bool" or not got[-1, -1].any()

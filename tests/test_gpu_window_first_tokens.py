@@ -457,3 +457,33 @@ def test_more_rows_and_key_heads_than_a_grid_dimension_has():
     want, square, *wants = _formula(*parts, d_o[at], _visible(s, s, 1, 1), 64**-0.5)
     _near(out[at], want, square)
     _check_gradients([g[at] for g in grads], wants, d_o[at], want, 64**-0.5)
+
+
+@pytest.mark.parametrize("bits", [None, 4, 8])
+def test_cached_steps_of_a_windowed_decoder_see_the_window(bits):
+    """Prompt and single tokens of left-padded rows: what the windowed model does by itself, the same weights without a window do under a mask of the window."""
+    from torchtune_b200.models.mistral import mistral
+
+    arch = dict(vocab_size=304, num_layers=2, num_heads=4, num_kv_heads=2, embed_dim=256, intermediate_dim=256, max_seq_len=256)
+    models = []
+    for kwargs in (dict(sliding_window_size=30, attention_sinks=3), {}):
+        torch.manual_seed(2)
+        with torch.device("cuda"):
+            model = mistral(**arch, **kwargs).to(torch.bfloat16).eval()
+            model.setup_caches(2, torch.bfloat16, decoder_max_seq_len=140, kv_cache_bits=bits)
+        models.append(model)
+    tokens = torch.randint(1, 304, (2, 130), generator=_gen(3), device="cuda")
+    start = torch.tensor([0, 21], device="cuda")[:, None, None]
+    i, j = torch.arange(130, device="cuda")[:, None], torch.arange(140, device="cuda")
+    causal = (j <= i) & ((j >= start) | (i == j))
+    window = causal & ((i - j < 30) | (j - start < 3))
+    with torch.no_grad():
+        for a, z in ((0, 120), (120, 121), (121, 129), (129, 130)):
+            pos = torch.arange(a, z, device="cuda").expand(2, -1)
+            own, given = (m(tokens[:, a:z], input_pos=pos, mask=mask[:, a:z]) for m, mask in zip(models, (causal, window)))
+            assert torch.equal(own, given)
+        # and the window counts
+        pos = torch.full((2, 1), 130, device="cuda")
+        last = (torch.arange(140, device="cuda") <= 130)[None, None].expand(2, 1, 140) & (j >= start)
+        own, all_keys = (m(tokens[:, :1], input_pos=pos, mask=last) for m in models)
+        assert not torch.equal(own, all_keys)
