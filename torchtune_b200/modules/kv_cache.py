@@ -85,7 +85,7 @@ class KVCache(nn.Module):
 class QuantizedKVCache(KVCache):
     """A :class:`KVCache` in 4 or 8 bits: 0.28 or 0.53 of the bytes of bf16, and of what a decode step reads.  Keys and values are quantised as they are appended, 32 channels of a token and
     head to a bf16 scale (:class:`~torchtune_b200.ops.QuantizedRows`), and attention goes through :meth:`attend`, which reads the codes; all queries, those of the prompt included, see the
-    keys and values that the cache stands for.  Head dimensions are multiples of 32."""
+    keys and values that the cache stands for.  Head dimensions are multiples of 32; prompts read all slots back for the ordinary attention, which has kernels for 64 and 128 channels."""
 
     def __init__(self, batch_size: int, max_seq_len: int, num_kv_heads: int, head_dim: int, bits: int = 4) -> None:
         nn.Module.__init__(self)

@@ -444,8 +444,8 @@ def attention(
 
 def quantized_append(k: torch.Tensor, v: torch.Tensor, k_rows: QuantizedRows, v_rows: QuantizedRows, slots: torch.Tensor) -> None:
     """Writes keys and values ``[b, s, heads, d]`` (bf16, fp16 or fp32) in 4 or 8 bits to the slots ``slots`` (int64 ``[s]``, consecutive) of the rows of a cache with as many batch rows.
-    No gradient flows through a cache in few bits.  On a CUDA device, where the slots are not known to the host, a token whose slot lies outside the cache or does not follow the one
-    before is not written and counted as an index violation; elsewhere it is an error."""
+    No gradient flows through a cache in few bits.  On a CUDA device, where the slots are not known to the host, a token whose slot lies outside the cache or is not as far behind the
+    first one's as the token is behind the first is not written and counted as an index violation; elsewhere it is an error."""
     b, h, n, d, bits = quantized.sizes(k_rows, v_rows)
     shape = k.shape
     if len(shape) != 4 or shape != v.shape or shape[0] != b or shape[2] != h or shape[3] != d:
@@ -488,7 +488,8 @@ def quantized_read(k_rows: QuantizedRows, v_rows: QuantizedRows, start: int = 0,
 def quantized_attention(q: torch.Tensor, k_rows: QuantizedRows, v_rows: QuantizedRows, mask: Optional[AttentionMask] = None, *, scale: Optional[float] = None, softcap: float = 0.0,
                         dropout_p: float = 0.0) -> torch.Tensor:
     """:func:`attention` of ``q`` ``[b, s, h, d]`` over all slots of a quantised cache (``k_rows.first(n)`` for the first ``n``).  Up to 16 query rows per key head (tokens times heads that share it; 8
-    of 256 channels) attend to the codes as they are; more of them, and calls that need gradients, read the cache back in ``q``'s type first.  Masks are those of :func:`attention`
+    of 256 channels) attend to the codes as they are; more of them, calls that need gradients, other head dimensions than 64, 96, 128 and 256, and more slots than a CTA's visibility words cover (349 440 for one query,
+    58 112 for sixteen) read all slots back in ``q``'s type first and take :func:`attention`, which has kernels for 64 and 128 channels.  Masks are those of :func:`attention`
     with other numbers of queries than of keys: causal ones put the queries into the last slots; documents and chunks have no meaning here."""
     mask = mask if mask is not None else AttentionMask(causal=False)
     size = b, h, n, d, _ = quantized.sizes(k_rows, v_rows)

@@ -15,7 +15,9 @@
 // FIRST: a causal window beside which the first positions stay visible; a tile visits the blocks of the first positions and then those of its window.  These visits are short, and what a CTA does in
 // front of them and behind them counts: one tile per CTA, and two CTAs per SM that hide it from one another (for 128 channels with one stage of K and V each).  Against two tiles per CTA, 32 / 8 heads,
 // 4 first positions: 1 x 6000 tokens of 128 channels, window 1024, 206 -> 184 us; 4 x 4096, window 512, 393 -> 342; 1 x 16384, window 4096, 1276 -> 1139; 4 x 1413 of 64, window 200, 103 -> 84 us.
-// With 64 channels the exponentials bound it (twice those of the visible pairs are taken at a window of 200), with 128 they and the products, which take turns within a tile.
+// The exponentials of the visited blocks (twice those of the visible pairs at a window of 200) do not bound it: at 16 per cycle and SM they take 16 of 80 us at 4 x 1413 of 64 channels, 71 of 300 at 4 x 4096
+// of 64, window 512, 45 of 180 at 1 x 6000 of 128, where the products take 62 more, in turns with them within a tile.  What the rest goes into, around three to ten blocks per CTA, was not measured
+// apart: tensor memory and barriers, the first loads, the chain from scores to weights to output, the epilogue.
 // Causal forward, head dim 64 (one-tile kernel before): 8 x 2048 tokens 788 -> 374 us, 1 x 16384 tokens 5079 -> 2042 us; exponentials bound it.
 // Soft-capped scores stay on the one-tile kernel in attention.cu.  Every wait is bounded and reports through the error word.
 #include "common/attn_math.cuh"

@@ -548,7 +548,7 @@ attention_kernel(const __grid_constant__ Params p) {
     else
       tile(std::true_type{}, drain, static_cast<int>(entry & kIndex));
     step(drain);
-    __syncwarp();  // the stage is refilled two iterations on
+    __syncwarp();  // the next iteration refills this stage: no lane may still read it
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncwarp();
