@@ -419,6 +419,8 @@ def attention(
             why = f"head_dim {q.shape[-1]}"
         elif _cuda_attention.takes_window(q, k, mask, softcap):
             why = _cuda_attention.window_reason(q, k, v, mask)
+            if why is None:
+                return _cuda_attention.window_attention(q, k, v, mask, scale)
         else:
             why = _cuda_attention.unsupported_reason(q, k, mask)
         if why is None:

@@ -7,6 +7,7 @@ from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
+from . import _fallback, _has_memory, reference
 from ._lib import check, err_word, lib, stream_ptr
 from .mask import AttentionMask
 
@@ -224,8 +225,6 @@ class _PlainWindowAttention(_WindowAttention):
     def backward(ctx, d_o):
         if not torch.is_grad_enabled():
             return _WindowAttention.backward(ctx, d_o)
-        from . import _fallback, reference
-
         leaves = [t.view_as(t) for t in ctx.saved_tensors[:3]]  # queries that come from the keys, or keys that are the values, have gradients of their own here
         window, _, scale = ctx.meta
         _fallback("attention", "a window's gradients that are to be differentiated", leaves[0])
@@ -245,8 +244,6 @@ def takes_window(q: torch.Tensor, k: torch.Tensor, mask: AttentionMask, softcap:
 def window_reason(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: AttentionMask) -> Optional[str]:
     """Why a call of ``takes_window`` cannot run on the kernels (``None`` = it can).  Without first tokens the statement's broadcasts and mixed types stay with the statement; with them
     :func:`attention` refuses what does not fit."""
-    from . import _has_memory
-
     if torch.autograd.forward_ad._current_level >= 0 or not _has_memory(q, k, v):
         return "forward-mode derivatives, transforms or traces of a window beside other numbers of keys, or of one with first tokens"
     if mask.sinks <= 0 and not _fits(q, k, v):
@@ -257,7 +254,8 @@ def window_reason(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Atten
 
 
 def _fits(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bool:
-    return k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[3] == q.shape[3] and q.dtype == k.dtype == v.dtype and q.device == k.device == v.device
+    a, b = q.shape, k.shape
+    return b == v.shape and b[0] == a[0] and b[3] == a[3] and q.dtype == k.dtype == v.dtype and q.device == k.device == v.device
 
 
 def unsupported_reason(q: torch.Tensor, k: torch.Tensor, mask: AttentionMask) -> Optional[str]:
@@ -277,6 +275,21 @@ def unsupported_reason(q: torch.Tensor, k: torch.Tensor, mask: AttentionMask) ->
     return None
 
 
+def window_attention(q, k, v, mask: AttentionMask, scale: Optional[float]) -> torch.Tensor:
+    """A call of ``takes_window`` that ``window_reason`` leaves to the kernels."""
+    b, s, _, d = q.shape
+    sk = k.shape[1]
+    if not _fits(q, k, v):
+        raise ValueError(f"queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not fit one another, or differ in type or device")
+    if mask.doc_ids is not None and tuple(mask.doc_ids.shape) not in ((b, s), (1, s)):
+        raise ValueError(f"document ids {tuple(mask.doc_ids.shape)} are not those of {b} rows of {s} tokens")
+    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q, k, v))
+    kernels = _WindowAttention if mask.sinks > 0 else _PlainWindowAttention
+    return kernels.apply(q, k, v, mask.doc_ids, min(mask.window, sk), min(max(mask.sinks, 0), sk), 1.0 / math.sqrt(d) if scale is None else float(scale))
+
+
 def attention(q, k, v, mask: AttentionMask, scale: Optional[float], softcap: float) -> torch.Tensor:
     """Self-attention with structured masks, cross-attention and cached decoding (``sk != s``), arbitrary boolean masks and
     soft-capped scores all run on the same pair of kernels; what differs is the mask description handed to them."""
@@ -285,13 +298,7 @@ def attention(q, k, v, mask: AttentionMask, scale: Optional[float], softcap: flo
     scale = (1.0 / math.sqrt(d)) if scale is None else scale
     softcap = max(0.0, float(softcap or 0.0))  # 0 and below: no cap
     if takes_window(q, k, mask, softcap):
-        if not _fits(q, k, v):
-            raise ValueError(f"queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not fit one another, or differ in type or device")
-        if mask.doc_ids is not None and tuple(mask.doc_ids.shape) not in ((b, s), (1, s)):
-            raise ValueError(f"document ids {tuple(mask.doc_ids.shape)} are not those of {b} rows of {s} tokens")
-        q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q.contiguous(), k.contiguous(), v.contiguous()))
-        kernels = _WindowAttention if mask.sinks > 0 else _PlainWindowAttention
-        return kernels.apply(q, k, v, mask.doc_ids, min(mask.window, sk), min(max(mask.sinks, 0), sk), float(scale))
+        return window_attention(q, k, v, mask, scale)
     lo = hi = kmask = dense = None
     monotone, causal = 1, bool(mask.causal)
     if mask.key_start is not None:
