@@ -20,7 +20,7 @@ import torch.nn.functional as F
 
 from . import reference
 from .mask import AttentionMask
-from . import quantized
+from . import qk_norm, quantized
 from .quantized import QuantizedRows
 
 __all__ = [
@@ -44,6 +44,8 @@ __all__ = [
     "rms_norm",
     "rope",
     "rope_append",
+    "qk_norm_rope",
+    "qk_norm_rope_append",
     "swiglu",
     "attention",
     "QuantizedRows",
@@ -385,6 +387,56 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: torch.
     from . import _cuda
 
     return _cuda.rope_append(q, k, v, cache, input_pos, interleaved, k_cache, v_cache, slots)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: Optional[torch.Tensor], cache: torch.Tensor, input_pos: Optional[torch.Tensor] = None, *,
+                 eps: float = 1e-6, interleaved: bool = True, norm_first: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every head of ``q`` and ``k`` ``[b, s, heads, d]``, times a gain ``[d]`` each (``None``: none), and :func:`rope`, in that order or (``norm_first=False``) the other way round, with
+    one rounding at the end where the two operators of their own make two.  One launch forward for CUDA tensors in bf16, fp16 or fp32 with ``d`` a multiple of 16 up to 512, and one backward (two
+    with gains' gradients).  ``input_pos``: ``[b, s]``, ``[s]``, or ``[b]`` for one token per row; the angles are constants.  On a CUDA device a position that the table does not have counts as
+    an index violation and position 0 stands in; elsewhere it is an error."""
+    qk_norm.check_arguments(q, k, (q_gain, k_gain), cache)
+    b, s = q.shape[:2]
+    pos = qk_norm.positions(input_pos, b, s, cache.shape[0])
+    if pos is not None and pos.device != q.device:
+        pos = pos.to(q.device)
+    if q.numel() == 0:
+        return torch.empty_like(q), torch.empty_like(k)
+    if cuda_ops_enabled(q) and qk_norm.suits(q, cache) and _has_memory(q, k, cache, *(t for t in (q_gain, k_gain, pos) if t is not None)) and torch.autograd.forward_ad._current_level < 0:
+        return qk_norm.norm_rope(q, k, q_gain, k_gain, cache, pos, float(eps), bool(interleaved), bool(norm_first), _differentiated(q, k, q_gain, k_gain))
+    _fallback("qk_norm_rope", f"head dimension {q.shape[-1]} or angles in {cache.dtype}", q)
+    return tuple(reference.norm_rope(x, gain, cache, pos, eps, interleaved, norm_first) for x, gain in ((q, q_gain), (k, k_gain)))
+
+
+def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: Optional[torch.Tensor], cache: torch.Tensor,
+                        input_pos: Optional[torch.Tensor], k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, *, eps: float = 1e-6, interleaved: bool = True,
+                        norm_first: bool = True) -> torch.Tensor:
+    """:func:`qk_norm_rope` of ``q`` (returned) and of ``k``, the latter and ``v`` written to ``k_cache`` / ``v_cache`` ``[b, max_seq, heads, d]`` at ``slots`` (int64 ``[s]``, no two the same), in one
+    launch.  No gradient flows through a cache: calls that would be differentiated are refused.  On a CUDA device a slot outside the cache counts as an index violation and nothing is written
+    for it; elsewhere it is an error."""
+    qk_norm.check_arguments(q, k, (q_gain, k_gain), cache)
+    b, s = q.shape[:2]
+    pos = qk_norm.positions(input_pos, b, s, cache.shape[0])
+    if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+        raise ValueError(f"values {tuple(v.shape)} of {v.dtype} on {v.device} are not like keys {tuple(k.shape)} of {k.dtype} on {k.device}")
+    to = k_cache.shape
+    if len(to) != 4 or to != v_cache.shape or to[0] != b or to[2:] != k.shape[2:] or not (k_cache.dtype == v_cache.dtype == k.dtype) or not (k_cache.device == v_cache.device == k.device):
+        raise ValueError(f"caches {tuple(to)} and {tuple(v_cache.shape)} of {k_cache.dtype} and {v_cache.dtype} are not [{b}, slots, {k.shape[2]}, {k.shape[3]}] of {k.dtype} on {k.device}")
+    if slots.dtype != torch.int64 or slots.shape != (s,) or not slots.is_contiguous() or slots.device != k.device:
+        raise ValueError(f"slots are contiguous int64 of [{s}] on {k.device}, not {slots.dtype} of {tuple(slots.shape)} on {slots.device}")
+    if _differentiated(q, k, v, q_gain, k_gain, k_cache, v_cache):
+        raise ValueError("no gradient flows through a cache: call this without autograd")
+    if pos is not None and pos.device != q.device:
+        pos = pos.to(q.device)
+    if q.numel() == 0:
+        return torch.empty_like(q)
+    if (cuda_ops_enabled(q) and qk_norm.suits(q, cache) and qk_norm.append_suits(k_cache, v_cache)
+            and _has_memory(q, k, v, cache, k_cache, v_cache, slots, *(t for t in (q_gain, k_gain, pos) if t is not None))):
+        return qk_norm.norm_rope_append(q, k, v, q_gain, k_gain, cache, pos, k_cache, v_cache, slots, float(eps), bool(interleaved), bool(norm_first))
+    _fallback("qk_norm_rope_append", f"head dimension {q.shape[-1]}, angles in {cache.dtype} or caches whose rows do not start on 16 bytes", q)
+    k_cache.index_copy_(1, slots, reference.norm_rope(k, k_gain, cache, pos, eps, interleaved, norm_first))
+    v_cache.index_copy_(1, slots, v)
+    return reference.norm_rope(q, q_gain, cache, pos, eps, interleaved, norm_first)
 
 
 def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:

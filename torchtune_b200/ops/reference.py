@@ -144,6 +144,31 @@ def rope_half(x: torch.Tensor, cache: torch.Tensor, input_pos: Optional[torch.Te
     return torch.cat([x1 * cos - x2 * sin, x2 * cos + x1 * sin], -1).type_as(x)
 
 
+def norm_rope(x: torch.Tensor, gain: Optional[torch.Tensor], cache: torch.Tensor, pos: Optional[torch.Tensor], eps: float, interleaved: bool, norm_first: bool) -> torch.Tensor:
+    """RMS norm of every head of ``x`` ``[b, s, h, d]`` times ``gain`` and rotation by the angles of ``cache`` ``[positions, d/2, 2]`` at ``pos`` ``[b, s]`` (``None``: 0 ... s - 1), in that order or the
+    other way round; fp32 (fp64 for fp64 inputs) with one rounding at the end."""
+    wide = torch.promote_types(x.dtype, torch.float32)
+    if pos is not None and not x.is_cuda and pos.numel() and (int(pos.min()) < 0 or int(pos.max()) >= cache.shape[0]):
+        raise ValueError(f"positions {int(pos.min())} to {int(pos.max())} and angles for {cache.shape[0]}")
+    if pos is not None and x.is_cuda:
+        pos = torch.where((pos >= 0) & (pos < cache.shape[0]), pos, torch.zeros_like(pos))
+    angles = (cache[: x.shape[1]] if pos is None else cache[pos.long()]).to(wide).unsqueeze(-3)  # [b or 1, s, 1, d/2, 2]
+    cos, sin = angles[..., 0], angles[..., 1]
+
+    def turn(t: torch.Tensor) -> torch.Tensor:
+        a, b = t.unflatten(-1, (-1, 2)).unbind(-1) if interleaved else t.chunk(2, -1)
+        a, b = a * cos - b * sin, b * cos + a * sin
+        return torch.stack([a, b], -1).flatten(-2) if interleaved else torch.cat([a, b], -1)
+
+    y = x.to(wide)
+    if not norm_first:
+        y = turn(y)
+    y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps)
+    if gain is not None:
+        y = y * gain.to(wide)
+    return (turn(y) if norm_first else y).to(x.dtype)
+
+
 def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     """``silu(gate) * up`` (torchtune/modules/feed_forward.py:50-53)."""
     return F.silu(gate) * up
