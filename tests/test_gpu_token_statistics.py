@@ -1,0 +1,200 @@
+"""Log-probabilities, entropies, alternatives and their gradients on the kernels, against the statement in 64 bits."""
+import pytest
+import torch
+
+from torchtune_b200 import ops
+from torchtune_b200.ops import _lib, reference
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+INF = float("inf")
+STEP = 2.0**-24
+
+
+def _logits(*shape, seed=0, dtype=torch.bfloat16, spread=3.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (spread * torch.randn(*shape, generator=g, device=DEV)).to(dtype)
+
+
+def _check(logits, tokens, temperature=1.0, top=0, grads=True, seed=1):
+    """All outputs and the gradient with random weights against 64 bits."""
+    v = logits.shape[-1]
+    x = logits.detach().clone().requires_grad_(grads)
+    with torch.set_grad_enabled(grads):
+        s = ops.token_statistics(x, tokens, temperature=temperature, top=top)
+    x64 = logits.double().requires_grad_(grads)
+    want = reference.token_statistics(x64, tokens, temperature, top, -100)
+    # a thread adds up v / 2048 vectors of 8, the CTA's threads 8 steps more; exponentials are 4 steps off and twice their argument's, which is below 60
+    sums = 140 + v / 2048
+    bound = STEP * (sums + 4 * want[0].abs())
+    assert ((s.logprobs.double() - want[0]).abs() <= bound).all(), float((s.logprobs.double() - want[0]).abs().max())
+    assert ((s.entropy.double() - want[1]).abs() <= STEP * 2 * sums * (1 + want[1])).all(), float((s.entropy.double() - want[1]).abs().max())
+    if top:
+        assert torch.equal(s.top_tokens, want[3])
+        assert ((s.top_logprobs.double() - want[2]).abs() <= STEP * (sums + 4 * want[2].abs())).all()
+    if not grads:
+        return s
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    weights = [torch.randn(t.shape, generator=g, device=DEV) for t in s[: 3 if top else 2]]
+    (got,) = torch.autograd.grad(s[: len(weights)], x, weights)
+    (exact,) = torch.autograd.grad(want[: len(weights)], x64, [w.double() for w in weights])
+    assert got.dtype == logits.dtype and got.shape == logits.shape
+    logp = torch.log_softmax(x64.detach() / temperature, -1)
+    each = sum(w.double().abs().reshape(*tokens.shape, -1).sum(-1) for w in (weights[0], *weights[2:]))[..., None] + weights[1].double().abs()[..., None] * (want[1].detach()[..., None] + logp.abs())
+    info = torch.finfo(got.dtype)
+    bound = info.eps / 2 * exact.abs().clamp(min=info.tiny) + STEP * ((sums + 4 * logp.abs()) * logp.exp() * each + 8 * (each if top else weights[0].abs()[..., None])) / temperature + 1e-36
+    bound = torch.where(torch.isfinite(bound), bound, torch.zeros_like(bound))
+    far = (got.double() - exact).abs() - bound
+    assert (far <= 0).all(), float(far.max())
+    return s
+
+
+@pytest.mark.parametrize("top", [0, 1, 20, 64])
+@pytest.mark.parametrize("rows,v,dtype,temperature", [
+    (1, 64, torch.float32, 1.0), (5, 257, torch.bfloat16, 0.7), (3, 2048, torch.float16, 1.3), (2, 4099, torch.bfloat16, 1.0), (40, 32003, torch.bfloat16, 0.9), (7, 50257, torch.float32, 0.5),
+    (16, 128256, torch.float32, 1.0), (3, 151936, torch.bfloat16, 1.0), (700, 5001, torch.float16, 1.0)])
+def test_against_64_bits(rows, v, dtype, temperature, top):
+    logits = _logits(rows, v, dtype=dtype)
+    tokens = torch.randint(0, v, (rows,), device=DEV)
+    tokens[0] = logits[0].argmax()
+    if rows > 2:
+        tokens[1], tokens[2] = v - 1, -100
+    _check(logits, tokens, temperature, top)
+
+
+@pytest.mark.parametrize("v", [1, 2, 7, 8, 9, 31, 255])
+def test_small_vocabularies(v):
+    for dtype in (torch.bfloat16, torch.float32):
+        _check(_logits(9, v, dtype=dtype), torch.arange(9, device=DEV) % v, top=min(v, 64))
+
+
+@pytest.mark.parametrize("order", ["up", "down", "equal", "blocks"])
+def test_alternatives_whatever_the_order(order):
+    """Rows whose largest logits lie together, which a choice by parts could miss, and rows of ties."""
+    v = 33000
+    x = torch.arange(v, device=DEV, dtype=torch.float32) / 1000
+    x = {"up": x, "down": x.flip(0), "equal": torch.zeros_like(x), "blocks": (torch.arange(v, device=DEV) // 300 % 7).float()}[order]
+    for rows in (1, 600):
+        s = _check(x.expand(rows, v).contiguous(), torch.zeros(rows, dtype=torch.int64, device=DEV), top=64, grads=rows == 1)
+        assert s.top_tokens[0].tolist() == torch.sort(x, descending=True, stable=True).indices[:64].tolist()
+
+
+def test_masked_and_non_finite_logits():
+    v, low = 5000, torch.finfo(torch.float32).min
+    x = _logits(8, v, dtype=torch.float32)
+    x[0, 3:] = -INF  # three tokens are left
+    x[1] = -INF
+    x[2] = low
+    x[3, 1:4999] = low
+    x[4, 17] = float("nan")
+    x[5, 4001] = INF
+    x[6, ::2] = -INF
+    x[7, :4096] = -INF  # whole segments
+    tokens = torch.tensor([2, 0, 9, 0, 1, 1, 1, 4999], device=DEV)
+    for case in (x, x[:, 1:]):  # rows that begin at odd addresses too
+        s = ops.token_statistics(case, tokens, top=5)
+        want = reference.token_statistics(case.double(), tokens, 1.0, 5, -100) if case.shape[1] == v else None
+        if want is None:
+            continue
+        assert torch.equal(s.top_tokens, want[3])
+        for a, b in zip(s[:3], want[:3]):
+            torch.testing.assert_close(a.double(), b, rtol=2e-5, atol=2e-5, equal_nan=True)
+        assert s.logprobs[[1, 4, 5]].isnan().all() and s.entropy[[1, 4, 5]].isnan().all() and s.logprobs[[0, 2, 3, 6, 7]].isfinite().all()
+    leaf = x[[0, 2, 3, 6, 7]].requires_grad_()
+    s = ops.token_statistics(leaf, tokens[[0, 2, 3, 6, 7]], top=2)
+    (g,) = torch.autograd.grad(s.logprobs.sum() + s.entropy.sum() + s.top_logprobs[:, 0].sum(), leaf)
+    assert g.isfinite().all() and not g[0, 3:].any() and not g[4, :4096].any()
+
+
+def test_layouts():
+    """Slices of a batch are read where they are; other layouts are copied; gradients have the logits' shape."""
+    whole = _logits(3, 40, 1003)
+    tokens = torch.randint(0, 1003, (3, 17), device=DEV)
+    part = whole[:, 5:22]
+    apart = ops.token_statistics(part.contiguous(), tokens, top=3)
+    before = torch.cuda.memory_stats()["allocated_bytes.all.allocated"]
+    s = ops.token_statistics(part, tokens, top=3)
+    assert torch.cuda.memory_stats()["allocated_bytes.all.allocated"] - before < part.numel() * 2  # no copy
+    # rows of an odd width begin at another address in a copy, and their sums run in another order: both are within the bound of _check
+    def near(a, b):
+        return bool(((a - b).abs() <= 2 * STEP * (141 + 4 * b.abs())).all())
+
+    assert near(s.logprobs, apart.logprobs) and near(s.top_logprobs, apart.top_logprobs) and torch.equal(s.top_tokens, apart.top_tokens)
+    assert ((s.entropy - apart.entropy).abs() <= 4 * STEP * 141 * (1 + apart.entropy)).all()
+    turned = part.transpose(-1, -2).contiguous().transpose(-1, -2)
+    assert torch.equal(ops.token_statistics(turned, tokens).logprobs, apart.logprobs)
+    _check(part, tokens, top=3)
+    leaf = whole.clone().requires_grad_()
+    ops.token_statistics(leaf[:, 5:22], tokens).logprobs.sum().backward()
+    assert not leaf.grad[:, :5].any() and not leaf.grad[:, 22:].any()
+    again = part.contiguous().requires_grad_()
+    ops.token_statistics(again, tokens).logprobs.sum().backward()
+    # two roundings to bf16 of values 2 * 141 roundings of 32 bits apart
+    assert ((leaf.grad[:, 5:22] - again.grad).abs() <= 2.0**-7 * again.grad.abs() + 2 * STEP * 141).all()
+    one = ops.token_statistics(part[0, 0], tokens[0, 0], top=3)
+    assert one.logprobs.shape == () and torch.equal(one.top_tokens, apart.top_tokens[0, 0])
+    strided = ops.token_statistics(part, torch.stack([tokens, tokens], -1)[..., 0], top=3)
+    assert torch.equal(strided.logprobs, s.logprobs)
+
+
+def test_gradients_of_parts_of_the_result():
+    logits, tokens = _logits(6, 3001), torch.randint(0, 3001, (6,), device=DEV)
+    x64 = logits.double().requires_grad_()
+    want = reference.token_statistics(x64, tokens, 1.0, 4, -100)
+    for i in range(3):
+        leaf = logits.clone().requires_grad_()
+        s = ops.token_statistics(leaf, tokens, top=4)
+        (g,) = torch.autograd.grad(s[i].sum(), leaf)
+        (exact,) = torch.autograd.grad(want[i].sum(), x64, retain_graph=True)
+        torch.testing.assert_close(g.double(), exact, rtol=2.0**-8, atol=1e-5)
+    assert not s.top_tokens.requires_grad
+
+
+def test_tokens_out_of_range_are_counted():
+    logits = _logits(4, 99)
+    _lib.index_violations()
+    leaf = logits.clone().requires_grad_()
+    s = ops.token_statistics(leaf, torch.tensor([99, -1, -100, 5], device=DEV))
+    assert _lib.index_violations() == 2 and not s.logprobs[:3].any() and s.logprobs[3] < 0
+    (g,) = torch.autograd.grad(s.logprobs.sum(), leaf)
+    assert not g[:3].any() and g[3].any()
+
+
+def test_results_do_not_change_and_recordings_hold_their_own():
+    logits, tokens = _logits(9, 32003), torch.randint(0, 32003, (9,), device=DEV)
+    leaf = logits.clone().requires_grad_()
+
+    def step():
+        s = ops.token_statistics(leaf, tokens, top=7)
+        (g,) = torch.autograd.grad(s.logprobs.sum() - s.entropy.sum(), leaf)
+        return (*(t.detach() for t in s), g)
+
+    eager = step()
+    assert all(torch.equal(a, b) for a, b in zip(eager, step()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert all(torch.equal(a, b) for a, b in zip(eager, step()))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for t in out:
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(eager, out))
+
+
+def test_rows_beyond_32_bits():
+    """Rows that begin behind 2^31 elements."""
+    v, rows = 128256, 17000
+    logits = torch.zeros(rows, v, dtype=torch.bfloat16, device=DEV)
+    logits[-1] = _logits(v)
+    tokens = torch.full((rows,), 7, device=DEV)
+    s = ops.token_statistics(logits, tokens, top=2)
+    want = reference.token_statistics(logits[-1:].double(), tokens[-1:], 1.0, 2, -100)
+    assert torch.equal(s.top_tokens[-1:], want[3])
+    torch.testing.assert_close(s.logprobs[-1:].double(), want[0], rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(s.entropy[-1:].double(), want[1], rtol=1e-5, atol=1e-5)

@@ -21,7 +21,9 @@ import torch.nn.functional as F
 from . import reference
 from .mask import AttentionMask
 from . import qk_norm, quantized
+from . import token_stats
 from .quantized import QuantizedRows
+from .token_stats import TokenStatistics
 
 __all__ = [
     "grouped_matmul",
@@ -55,6 +57,8 @@ __all__ = [
     "linear_cross_entropy",
     "linear_cross_entropy_mean",
     "token_logprobs",
+    "TokenStatistics",
+    "token_statistics",
     "embedding",
     "embed_tokens",
     "AttentionMask",
@@ -631,6 +635,20 @@ def logits_logprobs(logits: torch.Tensor, tokens: torch.Tensor, temperature: flo
         plain = _differentiated(logits) or isinstance(temperature, torch.Tensor) or not _has_memory(logits, tokens)
         return None if plain else _cuda.logits_logprobs_f32(logits, tokens, temperature)
     return _cuda.logits_logprobs(logits, tokens, temperature) if logits.shape[-1] % 8 == 0 else None
+
+
+def token_statistics(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0, top: int = 0, ignore_index: int = -100) -> TokenStatistics:
+    """Of ``softmax(logits / temperature)`` over the last dimension: the log-probability of ``tokens`` (int64, the shape of ``logits`` without it), the entropy, and the ``top`` (up to 64)
+    likeliest tokens with their log-probabilities, the largest logits first and of equal ones those of the lower index (NaN counts as largest).  CUDA logits in bf16, fp16 or fp32, of any width and
+    row pitch, are read once, and once more for the gradient of all three.  A token equal to ``ignore_index`` has log-probability 0 without a gradient (its row's entropy and alternatives are
+    still those of the row); so, counted as an index violation, has one outside the vocabulary on a CUDA device; elsewhere that is an error.  Infinitely low logits have probability 0 and no share
+    in the entropy; a row of nothing else, or one with a NaN or an infinitely high logit, has NaN for both."""
+    token_stats.check_arguments(logits, tokens, temperature, top)
+    if cuda_ops_enabled(logits) and _has_memory(logits, tokens) and token_stats.suits(logits, top) and torch.autograd.forward_ad._current_level < 0 and tokens.numel() > 0:
+        return token_stats.token_statistics(logits, tokens, float(temperature), int(top), int(ignore_index), _differentiated(logits))
+    if tokens.numel() > 0:
+        _fallback("token_statistics", f"{logits.shape[-1]} logits with {top} alternatives, or subclasses of tensors", logits)
+    return TokenStatistics(*reference.token_statistics(logits, tokens, temperature, top, ignore_index))
 
 
 def sample_tokens(logits: torch.Tensor, q: torch.Tensor, temperature: float, top_k: Optional[int]) -> Optional[torch.Tensor]:

@@ -169,6 +169,23 @@ def norm_rope(x: torch.Tensor, gain: Optional[torch.Tensor], cache: torch.Tensor
     return (turn(y) if norm_first else y).to(x.dtype)
 
 
+def token_statistics(logits: torch.Tensor, tokens: torch.Tensor, temperature: float, top: int, ignore_index: int):
+    """Log-probabilities of ``tokens`` under ``softmax(logits / temperature)``, entropies, and log-probabilities and indices of the ``top`` largest logits (of equal ones the lower index
+    first), in fp32 (fp64 for fp64 logits)."""
+    known = (tokens >= 0) & (tokens < logits.shape[-1])
+    if not logits.is_cuda and not bool((known | (tokens == ignore_index)).all()):
+        raise ValueError(f"a token is neither one of {logits.shape[-1]} nor {ignore_index}")
+    known &= tokens != ignore_index
+    dist = torch.log_softmax(logits.to(torch.promote_types(logits.dtype, torch.float32)) / temperature, -1)
+    picked = dist.gather(-1, torch.where(known, tokens, torch.zeros_like(tokens)).unsqueeze(-1)).squeeze(-1)
+    logprobs = torch.where(known, picked, torch.zeros_like(picked))
+    entropy = -(dist.exp() * dist.masked_fill(dist == float("-inf"), 0.0)).sum(-1)
+    if not top:
+        return logprobs, entropy, None, None
+    best = torch.sort(logits.detach(), dim=-1, descending=True, stable=True).indices[..., :top]
+    return logprobs, entropy, dist.gather(-1, best), best
+
+
 def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     """``silu(gate) * up`` (torchtune/modules/feed_forward.py:50-53)."""
     return F.silu(gate) * up
