@@ -21,7 +21,7 @@ import torch.nn.functional as F
 from . import reference
 from .mask import AttentionMask
 from . import qk_norm, quantized
-from . import token_stats
+from . import shared_prefix, token_stats
 from .quantized import QuantizedRows
 from .token_stats import TokenStatistics
 
@@ -54,6 +54,7 @@ __all__ = [
     "quantized_append",
     "quantized_read",
     "quantized_attention",
+    "shared_prefix_attention",
     "linear_cross_entropy",
     "linear_cross_entropy_mean",
     "token_logprobs",
@@ -578,6 +579,30 @@ def quantized_attention(q: torch.Tensor, k_rows: QuantizedRows, v_rows: Quantize
             return quantized.attention(q, mask, scale, size, steps)
     k, v = quantized_read(k_rows, v_rows, dtype=q.dtype)
     return attention(q, k, v, mask, scale=scale, softcap=softcap, dropout_p=dropout_p)
+
+
+def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, prefix_start: Optional[torch.Tensor] = None,
+                            prefix_stop: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of ``q`` ``[rows, s, h, d]`` over the keys and values of a prompt that several rows share, ``[prompts, n, h_kv, d]``, and over each row's own, ``[rows, slots, h_kv, d]``: row ``r``
+    belongs to prompt ``r // (rows // prompts)``, whose slots ``prefix_start[prompt]`` ... ``prefix_stop[prompt] - 1`` it sees (int32, by default all ``n``), and of its own the first ``lengths[row]``
+    (int32, by default all slots), of which its ``s`` queries are the last ones and see none behind their own.  Numbers out of range are cut off at it.  A query that sees no key gives 0, and what
+    lies in slots that no query of a row sees has no influence; one that only later tokens of the same call see should be finite.  The prefix is read once for all rows of a prompt.  bf16 CUDA
+    tensors with 64 or 128 channels outside autograd take the kernels (for keys and values in strides that are multiples of 16 bytes, where they lie); everything else takes the plain statement,
+    which has gradients."""
+    shared_prefix.check_arguments(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, lengths)
+    if q.numel() == 0:
+        return torch.empty_like(q)
+    if _native(q):
+        index = tuple(t for t in (prefix_start, prefix_stop, lengths) if t is not None)
+        if q.shape[3] not in shared_prefix.HEAD_DIMS:
+            _fallback("shared_prefix_attention", f"head dimension {q.shape[3]}", q)
+        elif _differentiated(q, k_prefix, v_prefix, k, v):
+            _fallback("shared_prefix_attention", "gradients", q)
+        elif not _has_memory(q, k_prefix, v_prefix, k, v, *index):
+            _fallback("shared_prefix_attention", "subclasses of tensors", q)
+        else:
+            return shared_prefix.attention(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, lengths, scale)
+    return reference.shared_prefix_attention(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, lengths, scale)
 
 
 def linear_cross_entropy(

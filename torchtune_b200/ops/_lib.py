@@ -193,6 +193,10 @@ def _declare(L: ctypes.CDLL) -> None:
     L.ttb_token_stats.restype = i32
     L.ttb_token_stats_bwd.argtypes = [c.c_char_p, f32, f32, vp]
     L.ttb_token_stats_bwd.restype = i32
+    L.ttb_shared_prefix_attention.argtypes = [c.c_char_p, f32, vp, vp]
+    L.ttb_shared_prefix_attention.restype = i32
+    L.ttb_shared_prefix_floats.argtypes = [c.c_char_p]
+    L.ttb_shared_prefix_floats.restype = i64
     L.ttb_qk_norm_rope_rows.argtypes = [c.c_char_p]
     L.ttb_qk_norm_rope_rows.restype = i64
     for fn in (L.ttb_span_decode_tile, L.ttb_span_prepare, L.ttb_span_prefill, L.ttb_span_decode, L.ttb_stream_step, L.ttb_embed_positions, L.ttb_clamped_glu, L.ttb_lightning_recurrent,

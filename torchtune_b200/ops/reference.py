@@ -169,6 +169,34 @@ def norm_rope(x: torch.Tensor, gain: Optional[torch.Tensor], cache: torch.Tensor
     return (turn(y) if norm_first else y).to(x.dtype)
 
 
+def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_start: Optional[torch.Tensor],
+                            prefix_stop: Optional[torch.Tensor], lengths: Optional[torch.Tensor], scale: Optional[float]) -> torch.Tensor:
+    """``q`` ``[rows, s, h, d]`` over the visible slots of the row's prompt ``[prompts, n, h_kv, d]`` and of its own ``[rows, slots, h_kv, d]``, in fp32 (fp64 for fp64 inputs); a query that sees no key
+    gives 0, and slots that no query of a row sees have no influence."""
+    rows, s, hq, d = q.shape
+    prompts, n, hkv, _ = k_prefix.shape
+    m, dev, wide = k.shape[1], q.device, torch.promote_types(q.dtype, torch.float32)
+    at = torch.arange(n, device=dev)
+    shared = torch.ones(prompts, n, dtype=torch.bool, device=dev)
+    if prefix_start is not None:
+        shared &= at >= prefix_start[:, None]
+    if prefix_stop is not None:
+        shared &= at < prefix_stop[:, None]
+    shared = shared.repeat_interleave(rows // prompts, 0)
+    length = torch.full((rows,), m, device=dev) if lengths is None else lengths.clamp(0, m).long()
+    last = length[:, None] - s + torch.arange(s, device=dev)
+    seen = torch.cat([shared[:, None].expand(rows, s, n), torch.arange(m, device=dev) <= last[..., None]], -1)  # [rows, s, n + m]
+    any_seen = torch.cat([shared, torch.arange(m, device=dev) < length[:, None]], -1)[..., None, None]
+    keys, values = (torch.cat([a.repeat_interleave(rows // prompts, 0), b], 1).to(wide).masked_fill(~any_seen, 0.0) for a, b in ((k_prefix, k), (v_prefix, v)))
+    qh = q.to(wide).view(rows, s, hkv, hq // hkv, d).permute(0, 2, 3, 1, 4)
+    score = (qh @ keys.permute(0, 2, 3, 1).unsqueeze(2)) * (d**-0.5 if scale is None else scale)
+    score = score.masked_fill(~seen[:, None, None], float("-inf"))
+    nothing = ~seen.any(-1)[:, None, None, :, None]
+    p = torch.softmax(score.masked_fill(nothing, 0.0), -1).masked_fill(nothing, 0.0)
+    out = p @ values.permute(0, 2, 1, 3).unsqueeze(2)
+    return out.permute(0, 3, 1, 2, 4).reshape(rows, s, hq, d).to(q.dtype)
+
+
 def token_statistics(logits: torch.Tensor, tokens: torch.Tensor, temperature: float, top: int, ignore_index: int):
     """Log-probabilities of ``tokens`` under ``softmax(logits / temperature)``, entropies, and log-probabilities and indices of the ``top`` largest logits (of equal ones the lower index
     first), in fp32 (fp64 for fp64 logits)."""

@@ -1,0 +1,66 @@
+"""Attention of rows that share a long prefix (``csrc/shared_prefix.cu``)."""
+from __future__ import annotations
+
+import math
+import struct
+from typing import Optional
+
+import torch
+
+from ._lib import check, err_word, lib
+from .quantized import _on
+
+HEAD_DIMS = (64, 128)  # that the kernel has
+_pack = struct.Struct("=31q").pack  # the kernel source's Call
+
+
+def check_arguments(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, lengths) -> None:
+    a, b, c = q.shape, k_prefix.shape, k.shape
+    if len(a) != 4 or len(b) != 4 or len(c) != 4 or b != v_prefix.shape or c != v.shape:
+        raise ValueError(f"queries {tuple(a)}, prefix {tuple(b)} and {tuple(v_prefix.shape)}, own {tuple(c)} and {tuple(v.shape)} are not [rows, tokens, heads, channels] with keys like values")
+    if a[0] != c[0] or b[2:] != c[2:] or a[3] != c[3] or c[2] == 0 or a[2] % c[2] or a[2] == 0 or (b[0] == 0) != (a[0] == 0) or (b[0] and a[0] % b[0]):
+        raise ValueError(f"{a[0]} rows of {a[2]} query heads of {a[3]} channels, {b[0]} prompts and {c[0]} rows with {b[2]} and {c[2]} key heads of {b[3]} and {c[3]}: rows are a multiple of the "
+                         "prompts, query heads of the key heads")
+    if not (q.dtype == k_prefix.dtype == v_prefix.dtype == k.dtype == v.dtype) or not q.dtype.is_floating_point:
+        raise ValueError(f"queries, keys and values have one floating-point type, not {q.dtype}, {k_prefix.dtype}, {v_prefix.dtype}, {k.dtype} and {v.dtype}")
+    if not (q.device == k_prefix.device == v_prefix.device == k.device == v.device):
+        raise ValueError("queries, keys and values are on one device")
+    for name, t, n in (("prefix_start", prefix_start, b[0]), ("prefix_stop", prefix_stop, b[0]), ("lengths", lengths, a[0])):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (n,) or t.device != q.device):
+            raise ValueError(f"{name} is int32 of [{n}] on {q.device}, not {t.dtype} of {tuple(t.shape)} on {t.device}")
+
+
+def _steady(t: torch.Tensor) -> torch.Tensor:
+    """``t``, if copies of tiles of one head can read it where it is, or a copy."""
+    steps = t.stride()
+    if steps[3] == 1 and t.data_ptr() & 15 == 0 and all(n == 1 or (step > 0 and step % 8 == 0) for n, step in zip(t.shape[:3], steps)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _steps(t: torch.Tensor):
+    """Steps of batch, slot and head; those of dimensions of size 1 are not used, but have to be in range."""
+    return [step if n > 1 else t.shape[3] for n, step in zip(t.shape[:3], t.stride())]
+
+
+def attention(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, lengths, scale: Optional[float]) -> torch.Tensor:
+    rows, s, hq, d = q.shape
+    q = q.contiguous()
+    if q.data_ptr() & 15:
+        q = q.clone()
+    o = torch.empty_like(q)
+    kv = [_steady(t) for t in (k_prefix, v_prefix, k, v)]
+    index = [None if t is None else t.contiguous() for t in (prefix_start, prefix_stop, lengths)]
+    sizes = (*(x for t in kv for x in _steps(t)), k_prefix.shape[0], rows, s, hq, k.shape[2], d, k_prefix.shape[1], k.shape[1])
+
+    def call(work: int, floats: int) -> bytes:
+        return _pack(q.data_ptr(), o.data_ptr(), *(t.data_ptr() for t in kv), *(0 if t is None else t.data_ptr() for t in index), work, floats, *sizes)
+
+    with torch.cuda.device(q.device):
+        floats = lib().ttb_shared_prefix_floats(call(0, 0))
+        if floats < 0:
+            check(floats, "attention over a shared prefix")
+        work = torch.empty(floats, dtype=torch.float32, device=q.device)
+        check(_on(q, lib().ttb_shared_prefix_attention, call(work.data_ptr(), floats), 1.0 / math.sqrt(d) if scale is None else float(scale), err_word(q.device).data_ptr()),
+              "attention over a shared prefix")
+    return o
