@@ -407,7 +407,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gain: Optional[torch.Tensor
         pos = pos.to(q.device)
     if q.numel() == 0:
         return torch.empty_like(q), torch.empty_like(k)
-    if cuda_ops_enabled(q) and qk_norm.suits(q, cache) and _has_memory(q, k, cache, *(t for t in (q_gain, k_gain, pos) if t is not None)) and torch.autograd.forward_ad._current_level < 0:
+    if cuda_ops_enabled(q) and qk_norm.suits(q, k, cache) and _has_memory(q, k, cache, *(t for t in (q_gain, k_gain, pos) if t is not None)) and torch.autograd.forward_ad._current_level < 0:
         return qk_norm.norm_rope(q, k, q_gain, k_gain, cache, pos, float(eps), bool(interleaved), bool(norm_first), _differentiated(q, k, q_gain, k_gain))
     _fallback("qk_norm_rope", f"head dimension {q.shape[-1]} or angles in {cache.dtype}", q)
     return tuple(reference.norm_rope(x, gain, cache, pos, eps, interleaved, norm_first) for x, gain in ((q, q_gain), (k, k_gain)))
@@ -435,7 +435,7 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_gai
         pos = pos.to(q.device)
     if q.numel() == 0:
         return torch.empty_like(q)
-    if (cuda_ops_enabled(q) and qk_norm.suits(q, cache) and qk_norm.append_suits(k_cache, v_cache)
+    if (cuda_ops_enabled(q) and qk_norm.suits(q, k, cache) and qk_norm.append_suits(k_cache, v_cache)
             and _has_memory(q, k, v, cache, k_cache, v_cache, slots, *(t for t in (q_gain, k_gain, pos) if t is not None))):
         return qk_norm.norm_rope_append(q, k, v, q_gain, k_gain, cache, pos, k_cache, v_cache, slots, float(eps), bool(interleaved), bool(norm_first))
     _fallback("qk_norm_rope_append", f"head dimension {q.shape[-1]}, angles in {cache.dtype} or caches whose rows do not start on 16 bytes", q)

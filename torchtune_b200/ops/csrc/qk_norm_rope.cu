@@ -7,8 +7,8 @@
 //   dw = sum dz n over tokens and heads,   dx (or du) = r (dn - n mean(dn n)),   dx = R^T du in the second order.
 // All of it is fp32 with one rounding at the end; as a norm and a rotation of their own it is two roundings and, of two tensors, four launches and twice the traffic.
 //
-// A head row is shared by G lanes (a power of two), each with eight channels of the first half and the same eight of the second: in the half-split layout these are pairs, in the interleaved one
-// pairs lie within the eight, so that no value crosses lanes but the sums.  A group of lanes takes up to HEADS heads of one token, whose angles it keeps.
+// A head row is shared by G lanes (a power of two), each with N channels of the first half and the same N of the second: in the half-split layout these are pairs, in the interleaved one
+// pairs lie within the N, so that no value crosses lanes but the sums.  A group of lanes takes up to HEADS heads of one token, whose angles it keeps.
 // The gains' gradients are sums in registers over all that a CTA does, then rows of a workspace that a second launch adds up, both in an order that depends on sizes alone.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -56,58 +56,68 @@ __device__ __forceinline__ T narrowed(float x) {
   else return __float2bfloat16_rn(x);
 }
 
-template <typename T>
-struct alignas(16) Eight {  // as they lie in memory
-  T v[8];
+template <typename T, int N>
+struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Run {  // channels as they lie in memory
+  T v[N];
+  static constexpr int kBytes = N * sizeof(T);
   __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(p);
+    } else {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
+      for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
   }
   __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
+    } else {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
+      for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
+    }
   }
 };
-// Sixteen channels of a lane: [0, 8) of the first half, [8, 16) of the second.
-template <typename T>
-__device__ __forceinline__ void widen16(const Eight<T> (&from)[2], float (&f)[16]) {
+
+// The channels of a lane: [0, N) of the first half, [N, 2N) of the second.
+template <typename T, int N>
+__device__ __forceinline__ void widen(const Run<T, N> (&from)[2], float (&f)[2 * N]) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) f[i] = widened(from[i >> 3].v[i & 7]);
+  for (int i = 0; i < 2 * N; ++i) f[i] = widened(from[i / N].v[i % N]);
 }
-template <bool INTERLEAVED>
-__device__ __forceinline__ void load_angles(const float* at, int d, int v, float (&cs)[16]) {  // pair i: cs[2i], cs[2i + 1]
-  const float* a = INTERLEAVED ? at + 8 * v : at + 16 * v;
-  const float* b = INTERLEAVED ? at + d / 2 + 8 * v : at + 16 * v + 8;
+template <bool INTERLEAVED, int N>
+__device__ __forceinline__ void load_angles(const float* at, int d, int v, float (&cs)[2 * N]) {  // pair i: cs[2i], cs[2i + 1]
+  const float* a = INTERLEAVED ? at + N * v : at + 2 * N * v;
+  const float* b = INTERLEAVED ? at + d / 2 + N * v : at + 2 * N * v + N;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < N / 4; ++i) {
     *reinterpret_cast<float4*>(cs + 4 * i) = reinterpret_cast<const float4*>(a)[i];
-    *reinterpret_cast<float4*>(cs + 8 + 4 * i) = reinterpret_cast<const float4*>(b)[i];
+    *reinterpret_cast<float4*>(cs + N + 4 * i) = reinterpret_cast<const float4*>(b)[i];
   }
 }
-template <bool INTERLEAVED, bool BACK>
-__device__ __forceinline__ void turn(float (&f)[16], const float (&cs)[16]) {
+template <bool INTERLEAVED, bool BACK, int N>
+__device__ __forceinline__ void turn(float (&f)[2 * N], const float (&cs)[2 * N]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < N; ++i) {
     float& x = f[INTERLEAVED ? 2 * i : i];
-    float& y = f[INTERLEAVED ? 2 * i + 1 : i + 8];
+    float& y = f[INTERLEAVED ? 2 * i + 1 : i + N];
     const float c = cs[2 * i], s = BACK ? -cs[2 * i + 1] : cs[2 * i + 1], x0 = x;
     x = x0 * c - y * s;
     y = y * c + x0 * s;
   }
 }
-template <typename T>
-__device__ __forceinline__ void load_gain(const void* gain, int wide, int d, int v, float (&w)[16]) {
+template <typename T, int N>
+__device__ __forceinline__ void load_gain(const void* gain, int wide, int d, int v, float (&w)[2 * N]) {
   if (gain == nullptr) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = 1.f;
+    for (int i = 0; i < 2 * N; ++i) w[i] = 1.f;
   } else if (wide) {
-    Eight<float> t[2];
-    t[0].load(static_cast<const float*>(gain) + 8 * v), t[1].load(static_cast<const float*>(gain) + d / 2 + 8 * v);
-    widen16(t, w);
+    Run<float, N> t[2];
+    t[0].load(static_cast<const float*>(gain) + N * v), t[1].load(static_cast<const float*>(gain) + d / 2 + N * v);
+    widen(t, w);
   } else {
-    Eight<T> t[2];
-    t[0].load(static_cast<const T*>(gain) + 8 * v), t[1].load(static_cast<const T*>(gain) + d / 2 + 8 * v);
-    widen16(t, w);
+    Run<T, N> t[2];
+    t[0].load(static_cast<const T*>(gain) + N * v), t[1].load(static_cast<const T*>(gain) + d / 2 + N * v);
+    widen(t, w);
   }
 }
 template <int G>
@@ -125,20 +135,19 @@ __device__ __forceinline__ int position(const Params& p, long long token, int i,
 }
 
 // A unit is a chunk of HEADS heads of one token; units are dealt to groups of G lanes.
-template <typename T, bool INTERLEAVED, bool AFTER, int G, int HEADS>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Params p) {
+template <typename T, bool INTERLEAVED, bool AFTER, int N, int G, int HEADS>
+__global__ void __launch_bounds__(kThreads, N * sizeof(T) <= 8 ? 4 : 2) forward_kernel(const __grid_constant__ Params p) {
   const int v = threadIdx.x & (G - 1);
-  const long long unit = (blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x) / G;
-  const long long tokens = static_cast<long long>(p.b) * p.s;
-  const bool live = unit < tokens * p.chunks && v < p.d / 16;  // a group's lanes stay together: its sums take all of them
-  const long long token = live ? unit / p.chunks : 0;
+  const uint32_t unit = blockIdx.x * (kThreads / G) + threadIdx.x / G;
+  const bool live = unit < static_cast<uint32_t>(p.b) * p.s * p.chunks && v < p.d / (2 * N);  // a group's lanes stay together: its sums take all of them
+  const uint32_t token = live ? unit / p.chunks : 0;
   int chunk = live ? static_cast<int>(unit - token * p.chunks) : 0, which = 0;
   while (chunk >= p.part[which].chunks) chunk -= p.part[which].chunks, ++which;
   const Part& part = p.part[which];
-  const int bi = static_cast<int>(token / p.s), i = static_cast<int>(token - static_cast<long long>(bi) * p.s);
+  const int bi = static_cast<int>(token / p.s), i = static_cast<int>(token - static_cast<uint32_t>(bi) * p.s);
   const int h0 = chunk * HEADS, count = live ? min(HEADS, part.heads - h0) : 0;
-  const T* x = static_cast<const T*>(part.x) + bi * part.x_b + i * part.x_s + h0 * part.x_h + 8 * v;
-  Eight<T> raw[HEADS][2];
+  const T* x = static_cast<const T*>(part.x) + bi * part.x_b + i * part.x_s + h0 * part.x_h + N * v;
+  Run<T, N> raw[HEADS][2];
 #pragma unroll
   for (int h = 0; h < HEADS; ++h)
     if (h < count) raw[h][0].load(x + h * part.x_h), raw[h][1].load(x + h * part.x_h + p.d / 2);
@@ -151,103 +160,103 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
       kept = false, to = 0;
     }
   }
-  T* y = static_cast<T*>(part.y) + bi * part.y_b + to * part.y_s + h0 * part.y_h + 8 * v;
+  T* y = static_cast<T*>(part.y) + bi * part.y_b + to * part.y_s + h0 * part.y_h + N * v;
   if (which == 2) {
 #pragma unroll
     for (int h = 0; h < HEADS; ++h)
       if (kept && h < count) raw[h][0].store(y + h * part.y_h), raw[h][1].store(y + h * part.y_h + p.d / 2);
   }
-  float cs[16], w[16];
+  float cs[2 * N], w[2 * N];
   const int at = live ? position(p, token, i, which == 0 && chunk == 0 && v == 0) : 0, lane = live ? v : 0;
-  load_angles<INTERLEAVED>(p.table + static_cast<long long>(at) * p.d, p.d, lane, cs);
-  load_gain<T>(part.gain, p.wide_gain, p.d, lane, w);
+  load_angles<INTERLEAVED, N>(p.table + static_cast<long long>(at) * p.d, p.d, lane, cs);
+  load_gain<T, N>(part.gain, p.wide_gain, p.d, lane, w);
 #pragma unroll
   for (int h = 0; h < HEADS; ++h) {
-    float f[16];
+    float f[2 * N];
     if (h < count) {
-      widen16(raw[h], f);
+      widen(raw[h], f);
     } else {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) f[j] = 0.f;
+      for (int j = 0; j < 2 * N; ++j) f[j] = 0.f;
     }
-    if (AFTER) turn<INTERLEAVED, false>(f, cs);
+    if (AFTER) turn<INTERLEAVED, false, N>(f, cs);
     float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) sum += f[j] * f[j];
+    for (int j = 0; j < 2 * N; ++j) sum += f[j] * f[j];
     const float r = rsqrtf(group_sum<G>(sum) / p.d + p.eps);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) f[j] = f[j] * r * w[j];
-    if (!AFTER) turn<INTERLEAVED, false>(f, cs);
+    for (int j = 0; j < 2 * N; ++j) f[j] = f[j] * r * w[j];
+    if (!AFTER) turn<INTERLEAVED, false, N>(f, cs);
     if (kept && which < 2 && h < count) {
-      Eight<T> out[2];
+      Run<T, N> out[2];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) out[j >> 3].v[j & 7] = narrowed<T>(f[j]);
+      for (int j = 0; j < 2 * N; ++j) out[j / N].v[j % N] = narrowed<T>(f[j]);
       out[0].store(y + h * part.y_h), out[1].store(y + h * part.y_h + p.d / 2);
     }
   }
 }
 
-template <typename T, bool INTERLEAVED, bool AFTER, int G, int HEADS>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constant__ Params p) {
-  __shared__ float sums[kThreads / 32][16 * G];
+template <typename T, bool INTERLEAVED, bool AFTER, int N, int G, int HEADS>
+__global__ void __launch_bounds__(kThreads, N * sizeof(T) <= 8 ? 3 : N == 4 ? 2 : 1) backward_kernel(const __grid_constant__ Params p) {
+  __shared__ float sums[kThreads / 32][2 * N * G];
   const int v = threadIdx.x & (G - 1);
   const int which = static_cast<int>(blockIdx.x) >= p.ctas_q;
   const Part& part = p.part[which];
   const int cta = blockIdx.x - (which ? p.ctas_q : 0), ctas = which ? gridDim.x - p.ctas_q : p.ctas_q;
-  const long long units = static_cast<long long>(p.b) * p.s * part.chunks;
+  const uint32_t units = static_cast<uint32_t>(p.b) * p.s * part.chunks;
   constexpr int kGroups = kThreads / G;
-  const bool lane_live = v < p.d / 16;
+  const bool lane_live = v < p.d / (2 * N);
   const int lane = lane_live ? v : 0;
-  float w[16], dw[16];
-  load_gain<T>(part.gain, p.wide_gain, p.d, lane, w);
+  float w[2 * N], dw[2 * N];
+  load_gain<T, N>(part.gain, p.wide_gain, p.d, lane, w);
 #pragma unroll
-  for (int j = 0; j < 16; ++j) dw[j] = 0.f;
-  for (long long first = static_cast<long long>(cta) * kGroups; first < units; first += static_cast<long long>(ctas) * kGroups) {  // the same for all lanes of a warp
-    const long long unit = first + threadIdx.x / G;
+  for (int j = 0; j < 2 * N; ++j) dw[j] = 0.f;
+  for (uint32_t first = cta * kGroups; first < units; first += ctas * kGroups) {  // the same for all lanes of a warp; units are below 2^31
+    const uint32_t unit = first + threadIdx.x / G;
     const bool live = unit < units && lane_live;
-    const long long token = live ? unit / part.chunks : 0;
+    const uint32_t token = live ? unit / part.chunks : 0;
     const int chunk = live ? static_cast<int>(unit - token * part.chunks) : 0;
-    const int bi = static_cast<int>(token / p.s), i = static_cast<int>(token - static_cast<long long>(bi) * p.s);
+    const int bi = static_cast<int>(token / p.s), i = static_cast<int>(token - static_cast<uint32_t>(bi) * p.s);
     const int h0 = chunk * HEADS, count = live ? min(HEADS, part.heads - h0) : 0;
-    const T* x = static_cast<const T*>(part.x) + bi * part.x_b + i * part.x_s + h0 * part.x_h + 8 * v;
-    const T* dy = static_cast<const T*>(part.dy) + bi * part.dy_b + i * part.dy_s + h0 * part.dy_h + 8 * v;
-    T* dx = static_cast<T*>(part.y) + bi * part.y_b + i * part.y_s + h0 * part.y_h + 8 * v;
-    Eight<T> raw_x[HEADS][2], raw_dy[HEADS][2];
+    const T* x = static_cast<const T*>(part.x) + bi * part.x_b + i * part.x_s + h0 * part.x_h + N * v;
+    const T* dy = static_cast<const T*>(part.dy) + bi * part.dy_b + i * part.dy_s + h0 * part.dy_h + N * v;
+    T* dx = static_cast<T*>(part.y) + bi * part.y_b + i * part.y_s + h0 * part.y_h + N * v;
+    Run<T, N> raw_x[HEADS][2], raw_dy[HEADS][2];
 #pragma unroll
     for (int h = 0; h < HEADS; ++h)
       if (h < count) {
         raw_x[h][0].load(x + h * part.x_h), raw_x[h][1].load(x + h * part.x_h + p.d / 2);
         raw_dy[h][0].load(dy + h * part.dy_h), raw_dy[h][1].load(dy + h * part.dy_h + p.d / 2);
       }
-    float cs[16];
-    load_angles<INTERLEAVED>(p.table + static_cast<long long>(live ? position(p, token, i, false) : 0) * p.d, p.d, lane, cs);
+    float cs[2 * N];
+    load_angles<INTERLEAVED, N>(p.table + static_cast<long long>(live ? position(p, token, i, false) : 0) * p.d, p.d, lane, cs);
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
-      float f[16], g[16];
+      float f[2 * N], g[2 * N];
       if (h < count) {
-        widen16(raw_x[h], f), widen16(raw_dy[h], g);
+        widen(raw_x[h], f), widen(raw_dy[h], g);
       } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) f[j] = g[j] = 0.f;
+        for (int j = 0; j < 2 * N; ++j) f[j] = g[j] = 0.f;
       }
-      if (AFTER) turn<INTERLEAVED, false>(f, cs);
-      else turn<INTERLEAVED, true>(g, cs);
+      if (AFTER) turn<INTERLEAVED, false, N>(f, cs);
+      else turn<INTERLEAVED, true, N>(g, cs);
       float sum = 0.f, dot = 0.f;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sum += f[j] * f[j], dot += g[j] * w[j] * f[j];
+      for (int j = 0; j < 2 * N; ++j) sum += f[j] * f[j], dot += g[j] * w[j] * f[j];
       const float r = rsqrtf(group_sum<G>(sum) / p.d + p.eps);
       const float mean = group_sum<G>(dot) / p.d * r;  // of dn n
       if (h < count) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = 0; j < 2 * N; ++j) {
           const float n = f[j] * r;
           dw[j] += g[j] * n;
           f[j] = r * (g[j] * w[j] - n * mean);
         }
-        if (AFTER) turn<INTERLEAVED, true>(f, cs);
-        Eight<T> out[2];
+        if (AFTER) turn<INTERLEAVED, true, N>(f, cs);
+        Run<T, N> out[2];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) out[j >> 3].v[j & 7] = narrowed<T>(f[j]);
+        for (int j = 0; j < 2 * N; ++j) out[j / N].v[j % N] = narrowed<T>(f[j]);
         out[0].store(dx + h * part.y_h), out[1].store(dx + h * part.y_h + p.d / 2);
       }
     }
@@ -255,20 +264,20 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
   if (p.work == nullptr) return;
   // groups of a warp, then warps, in a fixed order
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
+  for (int j = 0; j < 2 * N; ++j) {
 #pragma unroll
     for (int o = G; o < 32; o <<= 1) dw[j] += __shfl_xor_sync(0xffffffffu, dw[j], o);
   }
   if ((threadIdx.x & 31) < G) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) sums[threadIdx.x >> 5][j * G + v] = dw[j];
+    for (int j = 0; j < 2 * N; ++j) sums[threadIdx.x >> 5][j * G + v] = dw[j];
   }
   __syncthreads();
   for (int c = threadIdx.x; c < p.d; c += kThreads) {
     const int half = c >= p.d / 2, in = c - half * (p.d / 2);
     float t = 0.f;
 #pragma unroll
-    for (int k = 0; k < kThreads / 32; ++k) t += sums[k][(half * 8 + (in & 7)) * G + (in >> 3)];
+    for (int k = 0; k < kThreads / 32; ++k) t += sums[k][(half * N + in % N) * G + in / N];
     p.work[static_cast<long long>(blockIdx.x) * p.d + c] = t;
   }
 }
@@ -310,13 +319,15 @@ static int by_type(long long type, F f) {
   if (type == 1) return f(__half());
   return f(0.f);
 }
+// Channels of a half per lane and lanes of a head row: four channels keep the backward pass in 80 registers, of which three CTAs find room on an SM; more than 256 channels need eight.
 template <typename F>
-static int by_size(int d, F f) {  // lanes of a head row
-  const int lanes = d / 16;
-  if (lanes <= 4) return f(std::integral_constant<int, 4>());
-  if (lanes <= 8) return f(std::integral_constant<int, 8>());
-  if (lanes <= 16) return f(std::integral_constant<int, 16>());
-  return f(std::integral_constant<int, 32>());
+static int by_size(int d, F f) {
+  using Four = std::integral_constant<int, 4>;
+  if (d <= 32) return f(Four(), std::integral_constant<int, 4>());
+  if (d <= 64) return f(Four(), std::integral_constant<int, 8>());
+  if (d <= 128) return f(Four(), std::integral_constant<int, 16>());
+  if (d <= 256) return f(Four(), std::integral_constant<int, 32>());
+  return f(std::integral_constant<int, 8>(), std::integral_constant<int, 32>());
 }
 template <typename F>
 static int by_order(const Call& c, F f) {
@@ -326,7 +337,8 @@ static int by_order(const Call& c, F f) {
 
 static int params_of(const Call& c, Params& p, int parts, int heads_of_unit) {
   if (c.b <= 0 || c.s <= 0 || c.d <= 0 || c.d % 16 || c.d > 512 || c.b > 0x7fffffff || c.s > 0x7fffffff || c.table_len <= 0) return kErrBadShape;
-  if (c.b * c.s > 0x7fffffffll || (c.table & 15)) return kErrTooLarge;
+  if (c.b * c.s * (c.heads[0] + c.heads[1] + c.heads[2]) > 0x7fffffffll) return kErrTooLarge;
+  if (c.table & 15) return kErrBadShape;
   p.table = reinterpret_cast<const float*>(c.table), p.pos = reinterpret_cast<const int*>(c.pos), p.slots = reinterpret_cast<const long long*>(c.slots);
   p.work = reinterpret_cast<float*>(c.work);
   p.b = static_cast<int>(c.b), p.s = static_cast<int>(c.s), p.d = static_cast<int>(c.d), p.table_len = static_cast<int>(c.table_len), p.slot_count = static_cast<int>(c.slot_count);
@@ -379,8 +391,8 @@ extern "C" int ttb_qk_norm_rope(const char* call, float eps, void* stream) {
   const int parts = c.heads[2] > 0 ? 3 : 2;
   return by_type(c.type, [&](auto t) {
     using T = decltype(t);
-    return by_size(static_cast<int>(c.d), [&](auto g) {
-      constexpr int G = decltype(g)::value;
+    return by_size(static_cast<int>(c.d), [&](auto n, auto g) {
+      constexpr int N = decltype(n)::value, G = decltype(g)::value;
       return by_order(c, [&](auto interleaved, auto after) {
         auto go = [&](auto heads) {
           constexpr int H = decltype(heads)::value;
@@ -391,12 +403,12 @@ extern "C" int ttb_qk_norm_rope(const char* call, float eps, void* stream) {
           const long long units = c.b * c.s * p.chunks, ctas = (units * G + kThreads - 1) / kThreads;
           if (ctas > 0x7fffffff) return static_cast<int>(kErrTooLarge);
           TTB_COUNT_LAUNCH(1);
-          forward_kernel<T, decltype(interleaved)::value, decltype(after)::value, G, H><<<static_cast<unsigned>(ctas), kThreads, 0, st>>>(p);
+          forward_kernel<T, decltype(interleaved)::value, decltype(after)::value, N, G, H><<<static_cast<unsigned>(ctas), kThreads, 0, st>>>(p);
           return cudaGetLastError() == cudaSuccess ? static_cast<int>(kOk) : static_cast<int>(kErrDriver);
         };
         // several heads to a group once there is work for all SMs
         const long long rows = c.b * c.s * (c.heads[0] + c.heads[1] + c.heads[2]);
-        return rows * G < 148ll * 2048 * 2 ? go(std::integral_constant<int, 1>()) : go(std::integral_constant<int, 4>());
+        return rows * G < 2048ll * sm_count() ? go(std::integral_constant<int, 1>()) : go(std::integral_constant<int, 4>());
       });
     });
   });
@@ -407,7 +419,7 @@ extern "C" long long ttb_qk_norm_rope_rows(const char* call) {
   using namespace ttb::qkn;
   const Call& c = *reinterpret_cast<const Call*>(call);
   int q = 0, k = 0;
-  by_size(static_cast<int>(c.d), [&](auto g) {
+  by_size(static_cast<int>(c.d), [&](auto, auto g) {
     ctas_of(c, kThreads / decltype(g)::value, kBackHeads, q, k);
     return 0;
   });
@@ -421,8 +433,8 @@ extern "C" int ttb_qk_norm_rope_bwd(const char* call, float eps, void* stream) {
   auto st = static_cast<cudaStream_t>(stream);
   return by_type(c.type, [&](auto t) {
     using T = decltype(t);
-    return by_size(static_cast<int>(c.d), [&](auto g) {
-      constexpr int G = decltype(g)::value;
+    return by_size(static_cast<int>(c.d), [&](auto n, auto g) {
+      constexpr int N = decltype(n)::value, G = decltype(g)::value;
       return by_order(c, [&](auto interleaved, auto after) {
         Params p{};
         p.eps = eps;
@@ -433,7 +445,7 @@ extern "C" int ttb_qk_norm_rope_bwd(const char* call, float eps, void* stream) {
         p.ctas_q = q;
         if (p.work != nullptr && c.work_rows < q + k) return static_cast<int>(kErrBadShape);
         TTB_COUNT_LAUNCH(1);
-        backward_kernel<T, decltype(interleaved)::value, decltype(after)::value, G, kBackHeads><<<q + k, kThreads, 0, st>>>(p);
+        backward_kernel<T, decltype(interleaved)::value, decltype(after)::value, N, G, kBackHeads><<<q + k, kThreads, 0, st>>>(p);
         if (cudaGetLastError() != cudaSuccess) return static_cast<int>(kErrDriver);
         if (p.work != nullptr) {
           TTB_COUNT_LAUNCH(1);

@@ -314,48 +314,74 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
   if (warp == 5) tmem_dealloc(tO, L::kColumns);
 }
 
-// A warp per token and query head joins its pieces: those of the prefix, then its own, each in their order.
+// A warp per token and query head joins its pieces, those of the prefix and then its own: a lane per piece finds where it lies, its maximum and sum, and the weights go around, so that all loads but
+// the first two are independent.  32 pieces at a time.
 static constexpr int kJoinWarps = 8;
 template <int D>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ Params p) {
-  const long long w = blockIdx.x * static_cast<long long>(kJoinWarps) + (threadIdx.x >> 5);
+  const uint32_t w = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  const long long token = w / p.hq;
-  if (token >= static_cast<long long>(p.rows) * p.s) return;
+  const uint32_t token = w / p.hq;
+  if (token >= static_cast<uint32_t>(p.rows) * p.s) return;
   const int h = static_cast<int>(w - token * p.hq), head = h / p.group, a = h - head * p.group;
-  const int row = static_cast<int>(token / p.s), i = static_cast<int>(token - static_cast<long long>(row) * p.s);
+  const int row = static_cast<int>(token / p.s), i = static_cast<int>(token - static_cast<uint32_t>(row) * p.s);
   const int per = p.rows / p.prompts, prompt = row / per;
   constexpr int kMine = D / 32;
   float m = -INFINITY, l = 0.f, o[kMine];
 #pragma unroll
   for (int x = 0; x < kMine; ++x) o[x] = 0.f;
-  auto join = [&](bool prefix, int owner, int cuts, int rows, long long base, int r) {
-    for (int cut = 0; cut < cuts; ++cut) {
+  const int pieces = p.cuts_p + p.cuts_o;
+  for (int first_piece = 0; first_piece < pieces; first_piece += 32) {
+    const int piece = first_piece + lane;
+    long long at = 0;
+    float2 t = make_float2(-INFINITY, 0.f);
+    if (piece < pieces) {
+      const bool prefix = piece < p.cuts_p;
+      const int cut = prefix ? piece : piece - p.cuts_p, owner = prefix ? prompt : row;
       int first, last;
       range_of(p, prefix, owner, cut, first, last);
-      if (first >= last) continue;
-      const long long at = base + ((static_cast<long long>(owner) * cuts + cut) * p.hkv + head) * rows + r;
-      const float2 t = p.ml[at];
-      if (t.x == -INFINITY && t.y == 0.f) continue;  // no key of this piece is seen
-      const float top = fmaxf(m, t.x);
-      const float f = m == -INFINITY ? 0.f : exp2f(m - top), g = exp2f(t.x - top);
-      l = l * f + t.y * g;
-      m = top;
-      const float* v = p.part + at * D + lane * kMine;
-      float x[kMine];
-      if constexpr (kMine == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(v);
-      else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(v);
-#pragma unroll
-      for (int y = 0; y < kMine; ++y) o[y] = o[y] * f + x[y] * g;
+      if (first < last) {  // otherwise nobody has written it
+        at = prefix ? ((static_cast<long long>(prompt) * p.cuts_p + cut) * p.hkv + head) * p.rows_p + ((row - prompt * per) * p.s + i) * p.group + a
+                    : static_cast<long long>(p.prompts) * p.cuts_p * p.hkv * p.rows_p + ((static_cast<long long>(row) * p.cuts_o + cut) * p.hkv + head) * p.rows_o + i * p.group + a;
+        t = p.ml[at];
+      }
     }
-  };
-  join(true, prompt, p.cuts_p, p.rows_p, 0, ((row - prompt * per) * p.s + i) * p.group + a);
-  join(false, row, p.cuts_o, p.rows_o, static_cast<long long>(p.prompts) * p.cuts_p * p.hkv * p.rows_p, i * p.group + a);
+    float top = fmaxf(m, t.x);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), weight = exp2f(t.x - base);
+    float sum = t.y * weight;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    l = l * f + sum;
+    m = top;
+#pragma unroll
+    for (int y = 0; y < kMine; ++y) o[y] *= f;
+    const int n = min(32, pieces - first_piece);
+    for (int x0 = 0; x0 < n; x0 += 4) {
+      float v[4][kMine], g[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        g[x] = __shfl_sync(0xffffffffu, weight, x0 + x);  // 0 where no key is seen
+        const float* from = p.part + __shfl_sync(0xffffffffu, at, x0 + x) * D + lane * kMine;
+        if (g[x] != 0.f) {
+          if constexpr (kMine == 4) *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(from);
+          else *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(from);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (g[x] != 0.f) {
+#pragma unroll
+          for (int y = 0; y < kMine; ++y) o[y] += v[x][y] * g[x];
+        }
+    }
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;  // a query without a key gives 0
   uint32_t out[kMine / 2];
 #pragma unroll
   for (int y = 0; y < kMine / 2; ++y) out[y] = pack_bf16x2(o[2 * y] * inv, o[2 * y + 1] * inv);
-  __nv_bfloat16* to = p.o + (token * p.hq + h) * D + lane * kMine;
+  __nv_bfloat16* to = p.o + (static_cast<long long>(token) * p.hq + h) * D + lane * kMine;
   if constexpr (kMine == 4) *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[1]);
   else *reinterpret_cast<uint32_t*>(to) = out[0];
 }

@@ -67,8 +67,7 @@ struct GradParams {
   const float *g, *h, *k;  // gradients of log-probabilities, entropy and alternatives; nullptr: none
   void* dx;                // [rows, vocab]
   long long ignore;
-  long long parts;         // CTAs of a row
-  int inner, vocab, top;
+  int inner, vocab, top, parts;  // parts: CTAs of a row
   float c, rate;           // rate = 1 / T
 };
 
@@ -101,28 +100,40 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 // A row as eight-element vectors on 16 bytes, the first of which may begin before it.
 template <typename T>
 struct Row {
+  struct alignas(16) Vector {
+    T v[8];
+  };
   const T* x;
   int vocab, off;  // off: elements of vector 0 in front of the row
   __device__ __forceinline__ Row(const T* row, int n) : x(row), vocab(n), off(static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T))) {}
   __device__ __forceinline__ int vectors() const { return static_cast<int>((static_cast<long long>(vocab) + off + 7) / 8); }
-  __device__ __forceinline__ bool whole(int j) const { return (j > 0 || off == 0) && j * 8ll + 8 - off <= vocab; }
-  struct alignas(16) Vector {
-    T v[8];
-  };
+  // vectors [whole_from(), whole_to()) hold no element outside the row
+  __device__ __forceinline__ int whole_from() const { return off != 0; }
+  __device__ __forceinline__ int whole_to() const { return static_cast<int>((static_cast<long long>(vocab) + off) / 8); }
+  __device__ __forceinline__ const Vector* vector(int j) const { return reinterpret_cast<const Vector*>(x - off) + j; }
+  __device__ __forceinline__ static Vector whole(const Vector* at) {
+    Vector r;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(r.v)[i] = reinterpret_cast<const uint4*>(at)[i];
+    return r;
+  }
   __device__ __forceinline__ Vector load(int j) const {  // elements outside the row: the lowest value
+    if (j >= whole_from() && j < whole_to()) return whole(vector(j));
     Vector r;
     const long long e = j * 8ll - off;
-    if (whole(j)) {
 #pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(r.v)[i] = reinterpret_cast<const uint4*>(x + e)[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) r.v[i] = e + i >= 0 && e + i < vocab ? x[e + i] : narrowed<T>(-INFINITY);
-    }
+    for (int i = 0; i < 8; ++i) r.v[i] = e + i >= 0 && e + i < vocab ? x[e + i] : narrowed<T>(-INFINITY);
     return r;
   }
   __device__ __forceinline__ uint32_t key(long long e) const { return e >= 0 && e < vocab ? key_of(widened(x[e])) : 0u; }
 };
+// Eight values in 32 bits, two by two.
+template <typename Vector>
+__device__ __forceinline__ void widen8(const Vector& raw, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = widened(raw.v[i]);
+}
+__device__ __forceinline__ float most_of(const float (&f)[8]) { return max3_nan(max3_nan(f[0], f[1], f[2]), max3_nan(f[3], f[4], f[5]), max3_nan(f[6], f[7], f[7])); }
 
 // base, s and t of a part of a row
 struct Sums {
@@ -203,56 +214,76 @@ __global__ void __launch_bounds__(kThreads, 4) stats_kernel(const __grid_constan
   const uint64_t c2 = pack_f32x2(p.c, p.c);
   float top_x = -INFINITY, base = 0.f;  // 0 until there is a logit above the infinitely low ones
   uint64_t s2 = 0, t2 = 0;
-  for (int j0 = first; j0 < first + segments * 32; j0 += kThreads * kAhead) {
-    typename Row<T>::Vector raw[kAhead];
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int j = j0 + a * kThreads + threadIdx.x;
-      if (j < end) raw[a] = row.load(j);
+  auto take = [&](const float (&f)[8], float most) {
+    if (!(most <= top_x)) {  // NaN too
+      const float d = fminf(fmaxf((base - most) * p.c, kLowest), 0.f), g = fast_exp2(d);
+      float s0, s1, t0, t1;
+      unpack_f32x2(s2, s0, s1), unpack_f32x2(t2, t0, t1);
+      const float s = s0 + s1, t = t0 + t1;
+      s2 = pack_f32x2(s * g, 0.f), t2 = pack_f32x2((t + s * d) * g, 0.f);
+      top_x = base = most;
     }
+    const uint64_t b2 = pack_f32x2(-base, -base);
+    uint64_t tv = 0;
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int j = j0 + a * kThreads + threadIdx.x;
-      if (j - lane >= first + segments * 32) break;  // the same for a warp
-      float f[8];
+    for (int i = 0; i < 8; i += 2) {
+      const uint64_t d = mul_f32x2(add_f32x2(pack_f32x2(f[i], f[i + 1]), b2), c2);
+      float d0, d1;
+      unpack_f32x2(d, d0, d1);
+      const uint64_t e = pack_f32x2(fast_exp2(d0), fast_exp2(d1));
+      s2 = add_f32x2(s2, e);
+      tv = fma_f32x2(e, d, tv);
+    }
+    float t0, t1;
+    unpack_f32x2(tv, t0, t1);
+    if (!(t0 + t1 <= 0.f)) {  // an infinitely low logit (0 * -inf); its share is 0
+      t0 = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = j < end ? widened(raw[a].v[i]) : -INFINITY;
-      const float most = max3_nan(max3_nan(f[0], f[1], f[2]), max3_nan(f[3], f[4], f[5]), max3_nan(f[6], f[7], f[7]));
-      if constexpr (TOP) {
-        const float m = warp_max_nan(most);
-        if (lane == 0) sh.segments[(j - first) >> 5] = key_of(m);
+      for (int i = 0; i < 8; ++i) {
+        const float d = (f[i] - base) * p.c;
+        t0 += fast_exp2(d) * (d < kLowest ? kLowest : d);
       }
-      if (!(most <= top_x)) {  // NaN too
-        const float d = fminf(fmaxf((base - most) * p.c, kLowest), 0.f), g = fast_exp2(d);
-        float s0, s1, t0, t1;
-        unpack_f32x2(s2, s0, s1), unpack_f32x2(t2, t0, t1);
-        const float s = s0 + s1, t = t0 + t1;
-        s2 = pack_f32x2(s * g, 0.f), t2 = pack_f32x2((t + s * d) * g, 0.f);
-        top_x = base = most;
-      }
-      const uint64_t b2 = pack_f32x2(-base, -base);
-      uint64_t sv = 0, tv = 0;
+      tv = pack_f32x2(t0, 0.f);
+    }
+    t2 = add_f32x2(t2, tv);
+  };
+  auto note = [&](int j, float most) {  // the maximum of a segment
+    if constexpr (TOP) {
+      const float m = warp_max_nan(most);
+      if (lane == 0) sh.segments[(j - first) >> 5] = key_of(m);
+    }
+  };
+  constexpr int kBlock = kThreads * kAhead;
+  for (int j0 = first; j0 < end; j0 += kBlock) {
+    if (j0 >= row.whole_from() && j0 + kBlock <= min(end, row.whole_to())) {  // the same for the CTA
+      const typename Row<T>::Vector* at = row.vector(j0 + threadIdx.x);
+      typename Row<T>::Vector raw[kAhead];
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        const uint64_t d = mul_f32x2(add_f32x2(pack_f32x2(f[i], f[i + 1]), b2), c2);
-        float d0, d1;
-        unpack_f32x2(d, d0, d1);
-        const uint64_t e = pack_f32x2(fast_exp2(d0), fast_exp2(d1));
-        sv = add_f32x2(sv, e);
-        tv = fma_f32x2(e, d, tv);
-      }
-      float t0, t1;
-      unpack_f32x2(tv, t0, t1);
-      if (!(t0 + t1 <= 0.f)) {  // an infinitely low logit (0 * -inf); its share is 0
-        t0 = 0.f;
+      for (int a = 0; a < kAhead; ++a) raw[a] = Row<T>::whole(at + a * kThreads);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float d = (f[i] - base) * p.c;
-          t0 += fast_exp2(d) * (d < kLowest ? kLowest : d);
+      for (int a = 0; a < kAhead; ++a) {
+        float f[8];
+        widen8(raw[a], f);
+        const float most = most_of(f);
+        note(j0 + a * kThreads + threadIdx.x, most);
+        take(f, most);
+      }
+    } else {
+#pragma unroll 1
+      for (int a = 0; a < kAhead; ++a) {
+        const int j = j0 + a * kThreads + threadIdx.x;
+        if (j - lane >= end) break;  // the same for a warp
+        float f[8];
+        if (j < end) {
+          widen8(row.load(j), f);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = -INFINITY;
         }
-        tv = pack_f32x2(t0, 0.f);
+        const float most = most_of(f);
+        note(j, most);
+        take(f, most);
       }
-      s2 = add_f32x2(s2, sv), t2 = add_f32x2(t2, tv);
     }
   }
   Sums mine;
@@ -364,56 +395,87 @@ __global__ void __launch_bounds__(kThreads, 4) stats_kernel(const __grid_constan
 static constexpr int kGradVectors = 4;  // of a thread
 // grid: rows * parts
 template <typename T>
-__global__ void __launch_bounds__(kThreads) grad_kernel(const __grid_constant__ GradParams p) {
-  const long long r = blockIdx.x / p.parts;
-  const int part = static_cast<int>(blockIdx.x - r * p.parts);
+__global__ void __launch_bounds__(kThreads, 4) grad_kernel(const __grid_constant__ GradParams p) {
+  constexpr int kBlock = kThreads * kGradVectors;
+  const int r = blockIdx.x / p.parts, part = blockIdx.x - r * p.parts;
   const Row<T> row(static_cast<const T*>(p.x) + r / p.inner * p.step_outer + r % p.inner * p.step_inner, p.vocab);
-  T* out = static_cast<T*>(p.dx) + r * p.vocab;
+  T* out = static_cast<T*>(p.dx) + static_cast<long long>(r) * p.vocab;
   const bool same = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(row.x)) & 15) == 0;  // whole vectors of the row are such of the gradient
-  const int vectors = row.vectors(), j0 = part * (kThreads * kGradVectors) + threadIdx.x;
+  const int vectors = row.vectors(), j0 = part * kBlock;
+  const bool whole = same && j0 >= row.whole_from() && j0 + kBlock <= row.whole_to();
   typename Row<T>::Vector raw[kGradVectors];
+  if (whole) {
+    const typename Row<T>::Vector* at = row.vector(j0 + threadIdx.x);
 #pragma unroll
-  for (int a = 0; a < kGradVectors; ++a)
-    if (j0 + a * kThreads < vectors) raw[a] = row.load(j0 + a * kThreads);
+    for (int a = 0; a < kGradVectors; ++a)
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(raw[a].v)[i] = __ldcs(reinterpret_cast<const uint4*>(at + a * kThreads) + i);
+  }
   const long long token = p.tokens[r];
   const bool counts = token != p.ignore && token >= 0 && token < p.vocab;
-  const float base = p.stats[2 * r], log_s = p.stats[2 * r + 1];
+  const float base = p.stats[2ll * r], log_s = p.stats[2ll * r + 1];
   const float g = p.g != nullptr && counts ? p.g[r] : 0.f, h = p.h != nullptr ? p.h[r] : 0.f;
   float all = g;
   if (p.k != nullptr)
-    for (int i = 0; i < p.top; ++i) all += p.k[r * p.top + i];
+    for (int i = 0; i < p.top; ++i) all += p.k[static_cast<long long>(r) * p.top + i];
   // -p (all + h (H + ln2 q)) / T with q = log2 p
   const float offset = -(all + (h != 0.f ? h * p.entropy[r] : 0.f)) * p.rate, slope = -h * kLn2 * p.rate;
-  auto value = [&](float x) {
-    const float q = fmaxf(fmaf(x - base, p.c, -log_s), kLowest);
-    return fast_exp2(q) * fmaf(slope, q, offset);
+  const uint64_t base2 = pack_f32x2(-base, -base), c2 = pack_f32x2(p.c, p.c), log2s = pack_f32x2(-log_s, -log_s), offset2 = pack_f32x2(offset, offset), slope2 = pack_f32x2(slope, slope);
+  auto two = [&](float x0, float x1, float& d0, float& d1) {
+    float q0, q1;
+    unpack_f32x2(fma_f32x2(add_f32x2(pack_f32x2(x0, x1), base2), c2, log2s), q0, q1);
+    q0 = fmaxf(q0, kLowest), q1 = fmaxf(q1, kLowest);
+    unpack_f32x2(mul_f32x2(pack_f32x2(fast_exp2(q0), fast_exp2(q1)), fma_f32x2(slope2, pack_f32x2(q0, q1), offset2)), d0, d1);
   };
-#pragma unroll
-  for (int a = 0; a < kGradVectors; ++a) {
-    const int j = j0 + a * kThreads;
-    if (j >= vectors) break;
+  auto eight = [&](const typename Row<T>::Vector& x) {
     typename Row<T>::Vector d;
+    float f[8];
+    widen8(x, f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) d.v[i] = narrowed<T>(value(widened(raw[a].v[i])));
-    const long long e = j * 8ll - row.off;
-    if (same && row.whole(j)) {
+    for (int i = 0; i < 8; i += 2) {
+      float d0, d1;
+      two(f[i], f[i + 1], d0, d1);
+      d.v[i] = narrowed<T>(d0), d.v[i + 1] = narrowed<T>(d1);
+    }
+    return d;
+  };
+  if (whole) {
+    typename Row<T>::Vector* to = reinterpret_cast<typename Row<T>::Vector*>(out - row.off) + j0 + threadIdx.x;
 #pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) __stcs(reinterpret_cast<uint4*>(out + e) + i, reinterpret_cast<const uint4*>(d.v)[i]);
-    } else {
+    for (int a = 0; a < kGradVectors; ++a) {
+      const typename Row<T>::Vector d = eight(raw[a]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (e + i >= 0 && e + i < p.vocab) out[e + i] = d.v[i];
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) __stcs(reinterpret_cast<uint4*>(to + a * kThreads) + i, reinterpret_cast<const uint4*>(d.v)[i]);
+    }
+  } else {
+#pragma unroll 1
+    for (int a = 0; a < kGradVectors; ++a) {
+      const int j = j0 + a * kThreads + threadIdx.x;
+      if (j >= vectors) break;
+      const typename Row<T>::Vector d = eight(row.load(j));
+      const long long e = j * 8ll - row.off;
+      if (same && j >= row.whole_from() && j < row.whole_to()) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) __stcs(reinterpret_cast<uint4*>(out + e) + i, reinterpret_cast<const uint4*>(d.v)[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (e + i >= 0 && e + i < p.vocab) out[e + i] = d.v[i];
+      }
     }
   }
   // the token and the alternatives again, with what is theirs; of two equal ones both write the same
-  __syncthreads();
   const int targets = (p.k != nullptr ? p.top : 0) + 1;
+  __syncthreads();
   if (static_cast<int>(threadIdx.x) < targets) {
-    const long long mine = threadIdx.x == 0 ? (counts ? token : -1) : p.top_tokens[r * p.top + threadIdx.x - 1];
-    if (mine >= 0 && (mine + row.off) / 8 / (kThreads * kGradVectors) == part) {
-      float extra = counts && token == mine ? g : 0.f;
-      for (int i = 0; i + 1 < targets; ++i) extra += p.top_tokens[r * p.top + i] == mine ? p.k[r * p.top + i] : 0.f;
-      out[mine] = narrowed<T>(fmaf(extra, p.rate, value(widened(row.x[mine]))));
+    const long long* best = p.top_tokens + static_cast<long long>(r) * p.top;
+    const float* of_best = p.k + static_cast<long long>(r) * p.top;
+    const long long mine = threadIdx.x == 0 ? (counts ? token : -1) : best[threadIdx.x - 1];
+    if (mine >= 0 && (mine + row.off) / 8 / kBlock == part) {
+      float extra = counts && token == mine ? g : 0.f, d, unused;
+      for (int i = 0; i + 1 < targets; ++i) extra += best[i] == mine ? of_best[i] : 0.f;
+      two(widened(row.x[mine]), 0.f, d, unused);
+      out[mine] = narrowed<T>(fmaf(extra, p.rate, d));
     }
   }
 }
@@ -462,7 +524,7 @@ static int launch_grad(const Call& c, float log2_rate, float rate, cudaStream_t 
   p.g = reinterpret_cast<const float*>(c.g), p.h = reinterpret_cast<const float*>(c.h), p.k = reinterpret_cast<const float*>(c.k), p.dx = reinterpret_cast<void*>(c.dx);
   p.ignore = c.ignore, p.inner = static_cast<int>(c.inner), p.vocab = static_cast<int>(c.vocab), p.top = static_cast<int>(c.top), p.c = log2_rate, p.rate = rate;
   const long long vectors = (c.vocab + 7 + 7) / 8;
-  p.parts = (vectors + kThreads * kGradVectors - 1) / (kThreads * kGradVectors);
+  p.parts = static_cast<int>((vectors + kThreads * kGradVectors - 1) / (kThreads * kGradVectors));
   if (c.rows * p.parts > 0x7fffffffll) return kErrTooLarge;
   TTB_COUNT_LAUNCH(1);
   grad_kernel<T><<<static_cast<unsigned>(c.rows * p.parts), kThreads, 0, st>>>(p);

@@ -48,9 +48,10 @@ def check_arguments(q: torch.Tensor, k: torch.Tensor, gains: Tuple[Optional[torc
             raise ValueError(f"a gain {tuple(gain.shape)} of {gain.dtype} on {gain.device} is not [{a[3]}] on {q.device}")
 
 
-def suits(q: torch.Tensor, cache: torch.Tensor) -> bool:
+def suits(q: torch.Tensor, k: torch.Tensor, cache: torch.Tensor) -> bool:
     """Whether the kernels have this type and size."""
-    return q.dtype in _TYPES and q.shape[3] % 16 == 0 and q.shape[3] <= 512 and cache.dtype == torch.float32 and q.shape[0] * q.shape[1] < 2**31
+    b, s, h, d = q.shape
+    return q.dtype in _TYPES and d % 16 == 0 and d <= 512 and cache.dtype == torch.float32 and b * s * (h + 2 * k.shape[2]) < 2**31
 
 
 def _steady(t: torch.Tensor) -> torch.Tensor:
