@@ -195,9 +195,9 @@ def _declare(L: ctypes.CDLL) -> None:
     L.ttb_token_stats_bwd.restype = i32
     L.ttb_shared_prefix_attention.argtypes = [c.c_char_p, f32, vp, vp]
     L.ttb_shared_prefix_attention.restype = i32
-    L.ttb_shared_prefix_floats.argtypes = [c.c_char_p]
+    L.ttb_shared_prefix_floats.argtypes = [c.c_char_p, vp]
     L.ttb_shared_prefix_floats.restype = i64
-    L.ttb_qk_norm_rope_rows.argtypes = [c.c_char_p]
+    L.ttb_qk_norm_rope_rows.argtypes = []
     L.ttb_qk_norm_rope_rows.restype = i64
     for fn in (L.ttb_span_decode_tile, L.ttb_span_prepare, L.ttb_span_prefill, L.ttb_span_decode, L.ttb_stream_step, L.ttb_embed_positions, L.ttb_clamped_glu, L.ttb_lightning_recurrent,
                L.ttb_lightning_chunks, L.ttb_silu_rows, L.ttb_gated_norm):
@@ -226,6 +226,16 @@ def stream_ptr() -> int:
     device = torch.cuda.current_device()  # also initialises CUDA in the first call of a program
     lib().ttb_ensure_device(device)
     return torch._C._cuda_getCurrentRawStream(device)  # without the Python object around it, which takes longer to make than a launch does
+
+
+def launch(t: torch.Tensor, call, *args) -> int:
+    """Calls a kernel's entry with ``t``'s device as the current one and that device's current stream as its last argument."""
+    device = t.get_device()
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return launch(t, call, *args)
+    _lib.ttb_ensure_device(device)  # ``call`` is one of the library's, which therefore is loaded
+    return call(*args, torch._C._cuda_getCurrentRawStream(device))
 
 
 def err_word(device: torch.device) -> torch.Tensor:

@@ -414,17 +414,8 @@ extern "C" int ttb_qk_norm_rope(const char* call, float eps, void* stream) {
   });
 }
 
-// Rows of d floats that the backward pass needs as a workspace where a gain has a gradient.
-extern "C" long long ttb_qk_norm_rope_rows(const char* call) {
-  using namespace ttb::qkn;
-  const Call& c = *reinterpret_cast<const Call*>(call);
-  int q = 0, k = 0;
-  by_size(static_cast<int>(c.d), [&](auto, auto g) {
-    ctas_of(c, kThreads / decltype(g)::value, kBackHeads, q, k);
-    return 0;
-  });
-  return q + k;
-}
+// Rows of d floats that suffice as a workspace of the backward pass where a gain has a gradient: one for each CTA.
+extern "C" long long ttb_qk_norm_rope_rows() { return 4ll * ttb::sm_count(); }
 
 extern "C" int ttb_qk_norm_rope_bwd(const char* call, float eps, void* stream) {
   using namespace ttb;

@@ -434,8 +434,9 @@ struct Call {
   long long prompts, rows, s, hq, hkv, d, prefix, own;
 };
 
-// How long pieces are.  CTAs (two to an SM) take pieces in turn, those of the prefix first: the one with the most of both is done last.  A piece costs its tiles and an overhead of `kOverhead` tiles.
-static constexpr double kOverhead = 2.0;
+// How long pieces are.  CTAs (two to an SM) take pieces in turn, those of the prefix first: the one with the most of both is done last.  A piece costs its tiles and an overhead that grows with its
+// rows, whose queries and outputs move between the pieces: in tiles, 0.3 and one for each 64 rows.
+static double overhead_of(int rows) { return 0.3 + (rows < kRows ? rows : kRows) / 64.0; }
 static int plan_of(const Call& c, Params& p) {
   if (c.prompts <= 0 || c.rows <= 0 || c.rows % c.prompts || c.s <= 0 || c.hkv <= 0 || c.hq <= 0 || c.hq % c.hkv || (c.d != 64 && c.d != 128) || c.prefix < 0 || c.own < 0) return kErrBadShape;
   if (c.rows > 0x7fffffff || c.prefix > 0x3fffffff || c.own > 0x3fffffff || c.rows * c.s > 0x7fffffff / c.hq) return kErrTooLarge;
@@ -445,11 +446,12 @@ static int plan_of(const Call& c, Params& p) {
   p.tiles_p = (p.rows_p + kRows - 1) / kRows, p.tiles_o = (p.rows_o + kRows - 1) / kRows;
   const long long np = (c.prefix + kKeys - 1) / kKeys, no = (c.own + kKeys - 1) / kKeys;  // tiles of keys
   const long long heads_p = c.prompts * c.hkv * p.tiles_p, heads_o = c.rows * c.hkv * p.tiles_o, ctas = 2ll * sm_count();
+  const double over_p = overhead_of(p.rows_p), over_o = overhead_of(p.rows_o);
   double best = 0;
   long long run = 1;
   for (long long t = 2; t <= 4096; t += t < 32 ? 1 : t / 8) {
     const long long cuts_p = (np + t - 1) / t, cuts_o = (no + t - 1) / t;
-    const double each_p = cuts_p ? (np + cuts_p - 1) / cuts_p + kOverhead : 0, each_o = cuts_o ? (no + cuts_o - 1) / cuts_o + kOverhead : 0;
+    const double each_p = cuts_p ? (np + cuts_p - 1) / cuts_p + over_p : 0, each_o = cuts_o ? (no + cuts_o - 1) / cuts_o + over_o : 0;
     const long long pieces_p = heads_p * cuts_p, pieces = pieces_p + heads_o * cuts_o;
     auto of = [&](long long cta) {  // what a CTA has to do
       const long long first = pieces_p > cta ? (pieces_p - cta + ctas - 1) / ctas : 0, all = pieces > cta ? (pieces - cta + ctas - 1) / ctas : 0;
@@ -520,7 +522,7 @@ static int launch(const Call& c, Params& p, cudaStream_t st) {
 }  // namespace ttb
 
 // Floats of the workspace of a call (an sprefix::Call), or a negative error.
-extern "C" long long ttb_shared_prefix_floats(const char* call) {
+extern "C" long long ttb_shared_prefix_floats(const char* call, void*) {
   using namespace ttb::sprefix;
   const Call& c = *reinterpret_cast<const Call*>(call);
   Params p{};

@@ -5,10 +5,8 @@ import struct
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ._lib import check, lib
-from .quantized import _on
+from ._lib import check, launch, lib
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _pack = struct.Struct("=53q").pack  # the kernel source's Call
@@ -34,24 +32,24 @@ def positions(input_pos: Optional[torch.Tensor], b: int, s: int, table_len: int)
 
 
 def check_arguments(q: torch.Tensor, k: torch.Tensor, gains: Tuple[Optional[torch.Tensor], Optional[torch.Tensor]], cache: torch.Tensor) -> None:
-    a, c = q.shape, k.shape
+    a, c, t, device = q.shape, k.shape, cache.shape, q.device
     if len(a) != 4 or len(c) != 4 or a[:2] != c[:2] or a[3] != c[3] or a[3] % 2 or a[2] == 0 or c[2] == 0 or a[3] == 0:
         raise ValueError(f"queries {tuple(a)} and keys {tuple(c)} are not [rows, tokens, heads, channels] of the same rows, tokens and (even) channels")
-    if q.dtype != k.dtype or not q.dtype.is_floating_point:
+    if q.dtype is not k.dtype or not q.dtype.is_floating_point:
         raise ValueError(f"queries and keys have one floating-point type, not {q.dtype} and {k.dtype}")
-    if k.device != q.device or cache.device != q.device:
+    if k.device != device or cache.device != device:
         raise ValueError(f"queries on {q.device}, keys on {k.device} and angles on {cache.device} are not on one device")
-    if cache.dim() != 3 or cache.shape[0] == 0 or cache.shape[1] * 2 != a[3] or cache.shape[2] != 2 or not cache.dtype.is_floating_point:
-        raise ValueError(f"angles {tuple(cache.shape)} are not [positions, {a[3] // 2}, 2] (cosine and sine)")
+    if len(t) != 3 or t[0] == 0 or t[1] * 2 != a[3] or t[2] != 2 or not cache.dtype.is_floating_point:
+        raise ValueError(f"angles {tuple(t)} are not [positions, {a[3] // 2}, 2] (cosine and sine)")
     for gain in gains:
-        if gain is not None and (gain.shape != (a[3],) or gain.device != q.device or not gain.dtype.is_floating_point):
+        if gain is not None and (gain.shape != (a[3],) or gain.device != device or not gain.dtype.is_floating_point):
             raise ValueError(f"a gain {tuple(gain.shape)} of {gain.dtype} on {gain.device} is not [{a[3]}] on {q.device}")
 
 
 def suits(q: torch.Tensor, k: torch.Tensor, cache: torch.Tensor) -> bool:
     """Whether the kernels have this type and size."""
     b, s, h, d = q.shape
-    return q.dtype in _TYPES and d % 16 == 0 and d <= 512 and cache.dtype == torch.float32 and b * s * (h + 2 * k.shape[2]) < 2**31
+    return q.dtype in _TYPES and d % 16 == 0 and d <= 512 and cache.dtype is torch.float32 and b * s * (h + 2 * k.shape[2]) < 2**31
 
 
 def _steady(t: torch.Tensor) -> torch.Tensor:
@@ -72,37 +70,41 @@ def _at(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _gains(q: torch.Tensor, gain_q: Optional[torch.Tensor], gain_k: Optional[torch.Tensor]):
-    """Both in the type of the queries, or both in 32 bits."""
-    if all(g is None or g.dtype == q.dtype for g in (gain_q, gain_k)):
-        return gain_q, gain_k
-    return tuple(g if g is None else g.float() for g in (gain_q, gain_k))
-
-
 def _launch_pos(pos: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     if pos is None:
         return None
-    if pos.dtype != torch.int32:
+    if pos.dtype is not torch.int32:
         pos = pos.clamp(-1, 2**31 - 1).to(torch.int32)  # what does not fit stays out of range
     return pos.contiguous()
 
 
+def _gains(q: torch.Tensor, gain_q: Optional[torch.Tensor], gain_k: Optional[torch.Tensor]):
+    """Both in the type of the queries, or both in 32 bits."""
+    if (gain_q is None or gain_q.dtype is q.dtype) and (gain_k is None or gain_k.dtype is q.dtype):
+        return gain_q, gain_k
+    return tuple(g if g is None else g.float() for g in (gain_q, gain_k))
+
+
+def _is_wide(gain_q: Optional[torch.Tensor], gain_k: Optional[torch.Tensor]) -> bool:
+    gain = gain_q if gain_q is not None else gain_k
+    return gain is not None and gain.dtype is torch.float32
+
+
 def _forward(q, k, v, gain_q, gain_k, cache, pos, eps, interleaved, norm_first, out_k, out_v, slots):
     b, s, hq, d = q.shape
+    hk, held = k.shape[2], cache.shape[0]
     q, k, cache, gain_q, gain_k = _steady(q), _steady(k), _aligned(cache), _aligned(gain_q), _aligned(gain_k)
-    out_q = torch.empty((b, s, hq, d), dtype=q.dtype, device=q.device)
+    out_q = q.new_empty((b, s, hq, d))
     if v is None:
-        out_k = torch.empty((b, s, k.shape[2], d), dtype=k.dtype, device=k.device)
-        xv, yv, steps_v, to_v, heads_v, slot_count = 0, 0, _NONE, _NONE, 0, 0
+        out_k = k.new_empty((b, s, hk, d))
+        xv, yv, steps_v, to_k, to_v, heads_v, slot_count = 0, 0, _NONE, (s * hk * d, hk * d, d), _NONE, 0, 0
     else:
         v = _steady(v)
-        xv, yv, steps_v, to_v, heads_v, slot_count = v.data_ptr(), out_v.data_ptr(), v.stride()[:3], out_v.stride()[:3], v.shape[2], out_k.shape[1]
-    gain = gain_q if gain_q is not None else gain_k
-    wide = gain is not None and gain.dtype == torch.float32
+        xv, yv, steps_v, to_k, to_v, heads_v, slot_count = v.data_ptr(), out_v.data_ptr(), v.stride()[:3], out_k.stride()[:3], out_v.stride()[:3], hk, out_k.shape[1]
     call = _pack(q.data_ptr(), k.data_ptr(), xv, out_q.data_ptr(), out_k.data_ptr(), yv, 0, 0, _at(gain_q), _at(gain_k), *q.stride()[:3], *k.stride()[:3], *steps_v,
-                 *out_q.stride()[:3], *out_k.stride()[:3], *to_v, 0, 0, 0, 0, 0, 0, cache.data_ptr(), _at(pos), _at(slots), 0, 0, 0, 0, b, s, hq, k.shape[2], heads_v, d,
-                 cache.shape[0], slot_count, _TYPES[q.dtype], wide, interleaved, not norm_first)
-    check(_on(q, lib().ttb_qk_norm_rope, call, eps), "norm and rotation of queries and keys")
+                 s * hq * d, hq * d, d, *to_k, *to_v, 0, 0, 0, 0, 0, 0, cache.data_ptr(), _at(pos), _at(slots), 0, 0, 0, 0, b, s, hq, hk, heads_v, d,
+                 held, slot_count, _TYPES[q.dtype], _is_wide(gain_q, gain_k), interleaved, not norm_first)
+    check(launch(q, lib().ttb_qk_norm_rope, call, eps), "norm and rotation of queries and keys")
     return out_q, out_k
 
 
@@ -115,29 +117,27 @@ class _QKNormRope(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy_q, dy_k):
+        if torch.is_grad_enabled():
+            raise RuntimeError("the gradients of qk_norm_rope are not differentiable themselves")
         q, k, gain_q, gain_k, cache, pos = ctx.saved_tensors
         eps, interleaved, norm_first = ctx.how
+        need_q, need_k, need_gq, need_gk = ctx.needs_input_grad[:4]
         b, s, hq, d = q.shape
-        q, k, dy_q, dy_k, cache, at_q, at_k = _steady(q), _steady(k), _steady(dy_q), _steady(dy_k), _aligned(cache), _aligned(gain_q), _aligned(gain_k)
-        dq = torch.empty((b, s, hq, d), dtype=q.dtype, device=q.device)
-        dk = torch.empty((b, s, k.shape[2], d), dtype=k.dtype, device=k.device)
-        needs = ctx.needs_input_grad
-        d_gains = [torch.empty_like(g) if g is not None and need else None for g, need in ((at_q, needs[2]), (at_k, needs[3]))]
-        gain = gain_q if gain_q is not None else gain_k
-        wide = gain is not None and gain.dtype == torch.float32
-
-        def call(work: Optional[torch.Tensor]) -> bytes:
-            return _pack(q.data_ptr(), k.data_ptr(), 0, dq.data_ptr(), dk.data_ptr(), 0, dy_q.data_ptr(), dy_k.data_ptr(), _at(at_q), _at(at_k), *q.stride()[:3], *k.stride()[:3], *_NONE,
-                         *dq.stride()[:3], *dk.stride()[:3], *_NONE, *dy_q.stride()[:3], *dy_k.stride()[:3], cache.data_ptr(), _at(pos), 0, _at(work), 0 if work is None else work.shape[0],
-                         _at(d_gains[0]), _at(d_gains[1]), b, s, hq, k.shape[2], 0, d, cache.shape[0], 0, _TYPES[q.dtype], wide, interleaved, not norm_first)
-
-        work = None
-        if d_gains[0] is not None or d_gains[1] is not None:
-            work = torch.empty((lib().ttb_qk_norm_rope_rows(call(None)), d), dtype=torch.float32, device=q.device)
-        check(_on(q, lib().ttb_qk_norm_rope_bwd, call(work), eps), "gradients of the norm and rotation of queries and keys")
-        return dq if needs[0] else None, dk if needs[1] else None, d_gains[0], d_gains[1], None, None, None, None, None
+        hk, held = k.shape[2], cache.shape[0]
+        q, k, dy_q, dy_k, cache, gain_q, gain_k = _steady(q), _steady(k), _steady(dy_q), _steady(dy_k), _aligned(cache), _aligned(gain_q), _aligned(gain_k)
+        dq, dk = q.new_empty((b, s, hq, d)), k.new_empty((b, s, hk, d))
+        d_gq = torch.empty_like(gain_q) if need_gq and gain_q is not None else None
+        d_gk = torch.empty_like(gain_k) if need_gk and gain_k is not None else None
+        work, rows = None, 0
+        if d_gq is not None or d_gk is not None:
+            rows = lib().ttb_qk_norm_rope_rows()
+            work = q.new_empty((rows, d), dtype=torch.float32)
+        call = _pack(q.data_ptr(), k.data_ptr(), 0, dq.data_ptr(), dk.data_ptr(), 0, dy_q.data_ptr(), dy_k.data_ptr(), _at(gain_q), _at(gain_k), *q.stride()[:3], *k.stride()[:3], 0, 0, 0,
+                     s * hq * d, hq * d, d, s * hk * d, hk * d, d, 0, 0, 0, *dy_q.stride()[:3], *dy_k.stride()[:3], cache.data_ptr(), _at(pos), 0, _at(work), rows,
+                     _at(d_gq), _at(d_gk), b, s, hq, hk, 0, d, held, 0, _TYPES[q.dtype], _is_wide(gain_q, gain_k), interleaved, not norm_first)
+        check(launch(q, lib().ttb_qk_norm_rope_bwd, call, eps), "gradients of the norm and rotation of queries and keys")
+        return dq if need_q else None, dk if need_k else None, d_gq, d_gk, None, None, None, None, None
 
 
 def norm_rope(q, k, gain_q, gain_k, cache, pos, eps: float, interleaved: bool, norm_first: bool, differentiated: bool) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -7,11 +7,11 @@ from typing import Optional
 
 import torch
 
-from ._lib import check, err_word, lib
-from .quantized import _on
+from ._lib import check, err_word, launch, lib
 
 HEAD_DIMS = (64, 128)  # that the kernel has
 _pack = struct.Struct("=31q").pack  # the kernel source's Call
+_WITHOUT = (0,) * 23  # addresses and steps, where only sizes count
 
 
 def check_arguments(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, lengths) -> None:
@@ -32,6 +32,8 @@ def check_arguments(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, leng
 
 def _steady(t: torch.Tensor) -> torch.Tensor:
     """``t``, if copies of tiles of one head can read it where it is, or a copy."""
+    if t.is_contiguous():
+        return t if t.data_ptr() & 15 == 0 else t.clone()
     steps = t.stride()
     if steps[3] == 1 and t.data_ptr() & 15 == 0 and all(n == 1 or (step > 0 and step % 8 == 0) for n, step in zip(t.shape[:3], steps)):
         return t
@@ -40,7 +42,10 @@ def _steady(t: torch.Tensor) -> torch.Tensor:
 
 def _steps(t: torch.Tensor):
     """Steps of batch, slot and head; those of dimensions of size 1 are not used, but have to be in range."""
-    return [step if n > 1 else t.shape[3] for n, step in zip(t.shape[:3], t.stride())]
+    b, n, h, d = t.shape
+    if t.is_contiguous():
+        return n * h * d, h * d, d
+    return [step if n > 1 else d for n, step in zip((b, n, h), t.stride())]
 
 
 def attention(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, lengths, scale: Optional[float]) -> torch.Tensor:
@@ -49,18 +54,19 @@ def attention(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, lengths, s
     if q.data_ptr() & 15:
         q = q.clone()
     o = torch.empty_like(q)
-    kv = [_steady(t) for t in (k_prefix, v_prefix, k, v)]
-    index = [None if t is None else t.contiguous() for t in (prefix_start, prefix_stop, lengths)]
-    sizes = (*(x for t in kv for x in _steps(t)), k_prefix.shape[0], rows, s, hq, k.shape[2], d, k_prefix.shape[1], k.shape[1])
-
-    def call(work: int, floats: int) -> bytes:
-        return _pack(q.data_ptr(), o.data_ptr(), *(t.data_ptr() for t in kv), *(0 if t is None else t.data_ptr() for t in index), work, floats, *sizes)
-
-    with torch.cuda.device(q.device):
-        floats = lib().ttb_shared_prefix_floats(call(0, 0))
-        if floats < 0:
-            check(floats, "attention over a shared prefix")
-        work = torch.empty(floats, dtype=torch.float32, device=q.device)
-        check(_on(q, lib().ttb_shared_prefix_attention, call(work.data_ptr(), floats), 1.0 / math.sqrt(d) if scale is None else float(scale), err_word(q.device).data_ptr()),
-              "attention over a shared prefix")
+    k_prefix, v_prefix, k, v = _steady(k_prefix), _steady(v_prefix), _steady(k), _steady(v)
+    prefix_start, prefix_stop, lengths = (t if t is None or t.is_contiguous() else t.contiguous() for t in (prefix_start, prefix_stop, lengths))
+    library = lib()
+    sizes = (k_prefix.shape[0], rows, s, hq, k.shape[2], d, k_prefix.shape[1], k.shape[1])
+    floats = launch(q, library.ttb_shared_prefix_floats, _pack(*_WITHOUT, *sizes))
+    if floats < 0:
+        check(floats, "attention over a shared prefix")
+    work = q.new_empty((floats,), dtype=torch.float32)
+    call = _pack(q.data_ptr(), o.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k.data_ptr(), v.data_ptr(), _at(prefix_start), _at(prefix_stop), _at(lengths), work.data_ptr(), floats,
+                 *_steps(k_prefix), *_steps(v_prefix), *_steps(k), *_steps(v), *sizes)
+    check(launch(q, library.ttb_shared_prefix_attention, call, 1.0 / math.sqrt(d) if scale is None else float(scale), err_word(q.device).data_ptr()), "attention over a shared prefix")
     return o
+
+
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()

@@ -6,10 +6,8 @@ import struct
 from typing import NamedTuple, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ._lib import check, lib
-from .quantized import _on
+from ._lib import check, launch, lib
 
 MAX_TOP = 64
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -50,21 +48,21 @@ def _rows(logits: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
     return flat, 0, flat.stride(0), flat.shape[0]
 
 
-def _call(x, steps, rows, v, top, ignore, tokens, logprobs, entropy, stats, top_logprobs, top_tokens, g=None, h=None, k=None, dx=None) -> bytes:
-    at = [0 if t is None else t.data_ptr() for t in (tokens, logprobs, entropy, stats, top_logprobs, top_tokens, g, h, k, dx)]
-    return _pack(x.data_ptr(), *steps, rows, v, _TYPES[x.dtype], top, ignore, *at)
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def forward(logits, tokens, temperature: float, top: int, ignore: int, keep: bool):
     x, *steps = _rows(logits)
-    v, rows, dev = logits.shape[-1], tokens.numel(), logits.device
+    v, rows, shape = logits.shape[-1], tokens.numel(), tokens.shape
     tokens = tokens.contiguous()
-    logprobs, entropy = (torch.empty(tokens.shape, dtype=torch.float32, device=dev) for _ in range(2))
-    top_logprobs = torch.empty(tokens.shape + (top,), dtype=torch.float32, device=dev) if top else None
-    top_tokens = torch.empty(tokens.shape + (top,), dtype=torch.int64, device=dev) if top else None
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if keep else None
-    call = _call(x, steps, rows, v, top, ignore, tokens, logprobs, entropy, stats, top_logprobs, top_tokens)
-    check(_on(x, lib().ttb_token_stats, call, _LOG2E / temperature, 1.0 / temperature), "statistics of tokens")
+    logprobs = logits.new_empty(shape, dtype=torch.float32)
+    entropy = torch.empty_like(logprobs)
+    top_logprobs = logits.new_empty((*shape, top), dtype=torch.float32) if top else None
+    top_tokens = tokens.new_empty((*shape, top)) if top else None
+    stats = logprobs.new_empty((rows, 2)) if keep else None
+    call = _pack(x.data_ptr(), *steps, rows, v, _TYPES[x.dtype], top, ignore, tokens.data_ptr(), logprobs.data_ptr(), entropy.data_ptr(), _at(stats), _at(top_logprobs), _at(top_tokens), 0, 0, 0, 0)
+    check(launch(x, lib().ttb_token_stats, call, _LOG2E / temperature, 1.0 / temperature), "statistics of tokens")
     return TokenStatistics(logprobs, entropy, top_logprobs, top_tokens), tokens, stats
 
 
@@ -80,17 +78,19 @@ class _TokenStatistics(torch.autograd.Function):
         return tuple(out)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g, h, k, _):
+        if torch.is_grad_enabled():
+            raise RuntimeError("the gradients of token_statistics are not differentiable themselves")
         logits, tokens, stats, entropy, top_tokens = ctx.saved_tensors
         temperature, top, ignore = ctx.how
         if g is None and h is None and k is None:
             return None, None, None, None, None
-        g, h, k = (t if t is None else t.contiguous() for t in (g, h, k))
+        g, h, k = (t if t is None or t.is_contiguous() else t.contiguous() for t in (g, h, k))
         x, *steps = _rows(logits)
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        call = _call(x, steps, tokens.numel(), logits.shape[-1], top, ignore, tokens, None, entropy, stats, None, top_tokens, g, h, k, dx)
-        check(_on(x, lib().ttb_token_stats_bwd, call, _LOG2E / temperature, 1.0 / temperature), "gradient of statistics of tokens")
+        dx = logits.new_empty(logits.shape)
+        call = _pack(x.data_ptr(), *steps, tokens.numel(), logits.shape[-1], _TYPES[x.dtype], top, ignore, tokens.data_ptr(), 0, entropy.data_ptr(), stats.data_ptr(), 0, _at(top_tokens),
+                     _at(g), _at(h), _at(k), dx.data_ptr())
+        check(launch(x, lib().ttb_token_stats_bwd, call, _LOG2E / temperature, 1.0 / temperature), "gradient of statistics of tokens")
         return dx, None, None, None, None
 
 
