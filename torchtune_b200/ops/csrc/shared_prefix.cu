@@ -7,9 +7,10 @@
 // same work: scores of 128 rows and 64 keys on tcgen05 tensor cores, a thread per row for the softmax, probabilities in the scores' place in tensor memory as the A operand of the second
 // product, its accumulator next to them.  A tile of 64 keys and values is 32 KB: an SM's share of the memory's rate brings it in 1400 cycles, and 128 rows keep the tensor cores busy for 260 of them and the
 // exponentials' unit for 512, so that padding a single token's four rows to 128 costs nothing that is not idle; warps without rows have no part in the softmax.
-// Two CTAs to an SM take pieces in turn, a fixed share each.  A ring of slots that K and V fill in turn runs on over the end of a piece, so that the keys of the next one arrive while the output of the
-// last is written; the scores of a tile are computed while the softmax of the one before is.  Pieces are as long as a model of their number and overhead says (plan_of), and lie in a
-// workspace that a second launch joins in a fixed order.
+// Two CTAs to an SM share the tiles of all key heads out evenly, as they are: tiles of the prefixes in their order are one line, those of the rows another, CTAs get a stretch of one of them each
+// (with more than 128 query rows to a head, as many CTAs next to each other as there are tiles of rows, so that all but one find the keys in L2), and a piece ends where a head or a
+// stretch does.  Lengths are read on the device, so a recorded launch follows them.  A ring of slots that K and V fill in turn runs on over the end of a piece, so that the keys of the next one
+// arrive while the output of the last is written; the scores of a tile are computed while the softmax of the one before is.  Pieces lie in a workspace that a second launch joins in a fixed order.
 //
 // What lies behind the last visible key may be anything: scores are masked by selection, and the values of a piece's last tile that nobody sees are overwritten with zeros before they are
 // multiplied.  Every wait is bounded and reports through the error word.
@@ -32,17 +33,88 @@ struct Params {
   __nv_bfloat16* o;
   const int *start, *stop;  // [prompts] or nullptr: 0, prefix
   const int* lengths;       // [rows] or nullptr: own
+  int* shared_out;          // what the CTAs have agreed on: groups of the prefix and of rows, tiles in front of every prompt and of all, of every row and of all
   float* part;              // pieces' outputs: rows of D floats
   float2* ml;               // their maxima (log2) and sums
   int prompts, rows, s, hq, hkv, group;
   int prefix, own;          // slots
   int rows_p, rows_o;       // query rows of a prompt and of a row, per key head
-  int tiles_p, tiles_o;     // of 128 of them
-  int run_p, run_o;         // keys of a piece
-  int cuts_p, cuts_o;       // pieces of a key head's keys
-  int pieces_p, pieces;     // of all prompts; with those of rows, which follow
+  int pieces_p;             // most pieces of the prefix: those of rows lie behind them
+  uint32_t per_group;       // 2^32 / group, rounded up: the high word of a row times that is row / group, for rows below 2^32 / group
   float scale;
   int* err;
+};
+static constexpr int kSide = 8;  // CTAs next to each other for the tiles of rows of a head; more tiles than that are a CTA's one after the other
+__host__ __device__ __forceinline__ int tiles_of(int rows) { return (rows + kRows - 1) / kRows; }
+__host__ __device__ __forceinline__ int side_of(int rows) { return tiles_of(rows) < kSide ? tiles_of(rows) : kSide; }
+
+// Token of a query row.
+__device__ __forceinline__ int token_of(const Params& p, int row) { return p.group == 1 ? row : static_cast<int>(__umulhi(row, p.per_group)); }
+
+// Visible slots [lo, hi) of a prompt or a row.
+__device__ __forceinline__ void slots_of(const Params& p, bool prefix, int owner, int& lo, int& hi) {
+  if (prefix) {
+    lo = p.start != nullptr ? max(p.start[owner], 0) : 0;
+    hi = p.stop != nullptr ? min(p.stop[owner], p.prefix) : p.prefix;
+  } else {
+    lo = 0;
+    hi = p.lengths != nullptr ? min(p.lengths[owner], p.own) : p.own;
+  }
+}
+__device__ __forceinline__ int key_tiles(const Params& p, bool prefix, int owner) {
+  int lo, hi;
+  slots_of(p, prefix, owner, lo, hi);
+  return lo < hi ? (hi - lo + kKeys - 1) / kKeys : 0;
+}
+
+// n tiles over g groups: group i has [i n / g, (i + 1) n / g).  Quotients of whole numbers below 2^40 by such below 2^31: those that are no whole number are further from one than a double's
+// rounding, and the others are exact; a division of doubles is a tenth of one of 64-bit integers.
+__device__ __forceinline__ long long border(long long n, int g, int i) { return static_cast<long long>(static_cast<double>(n * i) / g); }
+__device__ __forceinline__ int group_of(long long n, int g, long long tile) { return static_cast<int>(static_cast<double>((tile + 1) * g - 1) / static_cast<double>(n)); }
+
+// A CTA's part: a stretch of the tiles of the prefixes or of the rows.
+struct Share {
+  bool prefix;
+  int group, side, sides, owner, head, tile;  // where it begins
+  int count;                                  // tiles of keys
+};
+// The pieces of a share, for each of its tiles of query rows.
+struct Walk {
+  int owner, head, tile, left;  // left: of the stretch
+  int row_tile;
+  int lo, hi, n;                // of the owner
+  __device__ __forceinline__ Walk(const Params& p, const Share& s) : row_tile(s.side) { restart(p, s); }
+  __device__ __forceinline__ void restart(const Params& p, const Share& s) {
+    owner = s.owner, head = s.head, tile = s.tile, left = s.count;
+    if (left > 0) enter(p, s.prefix);
+  }
+  __device__ __forceinline__ void enter(const Params& p, bool prefix) {
+    slots_of(p, prefix, owner, lo, hi);
+    n = lo < hi ? (hi - lo + kKeys - 1) / kKeys : 0;
+  }
+  __device__ __forceinline__ int count() const { return min(n - tile, left); }  // tiles of the piece
+  __device__ __forceinline__ int first() const { return lo + tile * kKeys; }
+  __device__ __forceinline__ int last() const { return min(hi, lo + (tile + count()) * kKeys); }
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  __device__ __forceinline__ void next(const Params& p, const Share& s) {
+    left -= count();
+    tile = 0;
+    if (left > 0) {
+      if (++head == p.hkv) {
+        head = 0;
+        n = 0;
+        while (n == 0 && ++owner < (s.prefix ? p.prompts : p.rows)) enter(p, s.prefix);
+        if (n == 0) left = 0;  // not unless the lengths have changed meanwhile
+      }
+    } else if ((row_tile += s.sides) < tiles_of(s.prefix ? p.rows_p : p.rows_o)) {
+      restart(p, s);
+    }
+  }
+  // first row of the piece in the workspace
+  __device__ __forceinline__ long long base(const Params& p, const Share& s) const {
+    const long long piece = static_cast<long long>(owner) * p.hkv + head + s.group;  // pieces are one for every head and one for every border within a head
+    return (s.prefix ? piece * p.rows_p : static_cast<long long>(p.pieces_p) * p.rows_p + piece * p.rows_o) + row_tile * kRows;
+  }
 };
 
 template <int D>
@@ -52,42 +124,63 @@ struct Layout {
   static constexpr int kSlot = kPanels * kPanel;
   static constexpr int kSlots = D == 128 ? 4 : 8;
   static constexpr int kBars = kQuery + kSlots * kSlot;
-  static constexpr int kBytes = kBars + (2 * kSlots + 6) * 8 + 16 + 1024;
+  static constexpr int kBytes = kBars + (2 * kSlots + 7) * 8 + 16 + 1024;
   static constexpr int kColumns = 256;  // of tensor memory: outputs, then two tiles of scores
   static_assert(4 * 32 * 32 * 4 <= kQuery, "four warps' 32 x 32 outputs take the queries' place");
 };
 
-// The keys of a piece: [first, last) of the prompt's or row's slots.
-__device__ __forceinline__ void range_of(const Params& p, bool prefix, int owner, int cut, int& first, int& last) {
-  int lo = 0, hi;
-  if (prefix) {
-    lo = p.start != nullptr ? p.start[owner] : 0;
-    hi = p.stop != nullptr ? p.stop[owner] : p.prefix;
-    lo = max(lo, 0), hi = min(hi, p.prefix);
-  } else {
-    hi = p.lengths != nullptr ? p.lengths[owner] : p.own;
-    hi = min(hi, p.own);
+// Every CTA adds up the tiles of all prompts and rows, a run of them to a thread, and finds its share; the first one leaves the sums for the joining launch.
+__device__ __forceinline__ void find_share(const Params& p, Share& share, int (*sums)[2]) {
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int run_p = (p.prompts + kThreads - 1) / kThreads, run_o = (p.rows + kThreads - 1) / kThreads;
+  int mine[2] = {0, 0};
+  for (int i = t * run_p; i < min(p.prompts, (t + 1) * run_p); ++i) mine[0] += key_tiles(p, true, i);
+  for (int i = t * run_o; i < min(p.rows, (t + 1) * run_o); ++i) mine[1] += key_tiles(p, false, i);
+  int upto[2] = {mine[0], mine[1]};
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int up = __shfl_up_sync(0xffffffffu, upto[k], x);
+      if (lane >= x) upto[k] += up;
+    }
   }
-  const int run = prefix ? p.run_p : p.run_o;
-  first = max(lo, cut * run);
-  last = min(static_cast<long long>(hi), (cut + 1ll) * run);
+  if (lane == 31) sums[warp][0] = upto[0], sums[warp][1] = upto[1];
+  __syncthreads();
+  int before[2] = {upto[0] - mine[0], upto[1] - mine[1]}, all[2] = {0, 0};
+  for (int w = 0; w < kThreads / 32; ++w)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) before[k] += w < warp ? sums[w][k] : 0, all[k] += sums[w][k];
+  // CTAs in proportion to the tiles, at most one to a tile of few rows or to three of 128
+  const int ctas = gridDim.x, side_p = side_of(p.rows_p), side_o = side_of(p.rows_o);
+  const long long n_p = static_cast<long long>(all[0]) * p.hkv, n_o = static_cast<long long>(all[1]) * p.hkv;
+  const long long work_p = n_p * tiles_of(p.rows_p), work_o = n_o * tiles_of(p.rows_o);
+  int ctas_p = n_p == 0 ? 0 : n_o == 0 ? ctas : static_cast<int>(static_cast<float>(work_p) / static_cast<float>(work_p + work_o) * ctas / side_p + 0.5f) * side_p;
+  if (n_p > 0 && n_o > 0) ctas_p = max(side_p, min(ctas_p, (ctas - side_o) / side_p * side_p));
+  auto groups_of = [](long long n, int room, int rows) { return n == 0 ? 0 : static_cast<int>(max(1ll, min(static_cast<long long>(room), n / (1 + min(rows, kRows) / 64)))); };
+  const int groups[2] = {groups_of(n_p, ctas_p / side_p, p.rows_p), groups_of(n_o, (ctas - ctas_p) / side_o, p.rows_o)};
+  const int cta = blockIdx.x, which = cta >= ctas_p, side = which ? side_o : side_p, at = which ? cta - ctas_p : cta;
+  share.prefix = !which, share.group = at / side, share.side = at % side, share.sides = side, share.count = 0;
+  __shared__ int found[3];
+  if (share.group < groups[which]) {
+    const long long n = which ? n_o : n_p, from = border(n, groups[which], share.group);
+    share.count = static_cast<int>(border(n, groups[which], share.group + 1) - from);
+    if (from >= static_cast<long long>(before[which]) * p.hkv && from < static_cast<long long>(before[which] + mine[which]) * p.hkv) {  // in this thread's run
+      long long at_owner = static_cast<long long>(before[which]) * p.hkv;
+      int owner = t * (which ? run_o : run_p), tiles = key_tiles(p, share.prefix, owner);
+      while (from >= at_owner + static_cast<long long>(tiles) * p.hkv) at_owner += static_cast<long long>(tiles) * p.hkv, tiles = key_tiles(p, share.prefix, ++owner);
+      const int in = static_cast<int>(from - at_owner);  // below 2^24 tiles times 256 heads, at most 2^31 - 1 by the check of sizes
+      found[0] = owner, found[1] = in / tiles, found[2] = in % tiles;
+    }
+  }
+  if (cta == 0) {
+    if (t == 0) p.shared_out[0] = groups[0], p.shared_out[1] = groups[1], p.shared_out[2 + p.prompts] = all[0], p.shared_out[3 + p.prompts + p.rows] = all[1];
+    for (int i = t * run_p; i < min(p.prompts, (t + 1) * run_p); ++i) p.shared_out[2 + i] = before[0], before[0] += key_tiles(p, true, i);
+    for (int i = t * run_o; i < min(p.rows, (t + 1) * run_o); ++i) p.shared_out[3 + p.prompts + i] = before[1], before[1] += key_tiles(p, false, i);
+  }
+  __syncthreads();
+  share.owner = found[0], share.head = found[1], share.tile = found[2];
 }
-
-// Which piece: tiles of query rows are neighbours, so that the second of them finds the keys in L2.
-struct Piece {
-  bool prefix;
-  int tile, head, cut, owner, first, last;
-  __device__ __forceinline__ Piece(const Params& p, int at) {
-    prefix = at < p.pieces_p;
-    at -= prefix ? 0 : p.pieces_p;
-    const int tiles = prefix ? p.tiles_p : p.tiles_o, cuts = prefix ? p.cuts_p : p.cuts_o;
-    tile = at % tiles, at /= tiles;
-    head = at % p.hkv, at /= p.hkv;
-    cut = at % cuts, owner = at / cuts;
-    range_of(p, prefix, owner, cut, first, last);
-  }
-  __device__ __forceinline__ int key_tiles() const { return first < last ? (last - first + kKeys - 1) / kKeys : 0; }  // 0: nothing to see; whoever joins the pieces knows that too
-};
 
 // A barrier of the four warps of the softmax; whether any of them says yes.
 __device__ __forceinline__ bool any_of_four(bool mine) {
@@ -117,17 +210,17 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
   uint64_t* q_full = empty + L::kSlots;
   uint64_t* s_full = q_full + 1;   // [2] scores of a tile are there
   uint64_t* p_full = q_full + 3;   // [2] its probabilities are
-  uint64_t* pv_done = q_full + 5;  // its second product is
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 6);
+  uint64_t* pv_done = q_full + 5;  // [2] its second product is done: one for odd and one for even tiles, since who waits knows only that the tile before the last is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 7);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;");  // the joining launch may take its place; it waits for the end of this one
+  if (threadIdx.x == 128) prefetch_tmap(&tm_kp), prefetch_tmap(&tm_vp), prefetch_tmap(&tm_ko), prefetch_tmap(&tm_vo);
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kSlots; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     mbar_init(q_full, 4);
-    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
-    mbar_init(pv_done, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&pv_done[i], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -136,27 +229,28 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  __shared__ int sums[kThreads / 32][2];
+  Share share;
+  find_share(p, share, sums);  // with two barriers
   tc_fence_after();
   const uint32_t tO = *tmem_slot, tS = tO + D;
 
   if (warp == 4) {
     // ---------------------------------------------------------------- loads: K and V of a tile in turn
-    if (lane == 0) prefetch_tmap(&tm_kp), prefetch_tmap(&tm_vp), prefetch_tmap(&tm_ko), prefetch_tmap(&tm_vo);
     int slot = 0, n = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int at = blockIdx.x; at < p.pieces && ok; at += gridDim.x) {
-      const Piece c(p, at);
-      const CUtensorMap *map_k = c.prefix ? &tm_kp : &tm_ko, *map_v = c.prefix ? &tm_vp : &tm_vo;
-      for (int x = 0; x < 2 * c.key_tiles() && !*abort_flag; ++x, ++n) {
+    const CUtensorMap *map_k = share.prefix ? &tm_kp : &tm_ko, *map_v = share.prefix ? &tm_vp : &tm_vo;
+    for (Walk w(p, share); w.more() && ok && !*abort_flag; w.next(p, share)) {
+      const int first = w.first(), loads = 2 * w.count();
+      for (int x = 0; x < loads && !*abort_flag; ++x, ++n) {
         if (!(ok = mbar_wait(&empty[slot], phase ^ 1))) {
           fail(abort_flag, p.err, 301);
           break;
         }
         if (lane == 0) {
           mbar_arrive_expect_tx(&full[slot], L::kSlot);
-          for (int y = 0; y < L::kPanels; ++y) tma_load_4d(ring + slot * L::kSlot + y * kPanel, x & 1 ? map_v : map_k, &full[slot], y * 64, c.head, c.first + (x >> 1) * kKeys, c.owner);
+          for (int y = 0; y < L::kPanels; ++y) tma_load_4d(ring + slot * L::kSlot + y * kPanel, x & 1 ? map_v : map_k, &full[slot], y * 64, w.head, first + (x >> 1) * kKeys, w.owner);
         }
         __syncwarp();
         if (++slot == L::kSlots) slot = 0, phase ^= 1;
@@ -186,9 +280,8 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
       __syncwarp();
       return true;
     };
-    for (int at = blockIdx.x; at < p.pieces && ok && !*abort_flag; at += gridDim.x) {
-      const int n = Piece(p, at).key_tiles();
-      if (n == 0) continue;
+    for (Walk w(p, share); w.more() && ok && !*abort_flag; w.next(p, share)) {
+      const int n = w.count();
       ok = mbar_wait(q_full, pieces++ & 1) && issue_s(done);
       for (int j = 0; j < n && ok && !*abort_flag; ++j, ++done) {
         if (j + 1 < n && !(ok = issue_s(done + 1))) break;  // while the softmax of this tile runs
@@ -201,7 +294,7 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k) umma_f16_ts(tO, from + k * 8, make_smem_desc_sw128(v_base + k * 2048, kPanel, 1024), idesc_o, (j | k) != 0);
           umma_commit(&empty[slot]);
-          umma_commit(pv_done);
+          umma_commit(&pv_done[done & 1]);
         }
         __syncwarp();
       }
@@ -216,26 +309,39 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
     const uint64_t c2 = pack_f32x2(cc, cc);
     bool ok = true, stop = false;
     uint32_t done = 0;  // tiles so far
-    for (int at = blockIdx.x; at < p.pieces && !stop; at += gridDim.x) {
-      const Piece piece(p, at);
-      const int n_tiles = piece.key_tiles(), first = piece.first, last = piece.last;
-      if (n_tiles == 0) continue;
-      const int rows = piece.prefix ? p.rows_p : p.rows_o, row0 = piece.tile * kRows, live = min(kRows, rows - row0), live_warps = (live + 31) / 32;
-      const long long token0 = static_cast<long long>(piece.owner) * (piece.prefix ? p.rows / p.prompts * p.s : p.s);
-      for (int x = threadIdx.x; x < live * (D / 8); x += 128) {
-        const int r = x / (D / 8), ch = x % (D / 8), row = row0 + r, token = row / p.group;
-        const uint4 v = *reinterpret_cast<const uint4*>(p.q + ((token0 + token) * p.hq + piece.head * p.group + row - token * p.group) * D + ch * 8);
-        *reinterpret_cast<uint4*>(sQ + (ch >> 3) * kPanelBytes + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+    for (Walk w(p, share); w.more() && !stop; w.next(p, share)) {
+      const int n_tiles = w.count(), first = w.first(), last = w.last();
+      const int rows = share.prefix ? p.rows_p : p.rows_o, row0 = w.row_tile * kRows, live = min(kRows, rows - row0), live_warps = (live + 31) / 32;
+      const long long token0 = static_cast<long long>(w.owner) * (share.prefix ? p.rows / p.prompts * p.s : p.s);
+      {
+        constexpr int kChunks = D / 8, kStep = 128 / kChunks;  // 16-byte pieces of a row; rows at a time
+        const int ch = threadIdx.x % kChunks, r0 = threadIdx.x / kChunks;
+        const __nv_bfloat16* from = p.q + (token0 * p.hq + w.head * p.group) * D + ch * 8;
+        uint8_t* to = sQ + (ch >> 3) * kPanelBytes;
+#pragma unroll 1
+        for (int r = r0; r < live; r += 8 * kStep) {
+          uint4 v[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int row = row0 + r + x * kStep;
+            if (r + x * kStep < live) {
+              const uint32_t token = token_of(p, row);
+              v[x] = *reinterpret_cast<const uint4*>(from + static_cast<long long>(token * p.hq + row - token * p.group) * D);
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int y = r + x * kStep;
+            if (y < live) *reinterpret_cast<uint4*>(to + y * 128 + (((ch & 7) ^ (y & 7)) << 4)) = v[x];
+          }
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
       const int r = warp * 32 + lane;
       int mine = r < live ? last : first;  // keys of this row end here
-      if (!piece.prefix && r < live) {
-        const int length = min(p.lengths != nullptr ? p.lengths[piece.owner] : p.own, p.own);
-        mine = min(last, length - p.s + (row0 + r) / p.group + 1);
-      }
+      if (!share.prefix && r < live) mine = min(last, w.hi - p.s + token_of(p, row0 + r) + 1);
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < n_tiles && !*abort_flag; ++j, ++done) {
         const int k0 = first + j * kKeys, seen = mine - k0;
@@ -289,7 +395,7 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
           l = l * alpha + (s0 + s1) + (s2 + s3);
           tmem_st_32x32(tile, pk);
           if (j > 0 && __any_sync(0xffffffffu, rescale)) {
-            if (!(ok = mbar_wait(pv_done, (done - 1) & 1))) break;  // the second product before this one has left the output
+            if (!(ok = mbar_wait(&pv_done[(done - 1) & 1], ((done - 1) >> 1) & 1))) break;  // the second product before this one has left the output
             tc_fence_after();
 #pragma unroll 1
             for (int ch = 0; ch < D / 32; ++ch) {
@@ -318,26 +424,27 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[done & 1]);
       }
-      if (ok && !*abort_flag) ok = mbar_wait(pv_done, (done - 1) & 1);
+      if (ok && !*abort_flag) ok = mbar_wait(&pv_done[(done - 1) & 1], ((done - 1) >> 1) & 1);
       if (ok && !*abort_flag && warp < live_warps) {
         tc_fence_after();
         // the output, unnormalised, by way of shared memory, where the queries are no longer needed, so that a row's values are written side by side
-        const long long base = piece.prefix ? ((static_cast<long long>(piece.owner) * p.cuts_p + piece.cut) * p.hkv + piece.head) * p.rows_p + row0
-                                            : static_cast<long long>(p.prompts) * p.cuts_p * p.hkv * p.rows_p +
-                                                  ((static_cast<long long>(piece.owner) * p.cuts_o + piece.cut) * p.hkv + piece.head) * p.rows_o + row0;
-        float* stage = reinterpret_cast<float*>(sQ) + warp * 1024;
-        const int count = min(32, live - warp * 32);
+        const long long base = w.base(p, share);
+        float4* stage = reinterpret_cast<float4*>(sQ) + warp * 256;
+        const int count = live - warp * 32;
+        float* to = p.part + (base + warp * 32 + (lane >> 3)) * D + (lane & 7) * 4;
 #pragma unroll 1
         for (int ch = 0; ch < D / 32; ++ch) {
           uint32_t v[32];
           tmem_ld_32x32(tO + lanes + ch * 32, v);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) stage[lane * 32 + (i ^ lane)] = __uint_as_float(v[i]);
+          for (int i = 0; i < 8; ++i) stage[lane * 8 + (i ^ (lane & 7))] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
           __syncwarp();
-          float* to = p.part + (base + warp * 32) * D + ch * 32 + lane;
-#pragma unroll 4
-          for (int i = 0; i < count; ++i) to[static_cast<long long>(i) * D] = stage[i * 32 + (lane ^ i)];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {  // four rows at a time
+            const int y = i * 4 + (lane >> 3);
+            if (y < count) *reinterpret_cast<float4*>(to + i * 4 * D + ch * 32) = stage[y * 8 + ((lane & 7) ^ (y & 7))];
+          }
           __syncwarp();
         }
         if (r < live) p.ml[base + r] = make_float2(m_used, l);
@@ -371,21 +478,27 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
   float m = -INFINITY, l = 0.f, o[kMine];
 #pragma unroll
   for (int x = 0; x < kMine; ++x) o[x] = 0.f;
-  const int pieces = p.cuts_p + p.cuts_o;
+  // pieces of the prompt's head, then of the row's own: those of all groups of CTAs with a tile of it
+  const int* before_p = p.shared_out + 2;
+  const int* before_o = before_p + p.prompts + 1;
+  int from[2], count[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int* before = k ? before_o : before_p;
+    const int owner = k ? row : prompt, groups = p.shared_out[k], n = before[owner + 1] - before[owner];
+    const long long all = static_cast<long long>(before[k ? p.rows : p.prompts]) * p.hkv, first = static_cast<long long>(before[owner]) * p.hkv + static_cast<long long>(head) * n;
+    from[k] = n > 0 ? group_of(all, groups, first) : 0;
+    count[k] = n > 0 ? group_of(all, groups, first + n - 1) - from[k] + 1 : 0;
+  }
+  const int pieces = count[0] + count[1];
   for (int first_piece = 0; first_piece < pieces; first_piece += 32) {
     const int piece = first_piece + lane;
     long long at = 0;
     float2 t = make_float2(-INFINITY, 0.f);
     if (piece < pieces) {
-      const bool prefix = piece < p.cuts_p;
-      const int cut = prefix ? piece : piece - p.cuts_p, owner = prefix ? prompt : row;
-      int first, last;
-      range_of(p, prefix, owner, cut, first, last);
-      if (first < last) {  // otherwise nobody has written it
-        at = prefix ? ((static_cast<long long>(prompt) * p.cuts_p + cut) * p.hkv + head) * p.rows_p + ((row - prompt * per) * p.s + i) * p.group + a
-                    : static_cast<long long>(p.prompts) * p.cuts_p * p.hkv * p.rows_p + ((static_cast<long long>(row) * p.cuts_o + cut) * p.hkv + head) * p.rows_o + i * p.group + a;
-        t = p.ml[at];
-      }
+      at = piece < count[0] ? (static_cast<long long>(prompt) * p.hkv + head + from[0] + piece) * p.rows_p + ((row - prompt * per) * p.s + i) * p.group + a
+                            : static_cast<long long>(p.pieces_p) * p.rows_p + (static_cast<long long>(row) * p.hkv + head + from[1] + piece - count[0]) * p.rows_o + i * p.group + a;
+      t = p.ml[at];
     }
     float top = fmaxf(m, t.x);
 #pragma unroll
@@ -434,50 +547,30 @@ struct Call {
   long long prompts, rows, s, hq, hkv, d, prefix, own;
 };
 
-// How long pieces are.  CTAs (two to an SM) take pieces in turn, those of the prefix first: the one with the most of both is done last.  A piece costs its tiles and an overhead that grows with its
-// rows, whose queries and outputs move between the pieces: in tiles, 0.3 and one for each 64 rows.
-static double overhead_of(int rows) { return 0.3 + (rows < kRows ? rows : kRows) / 64.0; }
-static int plan_of(const Call& c, Params& p) {
+// Sizes, and rows of the workspace: a piece for every head and one for every group of CTAs, of the prefixes and of the rows.
+static int plan_of(const Call& c, Params& p, long long& rows, long long& head_floats, int& ctas) {
   if (c.prompts <= 0 || c.rows <= 0 || c.rows % c.prompts || c.s <= 0 || c.hkv <= 0 || c.hq <= 0 || c.hq % c.hkv || (c.d != 64 && c.d != 128) || c.prefix < 0 || c.own < 0) return kErrBadShape;
-  if (c.rows > 0x7fffffff || c.prefix > 0x3fffffff || c.own > 0x3fffffff || c.rows * c.s > 0x7fffffff / c.hq) return kErrTooLarge;
+  if (c.rows > 0x3fffffff || c.prefix > 0x3fffffff || c.own > 0x3fffffff || c.rows * c.s > 0x7fffffff / c.hq || c.hkv > 256 || c.rows * (c.own / kKeys + 1) > 0x3fffffff ||
+      c.prompts * (c.prefix / kKeys + 1) > 0x3fffffff || (c.prefix / kKeys + 1) * c.hkv > 0x3fffffff || (c.own / kKeys + 1) * c.hkv > 0x3fffffff)
+    return kErrTooLarge;
   p.prompts = static_cast<int>(c.prompts), p.rows = static_cast<int>(c.rows), p.s = static_cast<int>(c.s), p.hq = static_cast<int>(c.hq), p.hkv = static_cast<int>(c.hkv);
   p.group = p.hq / p.hkv, p.prefix = static_cast<int>(c.prefix), p.own = static_cast<int>(c.own);
+  p.per_group = p.group == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + p.group - 1) / p.group);
   p.rows_p = static_cast<int>(c.rows / c.prompts * c.s * p.group), p.rows_o = static_cast<int>(c.s * p.group);
-  p.tiles_p = (p.rows_p + kRows - 1) / kRows, p.tiles_o = (p.rows_o + kRows - 1) / kRows;
   const long long np = (c.prefix + kKeys - 1) / kKeys, no = (c.own + kKeys - 1) / kKeys;  // tiles of keys
-  const long long heads_p = c.prompts * c.hkv * p.tiles_p, heads_o = c.rows * c.hkv * p.tiles_o, ctas = 2ll * sm_count();
-  const double over_p = overhead_of(p.rows_p), over_o = overhead_of(p.rows_o);
-  double best = 0;
-  long long run = 1;
-  for (long long t = 2; t <= 4096; t += t < 32 ? 1 : t / 8) {
-    const long long cuts_p = (np + t - 1) / t, cuts_o = (no + t - 1) / t;
-    const double each_p = cuts_p ? (np + cuts_p - 1) / cuts_p + over_p : 0, each_o = cuts_o ? (no + cuts_o - 1) / cuts_o + over_o : 0;
-    const long long pieces_p = heads_p * cuts_p, pieces = pieces_p + heads_o * cuts_o;
-    auto of = [&](long long cta) {  // what a CTA has to do
-      const long long first = pieces_p > cta ? (pieces_p - cta + ctas - 1) / ctas : 0, all = pieces > cta ? (pieces - cta + ctas - 1) / ctas : 0;
-      return first * each_p + (all - first) * each_o;
-    };
-    double time = of(0);
-    for (long long cta : {pieces_p % ctas, (pieces_p + ctas - 1) % ctas, (pieces + ctas - 1) % ctas}) time = of(cta) > time ? of(cta) : time;
-    if (best == 0 || time < best) best = time, run = t;
-    if (t > np && t > no) break;
-  }
-  auto cut = [&](long long n, int& cuts, int& keys) {
-    cuts = static_cast<int>((n + run - 1) / run);
-    keys = cuts == 0 ? kKeys : static_cast<int>((n + cuts - 1) / cuts) * kKeys;
-  };
-  cut(np, p.cuts_p, p.run_p), cut(no, p.cuts_o, p.run_o);
-  const double pieces_p = static_cast<double>(heads_p) * p.cuts_p, pieces_o = static_cast<double>(heads_o) * p.cuts_o;
-  if (pieces_p + pieces_o > 2e9) return kErrTooLarge;
-  p.pieces_p = static_cast<int>(pieces_p), p.pieces = static_cast<int>(pieces_p + pieces_o);
+  const long long most = c.prompts * c.hkv * np * tiles_of(p.rows_p) + c.rows * c.hkv * no * tiles_of(p.rows_o);
+  const int all = 2 * sm_count();
+  ctas = most < 2 * kSide ? 2 * kSide : most < all ? static_cast<int>(most) : all;
+  const long long pieces_p = np > 0 ? c.prompts * c.hkv + ctas / side_of(p.rows_p) : 0, pieces_o = no > 0 ? c.rows * c.hkv + ctas / side_of(p.rows_o) : 0;
+  if (pieces_p > 0x7fffffff) return kErrTooLarge;
+  p.pieces_p = static_cast<int>(pieces_p);
+  rows = pieces_p * p.rows_p + pieces_o * p.rows_o;
+  head_floats = (4 + c.prompts + c.rows + 3) / 4 * 4;
   return kOk;
-}
-static long long piece_rows(const Params& p) {
-  return static_cast<long long>(p.prompts) * p.cuts_p * p.hkv * p.rows_p + static_cast<long long>(p.rows) * p.cuts_o * p.hkv * p.rows_o;
 }
 
 template <int D>
-static int launch(const Call& c, Params& p, cudaStream_t st) {
+static int launch(const Call& c, Params& p, int ctas, cudaStream_t st) {
   using L = Layout<D>;
   CUtensorMap maps[4];
   const long long at[4] = {c.kp, c.vp, c.k, c.v};
@@ -499,12 +592,9 @@ static int launch(const Call& c, Params& p, cudaStream_t st) {
     if (cudaFuncSetAttribute(piece_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess) return kErrDriver;
     attr[device] = true;
   }
-  if (p.pieces > 0) {
-    const int ctas = 2 * sm_count();
-    TTB_COUNT_LAUNCH(1);
-    piece_kernel<D><<<p.pieces < ctas ? p.pieces : ctas, kThreads, L::kBytes, st>>>(maps[0], maps[1], maps[2], maps[3], p);
-    if (cudaGetLastError() != cudaSuccess) return kErrDriver;
-  }
+  TTB_COUNT_LAUNCH(2);
+  piece_kernel<D><<<ctas, kThreads, L::kBytes, st>>>(maps[0], maps[1], maps[2], maps[3], p);
+  if (cudaGetLastError() != cudaSuccess) return kErrDriver;
   const long long warps = static_cast<long long>(p.rows) * p.s * p.hq;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((warps + kJoinWarps - 1) / kJoinWarps));
@@ -513,8 +603,7 @@ static int launch(const Call& c, Params& p, cudaStream_t st) {
   cudaLaunchAttribute early[1];
   early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = early, cfg.numAttrs = p.pieces > 0 ? 1 : 0;
-  TTB_COUNT_LAUNCH(1);
+  cfg.attrs = early, cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, join_kernel<D>, p) == cudaSuccess ? kOk : kErrDriver;
 }
 
@@ -526,8 +615,10 @@ extern "C" long long ttb_shared_prefix_floats(const char* call, void*) {
   using namespace ttb::sprefix;
   const Call& c = *reinterpret_cast<const Call*>(call);
   Params p{};
-  const int rc = plan_of(c, p);
-  return rc != ttb::kOk ? rc : piece_rows(p) * (c.d + 2);
+  long long rows = 0, head = 0;
+  int ctas = 0;
+  const int rc = plan_of(c, p, rows, head, ctas);
+  return rc != ttb::kOk ? rc : head + rows * (c.d + 2);
 }
 
 extern "C" int ttb_shared_prefix_attention(const char* call, float scale, int* err, void* stream) {
@@ -535,15 +626,18 @@ extern "C" int ttb_shared_prefix_attention(const char* call, float scale, int* e
   using namespace ttb::sprefix;
   const Call& c = *reinterpret_cast<const Call*>(call);
   Params p{};
-  const int rc = plan_of(c, p);
+  long long rows = 0, head = 0;
+  int ctas = 0;
+  const int rc = plan_of(c, p, rows, head, ctas);
   if (rc != kOk) return rc;
   if ((c.q | c.o | c.kp | c.vp | c.k | c.v | c.work) & 15) return kErrBadShape;
-  const long long rows = piece_rows(p);
-  if (c.work_floats < rows * (c.d + 2)) return kErrBadShape;
+  if (c.work_floats < head + rows * (c.d + 2)) return kErrBadShape;
   p.q = reinterpret_cast<const __nv_bfloat16*>(c.q), p.o = reinterpret_cast<__nv_bfloat16*>(c.o);
   p.start = reinterpret_cast<const int*>(c.start), p.stop = reinterpret_cast<const int*>(c.stop), p.lengths = reinterpret_cast<const int*>(c.lengths);
-  p.part = reinterpret_cast<float*>(c.work), p.ml = reinterpret_cast<float2*>(p.part + rows * c.d);
+  p.shared_out = reinterpret_cast<int*>(c.work);
+  p.part = reinterpret_cast<float*>(c.work) + head, p.ml = reinterpret_cast<float2*>(p.part + rows * c.d);
   p.scale = scale, p.err = err;
   auto st = static_cast<cudaStream_t>(stream);
-  return c.d == 128 ? launch<128>(c, p, st) : launch<64>(c, p, st);
+  if (c.prefix == 0 && c.own == 0) return cudaMemsetAsync(p.o, 0, c.rows * c.s * c.hq * c.d * 2, st) == cudaSuccess ? kOk : kErrDriver;
+  return c.d == 128 ? launch<128>(c, p, ctas, st) : launch<64>(c, p, ctas, st);
 }
