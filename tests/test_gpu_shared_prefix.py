@@ -118,8 +118,8 @@ def test_layouts():
     assert torch.equal(ops.shared_prefix_attention(q, kp, vp, k, odd), want)
     wide = torch.cat([q, q], 2)[:, :, 8:]
     assert torch.equal(ops.shared_prefix_attention(wide, kp, vp, k, v), want)
-    one = ops.shared_prefix_attention(q, kp[:1].expand(2, -1, -1, -1), vp[:1].expand(2, -1, -1, -1), k, v)
-    assert torch.equal(one, ops.shared_prefix_attention(q, kp[:1], vp[:1], k, v))
+    twice = kp[:1].expand(2, -1, -1, -1), vp[:1].expand(2, -1, -1, -1)
+    _check(ops.shared_prefix_attention(q, *twice, k, v), q, *twice, k, v)
 
 
 def test_what_has_no_kernel():

@@ -130,12 +130,16 @@ struct Layout {
 };
 
 // Every CTA adds up the tiles of all prompts and rows, a run of them to a thread, and finds its share; the first one leaves the sums for the joining launch.
-__device__ __forceinline__ void find_share(const Params& p, Share& share, int (*sums)[2]) {
+__device__ __forceinline__ void add_tiles(const Params& p, int (&mine)[2]) {
+  const int t = threadIdx.x, run_p = (p.prompts + kThreads - 1) / kThreads, run_o = (p.rows + kThreads - 1) / kThreads;
+  mine[0] = t * run_p < p.prompts ? key_tiles(p, true, t * run_p) : 0;  // the loads of these two go out together
+  mine[1] = t * run_o < p.rows ? key_tiles(p, false, t * run_o) : 0;
+  for (int i = t * run_p + 1; i < min(p.prompts, (t + 1) * run_p); ++i) mine[0] += key_tiles(p, true, i);
+  for (int i = t * run_o + 1; i < min(p.rows, (t + 1) * run_o); ++i) mine[1] += key_tiles(p, false, i);
+}
+__device__ __forceinline__ void find_share(const Params& p, const int (&mine)[2], Share& share, int (*sums)[2]) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int run_p = (p.prompts + kThreads - 1) / kThreads, run_o = (p.rows + kThreads - 1) / kThreads;
-  int mine[2] = {0, 0};
-  for (int i = t * run_p; i < min(p.prompts, (t + 1) * run_p); ++i) mine[0] += key_tiles(p, true, i);
-  for (int i = t * run_o; i < min(p.rows, (t + 1) * run_o); ++i) mine[1] += key_tiles(p, false, i);
   int upto[2] = {mine[0], mine[1]};
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) {
@@ -151,13 +155,14 @@ __device__ __forceinline__ void find_share(const Params& p, Share& share, int (*
   for (int w = 0; w < kThreads / 32; ++w)
 #pragma unroll
     for (int k = 0; k < 2; ++k) before[k] += w < warp ? sums[w][k] : 0, all[k] += sums[w][k];
-  // CTAs in proportion to the tiles, at most one to a tile of few rows or to three of 128
+  // CTAs in proportion to the tiles, at most one to a tile of few rows or to two of 64 and more
   const int ctas = gridDim.x, side_p = side_of(p.rows_p), side_o = side_of(p.rows_o);
   const long long n_p = static_cast<long long>(all[0]) * p.hkv, n_o = static_cast<long long>(all[1]) * p.hkv;
-  const long long work_p = n_p * tiles_of(p.rows_p), work_o = n_o * tiles_of(p.rows_o);
+  // the end of a piece costs about 1.5 tiles, and a head is one piece at least
+  const long long work_p = (n_p + 3ll * p.prompts * p.hkv / 2) * tiles_of(p.rows_p), work_o = (n_o + 3ll * p.rows * p.hkv / 2) * tiles_of(p.rows_o);
   int ctas_p = n_p == 0 ? 0 : n_o == 0 ? ctas : static_cast<int>(static_cast<float>(work_p) / static_cast<float>(work_p + work_o) * ctas / side_p + 0.5f) * side_p;
   if (n_p > 0 && n_o > 0) ctas_p = max(side_p, min(ctas_p, (ctas - side_o) / side_p * side_p));
-  auto groups_of = [](long long n, int room, int rows) { return n == 0 ? 0 : static_cast<int>(max(1ll, min(static_cast<long long>(room), n / (1 + min(rows, kRows) / 64)))); };
+  auto groups_of = [](long long n, int room, int rows) { return n == 0 ? 0 : static_cast<int>(max(1ll, min(static_cast<long long>(room), n >> (rows >= 64)))); };
   const int groups[2] = {groups_of(n_p, ctas_p / side_p, p.rows_p), groups_of(n_o, (ctas - ctas_p) / side_o, p.rows_o)};
   const int cta = blockIdx.x, which = cta >= ctas_p, side = which ? side_o : side_p, at = which ? cta - ctas_p : cta;
   share.prefix = !which, share.group = at / side, share.side = at % side, share.sides = side, share.count = 0;
@@ -216,6 +221,8 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;");  // the joining launch may take its place; it waits for the end of this one
+  int my_tiles[2];
+  add_tiles(p, my_tiles);
   if (threadIdx.x == 128) prefetch_tmap(&tm_kp), prefetch_tmap(&tm_vp), prefetch_tmap(&tm_ko), prefetch_tmap(&tm_vo);
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kSlots; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
@@ -231,7 +238,7 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
   tc_fence_before();
   __shared__ int sums[kThreads / 32][2];
   Share share;
-  find_share(p, share, sums);  // with two barriers
+  find_share(p, my_tiles, share, sums);  // with two barriers
   tc_fence_after();
   const uint32_t tO = *tmem_slot, tS = tO + D;
 
@@ -309,32 +316,41 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
     const uint64_t c2 = pack_f32x2(cc, cc);
     bool ok = true, stop = false;
     uint32_t done = 0;  // tiles so far
-    for (Walk w(p, share); w.more() && !stop; w.next(p, share)) {
-      const int n_tiles = w.count(), first = w.first(), last = w.last();
-      const int rows = share.prefix ? p.rows_p : p.rows_o, row0 = w.row_tile * kRows, live = min(kRows, rows - row0), live_warps = (live + 31) / 32;
+    // Queries are on their way while the output of the piece before is written: eight 16-byte parts per thread, which for 128 channels are 64 rows; more rows follow when their piece begins.
+    constexpr int kParts = D / 8, kStep = 128 / kParts;  // parts of a row; rows at a time
+    const int q_part = threadIdx.x % kParts, q_row = threadIdx.x / kParts;
+    const int rows = share.prefix ? p.rows_p : p.rows_o;
+    auto fetch = [&](const Walk& w, int r0, uint4 (&v)[8]) {
+      const int row0 = w.row_tile * kRows + r0, end = min(rows - w.row_tile * kRows, kRows) - r0;
       const long long token0 = static_cast<long long>(w.owner) * (share.prefix ? p.rows / p.prompts * p.s : p.s);
-      {
-        constexpr int kChunks = D / 8, kStep = 128 / kChunks;  // 16-byte pieces of a row; rows at a time
-        const int ch = threadIdx.x % kChunks, r0 = threadIdx.x / kChunks;
-        const __nv_bfloat16* from = p.q + (token0 * p.hq + w.head * p.group) * D + ch * 8;
-        uint8_t* to = sQ + (ch >> 3) * kPanelBytes;
-#pragma unroll 1
-        for (int r = r0; r < live; r += 8 * kStep) {
-          uint4 v[8];
+      const __nv_bfloat16* from = p.q + (token0 * p.hq + w.head * p.group) * D + q_part * 8;
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const int row = row0 + r + x * kStep;
-            if (r + x * kStep < live) {
-              const uint32_t token = token_of(p, row);
-              v[x] = *reinterpret_cast<const uint4*>(from + static_cast<long long>(token * p.hq + row - token * p.group) * D);
-            }
-          }
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const int y = r + x * kStep;
-            if (y < live) *reinterpret_cast<uint4*>(to + y * 128 + (((ch & 7) ^ (y & 7)) << 4)) = v[x];
-          }
+      for (int x = 0; x < 8; ++x) {
+        const int r = q_row + x * kStep;
+        if (r < end) {
+          const uint32_t row = row0 + r, token = token_of(p, row);
+          v[x] = *reinterpret_cast<const uint4*>(from + static_cast<long long>(token * p.hq + row - token * p.group) * D);
         }
+      }
+    };
+    auto put = [&](int r0, int live, const uint4 (&v)[8]) {
+      uint8_t* to = sQ + (q_part >> 3) * kPanelBytes;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int r = r0 + q_row + x * kStep;
+        if (r < live) *reinterpret_cast<uint4*>(to + r * 128 + (((q_part & 7) ^ (r & 7)) << 4)) = v[x];
+      }
+    };
+    Walk w(p, share);
+    uint4 queries[8];
+    if (w.more()) fetch(w, 0, queries);
+    while (w.more() && !stop) {
+      const int n_tiles = w.count(), first = w.first(), last = w.last();
+      const int row0 = w.row_tile * kRows, live = min(kRows, rows - row0), live_warps = (live + 31) / 32;
+      put(0, live, queries);
+      if (live > 8 * kStep) {
+        fetch(w, 8 * kStep, queries);
+        put(8 * kStep, live, queries);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -424,6 +440,9 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[done & 1]);
       }
+      Walk after = w;
+      after.next(p, share);
+      if (after.more()) fetch(after, 0, queries);
       if (ok && !*abort_flag) ok = mbar_wait(&pv_done[(done - 1) & 1], ((done - 1) >> 1) & 1);
       if (ok && !*abort_flag && warp < live_warps) {
         tc_fence_after();
@@ -452,6 +471,7 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
       }
       if (!ok) fail(abort_flag, p.err, 303);
       stop = any_of_four(!ok || *abort_flag);  // all outputs are out of the queries' place; the four warps go on together or not at all
+      w = after;
     }
   }
 
@@ -461,76 +481,96 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
   if (warp == 5) tmem_dealloc(tO, L::kColumns);
 }
 
-// A warp per token and query head joins its pieces, those of the prefix and then its own: a lane per piece finds where it lies, its maximum and sum, and the weights go around, so that all loads but
-// the first two are independent.  32 pieces at a time.
+// Joins the pieces of a token and query head, those of the prefix and then its own.  A warp of `wide` (a power of two up to 8) takes every wide-th run of 32 pieces or, of fewer, its part of them: a lane
+// per piece finds where it lies, its maximum and sum, and the weights go around, so that all loads but the first two are independent.  Warps meet in shared memory, in their order.
 static constexpr int kJoinWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ Params p) {
-  const uint32_t w = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ Params p, int wide) {
+  __shared__ float outputs[kJoinWarps][D];
+  __shared__ float2 sums[kJoinWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, member = warp & (wide - 1);
+  const uint32_t w = (blockIdx.x * kJoinWarps + warp) / wide;
   const uint32_t token = w / p.hq;
-  if (token >= static_cast<uint32_t>(p.rows) * p.s) return;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the pieces are written
+  const bool live = token < static_cast<uint32_t>(p.rows) * p.s;
   const int h = static_cast<int>(w - token * p.hq), head = h / p.group, a = h - head * p.group;
   const int row = static_cast<int>(token / p.s), i = static_cast<int>(token - static_cast<uint32_t>(row) * p.s);
   const int per = p.rows / p.prompts, prompt = row / per;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the pieces are written
   constexpr int kMine = D / 32;
   float m = -INFINITY, l = 0.f, o[kMine];
 #pragma unroll
   for (int x = 0; x < kMine; ++x) o[x] = 0.f;
-  // pieces of the prompt's head, then of the row's own: those of all groups of CTAs with a tile of it
-  const int* before_p = p.shared_out + 2;
-  const int* before_o = before_p + p.prompts + 1;
-  int from[2], count[2];
+  if (live) {
+    // pieces of the prompt's head, then of the row's own: those of all groups of CTAs with a tile of it
+    const int* before_p = p.shared_out + 2;
+    const int* before_o = before_p + p.prompts + 1;
+    const int owners[2] = {prompt, row}, groups[2] = {p.shared_out[0], p.shared_out[1]}, at[2] = {before_p[prompt], before_o[row]}, next[2] = {before_p[prompt + 1], before_o[row + 1]};
+    const int all[2] = {before_p[p.prompts], before_o[p.rows]};
+    int from[2], count[2];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int* before = k ? before_o : before_p;
-    const int owner = k ? row : prompt, groups = p.shared_out[k], n = before[owner + 1] - before[owner];
-    const long long all = static_cast<long long>(before[k ? p.rows : p.prompts]) * p.hkv, first = static_cast<long long>(before[owner]) * p.hkv + static_cast<long long>(head) * n;
-    from[k] = n > 0 ? group_of(all, groups, first) : 0;
-    count[k] = n > 0 ? group_of(all, groups, first + n - 1) - from[k] + 1 : 0;
-  }
-  const int pieces = count[0] + count[1];
-  for (int first_piece = 0; first_piece < pieces; first_piece += 32) {
-    const int piece = first_piece + lane;
-    long long at = 0;
-    float2 t = make_float2(-INFINITY, 0.f);
-    if (piece < pieces) {
-      at = piece < count[0] ? (static_cast<long long>(prompt) * p.hkv + head + from[0] + piece) * p.rows_p + ((row - prompt * per) * p.s + i) * p.group + a
-                            : static_cast<long long>(p.pieces_p) * p.rows_p + (static_cast<long long>(row) * p.hkv + head + from[1] + piece - count[0]) * p.rows_o + i * p.group + a;
-      t = p.ml[at];
+    for (int k = 0; k < 2; ++k) {
+      const int n = next[k] - at[k];
+      const long long total = static_cast<long long>(all[k]) * p.hkv, first = static_cast<long long>(at[k]) * p.hkv + static_cast<long long>(head) * n;
+      from[k] = n > 0 ? group_of(total, groups[k], first) : 0;
+      count[k] = n > 0 ? group_of(total, groups[k], first + n - 1) - from[k] + 1 : 0;
     }
-    float top = fmaxf(m, t.x);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    const float base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), weight = exp2f(t.x - base);
-    float sum = t.y * weight;
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    l = l * f + sum;
-    m = top;
-#pragma unroll
-    for (int y = 0; y < kMine; ++y) o[y] *= f;
-    const int n = min(32, pieces - first_piece);
-    for (int x0 = 0; x0 < n; x0 += 4) {
-      float v[4][kMine], g[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        g[x] = __shfl_sync(0xffffffffu, weight, x0 + x);  // 0 where no key is seen
-        const float* from = p.part + __shfl_sync(0xffffffffu, at, x0 + x) * D + lane * kMine;
-        if (g[x] != 0.f) {
-          if constexpr (kMine == 4) *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(from);
-          else *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(from);
-        }
+    const int pieces = count[0] + count[1], run = min(32, (pieces + wide - 1) / wide);
+    for (int first_piece = member * run; first_piece < pieces; first_piece += wide * run) {
+      const int piece = first_piece + lane, n = min(run, pieces - first_piece);
+      long long place = 0;
+      float2 t = make_float2(-INFINITY, 0.f);
+      if (lane < n) {
+        place = piece < count[0] ? (static_cast<long long>(owners[0]) * p.hkv + head + from[0] + piece) * p.rows_p + ((row - prompt * per) * p.s + i) * p.group + a
+                                 : static_cast<long long>(p.pieces_p) * p.rows_p + (static_cast<long long>(owners[1]) * p.hkv + head + from[1] + piece - count[0]) * p.rows_o + i * p.group + a;
+        t = p.ml[place];
       }
+      float top = fmaxf(m, t.x);
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (g[x] != 0.f) {
+      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), weight = exp2f(t.x - base);
+      float sum = t.y * weight;
 #pragma unroll
-          for (int y = 0; y < kMine; ++y) o[y] += v[x][y] * g[x];
+      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      l = l * f + sum;
+      m = top;
+#pragma unroll
+      for (int y = 0; y < kMine; ++y) o[y] *= f;
+      for (int x0 = 0; x0 < n; x0 += 4) {
+        float v[4][kMine], g[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          g[x] = __shfl_sync(0xffffffffu, weight, x0 + x);  // 0 where no key is seen
+          const float* of = p.part + __shfl_sync(0xffffffffu, place, x0 + x) * D + lane * kMine;
+          if (g[x] != 0.f) {
+            if constexpr (kMine == 4) *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(of);
+            else *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(of);
+          }
         }
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (g[x] != 0.f) {
+#pragma unroll
+            for (int y = 0; y < kMine; ++y) o[y] += v[x][y] * g[x];
+          }
+      }
     }
   }
+  if (wide > 1) {
+    if (lane == 0) sums[warp] = make_float2(m, l);
+#pragma unroll
+    for (int y = 0; y < kMine; ++y) outputs[warp][lane * kMine + y] = o[y];
+    __syncthreads();
+    if (member != 0) return;
+    for (int x = 1; x < wide; ++x) {
+      const float2 t = sums[warp + x];
+      const float top = fmaxf(m, t.x), base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), g = exp2f(t.x - base);
+      l = l * f + t.y * g;
+      m = top;
+#pragma unroll
+      for (int y = 0; y < kMine; ++y) o[y] = o[y] * f + outputs[warp + x][lane * kMine + y] * g;
+    }
+  }
+  if (!live) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;  // a query without a key gives 0
   uint32_t out[kMine / 2];
 #pragma unroll
@@ -596,15 +636,17 @@ static int launch(const Call& c, Params& p, int ctas, cudaStream_t st) {
   piece_kernel<D><<<ctas, kThreads, L::kBytes, st>>>(maps[0], maps[1], maps[2], maps[3], p);
   if (cudaGetLastError() != cudaSuccess) return kErrDriver;
   const long long warps = static_cast<long long>(p.rows) * p.s * p.hq;
+  int wide = 1;  // few results are joined by more warps each, until there are sixteen to an SM
+  while (wide < kJoinWarps && warps * wide * 2 <= 16ll * sm_count()) wide *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((warps + kJoinWarps - 1) / kJoinWarps));
+  cfg.gridDim = dim3(static_cast<unsigned>((warps * wide + kJoinWarps - 1) / kJoinWarps));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute early[1];
   early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = early, cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel<D>, p) == cudaSuccess ? kOk : kErrDriver;
+  return cudaLaunchKernelEx(&cfg, join_kernel<D>, p, wide) == cudaSuccess ? kOk : kErrDriver;
 }
 
 }  // namespace sprefix
