@@ -1,8 +1,9 @@
 // Log-probabilities of given tokens with the entropy and the likeliest alternatives, from one pass over the logits, and their gradient in one more.
 //
-// Of z = x / T, in units of log2 (c = log2(e) / T):  d = (x - base) c,  s = sum 2^d,  t = sum 2^d d,  base the largest x so far, so that
+// Of z = x / T, in units of log2 (c = log2(e) / T):  d = (x - base) c,  s = sum 2^d,  t = sum 2^d d,  base within 2^24 of the largest 2^z so far, so that
 //   log p = ln2 (d - log2 s)        H = -sum p log p = ln2 (log2 s - t / s),
-// two sums of one sign each: nothing cancels.  When the base moves up by a / c, s' = s 2^-a and t' = (t - a s) 2^-a.  Differences are taken before they are scaled: a row of a type's lowest values is
+// where both terms stay below some 40: little cancels.  When the base moves up by a / c, s' = s 2^-a and t' = (t - a s) 2^-a.  A base that followed every new maximum would move in nearly all
+// steps of a warp, since one of its 32 lanes has a new one; so it hardly ever moves after a thread's first elements.  Differences are taken before they are scaled: a row of a type's lowest values is
 // one of equal logits.
 // With g, h and k_j the gradients of the token's log-probability, of the entropy and of the alternatives' log-probabilities:
 //   dx_v = ([v = token] g + sum_j [v = alternative j] k_j - p_v (g + sum_j k_j + h (log p_v + H))) / T.
@@ -38,12 +39,14 @@ using attn::pack_f32x2;
 using attn::unpack_f32x2;
 
 static constexpr int kThreads = 256, kWarps = kThreads / 32;
-static constexpr int kAhead = 4;          // vectors in flight per thread
+static constexpr int kAhead = 4;  // vectors in flight per thread
+static constexpr int kBlock = kThreads * kAhead;
 static constexpr int kMaxTop = 64;
 static constexpr int kMaxSegments = 2048;  // of a CTA
 static constexpr int kMaxCluster = 8;
 static constexpr float kLn2 = 0.6931471805599453f;
 static constexpr float kLowest = -200.f;  // 2^kLowest is 0 in fp32
+static constexpr float kReach = 24.f;     // log2 of how far exponentials may be above 1
 
 struct Params {
   const void* x;  // row r at x + (r / inner) * step_outer + (r % inner) * step_inner, in elements
@@ -90,11 +93,13 @@ __device__ __forceinline__ float warp_max_nan(float x) {
   asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(x));
   return d;
 }
-// Order of logits as whole numbers: NaN above all, zeros of both signs equal, nothing below 1 (0 stands for no element).
+// Order of logits as whole numbers: NaN above all, zeros of both signs equal, nothing below 1 (0 stands for no element); bits that the type does not have are left out.
+template <typename T>
+static constexpr int kSpareBits = std::is_same_v<T, float> ? 0 : std::is_same_v<T, __half> ? 13 : 16;
+template <typename T>
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (x != x) return 0xffffffffu;
   const uint32_t u = __float_as_uint(x + 0.f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return (x != x ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u)) >> kSpareBits<T>;
 }
 
 // A row as eight-element vectors on 16 bytes, the first of which may begin before it.
@@ -125,13 +130,19 @@ struct Row {
     for (int i = 0; i < 8; ++i) r.v[i] = e + i >= 0 && e + i < vocab ? x[e + i] : narrowed<T>(-INFINITY);
     return r;
   }
-  __device__ __forceinline__ uint32_t key(long long e) const { return e >= 0 && e < vocab ? key_of(widened(x[e])) : 0u; }
+  __device__ __forceinline__ uint32_t key(long long e) const { return e >= 0 && e < vocab ? key_of<T>(widened(x[e])) : 0u; }
 };
-// Eight values in 32 bits, two by two.
+// Eight values in 32 bits.
 template <typename Vector>
 __device__ __forceinline__ void widen8(const Vector& raw, float (&f)[8]) {
+  if constexpr (std::is_same_v<decltype(+raw.v), const __nv_bfloat16*>) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(raw.v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = widened(raw.v[i]);
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = widened(raw.v[i]);
+  }
 }
 __device__ __forceinline__ float most_of(const float (&f)[8]) { return max3_nan(max3_nan(f[0], f[1], f[2]), max3_nan(f[3], f[4], f[5]), max3_nan(f[6], f[7], f[7])); }
 
@@ -147,36 +158,68 @@ __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b, float c) {
   return {hi.base, hi.s + lo.s * f, hi.t + (lo.t + lo.s * d) * f};
 }
 
-// The `want` largest of n keys, of equal ones the first, in order of their place: to[0 ...]; by one warp.  Returns how many (n, if there are no more).
-__device__ __forceinline__ int choose(const uint32_t* keys, int n, int want, uint16_t* to) {
+// The `want` largest of n keys, of equal ones the first, in order of their place: to[0 ...]; by one warp.  Returns how many (n, if there are no more).  The keys lie on 16 bytes and have room for zeros
+// up to the next multiple of 128.
+__device__ __forceinline__ int choose(uint32_t* keys, int n, int want, uint16_t* to) {
   const int lane = threadIdx.x & 31;
   if (n <= want) {
     for (int i = lane; i < n; i += 32) to[i] = static_cast<uint16_t>(i);
     __syncwarp();
     return n;
   }
-  auto count = [&](uint32_t least) {
+  uint32_t high = 0, low = 0xffffffffu;
+  for (int i = lane; i < n; i += 32) high = max(high, keys[i]), low = min(low, keys[i]);
+  high = __reduce_max_sync(0xffffffffu, high), low = __reduce_min_sync(0xffffffffu, low);
+  const int groups = (n + 127) / 128;
+  for (int i = n + lane; i < groups * 128; i += 32) keys[i] = 0;
+  __syncwarp();
+  const uint4* fours = reinterpret_cast<const uint4*>(keys);
+  auto count = [&](uint32_t least) {  // least > 0
     int c = 0;
-#pragma unroll 8
-    for (int i = lane; i < n; i += 32) c += keys[i] >= least;
+#pragma unroll 4
+    for (int g = 0; g < groups; ++g) {
+      const uint4 k = fours[g * 32 + lane];
+      c += (k.x >= least) + (k.y >= least) + (k.z >= least) + (k.w >= least);
+    }
     return static_cast<int>(__reduce_add_sync(0xffffffffu, c));
   };
-  uint32_t level = 0;  // at least `want` keys reach it
-  for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
-    const int c = count(level | bit);
-    if (c >= want) level |= bit;
+  // at least `want` keys reach the level; all share the bits above the first in which the highest and the lowest differ
+  const int differ = 32 - __clz(high ^ low);
+  uint32_t level = differ == 32 ? 0u : high >> differ << differ;
+  for (int bit = differ - 1; bit >= 0; --bit) {
+    const int c = count(level | 1u << bit);
+    if (c >= want) level |= 1u << bit;
     if (c == want) break;
   }
   int equal = level == 0xffffffffu ? want : want - count(level + 1);  // of those that just reach it so many are taken
   int at = 0;
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    const uint32_t k = i0 + lane < n ? keys[i0 + lane] : 0u;
-    const uint32_t same = __ballot_sync(0xffffffffu, i0 + lane < n && k == level), below = (1u << lane) - 1;
-    const bool taken = i0 + lane < n && (k > level || (k == level && __popc(same & below) < equal));
-    const uint32_t all = __ballot_sync(0xffffffffu, taken);
-    if (taken) to[at + __popc(all & below)] = static_cast<uint16_t>(i0 + lane);
-    at += __popc(all);
-    equal -= min(equal, __popc(same));
+  for (int g = 0; g < groups; ++g) {
+    const uint4 four = fours[g * 32 + lane];
+    const uint32_t k[4] = {four.x, four.y, four.z, four.w};
+    const int place = g * 128 + lane * 4;
+    if (!__any_sync(0xffffffffu, max(max(k[0], k[1]), max(k[2], k[3])) >= level)) continue;
+    const uint32_t below = (1u << lane) - 1;
+    int same_before = 0, same_all = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t same = __ballot_sync(0xffffffffu, place + c < n && k[c] == level);
+      same_before += __popc(same & below), same_all += __popc(same);
+    }
+    bool taken[4];
+    int taken_before = 0, taken_all = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const bool same = place + c < n && k[c] == level;
+      taken[c] = place + c < n && (k[c] > level || (same && same_before < equal));
+      same_before += same;
+      const uint32_t all = __ballot_sync(0xffffffffu, taken[c]);
+      taken_before += __popc(all & below), taken_all += __popc(all);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (taken[c]) to[at + taken_before++] = static_cast<uint16_t>(place + c);
+    at += taken_all;
+    equal -= min(equal, same_all);
   }
   __syncwarp();
   return at;
@@ -191,9 +234,9 @@ struct Shared {
   Sums part[kMaxCluster];
 };
 struct SharedTop : Shared {
-  uint32_t segments[kMaxSegments];
-  uint32_t lanes[kMaxTop * 32];      // also keys of the cluster's entries
-  uint32_t elements[kMaxTop * 8];
+  alignas(16) uint32_t segments[kMaxSegments];
+  alignas(16) uint32_t lanes[kMaxTop * 32];  // also keys of the cluster's entries
+  alignas(16) uint32_t elements[kMaxTop * 8];
   uint16_t chosen[3][kMaxTop];
   int counts[3];
   Entry entries[kMaxCluster][kMaxTop];  // in order of their index; the first CTA's are those of all
@@ -212,31 +255,34 @@ __global__ void __launch_bounds__(kThreads, 4) stats_kernel(const __grid_constan
   const int first = min(per * split, all_segments) * 32, segments = min(all_segments - first / 32, per), end = min(vectors, first + segments * 32);
 
   const uint64_t c2 = pack_f32x2(p.c, p.c);
-  float top_x = -INFINITY, base = 0.f;  // 0 until there is a logit above the infinitely low ones
+  float limit = -INFINITY, base = 0.f;  // 0 until there is a logit above the infinitely low ones
+  const float reach = kReach / p.c;
   uint64_t s2 = 0, t2 = 0;
-  auto take = [&](const float (&f)[8], float most) {
-    if (!(most <= top_x)) {  // NaN too
+  auto raise = [&](float most) {
+    if (!(most <= limit)) {  // NaN too
       const float d = fminf(fmaxf((base - most) * p.c, kLowest), 0.f), g = fast_exp2(d);
       float s0, s1, t0, t1;
       unpack_f32x2(s2, s0, s1), unpack_f32x2(t2, t0, t1);
       const float s = s0 + s1, t = t0 + t1;
       s2 = pack_f32x2(s * g, 0.f), t2 = pack_f32x2((t + s * d) * g, 0.f);
-      top_x = base = most;
+      base = most, limit = most + reach;
     }
+  };
+  auto take = [&](const float (&f)[8]) {
     const uint64_t b2 = pack_f32x2(-base, -base);
-    uint64_t tv = 0;
+    uint64_t sv = 0, tv = 0;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       const uint64_t d = mul_f32x2(add_f32x2(pack_f32x2(f[i], f[i + 1]), b2), c2);
       float d0, d1;
       unpack_f32x2(d, d0, d1);
       const uint64_t e = pack_f32x2(fast_exp2(d0), fast_exp2(d1));
-      s2 = add_f32x2(s2, e);
+      sv = add_f32x2(sv, e);
       tv = fma_f32x2(e, d, tv);
     }
     float t0, t1;
     unpack_f32x2(tv, t0, t1);
-    if (!(t0 + t1 <= 0.f)) {  // an infinitely low logit (0 * -inf); its share is 0
+    if (t0 + t1 != t0 + t1) {  // an infinitely low logit (0 * -inf); its share is 0
       t0 = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -245,15 +291,14 @@ __global__ void __launch_bounds__(kThreads, 4) stats_kernel(const __grid_constan
       }
       tv = pack_f32x2(t0, 0.f);
     }
-    t2 = add_f32x2(t2, tv);
+    s2 = add_f32x2(s2, sv), t2 = add_f32x2(t2, tv);
   };
   auto note = [&](int j, float most) {  // the maximum of a segment
     if constexpr (TOP) {
       const float m = warp_max_nan(most);
-      if (lane == 0) sh.segments[(j - first) >> 5] = key_of(m);
+      if (lane == 0) sh.segments[(j - first) >> 5] = key_of<T>(m);
     }
   };
-  constexpr int kBlock = kThreads * kAhead;
   for (int j0 = first; j0 < end; j0 += kBlock) {
     if (j0 >= row.whole_from() && j0 + kBlock <= min(end, row.whole_to())) {  // the same for the CTA
       const typename Row<T>::Vector* at = row.vector(j0 + threadIdx.x);
@@ -266,7 +311,8 @@ __global__ void __launch_bounds__(kThreads, 4) stats_kernel(const __grid_constan
         widen8(raw[a], f);
         const float most = most_of(f);
         note(j0 + a * kThreads + threadIdx.x, most);
-        take(f, most);
+        raise(most);
+        take(f);
       }
     } else {
 #pragma unroll 1
@@ -282,7 +328,8 @@ __global__ void __launch_bounds__(kThreads, 4) stats_kernel(const __grid_constan
         }
         const float most = most_of(f);
         note(j, most);
-        take(f, most);
+        raise(most);
+        take(f);
       }
     }
   }
@@ -323,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 4) stats_kernel(const __grid_constan
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const long long e = j * 8ll - row.off + k;
-          const uint32_t key = e >= 0 && e < p.vocab ? key_of(widened(v.v[k])) : 0u;
+          const uint32_t key = e >= 0 && e < p.vocab ? key_of<T>(widened(v.v[k])) : 0u;
           best = max(best, key);
         }
       }
