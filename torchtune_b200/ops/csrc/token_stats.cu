@@ -1,6 +1,6 @@
 // Log-probabilities of given tokens with the entropy and the likeliest alternatives, from one pass over the logits, and their gradient in one more.
 //
-// Of z = x / T, in units of log2 (c = log2(e) / T):  d = (x - base) c,  s = sum 2^d,  t = sum 2^d d,  base within 2^24 of the largest 2^z so far, so that
+// Of z = x / T, in units of log2 (c = log2(e) / T):  d = (x - base) c,  s = sum 2^d,  t = sum 2^d d,  base so that 2^d stays below 2^24, so that
 //   log p = ln2 (d - log2 s)        H = -sum p log p = ln2 (log2 s - t / s),
 // where both terms stay below some 40: little cancels.  When the base moves up by a / c, s' = s 2^-a and t' = (t - a s) 2^-a.  A base that followed every new maximum would move in nearly all
 // steps of a warp, since one of its 32 lanes has a new one; so it hardly ever moves after a thread's first elements.  Differences are taken before they are scaled: a row of a type's lowest values is
@@ -9,9 +9,13 @@
 //   dx_v = ([v = token] g + sum_j [v = alternative j] k_j - p_v (g + sum_j k_j + h (log p_v + H))) / T.
 //
 // The alternatives are the `top` largest logits, of equal ones those with the lower index.  The pass leaves the largest value of every segment of 256 elements (what a warp reads at once) in shared
-// memory; the `top` segments with the largest ones (of equal ones the first) hold all alternatives, since an element outside is beaten by `top` maxima.  The same choice among the 32 lanes of those
-// segments and then among their eight elements leaves the alternatives, whatever the order of the logits, with a few hundred reads.  A choice is a search for the `top`-th largest key,
-// bit by bit, by one warp, while the other CTAs of the SM stream.
+// memory; the `top` segments with the largest ones (of equal ones the first) hold all alternatives, since an element outside is beaten by `top` maxima.  Of their elements those count that reach the
+// least of these maxima: hardly more than `top` as a rule, whose ranks one warp finds by comparing each with each.  Where they are too many (logits in order, ties, few segments), the
+// choice is made among the segments' 32 lanes and then among their eight elements as among the segments, by a search for the `top`-th largest key bit by bit: a few hundred reads
+// whatever the order of the logits.
+//
+// CTAs go from row to row.  Warps that stream take runs of a row and go on to the next one without waiting for each other; a warp of its own ends the row before, from sums and segments that lie in
+// shared memory twice.  Every lane copies its vectors two runs ahead, over the ends of rows too, to slots of its own.
 //
 // Rows begin at any address: vectors lie on 16 bytes, and the first and last of a row are read element by element.  Few rows are split over clusters of up to eight CTAs, which meet in the shared
 // memory of the first.
@@ -38,15 +42,23 @@ using attn::mul_f32x2;
 using attn::pack_f32x2;
 using attn::unpack_f32x2;
 
-static constexpr int kThreads = 256, kWarps = kThreads / 32;
-static constexpr int kAhead = 4;  // vectors in flight per thread
-static constexpr int kBlock = kThreads * kAhead;
+static constexpr int kWarps = 16;      // that stream
+static constexpr int kThreads = (kWarps + 1) * 32;
+static constexpr int kCtas = 2;        // of an SM
+template <typename T, bool TOP>
+static constexpr int kEach = sizeof(T) == 4 ? (TOP ? 1 : 2) : (TOP ? 3 : 4);  // vectors that a lane takes at once; alternatives need room of their own in shared memory
+template <typename T, bool TOP>
+static constexpr int kRun = 32 * kEach<T, TOP>;
+template <typename T, bool TOP>
+static constexpr int kSlotBytes = kWarps * kRun<T, TOP> * 8 * sizeof(T);
+static constexpr int kSlots = 3;
+static constexpr int kGradThreads = 256;
 static constexpr int kMaxTop = 64;
-static constexpr int kMaxSegments = 2048;  // of a CTA
+static constexpr int kMaxSegments = 1024;  // of a CTA
 static constexpr int kMaxCluster = 8;
 static constexpr float kLn2 = 0.6931471805599453f;
 static constexpr float kLowest = -200.f;  // 2^kLowest is 0 in fp32
-static constexpr float kReach = 24.f;     // log2 of how far exponentials may be above 1
+static constexpr float kMostAllowed = 0x1p24f;  // sum of the exponentials of eight elements
 
 struct Params {
   const void* x;  // row r at x + (r / inner) * step_outer + (r % inner) * step_inner, in elements
@@ -57,7 +69,7 @@ struct Params {
   float* stats;          // [rows, 2]: base and log2 s, or nullptr
   float* top_logprobs;   // [rows, top]
   long long* top_tokens;
-  long long ignore;
+  long long ignore, rows;
   int inner, vocab, top;
   float c, rate;  // log2(e) / T and 1 / T
 };
@@ -100,6 +112,12 @@ template <typename T>
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return (x != x ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u)) >> kSpareBits<T>;
+}
+
+template <typename T>
+__device__ __forceinline__ float value_of(uint32_t key) {
+  const uint32_t u = key << kSpareBits<T>;
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~(u | ((1u << kSpareBits<T>) - 1)));
 }
 
 // A row as eight-element vectors on 16 bytes, the first of which may begin before it.
@@ -146,16 +164,50 @@ __device__ __forceinline__ void widen8(const Vector& raw, float (&f)[8]) {
 }
 __device__ __forceinline__ float most_of(const float (&f)[8]) { return max3_nan(max3_nan(f[0], f[1], f[2]), max3_nan(f[3], f[4], f[5]), max3_nan(f[6], f[7], f[7])); }
 
+// x - base of elements i and i + 1
+template <typename T, typename Vector>
+__device__ __forceinline__ uint64_t minus(const Vector& raw, int i, float base) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {  // the conversion is part of the sum
+    const uint32_t w = reinterpret_cast<const uint32_t*>(raw.v)[i >> 1];
+    float d0, d1;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tadd.rn.f32.bf16 %0, lo, %3;\n\tadd.rn.f32.bf16 %1, hi, %3;\n\t}" : "=f"(d0), "=f"(d1) : "r"(w), "f"(-base));
+    return pack_f32x2(d0, d1);
+  } else {
+    return add_f32x2(pack_f32x2(widened(raw.v[i]), widened(raw.v[i + 1])), pack_f32x2(-base, -base));
+  }
+}
+template <typename T, typename Vector>
+__device__ __forceinline__ float most_of_vector(const Vector& raw) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(raw.v);
+    uint32_t a, b;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(w[0]), "r"(w[1]));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(w[2]), "r"(w[3]));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
+    const float lo = __uint_as_float(a << 16), hi = __uint_as_float(a & 0xffff0000u);
+    return max3_nan(lo, hi, hi);
+  } else {
+    float f[8];
+    widen8(raw, f);
+    return most_of(f);
+  }
+}
+
 // base, s and t of a part of a row
 struct Sums {
   float base, s, t;
 };
-__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b, float c) {
-  if (b.s == 0.f) return a;  // NaN goes on
-  if (a.s == 0.f) return b;
-  const Sums &hi = a.base >= b.base ? a : b, &lo = a.base >= b.base ? b : a;
-  const float d = fmaxf((lo.base - hi.base) * c, kLowest), f = exp2f(d);
-  return {hi.base, hi.s + lo.s * f, hi.t + (lo.t + lo.s * d) * f};
+// The sums of all lanes of a warp, over the highest of their bases; one without a finite logit (s = 0) has none.  NaN goes on.
+__device__ __forceinline__ Sums joined_lanes(const Sums& mine, float c) {
+  float s = mine.s, t = mine.t;
+  const float highest = warp_max_nan(s == 0.f ? -INFINITY : mine.base);
+  if (s != 0.f) {
+    const float d = fmaxf((mine.base - highest) * c, kLowest), f = fast_exp2(d);
+    t = (t + s * d) * f, s *= f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), t += __shfl_xor_sync(0xffffffffu, t, o);
+  return {highest == -INFINITY ? 0.f : highest, s, t};
 }
 
 // The `want` largest of n keys, of equal ones the first, in order of their place: to[0 ...]; by one warp.  Returns how many (n, if there are no more).  The keys lie on 16 bytes and have room for zeros
@@ -225,225 +277,407 @@ __device__ __forceinline__ int choose(uint32_t* keys, int n, int want, uint16_t*
   return at;
 }
 
-struct Entry {  // an alternative; index -1: none
-  uint32_t key;
-  int index;
-};
+// An alternative, or a segment: its key above, and below it the complement of its index, so that the larger number comes first.  0: none.
+using Entry = unsigned long long;
+__device__ __forceinline__ Entry entry_of(uint32_t key, int index) { return static_cast<Entry>(key) << 32 | ~static_cast<uint32_t>(index); }
+__device__ __forceinline__ uint32_t key_in(Entry e) { return static_cast<uint32_t>(e >> 32); }
+__device__ __forceinline__ int index_in(Entry e) { return static_cast<int>(~static_cast<uint32_t>(e)); }
+static constexpr int kMostCandidates = 512;  // all entries of a cluster
+
+// The `want` largest of `count` candidates, in their order, to `to`; by one warp.
+__device__ __forceinline__ void rank(const Entry* list, int count, int want, Entry* to) {
+  const int lane = threadIdx.x & 31;
+  for (int i = lane; i < want; i += 32) to[i] = 0;
+  __syncwarp();
+  for (int i = lane; i < count; i += 64) {  // two per lane
+    const Entry a = list[i], b = i + 32 < count ? list[i + 32] : 0;
+    int rank_a = 0, rank_b = 0;
+#pragma unroll 8
+    for (int j = 0; j < count; ++j) {
+      const Entry e = list[j];
+      rank_a += e > a, rank_b += e > b;
+    }
+    if (rank_a < want) to[rank_a] = a;
+    if (i + 32 < count && rank_b < want) to[rank_b] = b;
+  }
+  __syncwarp();
+}
+__device__ __forceinline__ void append(Entry* list, int* count, Entry e) {  // as far as there is room
+  const int at = atomicAdd(count, 1);
+  if (at < kMostCandidates) list[at] = e;
+}
+// The `want` (up to 32) largest of n keys, of equal ones the first, with their places as indices and in order, to `to`; false, if there are too many candidates.  At least `want` keys reach the want-th
+// largest of the lanes' maxima, and hardly more than twice as many if keys are in no order.  *count is 0.
+__device__ __forceinline__ bool choose_few(const uint32_t* keys, int n, int want, Entry* list, int* count, Entry* to) {
+  const int lane = threadIdx.x & 31;
+  uint32_t most = 0;
+#pragma unroll 4
+  for (int i = lane; i < n; i += 32) most = max(most, keys[i]);
+  int above = 0;
+#pragma unroll
+  for (int x = 0; x < 32; ++x) {
+    const uint32_t other = __shfl_sync(0xffffffffu, most, x);
+    above += (other > most) | ((other == most) & (x < lane));
+  }
+  const uint32_t least = __shfl_sync(0xffffffffu, most, __ffs(__ballot_sync(0xffffffffu, above == want - 1)) - 1);
+#pragma unroll 4
+  for (int i = lane; i < n; i += 32) {
+    const uint32_t key = keys[i];
+    if (key >= least) append(list, count, entry_of(key, i));
+  }
+  __syncwarp();
+  const int found = *static_cast<volatile int*>(count);
+  __syncwarp();
+  if (lane == 0) *count = 0;
+  if (found <= kMostCandidates) rank(list, found, want, to);
+  __syncwarp();
+  return found <= kMostCandidates;
+}
+
 struct Shared {
-  Sums warp[kWarps];
+  Sums warp[2][kWarps];
   Sums part[kMaxCluster];
 };
 struct SharedTop : Shared {
-  alignas(16) uint32_t segments[kMaxSegments];
-  alignas(16) uint32_t lanes[kMaxTop * 32];  // also keys of the cluster's entries
+  alignas(16) uint32_t segments[2][kMaxSegments];
+  alignas(16) uint32_t lanes[kMaxTop * 32];
   alignas(16) uint32_t elements[kMaxTop * 8];
   uint16_t chosen[3][kMaxTop];
-  int counts[3];
-  Entry entries[kMaxCluster][kMaxTop];  // in order of their index; the first CTA's are those of all
+  Entry candidates[kMostCandidates];
+  Entry found[kMaxTop];                 // segments
+  Entry entries[kMaxCluster][kMaxTop];  // in their order; the first CTA's are those of all
+  int count, few;                       // candidates; whether `found` holds the segments to be looked at
 };
 
-// grid: rows, each of `cluster` CTAs
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void wait_at(int barrier) { asm volatile("barrier.cta.sync %0, %1;" ::"r"(barrier), "n"(kThreads) : "memory"); }
+__device__ __forceinline__ void wait_for_all() { asm volatile("barrier.cta.sync 5, %0;" ::"n"(kThreads) : "memory"); }
+__device__ __forceinline__ void arrive_at(int barrier) { asm volatile("barrier.cta.arrive %0, %1;" ::"r"(barrier), "n"(kThreads) : "memory"); }
+
+// grid: CTAs that take rows in turn, or for few rows a cluster for each
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, 4) stats_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(16) uint8_t slots[];
   __shared__ std::conditional_t<TOP, SharedTop, Shared> sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int splits = cluster.num_blocks(), split = cluster.block_rank();
-  const long long r = blockIdx.x / splits;
-  const Row<T> row(static_cast<const T*>(p.x) + r / p.inner * p.step_outer + r % p.inner * p.step_inner, p.vocab);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int vectors = row.vectors(), all_segments = (vectors + 31) / 32, per = (all_segments + splits - 1) / splits;
-  const int first = min(per * split, all_segments) * 32, segments = min(all_segments - first / 32, per), end = min(vectors, first + segments * 32);
+  const uint32_t step = gridDim.x / splits, rows = p.rows;  // below 2^31
+  auto row_of = [&](uint32_t r) {
+    const uint32_t outer = p.step_outer == 0 ? 0u : r / p.inner;
+    return Row<T>(static_cast<const T*>(p.x) + outer * p.step_outer + static_cast<long long>(r - outer * p.inner) * p.step_inner, p.vocab);
+  };
+  struct Part {  // of a row, in vectors and segments of 32 of them
+    int first, end, segments;
+  };
+  auto part_of = [&](const Row<T>& row) {
+    const int vectors = row.vectors(), all = (vectors + 31) / 32, per = splits == 1 ? all : (all + splits - 1) / splits, from = min(per * split, all), count = min(all - from, per);
+    return Part{from * 32, min(vectors, (from + count) * 32), count};
+  };
 
-  const uint64_t c2 = pack_f32x2(p.c, p.c);
-  float limit = -INFINITY, base = 0.f;  // 0 until there is a logit above the infinitely low ones
-  const float reach = kReach / p.c;
-  uint64_t s2 = 0, t2 = 0;
-  auto raise = [&](float most) {
-    if (!(most <= limit)) {  // NaN too
-      const float d = fminf(fmaxf((base - most) * p.c, kLowest), 0.f), g = fast_exp2(d);
+  [[maybe_unused]] auto keys_of = [&](const Row<T>& row, const Part& part, int j, uint32_t (&key)[8]) {  // of a vector's elements
+    if (j >= row.whole_from() && j < min(part.end, row.whole_to())) {
+      float f[8];
+      widen8(Row<T>::whole(row.vector(j)), f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) key[k] = key_of<T>(f[k]);
+    } else {
+      const long long e = j * 8ll - row.off;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) key[k] = j < part.end ? row.key(e + k) : 0u;
+    }
+  };
+  // The elements of the segments that were found which reach the least of their maxima; by one warp, or by all, `member` of which this is
+  [[maybe_unused]] auto gather = [&](const Row<T>& row, const Part& part, int member) {
+    if constexpr (TOP) {
+    const uint32_t least = key_in(sh.found[p.top - 1]);
+    const int members = splits > 1 ? kWarps + 1 : 1;
+    for (int i0 = member; i0 < p.top; i0 += 4 * members) {
+      uint32_t key[4][8];
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (i0 + x * members < p.top) keys_of(row, part, part.first + index_in(sh.found[i0 + x * members]) * 32 + lane, key[x]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (i0 + x * members >= p.top) break;
+        const int e = (part.first + index_in(sh.found[i0 + x * members]) * 32 + lane) * 8 - row.off;
+        uint32_t most = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) most = max(most, key[x][k]);
+        if (most >= least) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (key[x][k] >= least) append(sh.candidates, &sh.count, entry_of(key[x][k], e + k));
+        }
+      }
+    }
+    __syncwarp();
+    }
+  };
+  if constexpr (TOP) {
+    if (threadIdx.x == kWarps * 32) sh.count = 0;
+  }
+
+  if (warp < kWarps) {
+    const uint64_t c2 = pack_f32x2(p.c, p.c);
+    constexpr int kMine = kEach<T, TOP>, kPieces = sizeof(T) / 2;  // 16-byte pieces of a vector
+    using Vector = typename Row<T>::Vector;
+    uint8_t* my_slots = slots + (warp * kRun<T, TOP> + lane) * 16;  // piece x of vector a of slot s: (s * kPieces + x) slots' pieces and a * 32 vectors further on
+    constexpr int kPieceBytes = kWarps * kRun<T, TOP> * 16;
+    // the next run to be copied
+    uint32_t ahead_r = blockIdx.x / splits;
+    Row<T> ahead_row = row_of(ahead_r < rows ? ahead_r : 0);
+    Part ahead_part = part_of(ahead_row);
+    int ahead_j = ahead_part.first + warp * kRun<T, TOP>, ahead_slot = 0;
+    auto whole = [](const Row<T>& row, const Part& part, int j0) { return j0 >= row.whole_from() && j0 + kRun<T, TOP> <= min(part.end, row.whole_to()); };  // the same for a warp
+    auto copy_ahead = [&]() {
+      while (ahead_r < rows && ahead_j >= ahead_part.end) {
+        ahead_r += step;
+        if (ahead_r < rows) ahead_row = row_of(ahead_r), ahead_part = part_of(ahead_row), ahead_j = ahead_part.first + warp * kRun<T, TOP>;
+      }
+      if (ahead_r < rows) {
+        if (whole(ahead_row, ahead_part, ahead_j)) {
+          const Vector* from = ahead_row.vector(ahead_j + lane);
+          const uint32_t to = smem_u32(my_slots) + ahead_slot * kPieces * kPieceBytes;
+#pragma unroll
+          for (int a = 0; a < kMine; ++a)
+#pragma unroll
+            for (int x = 0; x < kPieces; ++x) copy16(to + x * kPieceBytes + a * 512, reinterpret_cast<const uint4*>(from + a * 32) + x);
+        }
+        ahead_j += kWarps * kRun<T, TOP>;
+        ahead_slot = ahead_slot + 1 == kSlots ? 0 : ahead_slot + 1;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    copy_ahead(), copy_ahead();
+    int buffer = 0, turn = 0, slot = 0;
+    for (uint32_t r = blockIdx.x / splits; r < rows; r += step, buffer ^= 1, ++turn) {
+      const Row<T> row = row_of(r);
+      const Part part = part_of(row);
+      if (turn > 1) wait_at(3 + buffer);  // what lies in this buffer has been used
+      float most_allowed = -1.f, base = 0.f;  // there is no base until there is a logit above the infinitely low ones
+      uint64_t s2 = 0, t2 = 0;
+      auto careful = [&](const float (&f)[8]) {  // moves the base, and takes what is infinitely low to have no share (0 * -inf)
+        const float most = most_of(f);
+        if (!(most <= (most_allowed < 0.f ? -INFINITY : base))) {  // NaN too
+          const float d = fminf(fmaxf((base - most) * p.c, kLowest), 0.f), g = fast_exp2(d);
+          float s0, s1, t0, t1;
+          unpack_f32x2(s2, s0, s1), unpack_f32x2(t2, t0, t1);
+          const float s = s0 + s1, t = t0 + t1;
+          s2 = pack_f32x2(s * g, 0.f), t2 = pack_f32x2((t + s * d) * g, 0.f);
+          base = most, most_allowed = kMostAllowed;
+        }
+        float s = 0.f, t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float d = (f[i] - base) * p.c, e = fast_exp2(d);
+          s += e, t += e * (d < kLowest ? kLowest : d);
+        }
+        s2 = add_f32x2(s2, pack_f32x2(s, 0.f)), t2 = add_f32x2(t2, pack_f32x2(t, 0.f));
+      };
+      auto take = [&](const Vector& raw) {
+        uint64_t sv = 0, tv = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const uint64_t d = mul_f32x2(minus<T>(raw, i, base), c2);
+          float d0, d1;
+          unpack_f32x2(d, d0, d1);
+          const uint64_t e = pack_f32x2(fast_exp2(d0), fast_exp2(d1));
+          sv = i == 0 ? e : add_f32x2(sv, e);
+          tv = i == 0 ? mul_f32x2(e, d) : fma_f32x2(e, d, tv);
+        }
+        float s0, s1, t0, t1;
+        unpack_f32x2(sv, s0, s1), unpack_f32x2(tv, t0, t1);
+        const float sum = s0 + s1, t = t0 + t1;
+        if (!(sum <= most_allowed) || t != t) {
+          float f[8];
+          widen8(raw, f);
+          careful(f);
+        } else {
+          s2 = add_f32x2(s2, sv), t2 = add_f32x2(t2, tv);
+        }
+      };
+      auto note = [&](int j, float most) {  // the maximum of a segment
+        if constexpr (TOP) {
+          const float m = warp_max_nan(most);
+          if (lane == 0) sh.segments[buffer][(j - part.first) >> 5] = __float_as_uint(m);  // the warp that ends the row makes a key of it
+        }
+      };
+      for (int j0 = part.first + warp * kRun<T, TOP>; j0 < part.end; j0 += kWarps * kRun<T, TOP>) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        copy_ahead();  // to the slot before this one
+        if (whole(row, part, j0)) {
+          const uint8_t* at = my_slots + slot * kPieces * kPieceBytes;
+#pragma unroll
+          for (int a = 0; a < kMine; ++a) {
+            Vector raw;
+#pragma unroll
+            for (int x = 0; x < kPieces; ++x) reinterpret_cast<uint4*>(raw.v)[x] = *reinterpret_cast<const uint4*>(at + x * kPieceBytes + a * 512);
+            if constexpr (TOP) note(j0 + a * 32, most_of_vector<T>(raw));
+            take(raw);
+          }
+        } else {
+#pragma unroll 1
+          for (int a = 0; a < kMine && j0 + a * 32 < part.end; ++a) {
+            const int j = j0 + a * 32 + lane;
+            float f[8];
+            if (j < part.end) {
+              widen8(row.load(j), f);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) f[i] = -INFINITY;
+            }
+            note(j0 + a * 32, most_of(f));
+            careful(f);
+          }
+        }
+        slot = slot + 1 == kSlots ? 0 : slot + 1;
+      }
       float s0, s1, t0, t1;
       unpack_f32x2(s2, s0, s1), unpack_f32x2(t2, t0, t1);
-      const float s = s0 + s1, t = t0 + t1;
-      s2 = pack_f32x2(s * g, 0.f), t2 = pack_f32x2((t + s * d) * g, 0.f);
-      base = most, limit = most + reach;
+      const Sums mine = joined_lanes({base, s0 + s1, t0 + t1}, p.c);
+      if (lane == 0) sh.warp[buffer][warp] = mine;
+      __syncwarp();
+      arrive_at(1 + buffer);
     }
-  };
-  auto take = [&](const float (&f)[8]) {
-    const uint64_t b2 = pack_f32x2(-base, -base);
-    uint64_t sv = 0, tv = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const uint64_t d = mul_f32x2(add_f32x2(pack_f32x2(f[i], f[i + 1]), b2), c2);
-      float d0, d1;
-      unpack_f32x2(d, d0, d1);
-      const uint64_t e = pack_f32x2(fast_exp2(d0), fast_exp2(d1));
-      sv = add_f32x2(sv, e);
-      tv = fma_f32x2(e, d, tv);
-    }
-    float t0, t1;
-    unpack_f32x2(tv, t0, t1);
-    if (t0 + t1 != t0 + t1) {  // an infinitely low logit (0 * -inf); its share is 0
-      t0 = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = (f[i] - base) * p.c;
-        t0 += fast_exp2(d) * (d < kLowest ? kLowest : d);
+    if (splits > 1) {
+      if constexpr (TOP) {
+        wait_for_all();
+        const Row<T> row = row_of(blockIdx.x / splits);
+        if (sh.few) gather(row, part_of(row), warp);
+        wait_for_all();
       }
-      tv = pack_f32x2(t0, 0.f);
+      cluster.sync(), cluster.sync();
     }
-    s2 = add_f32x2(s2, sv), t2 = add_f32x2(t2, tv);
-  };
-  auto note = [&](int j, float most) {  // the maximum of a segment
-    if constexpr (TOP) {
-      const float m = warp_max_nan(most);
-      if (lane == 0) sh.segments[(j - first) >> 5] = key_of<T>(m);
-    }
-  };
-  for (int j0 = first; j0 < end; j0 += kBlock) {
-    if (j0 >= row.whole_from() && j0 + kBlock <= min(end, row.whole_to())) {  // the same for the CTA
-      const typename Row<T>::Vector* at = row.vector(j0 + threadIdx.x);
-      typename Row<T>::Vector raw[kAhead];
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a) raw[a] = Row<T>::whole(at + a * kThreads);
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        float f[8];
-        widen8(raw[a], f);
-        const float most = most_of(f);
-        note(j0 + a * kThreads + threadIdx.x, most);
-        raise(most);
-        take(f);
-      }
-    } else {
-#pragma unroll 1
-      for (int a = 0; a < kAhead; ++a) {
-        const int j = j0 + a * kThreads + threadIdx.x;
-        if (j - lane >= end) break;  // the same for a warp
-        float f[8];
-        if (j < end) {
-          widen8(row.load(j), f);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = -INFINITY;
-        }
-        const float most = most_of(f);
-        note(j, most);
-        raise(most);
-        take(f);
-      }
-    }
-  }
-  Sums mine;
-  {
-    float a, b;
-    mine.base = base;
-    unpack_f32x2(s2, a, b), mine.s = a + b;
-    unpack_f32x2(t2, a, b), mine.t = a + b;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums other = {__shfl_xor_sync(0xffffffffu, mine.base, o), __shfl_xor_sync(0xffffffffu, mine.s, o), __shfl_xor_sync(0xffffffffu, mine.t, o)};
-    mine = lane & o ? joined(other, mine, p.c) : joined(mine, other, p.c);
-  }
-  if (lane == 0) sh.warp[warp] = mine;
-  if (splits > 1) cluster.sync();  // all CTAs have started: their shared memory may be written
-  else __syncthreads();
-  auto* home = cluster.map_shared_rank(&sh, 0);
-  if (threadIdx.x == 0) {
-    mine = sh.warp[0];
-    for (int w = 1; w < kWarps; ++w) mine = joined(mine, sh.warp[w], p.c);
-    home->part[split] = mine;
+    return;
   }
 
-  if constexpr (TOP) {
-    if (warp == 0) {
-      const int n = choose(sh.segments, segments, p.top, sh.chosen[0]);
-      if (lane == 0) sh.counts[0] = n;
+  // ------------------------------------------------------------------------------------------------ the warp that ends rows
+  auto choose_segments = [&](const Part& part, uint32_t* segments) {  // sh.few: whether it went without a search
+    if constexpr (TOP) {
+    for (int i = lane; i < part.segments; i += 32) segments[i] = key_of<T>(__uint_as_float(segments[i]));
+    __syncwarp();
+    const bool few = p.top <= 32 && part.segments > p.top && choose_few(segments, part.segments, p.top, sh.candidates, &sh.count, sh.found);
+    if (lane == 0) sh.few = few;
+    __syncwarp();
     }
-    __syncthreads();
-    const int n_segments = sh.counts[0];
-    for (int i = warp; i < n_segments; i += kWarps) {
-      const int j = first + sh.chosen[0][i] * 32 + lane;
-      uint32_t best = 0;
-      if (j < end) {
-        const typename Row<T>::Vector v = row.load(j);
+  };
+  auto select = [&](const Row<T>& row, const Part& part, uint32_t* segments, Entry* to) {  // the alternatives of a part, in their order, behind gather()
+    if constexpr (TOP) {
+    const int count = sh.few ? sh.count : kMostCandidates + 1;
+    __syncwarp();
+    if (lane == 0) sh.count = 0;
+    if (count <= kMostCandidates) {
+      rank(sh.candidates, count, p.top, to);
+      return;
+    }
+    const int n_segments = choose(segments, part.segments, p.top, sh.chosen[0]);
+    for (int i = 0; i < n_segments; ++i) {
+      uint32_t key[8], most = 0;
+      keys_of(row, part, part.first + sh.chosen[0][i] * 32 + lane, key);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const long long e = j * 8ll - row.off + k;
-          const uint32_t key = e >= 0 && e < p.vocab ? key_of<T>(widened(v.v[k])) : 0u;
-          best = max(best, key);
-        }
-      }
-      sh.lanes[i * 32 + lane] = best;
+      for (int k = 0; k < 8; ++k) most = max(most, key[k]);
+      sh.lanes[i * 32 + lane] = most;
     }
-    __syncthreads();
-    if (warp == 0) {
-      const int n = choose(sh.lanes, n_segments * 32, p.top, sh.chosen[1]);
-      if (lane == 0) sh.counts[1] = n;
-    }
-    __syncthreads();
-    const int n_lanes = sh.counts[1];
+    __syncwarp();
+    const int n_lanes = choose(sh.lanes, n_segments * 32, p.top, sh.chosen[1]);
     auto index_of = [&](int i) {  // of element i of the chosen lanes
       const int at = sh.chosen[1][i >> 3];
-      return (first + sh.chosen[0][at >> 5] * 32ll + (at & 31)) * 8 - row.off + (i & 7);
+      return (part.first + sh.chosen[0][at >> 5] * 32ll + (at & 31)) * 8 - row.off + (i & 7);
     };
-    for (int i = threadIdx.x; i < n_lanes * 8; i += kThreads) sh.elements[i] = row.key(index_of(i));
-    __syncthreads();
-    if (warp == 0) {
-      const int n = choose(sh.elements, n_lanes * 8, p.top, sh.chosen[2]);
-      for (int i = lane; i < p.top; i += 32) {
-        Entry e = {0u, -1};
-        if (i < n && sh.elements[sh.chosen[2][i]] != 0) e = {sh.elements[sh.chosen[2][i]], static_cast<int>(index_of(sh.chosen[2][i]))};
-        home->entries[split][i] = e;
+    for (int i = lane; i < n_lanes * 8; i += 32) sh.elements[i] = row.key(index_of(i));
+    __syncwarp();
+    const int n = choose(sh.elements, n_lanes * 8, p.top, sh.chosen[2]);
+    for (int i = lane; i < n; i += 32) {
+      const uint32_t key = sh.elements[sh.chosen[2][i]];
+      sh.candidates[i] = key != 0 ? entry_of(key, static_cast<int>(index_of(sh.chosen[2][i]))) : 0;
+    }
+    __syncwarp();
+    rank(sh.candidates, n, p.top, to);
+    }
+  };
+  auto finish = [&](long long r, long long token, float logit, const Sums& sum) {  // with the alternatives in entries[0]
+    const float log_s = log2f(sum.s);
+    if constexpr (TOP) {
+      for (int x = lane; x < p.top; x += 32) {
+        const Entry e = sh.entries[0][x];
+        p.top_tokens[r * p.top + x] = index_in(e);
+        p.top_logprobs[r * p.top + x] = (value_of<T>(key_in(e)) - sum.base) * p.rate - log_s * kLn2;
       }
+      __syncwarp();
     }
+    if (lane == 0) {
+      float lp = 0.f;
+      if (token >= 0 && token < p.vocab) lp = (logit - sum.base) * p.rate - log_s * kLn2;
+      else if (token != p.ignore) TTB_NOTE_VIOLATION(token_stats);  // as a row that is ignored
+      p.logprobs[r] = token == p.ignore ? 0.f : lp;
+      p.entropy[r] = (log_s - sum.t / sum.s) * kLn2;
+      if (p.stats != nullptr) p.stats[2 * r] = sum.base, p.stats[2 * r + 1] = log_s;
+    }
+  };
+  auto sum_of = [&](int buffer) {  // of the warps
+    return joined_lanes(lane < kWarps ? sh.warp[buffer][lane] : Sums{0.f, 0.f, 0.f}, p.c);
+  };
+  if (splits == 1) {
+    int buffer = 0;
+    for (uint32_t r = blockIdx.x; r < rows; r += step, buffer ^= 1) {
+      const Row<T> row = row_of(r);
+      const long long token = p.tokens[r];
+      const float logit = token >= 0 && token < p.vocab ? widened(row.x[token]) : 0.f;
+      wait_at(1 + buffer);
+      const Sums sum = sum_of(buffer);
+      if constexpr (TOP) {
+        const Part part = part_of(row);
+        choose_segments(part, sh.segments[buffer]);
+        if (sh.few) gather(row, part, 0);
+        select(row, part, sh.segments[buffer], sh.entries[0]);
+      }
+      __syncwarp();
+      if (r + 2 * step < rows) arrive_at(3 + buffer);
+      finish(r, token, logit, sum);
+    }
+    return;
   }
-  if (splits > 1) {
-    cluster.sync();
-    if (split != 0) return;
-  } else {
-    __syncthreads();
-  }
-  Sums sum = sh.part[0];
-  for (int i = 1; i < splits; ++i) sum = joined(sum, sh.part[i], p.c);
-  const float log_s = log2f(sum.s);
+  const uint32_t r = blockIdx.x / splits;
+  const Row<T> row = row_of(r);
+  const long long token = p.tokens[r];
+  const float logit = token >= 0 && token < p.vocab ? widened(row.x[token]) : 0.f;
+  wait_at(1);
   if constexpr (TOP) {
-    Entry* best = sh.entries[0];
-    if (splits > 1) {
-      for (int i = threadIdx.x; i < splits * p.top; i += kThreads) sh.lanes[i] = sh.entries[i / p.top][i % p.top].key;
-      __syncthreads();
-      Entry mine_too = {0u, -1};
-      if (warp == 0) choose(sh.lanes, splits * p.top, p.top, sh.chosen[0]);
-      __syncthreads();
-      if (threadIdx.x < p.top) mine_too = sh.entries[sh.chosen[0][threadIdx.x] / p.top][sh.chosen[0][threadIdx.x] % p.top];
-      __syncthreads();
-      if (threadIdx.x < p.top) best[threadIdx.x] = mine_too;
-      __syncthreads();
-    }
-    if (threadIdx.x < p.top) {
-      const Entry e = best[threadIdx.x];
-      int rank = 0;  // entries lie in order of their index
-      for (int i = 0; i < p.top; ++i) rank += best[i].key > e.key || (best[i].key == e.key && i < static_cast<int>(threadIdx.x));
-      p.top_tokens[r * p.top + rank] = e.index;
-      p.top_logprobs[r * p.top + rank] = (widened(row.x[e.index]) - sum.base) * p.rate - log_s * kLn2;
-    }
+    const Part part = part_of(row);
+    choose_segments(part, sh.segments[0]);
+    wait_for_all();
+    if (sh.few) gather(row, part, kWarps);
+    wait_for_all();
   }
-  if (threadIdx.x == 0) {
-    const long long token = p.tokens[r];
-    float lp = 0.f;
-    if (token >= 0 && token < p.vocab) lp = (widened(row.x[token]) - sum.base) * p.rate - log_s * kLn2;
-    else if (token != p.ignore) TTB_NOTE_VIOLATION(token_stats);  // as a row that is ignored
-    p.logprobs[r] = token == p.ignore ? 0.f : lp;
-    p.entropy[r] = (log_s - sum.t / sum.s) * kLn2;
-    if (p.stats != nullptr) p.stats[2 * r] = sum.base, p.stats[2 * r + 1] = log_s;
+  cluster.sync();  // all CTAs have started: their shared memory may be written
+  auto* home = cluster.map_shared_rank(&sh, 0);
+  const Sums mine = sum_of(0);
+  if (lane == 0) home->part[split] = mine;
+  if constexpr (TOP) select(row, part_of(row), sh.segments[0], home->entries[split]);
+  cluster.sync();
+  if (split != 0) return;
+  const Sums sum = joined_lanes(lane < splits ? sh.part[lane] : Sums{0.f, 0.f, 0.f}, p.c);
+  if constexpr (TOP) {
+    uint32_t least = 1;  // a part with as many entries has nothing lower to give
+    for (int i = 0; i < splits; ++i) least = max(least, key_in(sh.entries[i][p.top - 1]));
+    for (int i = lane; i < splits * kMaxTop; i += 32) {
+      const Entry e = i % kMaxTop < p.top ? sh.entries[i / kMaxTop][i % kMaxTop] : 0;
+      if (key_in(e) >= least) append(sh.candidates, &sh.count, e);
+    }
+    __syncwarp();
+    const int count = *static_cast<volatile int*>(&sh.count);
+    __syncwarp();
+    rank(sh.candidates, count, p.top, sh.entries[0]);
   }
+  finish(r, token, logit, sum);
 }
 
 static constexpr int kGradVectors = 4;  // of a thread
 // grid: rows * parts
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) grad_kernel(const __grid_constant__ GradParams p) {
-  constexpr int kBlock = kThreads * kGradVectors;
+__global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const __grid_constant__ GradParams p) {
+  constexpr int kBlock = kGradThreads * kGradVectors;
   const int r = blockIdx.x / p.parts, part = blockIdx.x - r * p.parts;
   const Row<T> row(static_cast<const T*>(p.x) + r / p.inner * p.step_outer + r % p.inner * p.step_inner, p.vocab);
   T* out = static_cast<T*>(p.dx) + static_cast<long long>(r) * p.vocab;
@@ -456,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 4) grad_kernel(const __grid_constant
 #pragma unroll
     for (int a = 0; a < kGradVectors; ++a)
 #pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(raw[a].v)[i] = __ldcs(reinterpret_cast<const uint4*>(at + a * kThreads) + i);
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(raw[a].v)[i] = __ldcs(reinterpret_cast<const uint4*>(at + a * kGradThreads) + i);
   }
   const long long token = p.tokens[r];
   const bool counts = token != p.ignore && token >= 0 && token < p.vocab;
@@ -492,12 +726,12 @@ __global__ void __launch_bounds__(kThreads, 4) grad_kernel(const __grid_constant
     for (int a = 0; a < kGradVectors; ++a) {
       const typename Row<T>::Vector d = eight(raw[a]);
 #pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) __stcs(reinterpret_cast<uint4*>(to + a * kThreads) + i, reinterpret_cast<const uint4*>(d.v)[i]);
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) __stcs(reinterpret_cast<uint4*>(to + a * kGradThreads) + i, reinterpret_cast<const uint4*>(d.v)[i]);
     }
   } else {
 #pragma unroll 1
     for (int a = 0; a < kGradVectors; ++a) {
-      const int j = j0 + a * kThreads + threadIdx.x;
+      const int j = j0 + a * kGradThreads + threadIdx.x;
       if (j >= vectors) break;
       const typename Row<T>::Vector d = eight(row.load(j));
       const long long e = j * 8ll - row.off;
@@ -546,14 +780,24 @@ static int launch(const Call& c, float log2_rate, float rate, cudaStream_t st) {
   p.x = reinterpret_cast<const void*>(c.x), p.step_outer = c.step_outer, p.step_inner = c.step_inner, p.tokens = reinterpret_cast<const long long*>(c.tokens);
   p.logprobs = reinterpret_cast<float*>(c.logprobs), p.entropy = reinterpret_cast<float*>(c.entropy), p.stats = reinterpret_cast<float*>(c.stats);
   p.top_logprobs = reinterpret_cast<float*>(c.top_logprobs), p.top_tokens = reinterpret_cast<long long*>(c.top_tokens);
-  p.ignore = c.ignore, p.inner = static_cast<int>(c.inner), p.vocab = static_cast<int>(c.vocab), p.top = static_cast<int>(c.top), p.c = log2_rate, p.rate = rate;
+  p.ignore = c.ignore, p.rows = c.rows, p.inner = static_cast<int>(c.inner), p.vocab = static_cast<int>(c.vocab), p.top = static_cast<int>(c.top), p.c = log2_rate, p.rate = rate;
   const long long segments = (c.vocab + 7 + 255) / 256;
-  // few rows: more CTAs to a row, up to two for an SM, while each has eight segments (one for every warp)
+  // few rows: a cluster to a row, while each of its CTAs has a run for every warp, as long as all are on an SM at once
+  const long long at_once = static_cast<long long>(kCtas) * sm_count();
   int splits = 1;
-  while (splits < kMaxCluster && ((c.rows * splits * 2 <= 2ll * sm_count() && segments >= splits * 2 * kWarps) || (TOP && segments > static_cast<long long>(splits) * kMaxSegments))) splits *= 2;
+  while (splits < kMaxCluster && ((c.rows * splits * 2 <= at_once && segments >= splits * 2 * kWarps) || (TOP && segments > static_cast<long long>(splits) * kMaxSegments))) splits *= 2;
   if ((TOP && segments > static_cast<long long>(splits) * kMaxSegments) || c.rows * splits > 0x7fffffffll) return kErrTooLarge;
+  constexpr int bytes = kSlots * kSlotBytes<T, TOP>;
+  static bool attr[64] = {};  // an attribute of the kernel on one device
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return kErrDriver;
+  if (!attr[device]) {
+    if (cudaFuncSetAttribute(stats_kernel<T, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return kErrDriver;
+    attr[device] = true;
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(c.rows * splits));
+  cfg.dynamicSmemBytes = bytes;
+  cfg.gridDim = dim3(static_cast<unsigned>(splits > 1 || c.rows < at_once ? c.rows * splits : at_once));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -571,10 +815,10 @@ static int launch_grad(const Call& c, float log2_rate, float rate, cudaStream_t 
   p.g = reinterpret_cast<const float*>(c.g), p.h = reinterpret_cast<const float*>(c.h), p.k = reinterpret_cast<const float*>(c.k), p.dx = reinterpret_cast<void*>(c.dx);
   p.ignore = c.ignore, p.inner = static_cast<int>(c.inner), p.vocab = static_cast<int>(c.vocab), p.top = static_cast<int>(c.top), p.c = log2_rate, p.rate = rate;
   const long long vectors = (c.vocab + 7 + 7) / 8;
-  p.parts = static_cast<int>((vectors + kThreads * kGradVectors - 1) / (kThreads * kGradVectors));
+  p.parts = static_cast<int>((vectors + kGradThreads * kGradVectors - 1) / (kGradThreads * kGradVectors));
   if (c.rows * p.parts > 0x7fffffffll) return kErrTooLarge;
   TTB_COUNT_LAUNCH(1);
-  grad_kernel<T><<<static_cast<unsigned>(c.rows * p.parts), kThreads, 0, st>>>(p);
+  grad_kernel<T><<<static_cast<unsigned>(c.rows * p.parts), kGradThreads, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrDriver;
 }
 

@@ -95,9 +95,9 @@ class _TokenStatistics(torch.autograd.Function):
 
 
 def suits(logits: torch.Tensor, top: int) -> bool:
-    """Whether the kernels take these: with alternatives, a CTA has room for the maxima of 2048 segments of 256 elements, and a row has eight CTAs."""
+    """Whether the kernels take these: with alternatives, a CTA has room for the maxima of 1024 segments of 256 elements, and a row has eight CTAs."""
     v = logits.shape[-1]
-    return logits.dtype in _TYPES and v <= (4_000_000 if top else 2**31 - 512) and logits.numel() // v < 2**27
+    return logits.dtype in _TYPES and v <= (2_000_000 if top else 2**31 - 512) and logits.numel() // v < 2**27
 
 
 def token_statistics(logits, tokens, temperature: float, top: int, ignore: int, differentiated: bool) -> TokenStatistics:
