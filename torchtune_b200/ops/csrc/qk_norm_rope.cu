@@ -120,13 +120,6 @@ __device__ __forceinline__ void load_gain(const void* gain, int wide, int d, int
     widen(t, w);
   }
 }
-template <int G>
-__device__ __forceinline__ float group_sum(float x) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
-}
-
 __device__ __forceinline__ int position(const Params& p, long long token, int i, bool first) {
   const int at = p.pos != nullptr ? p.pos[token] : i;
   if (at >= 0 && at < p.table_len) return at;
@@ -134,70 +127,97 @@ __device__ __forceinline__ int position(const Params& p, long long token, int i,
   return 0;
 }
 
-// A unit is a chunk of HEADS heads of one token; units are dealt to groups of G lanes.
-template <typename T, bool INTERLEAVED, bool AFTER, int N, int G, int HEADS>
-__global__ void __launch_bounds__(kThreads, N * sizeof(T) <= 8 ? 4 : 2) forward_kernel(const __grid_constant__ Params p) {
-  const int v = threadIdx.x & (G - 1);
-  const uint32_t unit = blockIdx.x * (kThreads / G) + threadIdx.x / G;
-  const bool live = unit < static_cast<uint32_t>(p.b) * p.s * p.chunks && v < p.d / (2 * N);  // a group's lanes stay together: its sums take all of them
-  const uint32_t token = live ? unit / p.chunks : 0;
-  int chunk = live ? static_cast<int>(unit - token * p.chunks) : 0, which = 0;
-  while (chunk >= p.part[which].chunks) chunk -= p.part[which].chunks, ++which;
+// A unit is a chunk of HEADS heads of one token, whose sums go around side by side: a head that a unit lacks counts as zeros, so that no branch keeps the chains of shuffles apart.
+struct Place {  // of a unit
+  long long x, dy, y;  // elements from the start of the part's tensors
+  int which, token_in_row, count;
+  uint32_t token;
+  bool first;  // of its part
+};
+template <int N, int HEADS>
+__device__ __forceinline__ Place place_of(const Params& p, uint32_t unit, uint32_t units, int chunks, int which, int v) {
+  Place u;
+  const bool live = unit < units;
+  u.token = live ? unit / chunks : 0;
+  int chunk = live ? static_cast<int>(unit - u.token * chunks) : 0;
+  if (which < 0) {
+    which = 0;
+    while (chunk >= p.part[which].chunks) chunk -= p.part[which].chunks, ++which;
+  }
+  u.which = which, u.first = live && chunk == 0;
   const Part& part = p.part[which];
-  const int bi = static_cast<int>(token / p.s), i = static_cast<int>(token - static_cast<uint32_t>(bi) * p.s);
-  const int h0 = chunk * HEADS, count = live ? min(HEADS, part.heads - h0) : 0;
-  const T* x = static_cast<const T*>(part.x) + bi * part.x_b + i * part.x_s + h0 * part.x_h + N * v;
+  const int bi = static_cast<int>(u.token / p.s), h0 = chunk * HEADS;
+  u.token_in_row = static_cast<int>(u.token - static_cast<uint32_t>(bi) * p.s);
+  u.count = live && v < p.d / (2 * N) ? min(HEADS, part.heads - h0) : 0;  // a group's lanes stay together: its sums take all of them
+  u.x = bi * part.x_b + u.token_in_row * part.x_s + h0 * part.x_h + N * v;
+  u.dy = bi * part.dy_b + u.token_in_row * part.dy_s + h0 * part.dy_h + N * v;
+  long long to = u.token_in_row;
+  if (which > 0 && p.slots != nullptr) {
+    to = p.slots[u.token_in_row];
+    if (to < 0 || to >= p.slot_count) to = -1;
+  }
+  u.y = to < 0 ? -1 : bi * part.y_b + to * part.y_s + h0 * part.y_h + N * v;
+  return u;
+}
+
+template <int HEADS, int G>
+__device__ __forceinline__ void group_sums(float (&x)[HEADS]) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) x[h] += __shfl_xor_sync(0xffffffffu, x[h], o);
+}
+
+template <typename T, bool INTERLEAVED, bool AFTER, int N, int G, int HEADS>
+__global__ void __launch_bounds__(kThreads, HEADS == 1 ? 4 : N * sizeof(T) <= 8 ? 3 : 1) forward_kernel(const __grid_constant__ Params p) {
+  const int v = threadIdx.x & (G - 1), lane = v < p.d / (2 * N) ? v : 0;
+  const uint32_t units = static_cast<uint32_t>(p.b) * p.s * p.chunks;
+  const Place u = place_of<N, HEADS>(p, blockIdx.x * (kThreads / G) + threadIdx.x / G, units, p.chunks, -1, v);
+  const Part& part = p.part[u.which];
+  const T* x = static_cast<const T*>(part.x) + u.x;
   Run<T, N> raw[HEADS][2];
 #pragma unroll
-  for (int h = 0; h < HEADS; ++h)
-    if (h < count) raw[h][0].load(x + h * part.x_h), raw[h][1].load(x + h * part.x_h + p.d / 2);
-  long long to = i;
-  bool kept = count > 0;
-  if (which > 0 && p.slots != nullptr) {
-    to = p.slots[i];
-    if (to < 0 || to >= p.slot_count) {  // nothing is written outside a cache
-      if (kept && which == 1 && chunk == 0 && v == 0) TTB_NOTE_VIOLATION(qk_norm);
-      kept = false, to = 0;
-    }
-  }
-  T* y = static_cast<T*>(part.y) + bi * part.y_b + to * part.y_s + h0 * part.y_h + N * v;
-  if (which == 2) {
-#pragma unroll
-    for (int h = 0; h < HEADS; ++h)
-      if (kept && h < count) raw[h][0].store(y + h * part.y_h), raw[h][1].store(y + h * part.y_h + p.d / 2);
+  for (int h = 0; h < HEADS; ++h) {
+    raw[h][0] = raw[h][1] = Run<T, N>{};
+    if (h < u.count) raw[h][0].load(x + h * part.x_h), raw[h][1].load(x + h * part.x_h + p.d / 2);
   }
   float cs[2 * N], w[2 * N];
-  const int at = live ? position(p, token, i, which == 0 && chunk == 0 && v == 0) : 0, lane = live ? v : 0;
+  const int at = u.count > 0 ? position(p, u.token, u.token_in_row, u.first && u.which == 0 && v == 0) : 0;
   load_angles<INTERLEAVED, N>(p.table + static_cast<long long>(at) * p.d, p.d, lane, cs);
   load_gain<T, N>(part.gain, p.wide_gain, p.d, lane, w);
+  T* y = static_cast<T*>(part.y) + u.y;
+  const int kept = u.y >= 0 ? u.count : 0;  // nothing is written outside a cache
+  if (u.y < 0 && u.first && u.which == 1 && v == 0) TTB_NOTE_VIOLATION(qk_norm);
+  if (u.which == 2) {
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h)
+      if (h < kept) raw[h][0].store(y + h * part.y_h), raw[h][1].store(y + h * part.y_h + p.d / 2);
+  }
+  float f[HEADS][2 * N], sum[HEADS];
 #pragma unroll
   for (int h = 0; h < HEADS; ++h) {
-    float f[2 * N];
-    if (h < count) {
-      widen(raw[h], f);
-    } else {
+    widen(raw[h], f[h]);
+    if (AFTER) turn<INTERLEAVED, false, N>(f[h], cs);
+    sum[h] = 0.f;
 #pragma unroll
-      for (int j = 0; j < 2 * N; ++j) f[j] = 0.f;
-    }
-    if (AFTER) turn<INTERLEAVED, false, N>(f, cs);
-    float sum = 0.f;
+    for (int j = 0; j < 2 * N; ++j) sum[h] += f[h][j] * f[h][j];
+  }
+  group_sums<HEADS, G>(sum);
 #pragma unroll
-    for (int j = 0; j < 2 * N; ++j) sum += f[j] * f[j];
-    const float r = rsqrtf(group_sum<G>(sum) / p.d + p.eps);
+  for (int h = 0; h < HEADS; ++h) {
+    const float r = rsqrtf(sum[h] / p.d + p.eps);
 #pragma unroll
-    for (int j = 0; j < 2 * N; ++j) f[j] = f[j] * r * w[j];
-    if (!AFTER) turn<INTERLEAVED, false, N>(f, cs);
-    if (kept && which < 2 && h < count) {
-      Run<T, N> out[2];
+    for (int j = 0; j < 2 * N; ++j) f[h][j] = f[h][j] * r * w[j];
+    if (!AFTER) turn<INTERLEAVED, false, N>(f[h], cs);
+    Run<T, N> out[2];
 #pragma unroll
-      for (int j = 0; j < 2 * N; ++j) out[j / N].v[j % N] = narrowed<T>(f[j]);
-      out[0].store(y + h * part.y_h), out[1].store(y + h * part.y_h + p.d / 2);
-    }
+    for (int j = 0; j < 2 * N; ++j) out[j / N].v[j % N] = narrowed<T>(f[h][j]);
+    if (u.which < 2 && h < kept) out[0].store(y + h * part.y_h), out[1].store(y + h * part.y_h + p.d / 2);
   }
 }
 
 template <typename T, bool INTERLEAVED, bool AFTER, int N, int G, int HEADS>
-__global__ void __launch_bounds__(kThreads, N * sizeof(T) <= 8 ? 3 : N == 4 ? 2 : 1) backward_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, N * sizeof(T) <= 8 ? 3 : 1) backward_kernel(const __grid_constant__ Params p) {
   __shared__ float sums[kThreads / 32][2 * N * G];
   const int v = threadIdx.x & (G - 1);
   const int which = static_cast<int>(blockIdx.x) >= p.ctas_q;
@@ -212,53 +232,47 @@ __global__ void __launch_bounds__(kThreads, N * sizeof(T) <= 8 ? 3 : N == 4 ? 2 
 #pragma unroll
   for (int j = 0; j < 2 * N; ++j) dw[j] = 0.f;
   for (uint32_t first = cta * kGroups; first < units; first += ctas * kGroups) {  // the same for all lanes of a warp; units are below 2^31
-    const uint32_t unit = first + threadIdx.x / G;
-    const bool live = unit < units && lane_live;
-    const uint32_t token = live ? unit / part.chunks : 0;
-    const int chunk = live ? static_cast<int>(unit - token * part.chunks) : 0;
-    const int bi = static_cast<int>(token / p.s), i = static_cast<int>(token - static_cast<uint32_t>(bi) * p.s);
-    const int h0 = chunk * HEADS, count = live ? min(HEADS, part.heads - h0) : 0;
-    const T* x = static_cast<const T*>(part.x) + bi * part.x_b + i * part.x_s + h0 * part.x_h + N * v;
-    const T* dy = static_cast<const T*>(part.dy) + bi * part.dy_b + i * part.dy_s + h0 * part.dy_h + N * v;
-    T* dx = static_cast<T*>(part.y) + bi * part.y_b + i * part.y_s + h0 * part.y_h + N * v;
+    const Place u = place_of<N, HEADS>(p, first + threadIdx.x / G, units, part.chunks, which, v);
+    const T* x = static_cast<const T*>(part.x) + u.x;
+    const T* dy = static_cast<const T*>(part.dy) + u.dy;
+    T* dx = static_cast<T*>(part.y) + u.y;
     Run<T, N> raw_x[HEADS][2], raw_dy[HEADS][2];
 #pragma unroll
-    for (int h = 0; h < HEADS; ++h)
-      if (h < count) {
+    for (int h = 0; h < HEADS; ++h) {
+      raw_x[h][0] = raw_x[h][1] = raw_dy[h][0] = raw_dy[h][1] = Run<T, N>{};
+      if (h < u.count) {
         raw_x[h][0].load(x + h * part.x_h), raw_x[h][1].load(x + h * part.x_h + p.d / 2);
         raw_dy[h][0].load(dy + h * part.dy_h), raw_dy[h][1].load(dy + h * part.dy_h + p.d / 2);
       }
-    float cs[2 * N];
-    load_angles<INTERLEAVED, N>(p.table + static_cast<long long>(live ? position(p, token, i, false) : 0) * p.d, p.d, lane, cs);
+    }
+    float cs[2 * N], f[HEADS][2 * N], g[HEADS][2 * N], sums_of[2 * HEADS];
+    load_angles<INTERLEAVED, N>(p.table + static_cast<long long>(u.count > 0 ? position(p, u.token, u.token_in_row, false) : 0) * p.d, p.d, lane, cs);
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
-      float f[2 * N], g[2 * N];
-      if (h < count) {
-        widen(raw_x[h], f), widen(raw_dy[h], g);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2 * N; ++j) f[j] = g[j] = 0.f;
-      }
-      if (AFTER) turn<INTERLEAVED, false, N>(f, cs);
-      else turn<INTERLEAVED, true, N>(g, cs);
+      widen(raw_x[h], f[h]), widen(raw_dy[h], g[h]);
+      if (AFTER) turn<INTERLEAVED, false, N>(f[h], cs);
+      else turn<INTERLEAVED, true, N>(g[h], cs);
       float sum = 0.f, dot = 0.f;
 #pragma unroll
-      for (int j = 0; j < 2 * N; ++j) sum += f[j] * f[j], dot += g[j] * w[j] * f[j];
-      const float r = rsqrtf(group_sum<G>(sum) / p.d + p.eps);
-      const float mean = group_sum<G>(dot) / p.d * r;  // of dn n
-      if (h < count) {
+      for (int j = 0; j < 2 * N; ++j) sum += f[h][j] * f[h][j], dot += g[h][j] * w[j] * f[h][j];
+      sums_of[2 * h] = sum, sums_of[2 * h + 1] = dot;
+    }
+    group_sums<2 * HEADS, G>(sums_of);
 #pragma unroll
-        for (int j = 0; j < 2 * N; ++j) {
-          const float n = f[j] * r;
-          dw[j] += g[j] * n;
-          f[j] = r * (g[j] * w[j] - n * mean);
-        }
-        if (AFTER) turn<INTERLEAVED, true, N>(f, cs);
-        Run<T, N> out[2];
+    for (int h = 0; h < HEADS; ++h) {
+      const float r = h < u.count ? rsqrtf(sums_of[2 * h] / p.d + p.eps) : 0.f;
+      const float mean = sums_of[2 * h + 1] / p.d * r;  // of dn n
 #pragma unroll
-        for (int j = 0; j < 2 * N; ++j) out[j / N].v[j % N] = narrowed<T>(f[j]);
-        out[0].store(dx + h * part.y_h), out[1].store(dx + h * part.y_h + p.d / 2);
+      for (int j = 0; j < 2 * N; ++j) {
+        const float n = f[h][j] * r;
+        dw[j] += g[h][j] * n;
+        f[h][j] = r * (g[h][j] * w[j] - n * mean);
       }
+      if (AFTER) turn<INTERLEAVED, true, N>(f[h], cs);
+      Run<T, N> out[2];
+#pragma unroll
+      for (int j = 0; j < 2 * N; ++j) out[j / N].v[j % N] = narrowed<T>(f[h][j]);
+      if (h < u.count) out[0].store(dx + h * part.y_h), out[1].store(dx + h * part.y_h + p.d / 2);
     }
   }
   if (p.work == nullptr) return;
@@ -319,7 +333,7 @@ static int by_type(long long type, F f) {
   if (type == 1) return f(__half());
   return f(0.f);
 }
-// Channels of a half per lane and lanes of a head row: four channels keep the backward pass in 80 registers, of which three CTAs find room on an SM; more than 256 channels need eight.
+// Channels of a half per lane and lanes of a head row: four channels leave registers for the next heads; more than 256 channels need eight.
 template <typename F>
 static int by_size(int d, F f) {
   using Four = std::integral_constant<int, 4>;
@@ -365,10 +379,10 @@ static int params_of(const Call& c, Params& p, int parts, int heads_of_unit) {
   return p.chunks > 0 ? kOk : kErrBadShape;
 }
 
-// Backward: CTAs, at most four to an SM, dealt to queries and keys by their heads.
+// Backward: CTAs, at most three to an SM, dealt to queries and keys by their heads.
 static void ctas_of(const Call& c, int groups, int heads_of_unit, int& q, int& k) {
   const long long uq = c.b * c.s * ((c.heads[0] + heads_of_unit - 1) / heads_of_unit), uk = c.b * c.s * ((c.heads[1] + heads_of_unit - 1) / heads_of_unit);
-  const long long nq = (uq + groups - 1) / groups, nk = (uk + groups - 1) / groups, most = 4ll * sm_count();
+  const long long nq = (uq + groups - 1) / groups, nk = (uk + groups - 1) / groups, most = 3ll * sm_count();
   if (nq + nk <= most) {
     q = static_cast<int>(nq), k = static_cast<int>(nk);
     return;
@@ -400,8 +414,7 @@ extern "C" int ttb_qk_norm_rope(const char* call, float eps, void* stream) {
           p.eps = eps;
           const int rc = params_of(c, p, parts, H);
           if (rc != kOk) return rc;
-          const long long units = c.b * c.s * p.chunks, ctas = (units * G + kThreads - 1) / kThreads;
-          if (ctas > 0x7fffffff) return static_cast<int>(kErrTooLarge);
+          const long long units = c.b * c.s * p.chunks, ctas = (units * G + kThreads - 1) / kThreads;  // fewer than 2^31 of the former
           TTB_COUNT_LAUNCH(1);
           forward_kernel<T, decltype(interleaved)::value, decltype(after)::value, N, G, H><<<static_cast<unsigned>(ctas), kThreads, 0, st>>>(p);
           return cudaGetLastError() == cudaSuccess ? static_cast<int>(kOk) : static_cast<int>(kErrDriver);
@@ -415,7 +428,7 @@ extern "C" int ttb_qk_norm_rope(const char* call, float eps, void* stream) {
 }
 
 // Rows of d floats that suffice as a workspace of the backward pass where a gain has a gradient: one for each CTA.
-extern "C" long long ttb_qk_norm_rope_rows() { return 4ll * ttb::sm_count(); }
+extern "C" long long ttb_qk_norm_rope_rows() { return 3ll * ttb::sm_count(); }
 
 extern "C" int ttb_qk_norm_rope_bwd(const char* call, float eps, void* stream) {
   using namespace ttb;
