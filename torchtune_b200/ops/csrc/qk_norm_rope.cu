@@ -42,7 +42,7 @@ struct Params {
   float* work;             // backward: rows of d sums, those of queries first
   int b, s, d, table_len, slot_count, wide_gain;
   int chunks;              // of a token, all parts
-  float eps;
+  float eps, per_d;        // per_d: 1 / d
   int ctas_q;              // backward: CTAs of queries; the others are of keys
 };
 
@@ -81,8 +81,26 @@ struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Run {  // channels as th
 // The channels of a lane: [0, N) of the first half, [N, 2N) of the second.
 template <typename T, int N>
 __device__ __forceinline__ void widen(const Run<T, N> (&from)[2], float (&f)[2 * N]) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
 #pragma unroll
-  for (int i = 0; i < 2 * N; ++i) f[i] = widened(from[i / N].v[i % N]);
+    for (int i = 0; i < N; ++i) {
+      const uint32_t w = reinterpret_cast<const uint32_t*>(from[i / (N / 2)].v)[i % (N / 2)];
+      f[2 * i] = __uint_as_float(w << 16), f[2 * i + 1] = __uint_as_float(w & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) f[i] = widened(from[i / N].v[i % N]);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void narrow(const float (&f)[2 * N], Run<T, N> (&to)[2]) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) reinterpret_cast<__nv_bfloat162*>(to[i / (N / 2)].v)[i % (N / 2)] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) to[i / N].v[i % N] = narrowed<T>(f[i]);
+  }
 }
 template <bool INTERLEAVED, int N>
 __device__ __forceinline__ void load_angles(const float* at, int d, int v, float (&cs)[2 * N]) {  // pair i: cs[2i], cs[2i + 1]
@@ -113,11 +131,11 @@ __device__ __forceinline__ void load_gain(const void* gain, int wide, int d, int
   } else if (wide) {
     Run<float, N> t[2];
     t[0].load(static_cast<const float*>(gain) + N * v), t[1].load(static_cast<const float*>(gain) + d / 2 + N * v);
-    widen(t, w);
+    widen<float, N>(t, w);
   } else {
     Run<T, N> t[2];
     t[0].load(static_cast<const T*>(gain) + N * v), t[1].load(static_cast<const T*>(gain) + d / 2 + N * v);
-    widen(t, w);
+    widen<T, N>(t, w);
   }
 }
 __device__ __forceinline__ int position(const Params& p, long long token, int i, bool first) {
@@ -196,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, HEADS == 1 ? 4 : N * sizeof(T) <= 8 
   float f[HEADS][2 * N], sum[HEADS];
 #pragma unroll
   for (int h = 0; h < HEADS; ++h) {
-    widen(raw[h], f[h]);
+    widen<T, N>(raw[h], f[h]);
     if (AFTER) turn<INTERLEAVED, false, N>(f[h], cs);
     sum[h] = 0.f;
 #pragma unroll
@@ -205,13 +223,12 @@ __global__ void __launch_bounds__(kThreads, HEADS == 1 ? 4 : N * sizeof(T) <= 8 
   group_sums<HEADS, G>(sum);
 #pragma unroll
   for (int h = 0; h < HEADS; ++h) {
-    const float r = rsqrtf(sum[h] / p.d + p.eps);
+    const float r = rsqrtf(sum[h] * p.per_d + p.eps);
 #pragma unroll
     for (int j = 0; j < 2 * N; ++j) f[h][j] = f[h][j] * r * w[j];
     if (!AFTER) turn<INTERLEAVED, false, N>(f[h], cs);
     Run<T, N> out[2];
-#pragma unroll
-    for (int j = 0; j < 2 * N; ++j) out[j / N].v[j % N] = narrowed<T>(f[h][j]);
+    narrow<T, N>(f[h], out);
     if (u.which < 2 && h < kept) out[0].store(y + h * part.y_h), out[1].store(y + h * part.y_h + p.d / 2);
   }
 }
@@ -249,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, N * sizeof(T) <= 8 ? 3 : 1) backward
     load_angles<INTERLEAVED, N>(p.table + static_cast<long long>(u.count > 0 ? position(p, u.token, u.token_in_row, false) : 0) * p.d, p.d, lane, cs);
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
-      widen(raw_x[h], f[h]), widen(raw_dy[h], g[h]);
+      widen<T, N>(raw_x[h], f[h]), widen<T, N>(raw_dy[h], g[h]);
       if (AFTER) turn<INTERLEAVED, false, N>(f[h], cs);
       else turn<INTERLEAVED, true, N>(g[h], cs);
       float sum = 0.f, dot = 0.f;
@@ -260,8 +277,8 @@ __global__ void __launch_bounds__(kThreads, N * sizeof(T) <= 8 ? 3 : 1) backward
     group_sums<2 * HEADS, G>(sums_of);
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
-      const float r = h < u.count ? rsqrtf(sums_of[2 * h] / p.d + p.eps) : 0.f;
-      const float mean = sums_of[2 * h + 1] / p.d * r;  // of dn n
+      const float r = h < u.count ? rsqrtf(sums_of[2 * h] * p.per_d + p.eps) : 0.f;
+      const float mean = sums_of[2 * h + 1] * p.per_d * r;  // of dn n
 #pragma unroll
       for (int j = 0; j < 2 * N; ++j) {
         const float n = f[h][j] * r;
@@ -270,8 +287,7 @@ __global__ void __launch_bounds__(kThreads, N * sizeof(T) <= 8 ? 3 : 1) backward
       }
       if (AFTER) turn<INTERLEAVED, true, N>(f[h], cs);
       Run<T, N> out[2];
-#pragma unroll
-      for (int j = 0; j < 2 * N; ++j) out[j / N].v[j % N] = narrowed<T>(f[h][j]);
+      narrow<T, N>(f[h], out);
       if (h < u.count) out[0].store(dx + h * part.y_h), out[1].store(dx + h * part.y_h + p.d / 2);
     }
   }
@@ -356,7 +372,7 @@ static int params_of(const Call& c, Params& p, int parts, int heads_of_unit) {
   p.table = reinterpret_cast<const float*>(c.table), p.pos = reinterpret_cast<const int*>(c.pos), p.slots = reinterpret_cast<const long long*>(c.slots);
   p.work = reinterpret_cast<float*>(c.work);
   p.b = static_cast<int>(c.b), p.s = static_cast<int>(c.s), p.d = static_cast<int>(c.d), p.table_len = static_cast<int>(c.table_len), p.slot_count = static_cast<int>(c.slot_count);
-  p.wide_gain = static_cast<int>(c.wide_gain), p.chunks = 0;
+  p.wide_gain = static_cast<int>(c.wide_gain), p.chunks = 0, p.per_d = 1.f / static_cast<float>(c.d);
   for (int i = 0; i < parts; ++i) {
     Part& t = p.part[i];
     t.x = reinterpret_cast<const void*>(c.x[i]), t.y = reinterpret_cast<void*>(c.y[i]);
