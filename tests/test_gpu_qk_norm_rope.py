@@ -99,6 +99,8 @@ def test_layouts():
     odd = torch.empty(q.numel() + 1, device=DEV, dtype=torch.bfloat16)[1:].view_as(q).copy_(q.detach())
     odd_gain = torch.ones(d + 1, device=DEV, dtype=torch.bfloat16)[1:]
     assert torch.equal(ops.qk_norm_rope(odd, k.detach(), odd_gain, gain, table)[0], apart[0])
+    rounded = table.to(torch.bfloat16)
+    assert torch.equal(ops.qk_norm_rope(q.detach(), k.detach(), gain, gain, rounded)[0], ops.qk_norm_rope(q.detach(), k.detach(), gain, gain, rounded.float())[0])
     spread = torch.ones((), device=DEV, dtype=torch.bfloat16).expand(b, s, 6, d)
     x = q.detach().clone().requires_grad_()
     (g1,) = torch.autograd.grad(ops.qk_norm_rope(x, k.detach(), gain, gain, table)[0], x, spread)

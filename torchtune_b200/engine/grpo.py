@@ -112,6 +112,9 @@ class GRPOTrainer:
         self._max_generated_tokens = cfg.max_generated_tokens
         self._temperature = cfg.get("temperature", 1.0)
         self._top_k = cfg.get("top_k")
+        self._share_prompts = cfg.get("share_prompts", False)  # a prompt's answers read its keys and values from one place (generation.generate_group)
+        self._entropy_coeff = cfg.get("entropy_coeff", 0.0)  # weight of the policy's mean entropy, which the loss is lowered by
+        self._log_entropy = cfg.get("log_entropy", False) or self._entropy_coeff != 0.0
         self._total_steps = cfg.num_steps
         self._total_epochs = cfg.get("epochs", 1)
         self._save_every_n_epochs = cfg.get("save_every_n_epochs", 1)
@@ -133,18 +136,33 @@ class GRPOTrainer:
         logits = rlhf.truncate_sequence_for_logprobs(logits, ctx)
         return rlhf.logits_to_logprobs(logits, query_responses[:, ctx:], self._temperature)
 
+    def _response_statistics(self, model: nn.Module, query_responses, masks, position_ids, ctx: int):
+        """Log-probabilities of the responses and the entropies of the distributions they were drawn from."""
+        logits = model(query_responses, input_pos=position_ids, mask=masks)
+        logits = rlhf.truncate_sequence_for_logprobs(logits, ctx)
+        return rlhf.logits_to_statistics(logits, query_responses[:, ctx:], self._temperature)[:2]
+
+    def _rollout(self, prompts: torch.Tensor) -> torch.Tensor:
+        """``[b * grpo_samples, ctx + max_generated_tokens]`` (or less): every prompt with its responses."""
+        b, ctx = prompts.shape
+        g = self.grpo_samples
+        how = dict(max_generated_tokens=self._max_generated_tokens, temperature=self._temperature, top_k=self._top_k, pad_id=self._pad_id, rng=self._rng,
+                   stop_tokens=self._stop_token_ids.tolist() or None, return_logits=False)  # log-probabilities are recomputed below; no [b, n, vocab] tensor is kept
+        prompts = _left_pad(prompts, self._pad_id)
+        if self._share_prompts:
+            return generation.generate_group(self._model, prompts, samples=g, **how)[0]
+        batch = prompts[:, None, :].expand(b, g, ctx).reshape(b * g, ctx)
+        self._model.setup_caches(batch_size=b * g, dtype=self._dtype, decoder_max_seq_len=ctx + self._max_generated_tokens)
+        try:
+            return generation.generate(model=self._model, prompt=batch, **how)[0]
+        finally:
+            delete_kv_caches(self._model)
+
     @torch.no_grad()
     def generate_trajectory(self, prompts: torch.Tensor, answers: List[str]) -> GRPOTrajectory:
         b, ctx = prompts.shape
         g = self.grpo_samples
-        batch = _left_pad(prompts, self._pad_id)[:, None, :].expand(b, g, ctx).reshape(b * g, ctx)
-        self._model.setup_caches(batch_size=b * g, dtype=self._dtype, decoder_max_seq_len=ctx + self._max_generated_tokens)
-        try:
-            query_responses, _ = generation.generate(model=self._model, prompt=batch, max_generated_tokens=self._max_generated_tokens, temperature=self._temperature, top_k=self._top_k,
-                                                     pad_id=self._pad_id, rng=self._rng, stop_tokens=self._stop_token_ids.tolist() or None,
-                                                     return_logits=False)  # log-probabilities are recomputed below; no [b, n, vocab] tensor is kept
-        finally:
-            delete_kv_caches(self._model)
+        query_responses = self._rollout(prompts)
         not_pad = query_responses != self._pad_id
         masks = generation.get_causal_mask_from_padding_mask(not_pad)
         position_ids = generation.get_position_ids_from_padding_mask(not_pad)
@@ -168,14 +186,20 @@ class GRPOTrainer:
         chunks = max(1, -(-n // self._forward_batch_size))
         totals = None
         for idx in torch.arange(n, device=self._device).tensor_split(chunks):
-            pi = self._response_logprobs(self._model, traj.query_responses[idx], traj.masks[idx], traj.position_ids[idx], ctx)
-            pad = traj.response_padding_masks[idx]
+            pad, entropy = traj.response_padding_masks[idx], None
+            if self._log_entropy:
+                pi, entropy = self._response_statistics(self._model, traj.query_responses[idx], traj.masks[idx], traj.position_ids[idx], ctx)
+                entropy = rlhf.masked_mean(entropy, ~pad)
+            else:
+                pi = self._response_logprobs(self._model, traj.query_responses[idx], traj.masks[idx], traj.position_ids[idx], ctx)
             pi = pi.masked_fill(pad, 1.0)
             loss, policy_loss, kl_loss, ratios, clipfrac = self._loss_fn(traj.logprobs[idx], pi, traj.ref_logprobs[idx], traj.advantages[idx], padding_masks=~pad)
+            if self._entropy_coeff != 0.0:
+                loss = loss - self._entropy_coeff * entropy
             (loss * (idx.numel() / n)).backward()
             with torch.no_grad():
                 approx_kl = (0.5 * (pi - traj.logprobs[idx]).pow(2)).mean()
-            part = [t.detach().float().to(self._device) * (idx.numel() / n) for t in (loss, policy_loss, kl_loss, ratios, clipfrac, approx_kl)]
+            part = [t.detach().float().to(self._device) * (idx.numel() / n) for t in (loss, policy_loss, kl_loss, ratios, clipfrac, approx_kl, *(() if entropy is None else (entropy,)))]
             totals = part if totals is None else [a + b for a, b in zip(totals, part)]
         grad_norm = None
         if self.parallel is not None:
@@ -188,7 +212,10 @@ class GRPOTrainer:
         if self._lr_scheduler is not None:
             self._lr_scheduler.step()
         self.global_step += 1
-        return GRPOStats(*totals, metadata={"grad_norm": grad_norm})
+        metadata = {"grad_norm": grad_norm}
+        if self._log_entropy:
+            metadata["entropy"] = totals.pop()
+        return GRPOStats(*totals, metadata=metadata)
 
     def train(self) -> None:
         if hasattr(self._optimizer, "zero_grad"):
@@ -225,6 +252,8 @@ class GRPOTrainer:
             "loss": mean("loss"), "policy_loss": mean("policy_loss"), "kl_loss": mean("kl_loss"), "ratios": mean("ratios"), "clipfrac": mean("clipfrac"), "approx_policy_kl": mean("approx_policy_kls"),
             "rewards": self._last_rewards.mean(), "successes": self._last_successes.mean(), "response_lengths": traj.seq_lens.float().mean(),
         }
+        if self._log_entropy:
+            vals["entropy"] = torch.stack([s.metadata["entropy"] for s in stats]).mean()
         keys = sorted(vals)
         packed = torch.stack([vals[k].float().to(self._device) for k in keys])
         if self.parallel is not None:

@@ -4,21 +4,21 @@ A step of a small model is a few hundred launches of a few microseconds each, an
 from __future__ import annotations
 
 import threading
-from typing import Optional, Set, Tuple
+from typing import Optional, Sequence, Set, Tuple
 
 import torch
 from torch import nn
 from torch.utils._device import DeviceContext
 
 from .. import ops
-from ..modules import FeedForward, KVCache, MultiHeadAttention, QuantizedKVCache, RMSNorm, TransformerDecoder, TransformerSelfAttentionLayer
+from ..modules import FeedForward, KVCache, MultiHeadAttention, QuantizedKVCache, RMSNorm, SharedPrefixKVCache, TransformerDecoder, TransformerSelfAttentionLayer
 from ..modules.linear import Linear, has_hooks
 from ..modules.position_embeddings import RotaryPositionalEmbeddings
 from ..modules.tied_linear import TiedLinear
 from ._native_layers import NativeLayers
 
 # Modules whose forward pass of one token is the same sequence of launches in every step and needs no look at the device.
-_PLAIN = (TransformerDecoder, TransformerSelfAttentionLayer, MultiHeadAttention, FeedForward, KVCache, QuantizedKVCache, RMSNorm, Linear, nn.Linear, nn.Embedding, nn.ModuleList, nn.Identity,
+_PLAIN = (TransformerDecoder, TransformerSelfAttentionLayer, MultiHeadAttention, FeedForward, KVCache, QuantizedKVCache, SharedPrefixKVCache, RMSNorm, Linear, nn.Linear, nn.Embedding, nn.ModuleList, nn.Identity,
           nn.SiLU, nn.GELU, nn.ReLU)
 
 
@@ -52,7 +52,7 @@ class StepGraph:
     these sizes choose stays out of the recording.  While the program has other threads, all calls run as they are."""
 
     @staticmethod
-    def suits(model: nn.Module, like: torch.Tensor) -> bool:
+    def suits(model: nn.Module, like: torch.Tensor, caches: Sequence[type] = (KVCache, QuantizedKVCache)) -> bool:
         if type(model) is not TransformerDecoder or not like.is_cuda or model.tok_embeddings.weight.dtype != torch.bfloat16 or model.loop is not None:
             return False
         if model.num_output_chunks or model.output_hidden_states or model.skip_output_layer or model.pos_embeddings is not None:
@@ -72,7 +72,7 @@ class StepGraph:
             if type(layer) is not TransformerSelfAttentionLayer or layer.mask_mod is not None or type(layer.attn) is not MultiHeadAttention:
                 return False
             attn = layer.attn
-            if type(attn.kv_cache) not in (KVCache, QuantizedKVCache) or not attn.cache_enabled or attn.kv_cache.cache_pos.is_inference() or getattr(attn, "context_parallel", None) is not None:
+            if type(attn.kv_cache) not in caches or not attn.cache_enabled or getattr(attn.kv_cache, "cache_pos", like).is_inference() or getattr(attn, "context_parallel", None) is not None:
                 return False
             if attn.training and attn.attn_dropout:
                 return False

@@ -85,6 +85,7 @@ class DecoderArch:
     activation: Callable[[], nn.Module] = nn.SiLU
     mlp_bias: bool = False
     qk_norm_before_rope: bool = False  # Qwen3 normalises q/k per head before the rotation
+    fuse_qk_norm: bool = False  # norms and rotation of q/k as one operator with one rounding
     post_norms: bool = False  # Gemma-2: extra norms on the attention / MLP outputs (sa_scale, mlp_scale)
     final_norm: Optional[Callable[[int, float], nn.Module]] = None  # defaults to `norm`
     attn_softcap: float = 0.0
@@ -141,6 +142,7 @@ def build_attention(arch: DecoderArch, ad: AdapterSpec, rope: Optional[nn.Module
         softcap=arch.attn_softcap,
         scale=arch.attn_scale,
         qk_norm_before_rope=arch.qk_norm_before_rope,
+        fuse_qk_norm=arch.fuse_qk_norm,
     )
 
 

@@ -9,13 +9,14 @@ from .._generic import component_builders, layer_builders
 from ..qwen2._convert_weights import qwen3_hf_to_tune, qwen3_tune_to_hf  # noqa: F401
 
 
-def _arch(vocab_size: int, num_layers: int, num_heads: int, num_kv_heads: int, embed_dim: int, intermediate_dim: int, max_seq_len: int, head_dim: Optional[int] = None, attn_dropout: float = 0.0, norm_eps: float = 1e-5, rope_base: float = 1_000_000.0, tie_word_embeddings: bool = False, q_proj_bias: bool = True, k_proj_bias: bool = True, v_proj_bias: bool = True, q_norm: bool = False, k_norm: bool = False) -> DecoderArch:
+def _arch(vocab_size: int, num_layers: int, num_heads: int, num_kv_heads: int, embed_dim: int, intermediate_dim: int, max_seq_len: int, head_dim: Optional[int] = None, attn_dropout: float = 0.0, norm_eps: float = 1e-5, rope_base: float = 1_000_000.0, tie_word_embeddings: bool = False, q_proj_bias: bool = True, k_proj_bias: bool = True, v_proj_bias: bool = True, q_norm: bool = False, k_norm: bool = False, fuse_qk_norm: bool = False) -> DecoderArch:
     if q_norm != k_norm:
         raise ValueError("q_norm and k_norm must be enabled together")
-    return DecoderArch(vocab_size=vocab_size, num_layers=num_layers, num_heads=num_heads, num_kv_heads=num_kv_heads, embed_dim=embed_dim, max_seq_len=max_seq_len, intermediate_dim=intermediate_dim, head_dim=head_dim, attn_dropout=attn_dropout, norm_eps=norm_eps, qkv_bias=q_proj_bias and k_proj_bias and v_proj_bias, tie_embeddings=tie_word_embeddings, qk_norm=(lambda hd, eps: RMSNorm(hd, eps=eps)) if q_norm else None, qk_norm_before_rope=True, rope=lambda hd, msl: Qwen2RotaryPositionalEmbeddings(dim=hd, max_seq_len=msl, base=rope_base))
+    return DecoderArch(vocab_size=vocab_size, num_layers=num_layers, num_heads=num_heads, num_kv_heads=num_kv_heads, embed_dim=embed_dim, max_seq_len=max_seq_len, intermediate_dim=intermediate_dim, head_dim=head_dim, attn_dropout=attn_dropout, norm_eps=norm_eps, qkv_bias=q_proj_bias and k_proj_bias and v_proj_bias, tie_embeddings=tie_word_embeddings, qk_norm=(lambda hd, eps: RMSNorm(hd, eps=eps)) if q_norm else None, qk_norm_before_rope=True, fuse_qk_norm=fuse_qk_norm, rope=lambda hd, msl: Qwen2RotaryPositionalEmbeddings(dim=hd, max_seq_len=msl, base=rope_base))
 
 
-qwen3, lora_qwen3 = component_builders("qwen3", _arch, "Qwen3 decoder: GQA with per-head q/k RMSNorm before RoPE, SwiGLU, RMSNorm.")
+qwen3, lora_qwen3 = component_builders("qwen3", _arch, "Qwen3 decoder: GQA with per-head q/k RMSNorm before RoPE, SwiGLU, RMSNorm.  ``fuse_qk_norm`` makes norm and rotation one operator with one rounding (the builders of all sizes "
+                                             "take it).")
 qwen3_mlp, lora_qwen3_self_attention, lora_qwen3_mlp = layer_builders(_arch)
 
 _B = dict(vocab_size=151936, head_dim=128, attn_dropout=0.0, norm_eps=1e-6, rope_base=1_000_000.0, q_proj_bias=False, k_proj_bias=False, v_proj_bias=False, q_norm=True, k_norm=True)
@@ -26,14 +27,15 @@ _ARCHS = {
     "8b": dict(num_layers=36, num_heads=32, num_kv_heads=8, embed_dim=4096, intermediate_dim=12288),
     "14b": dict(num_layers=40, num_heads=40, num_kv_heads=8, embed_dim=5120, intermediate_dim=17408),
 }
+_EXPOSED = dict(fuse_qk_norm=False)
 for _n, _s in _ARCHS.items():
     for _variant, _msl in (("base", 32768), ("instruct", 40960)):
         _name = f"qwen3_{_n}_{_variant}"
-        globals()[_name] = preset(qwen3, _name, f"Qwen3 {_n} ({_variant}).", max_seq_len=_msl, **_B, **_s)
-        globals()[f"lora_{_name}"] = lora_preset(lora_qwen3, f"lora_{_name}", f"Qwen3 {_n} ({_variant}) with adapters.", max_seq_len=_msl, **_B, **_s)
+        globals()[_name] = preset(qwen3, _name, f"Qwen3 {_n} ({_variant}).", exposed=_EXPOSED, max_seq_len=_msl, **_B, **_s)
+        globals()[f"lora_{_name}"] = lora_preset(lora_qwen3, f"lora_{_name}", f"Qwen3 {_n} ({_variant}) with adapters.", exposed=_EXPOSED, max_seq_len=_msl, **_B, **_s)
 _S32 = dict(num_layers=64, num_heads=64, num_kv_heads=8, embed_dim=5120, intermediate_dim=25600, max_seq_len=40960)
-qwen3_32b = preset(qwen3, "qwen3_32b", "Qwen3 32B.", **_B, **_S32)
-lora_qwen3_32b = lora_preset(lora_qwen3, "lora_qwen3_32b", "Qwen3 32B with adapters.", **_B, **_S32)
+qwen3_32b = preset(qwen3, "qwen3_32b", "Qwen3 32B.", exposed=_EXPOSED, **_B, **_S32)
+lora_qwen3_32b = lora_preset(lora_qwen3, "lora_qwen3_32b", "Qwen3 32B with adapters.", exposed=_EXPOSED, **_B, **_S32)
 
 
 def qwen3_tokenizer(path: str, merges_file: str, special_tokens_path: Optional[str] = None, max_seq_len: Optional[int] = None, prompt_template=None, truncation_type: str = "right", **kwargs):

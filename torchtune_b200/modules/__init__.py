@@ -12,7 +12,7 @@ from .embedding_utils import resize_token_embeddings
 from .cached_mixer import CachedMixer
 from .feed_forward import ClampedGLU, FeedForward
 from .hyper_connections import HyperConnection, LayerScale
-from .kv_cache import KVCache, PassCaches, QuantizedKVCache, RowCache, SpanKVCache, StateCache
+from .kv_cache import KVCache, PassCaches, PromptGroups, QuantizedKVCache, RowCache, SharedPrefixKVCache, SpanKVCache, StateCache
 from .latent_attention import LatentAttention, LatentCache
 from .layer_norm import Fp32LayerNorm
 from .linear import Linear
@@ -59,6 +59,8 @@ __all__ = [
     "HyperConnectionLayer",
     "KVCache",
     "QuantizedKVCache",
+    "PromptGroups",
+    "SharedPrefixKVCache",
     "LatentAttention",
     "LatentCache",
     "LayerScale",

@@ -2,16 +2,17 @@
 from __future__ import annotations
 
 import logging
-from typing import Optional, Union
+from typing import Optional, Tuple, Union
 
 import torch
 from torch import nn
 
 from .. import ops
 from ..ops.mask import AttentionMask
-from .kv_cache import KVCache, QuantizedKVCache
+from .kv_cache import KVCache, QuantizedKVCache, SharedPrefixKVCache
 from .linear import Linear, has_hooks, is_plain_linear
 from .position_embeddings import RotaryPositionalEmbeddings
+from .rms_norm import RMSNorm
 
 logger = logging.getLogger(__name__)
 
@@ -35,6 +36,9 @@ class MultiHeadAttention(nn.Module):
     :class:`~torchtune_b200.ops.AttentionMask` (structured, used for training) or a
     boolean tensor ``[b, s_q, s_kv]`` with True = attend.  With ``y`` given this is
     cross attention; ``y=None`` on a cross-attention layer reads the KV cache.
+
+    ``fuse_qk_norm``: the norms of queries and keys and the rotation are one operator (:func:`torchtune_b200.ops.qk_norm_rope`, with a plain KV cache its write too), which rounds
+    once where the two of their own round twice; it needs RMS norms of one epsilon and a plain rotary embedding, and has no effect without them.
     """
 
     def __init__(
@@ -58,6 +62,7 @@ class MultiHeadAttention(nn.Module):
         softcap: float = 0.0,
         scale: Optional[float] = None,
         qk_norm_before_rope: bool = False,
+        fuse_qk_norm: bool = False,
     ) -> None:
         super().__init__()
         if num_heads % num_kv_heads != 0:
@@ -86,6 +91,7 @@ class MultiHeadAttention(nn.Module):
         self.k_norm = k_norm
         self.pos_embeddings = pos_embeddings
         self.qk_norm_before_rope = qk_norm_before_rope
+        self.fuse_qk_norm = fuse_qk_norm
         self.cache_enabled = False
 
     def setup_cache(self, batch_size: int, dtype: torch.dtype, max_seq_len: int, bits: Optional[int] = None) -> None:
@@ -112,7 +118,7 @@ class MultiHeadAttention(nn.Module):
         """Rotary embedding of ``q`` (returned) and of ``k``, the latter and ``v`` going straight to their slots of the cache; ``None``, with nothing
         done, for anything but a plain rotation in front of a plain cache."""
         cache, pe = self.kv_cache, self.pos_embeddings
-        if not self.cache_enabled or type(cache) is not KVCache or self.q_norm is not None or not isinstance(pe, RotaryPositionalEmbeddings):
+        if not self.cache_enabled or type(cache) not in (KVCache, SharedPrefixKVCache) or self.q_norm is not None or not isinstance(pe, RotaryPositionalEmbeddings):
             return None
         if type(pe).forward is not RotaryPositionalEmbeddings.forward or has_hooks(pe) or has_hooks(cache):
             return None
@@ -121,6 +127,26 @@ class MultiHeadAttention(nn.Module):
         if out is not None:
             cache.advance(s)
         return out
+
+    def _norms_and_rotates(self) -> bool:
+        """Whether norms and rotation of queries and keys may be one operator."""
+        pe, norms = self.pos_embeddings, (self.q_norm, self.k_norm)
+        if not self.fuse_qk_norm or any(type(m) is not RMSNorm or has_hooks(m) for m in norms) or norms[0].eps != norms[1].eps:
+            return False
+        return isinstance(pe, RotaryPositionalEmbeddings) and type(pe).forward is RotaryPositionalEmbeddings.forward and not has_hooks(pe)
+
+    def _norm_and_rotate(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, input_pos: Optional[torch.Tensor]) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+        """Queries and keys; ``None`` for the keys if they and the values have gone to the cache."""
+        pe, cache, gains = self.pos_embeddings, self.kv_cache, (self.q_norm.scale, self.k_norm.scale)
+        how = dict(eps=self.q_norm.eps, interleaved=pe.interleaved, norm_first=self.qk_norm_before_rope)
+        into = self.cache_enabled and type(cache) in (KVCache, SharedPrefixKVCache) and cache.k_cache.dtype == k.dtype and not has_hooks(cache)
+        if into and not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, *gains))) and torch.autograd.forward_ad._current_level < 0:
+            b, s = q.shape[:2]
+            slots = cache.reserve(b, s)
+            q = ops.qk_norm_rope_append(q, k, v, *gains, pe.cache, input_pos, cache.k_cache[:b], cache.v_cache[:b], slots, **how)
+            cache.advance(s)
+            return q, None
+        return ops.qk_norm_rope(q, k, *gains, pe.cache, input_pos, **how)
 
     def forward(
         self,
@@ -144,12 +170,24 @@ class MultiHeadAttention(nn.Module):
             q = self.q_proj(x)
         q = q.view(b, s_x, self.num_heads, self.head_dim)
         rotated = None
-        quantized = self.cache_enabled and isinstance(self.kv_cache, QuantizedKVCache)
+        attends = self.cache_enabled and isinstance(self.kv_cache, (QuantizedKVCache, SharedPrefixKVCache))  # with keys and values that are not simply its buffers
         if k is not None:
             k, v = (t.view(b, s_x, self.num_kv_heads, self.head_dim) for t in (k, v))
             rotated = self._rotate_into_cache(q, k, v, input_pos)
+        fused = rotated is None and y is x and self._norms_and_rotates()
         if rotated is not None:
-            q, k, v = rotated, self.kv_cache.k_cache[:b], self.kv_cache.v_cache[:b]
+            q, k, v = rotated, None, None
+        elif fused:
+            if k is None:
+                k, v = (proj(x).view(b, s_x, self.num_kv_heads, self.head_dim) for proj in (self.k_proj, self.v_proj))
+            q, k = self._norm_and_rotate(q, k, v, input_pos)
+        if rotated is not None or fused:
+            if k is not None and attends:
+                self.kv_cache.append(k, v)
+            elif k is not None and self.kv_cache is not None and self.cache_enabled:
+                k, v = self.kv_cache.update(k, v)
+            elif k is None and not attends:
+                k, v = self.kv_cache.k_cache[:b], self.kv_cache.v_cache[:b]
         else:
             if self.q_norm is not None and self.qk_norm_before_rope:
                 q = self.q_norm(q)
@@ -160,7 +198,7 @@ class MultiHeadAttention(nn.Module):
             if y is None:
                 if self.kv_cache is None or not self.cache_enabled:
                     raise ValueError("Must provide y input or use kv_cache to enable streaming decoding")
-                if not quantized:
+                if not attends:
                     k, v = self.kv_cache.k_cache[:b], self.kv_cache.v_cache[:b]
             else:
                 s_y = y.shape[1]
@@ -173,7 +211,7 @@ class MultiHeadAttention(nn.Module):
                     k = self.pos_embeddings(k, input_pos=input_pos)
                 if self.k_norm is not None and not self.qk_norm_before_rope:
                     k = self.k_norm(k)
-                if quantized:
+                if attends:
                     self.kv_cache.append(k, v)
                 elif self.kv_cache is not None and self.cache_enabled:
                     k, v = self.kv_cache.update(k, v)
@@ -184,7 +222,7 @@ class MultiHeadAttention(nn.Module):
         if cp is not None and plain:  # sequence-sharded activations: whole sequences for a subset of heads inside attention
             q, k, v = cp.seq_to_heads(q), cp.seq_to_heads(k), cp.seq_to_heads(v)
         how = dict(scale=self.scale, softcap=self.softcap, dropout_p=self.attn_dropout if self.training else 0.0)
-        out = self.kv_cache.attend(q, attn_mask, **how) if quantized else ops.attention(q, k, v, attn_mask, **how)
+        out = self.kv_cache.attend(q, attn_mask, **how) if attends else ops.attention(q, k, v, attn_mask, **how)
         if cp is not None and plain:
             out = cp.heads_to_seq(out)
         out = out.reshape(b, s_x, self.num_heads * self.head_dim)

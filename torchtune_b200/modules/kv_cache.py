@@ -139,6 +139,78 @@ class QuantizedKVCache(KVCache):
         return ops.quantized_read(*self.rows(k_val.shape[0]), dtype=k_val.dtype)
 
 
+class PromptGroups:
+    """Several rows (answers) to each of some prompts, in step: how many tokens the rows hold, and the prompts' first real slots.  The caches of all layers share one, and whoever runs the model
+    moves it on (:meth:`advance`) once per step; its numbers lie on the device, so that a recorded step reads those of its replay."""
+
+    def __init__(self, starts: torch.Tensor, rows: int) -> None:
+        self.starts = starts.to(torch.int32).contiguous()
+        self.prompts, self.rows = starts.shape[0], rows
+        self.lengths = torch.zeros(rows, dtype=torch.int32, device=starts.device)  # tokens of a row, the one of the step at hand included
+        self.slot = torch.zeros(1, dtype=torch.int64, device=starts.device)  # of the step at hand
+        self.answering = False  # False while the prompts are read
+
+    def begin(self) -> None:
+        """The prompts are read; the rows' first token comes next."""
+        self.answering = True
+        self.lengths.fill_(1)
+        self.slot.zero_()
+
+    def advance(self) -> None:
+        self.lengths.add_(1)
+        self.slot.add_(1)
+
+
+class SharedPrefixKVCache(nn.Module):
+    """Keys and values of prompts, held once, and of the rows that answer them: ``rows // prompts`` consecutive rows to a prompt.  While the prompts are read the batch is one row per prompt and the
+    mask is the prompts' own; after :meth:`PromptGroups.begin` it is all rows, one token per step, and attention goes over the prompt's real tokens and the row's own
+    (:func:`torchtune_b200.ops.shared_prefix_attention`)."""
+
+    def __init__(self, groups: PromptGroups, prompt_len: int, max_new_tokens: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype) -> None:
+        super().__init__()
+        self.groups = groups
+        self.max_seq_len = max_new_tokens
+        for name, (batch, slots) in (("prompt", (groups.prompts, prompt_len)), ("own", (groups.rows, max_new_tokens))):
+            for kv in "kv":
+                self.register_buffer(f"{name}_{kv}", torch.zeros(batch, slots, num_kv_heads, head_dim, dtype=dtype, device=groups.starts.device), persistent=False)
+
+    @property
+    def k_cache(self) -> torch.Tensor:
+        return self.own_k if self.groups.answering else self.prompt_k
+
+    @property
+    def v_cache(self) -> torch.Tensor:
+        return self.own_v if self.groups.answering else self.prompt_v
+
+    def reserve(self, bsz: int, seq_len: int) -> torch.Tensor:
+        groups = self.groups
+        if not groups.answering:
+            if bsz != groups.prompts or seq_len != self.prompt_k.shape[1]:
+                raise ValueError(f"the prompts are {groups.prompts} rows of {self.prompt_k.shape[1]} tokens, read at once, not {bsz} of {seq_len}")
+            return torch.arange(seq_len, device=groups.slot.device)
+        if bsz != groups.rows or seq_len != 1:
+            raise ValueError(f"{groups.rows} rows answer one token at a time, not {bsz} rows of {seq_len}")
+        return groups.slot
+
+    def advance(self, seq_len: int) -> None:
+        """All layers move on together (:meth:`PromptGroups.advance`)."""
+
+    def append(self, k_val: torch.Tensor, v_val: torch.Tensor) -> None:
+        slots = self.reserve(*k_val.shape[:2])
+        self.k_cache.index_copy_(1, slots, k_val)
+        self.v_cache.index_copy_(1, slots, v_val)
+
+    def attend(self, q: torch.Tensor, mask: ops.AttentionMask, *, scale: Optional[float] = None, softcap: float = 0.0, dropout_p: float = 0.0) -> torch.Tensor:
+        """Attention of ``q`` ``[b, s, n, d]``: over the prompts with their mask, then over prompts and rows, where the mask is causal and nothing else."""
+        if not self.groups.answering:
+            return ops.attention(q, self.prompt_k, self.prompt_v, mask, scale=scale, softcap=softcap, dropout_p=dropout_p)
+        plain = mask.causal and mask.bool_mask is None and mask.doc_ids is None and mask.key_start is None and mask.chunk == 0 and mask.window == 0
+        if softcap > 0.0 or dropout_p != 0.0 or not plain:
+            raise ValueError("rows that share a prompt see it and their own tokens: no other mask, soft cap or dropout")
+        g = self.groups
+        return ops.shared_prefix_attention(q, self.prompt_k, self.prompt_v, self.own_k, self.own_v, prefix_start=g.starts, lengths=g.lengths, scale=scale)
+
+
 @contextmanager
 def counted_appends(caches: Sequence[KVCache]) -> Iterator[None]:
     """Asks the device once how many tokens the caches hold and counts their appends on the host until the block is left, for a caller that alone writes

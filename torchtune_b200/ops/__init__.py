@@ -401,6 +401,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gain: Optional[torch.Tensor
     with gains' gradients).  ``input_pos``: ``[b, s]``, ``[s]``, or ``[b]`` for one token per row; the angles are constants.  On a CUDA device a position that the table does not have counts as
     an index violation and position 0 stands in; elsewhere it is an error."""
     qk_norm.check_arguments(q, k, (q_gain, k_gain), cache)
+    if cache.dtype in (torch.bfloat16, torch.float16):  # of a model that was converted as a whole
+        cache = cache.float()
     b, s = q.shape[:2]
     pos = qk_norm.positions(input_pos, b, s, cache.shape[0])
     if pos is not None and pos.device != q.device:
@@ -420,6 +422,8 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_gai
     launch.  No gradient flows through a cache: calls that would be differentiated are refused.  On a CUDA device a slot outside the cache counts as an index violation and nothing is written
     for it; elsewhere it is an error."""
     qk_norm.check_arguments(q, k, (q_gain, k_gain), cache)
+    if cache.dtype in (torch.bfloat16, torch.float16):  # of a model that was converted as a whole
+        cache = cache.float()
     b, s = q.shape[:2]
     pos = qk_norm.positions(input_pos, b, s, cache.shape[0])
     if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:

@@ -5,6 +5,7 @@ from .sequence_processing import (
     batched_logits_to_logprobs,
     get_batch_log_probs,
     logits_to_logprobs,
+    logits_to_statistics,
     truncate_sequence_at_first_stop_token,
     truncate_sequence_for_logprobs,
 )
@@ -25,6 +26,7 @@ __all__ = [
     "batched_logits_to_logprobs",
     "get_batch_log_probs",
     "logits_to_logprobs",
+    "logits_to_statistics",
     "truncate_sequence_at_first_stop_token",
     "truncate_sequence_for_logprobs",
 ]

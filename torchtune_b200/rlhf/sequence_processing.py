@@ -30,6 +30,14 @@ def logits_to_logprobs(logits: torch.Tensor, sequences: torch.Tensor, temperatur
     return torch.gather(F.log_softmax(logits / temperature, dim=-1), 2, sequences.unsqueeze(-1)).squeeze(-1)
 
 
+def logits_to_statistics(logits: torch.Tensor, sequences: torch.Tensor, temperature: float = 1.0, top: int = 0):
+    """:func:`logits_to_logprobs` with the entropy of every position's distribution and, with ``top``, the likeliest tokens: a :class:`torchtune_b200.ops.TokenStatistics` in fp32, differentiable in
+    ``logits``, from one pass over them."""
+    from .. import ops
+
+    return ops.token_statistics(logits, sequences, temperature=temperature, top=top)
+
+
 def batched_logits_to_logprobs(logits: torch.Tensor, sequences: torch.Tensor, temperature: float = 1.0, chunk_size: int = 1) -> torch.Tensor:
     """Same as :func:`logits_to_logprobs`, processed ``chunk_size`` rows at a time to bound memory."""
     out = torch.empty(sequences.shape, dtype=torch.float32, device=logits.device)
