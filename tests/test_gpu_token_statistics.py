@@ -107,6 +107,22 @@ def test_masked_and_non_finite_logits():
     assert g.isfinite().all() and not g[0, 3:].any() and not g[4, :4096].any()
 
 
+def test_gradients_of_rows_that_are_not_finite():
+    """NaN reaches the gradient of a row with any weight; a row without weight (padding, say) has zeros."""
+    x = _logits(6, 3000)
+    x[0, 17], x[1] = float("nan"), -INF
+    x[2, 5] = INF
+    x[3, 99] = float("nan")
+    leaf = x.requires_grad_()
+    s = ops.token_statistics(leaf, torch.tensor([1, 2, 3, -100, 4, -100], device=DEV), top=3)
+    for weight in (torch.ones(6, device=DEV), torch.zeros(6, device=DEV)):
+        (g,) = torch.autograd.grad(s.logprobs, leaf, weight, retain_graph=True)
+        assert not g[3].any() and not g[5].any() and g[4].isfinite().all()
+        assert bool(weight.any()) == bool(g[:3].isnan().all()) == bool(g[4].any()) and (bool(weight.any()) or not g.any())
+    (g,) = torch.autograd.grad(s.top_logprobs, leaf, torch.tensor([1.0, -1.0, 0.0], device=DEV).expand(6, 3))  # weights that add up to 0
+    assert g[:4].isnan().all() and g[4:].isfinite().all() and g[4:].any(1).all()
+
+
 def test_layouts():
     """Slices of a batch are read where they are; other layouts are copied; gradients have the logits' shape."""
     whole = _logits(3, 40, 1003)

@@ -100,6 +100,11 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 __device__ __forceinline__ float warp_max_nan(float x) {
   float d;
   asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(x));
@@ -696,20 +701,29 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const __grid_cons
   const bool counts = token != p.ignore && token >= 0 && token < p.vocab;
   const float base = p.stats[2ll * r], log_s = p.stats[2ll * r + 1];
   const float g = p.g != nullptr && counts ? p.g[r] : 0.f, h = p.h != nullptr ? p.h[r] : 0.f;
-  float all = g;
+  float all = g, any = fabsf(g) + fabsf(h);
   if (p.k != nullptr)
-    for (int i = 0; i < p.top; ++i) all += p.k[static_cast<long long>(r) * p.top + i];
+    for (int i = 0; i < p.top; ++i) {
+      const float k = p.k[static_cast<long long>(r) * p.top + i];
+      all += k, any += fabsf(k);
+    }
+  const bool none = any == 0.f;  // zeros then, whatever the logits are; else what is NaN in a row reaches its gradient
   // -p (all + h (H + ln2 q)) / T with q = log2 p
   const float offset = -(all + (h != 0.f ? h * p.entropy[r] : 0.f)) * p.rate, slope = -h * kLn2 * p.rate;
   const uint64_t base2 = pack_f32x2(-base, -base), c2 = pack_f32x2(p.c, p.c), log2s = pack_f32x2(-log_s, -log_s), offset2 = pack_f32x2(offset, offset), slope2 = pack_f32x2(slope, slope);
   auto two = [&](float x0, float x1, float& d0, float& d1) {
     float q0, q1;
     unpack_f32x2(fma_f32x2(add_f32x2(pack_f32x2(x0, x1), base2), c2, log2s), q0, q1);
-    q0 = fmaxf(q0, kLowest), q1 = fmaxf(q1, kLowest);
+    q0 = max_nan(q0, kLowest), q1 = max_nan(q1, kLowest);
     unpack_f32x2(mul_f32x2(pack_f32x2(fast_exp2(q0), fast_exp2(q1)), fma_f32x2(slope2, pack_f32x2(q0, q1), offset2)), d0, d1);
   };
   auto eight = [&](const typename Row<T>::Vector& x) {
     typename Row<T>::Vector d;
+    if (none) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d.v[i] = narrowed<T>(0.f);
+      return d;
+    }
     float f[8];
     widen8(x, f);
 #pragma unroll
@@ -748,7 +762,7 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const __grid_cons
   // the token and the alternatives again, with what is theirs; of two equal ones both write the same
   const int targets = (p.k != nullptr ? p.top : 0) + 1;
   __syncthreads();
-  if (static_cast<int>(threadIdx.x) < targets) {
+  if (!none && static_cast<int>(threadIdx.x) < targets) {
     const long long* best = p.top_tokens + static_cast<long long>(r) * p.top;
     const float* of_best = p.k + static_cast<long long>(r) * p.top;
     const long long mine = threadIdx.x == 0 ? (counts ? token : -1) : best[threadIdx.x - 1];
