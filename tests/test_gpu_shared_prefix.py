@@ -132,6 +132,13 @@ def test_what_has_no_kernel():
     torch.testing.assert_close(ops.shared_prefix_attention(*wide), reference.shared_prefix_attention(*(t.double() for t in wide), None, None, None, None).float(), rtol=1e-5, atol=1e-5)
 
 
+def test_sizes_beyond_the_kernels_indices():
+    with pytest.raises(ops.KernelFallbackError):
+        ops.shared_prefix_attention(*_inputs(1, 1, 1, 3, 2, 257, 257, 64))
+    with pytest.raises(ops.KernelFallbackError):
+        ops.shared_prefix_attention(*_inputs(1, 5, 1, 3, 2, 30011, 1, 64))
+
+
 def test_streams_recordings_and_lengths_that_move_on():
     t = _inputs(2, 8, 1, 400, 200, 8, 2, 128)
     lengths = _int([1] * 8)

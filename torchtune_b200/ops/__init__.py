@@ -397,7 +397,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: torch.
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: Optional[torch.Tensor], cache: torch.Tensor, input_pos: Optional[torch.Tensor] = None, *,
                  eps: float = 1e-6, interleaved: bool = True, norm_first: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
     """RMS norm of every head of ``q`` and ``k`` ``[b, s, heads, d]``, times a gain ``[d]`` each (``None``: none), and :func:`rope`, in that order or (``norm_first=False``) the other way round, with
-    one rounding at the end where the two operators of their own make two.  One launch forward for CUDA tensors in bf16, fp16 or fp32 with ``d`` a multiple of 16 up to 512, and one backward (two
+    one rounding at the end where the two operators of their own make two.  ``cache``: fp32 (angles in 16 bits are widened by a copy, per call).  One launch forward for CUDA tensors in bf16, fp16 or fp32 with ``d`` a multiple of 16 up to 512, and one backward (two
     with gains' gradients).  ``input_pos``: ``[b, s]``, ``[s]``, or ``[b]`` for one token per row; the angles are constants.  On a CUDA device a position that the table does not have counts as
     an index violation and position 0 stands in; elsewhere it is an error."""
     qk_norm.check_arguments(q, k, (q_gain, k_gain), cache)
@@ -598,8 +598,8 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
         return torch.empty_like(q)
     if _native(q):
         index = tuple(t for t in (prefix_start, prefix_stop, lengths) if t is not None)
-        if q.shape[3] not in shared_prefix.HEAD_DIMS:
-            _fallback("shared_prefix_attention", f"head dimension {q.shape[3]}", q)
+        if not shared_prefix.suits(q, k, k_prefix.shape[0]):
+            _fallback("shared_prefix_attention", f"{q.shape[2]} query and {k.shape[2]} key heads of {q.shape[3]} channels", q)
         elif _differentiated(q, k_prefix, v_prefix, k, v):
             _fallback("shared_prefix_attention", "gradients", q)
         elif not _has_memory(q, k_prefix, v_prefix, k, v, *index):
@@ -671,7 +671,7 @@ def token_statistics(logits: torch.Tensor, tokens: torch.Tensor, *, temperature:
     likeliest tokens with their log-probabilities, the largest logits first and of equal ones those of the lower index (NaN counts as largest).  CUDA logits in bf16, fp16 or fp32, of any width and
     row pitch, are read once, and once more for the gradient of all three.  A token equal to ``ignore_index`` has log-probability 0 without a gradient (its row's entropy and alternatives are
     still those of the row); so, counted as an index violation, has one outside the vocabulary on a CUDA device; elsewhere that is an error.  Infinitely low logits have probability 0 and no share
-    in the entropy; a row of nothing else, or one with a NaN or an infinitely high logit, has NaN for both."""
+    in the entropy; a row of nothing else, or one with a NaN or an infinitely high logit, has NaN for both and, on a CUDA device unless all its gradients are 0, in its logits' gradient."""
     token_stats.check_arguments(logits, tokens, temperature, top)
     if cuda_ops_enabled(logits) and _has_memory(logits, tokens) and token_stats.suits(logits, top) and torch.autograd.forward_ad._current_level < 0 and tokens.numel() > 0:
         return token_stats.token_statistics(logits, tokens, float(temperature), int(top), int(ignore_index), _differentiated(logits))

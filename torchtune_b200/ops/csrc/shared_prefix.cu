@@ -173,7 +173,8 @@ __device__ __forceinline__ void find_share(const Params& p, const int (&mine)[2]
     if (from >= static_cast<long long>(before[which]) * p.hkv && from < static_cast<long long>(before[which] + mine[which]) * p.hkv) {  // in this thread's run
       long long at_owner = static_cast<long long>(before[which]) * p.hkv;
       int owner = t * (which ? run_o : run_p), tiles = key_tiles(p, share.prefix, owner);
-      while (from >= at_owner + static_cast<long long>(tiles) * p.hkv) at_owner += static_cast<long long>(tiles) * p.hkv, tiles = key_tiles(p, share.prefix, ++owner);
+      const int owners = which ? p.rows : p.prompts;
+      while (owner + 1 < owners && from >= at_owner + static_cast<long long>(tiles) * p.hkv) at_owner += static_cast<long long>(tiles) * p.hkv, tiles = key_tiles(p, share.prefix, ++owner);
       const int in = static_cast<int>(from - at_owner);  // below 2^24 tiles times 256 heads, at most 2^31 - 1 by the check of sizes
       found[0] = owner, found[1] = in / tiles, found[2] = in % tiles;
     }
@@ -596,6 +597,7 @@ static int plan_of(const Call& c, Params& p, long long& rows, long long& head_fl
   p.prompts = static_cast<int>(c.prompts), p.rows = static_cast<int>(c.rows), p.s = static_cast<int>(c.s), p.hq = static_cast<int>(c.hq), p.hkv = static_cast<int>(c.hkv);
   p.group = p.hq / p.hkv, p.prefix = static_cast<int>(c.prefix), p.own = static_cast<int>(c.own);
   p.per_group = p.group == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + p.group - 1) / p.group);
+  if (c.rows / c.prompts * c.s * p.group * p.group > 0xffffffffll) return kErrTooLarge;
   p.rows_p = static_cast<int>(c.rows / c.prompts * c.s * p.group), p.rows_o = static_cast<int>(c.s * p.group);
   const long long np = (c.prefix + kKeys - 1) / kKeys, no = (c.own + kKeys - 1) / kKeys;  // tiles of keys
   const long long most = c.prompts * c.hkv * np * tiles_of(p.rows_p) + c.rows * c.hkv * no * tiles_of(p.rows_o);

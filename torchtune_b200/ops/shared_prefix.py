@@ -30,6 +30,13 @@ def check_arguments(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, leng
             raise ValueError(f"{name} is int32 of [{n}] on {q.device}, not {t.dtype} of {tuple(t.shape)} on {t.device}")
 
 
+def suits(q: torch.Tensor, k: torch.Tensor, prompts: int) -> bool:
+    """Whether the kernels have these sizes: query rows are numbered in 32 bits, and their tokens are found by a multiplication that is exact below 2^32 over the query heads of a key head."""
+    rows, s, hq, d = q.shape
+    group = hq // k.shape[2]
+    return d in HEAD_DIMS and k.shape[2] <= 256 and rows * s * hq < 2**31 and rows // prompts * s * group * group < 2**32
+
+
 def _steady(t: torch.Tensor) -> torch.Tensor:
     """``t``, if copies of tiles of one head can read it where it is, or a copy."""
     if t.is_contiguous():
