@@ -307,35 +307,64 @@ __device__ __forceinline__ void rank(const Entry* list, int count, int want, Ent
   }
   __syncwarp();
 }
-__device__ __forceinline__ void append(Entry* list, int* count, Entry e) {  // as far as there is room
-  const int at = atomicAdd(count, 1);
-  if (at < kMostCandidates) list[at] = e;
+// Entries go to the list's next places, as far as there is room, those of lower lanes first; by a whole warp.
+__device__ __forceinline__ void append(Entry* list, int& count, bool mine, Entry e) {
+  const uint32_t all = __ballot_sync(0xffffffffu, mine);
+  const int at = count + __popc(all & ((1u << (threadIdx.x & 31)) - 1));
+  if (mine && at < kMostCandidates) list[at] = e;
+  count += __popc(all);
 }
-// The `want` (up to 32) largest of n keys, of equal ones the first, with their places as indices and in order, to `to`; false, if there are too many candidates.  At least `want` keys reach the want-th
-// largest of the lanes' maxima, and hardly more than twice as many if keys are in no order.  *count is 0.
-__device__ __forceinline__ bool choose_few(const uint32_t* keys, int n, int want, Entry* list, int* count, Entry* to) {
-  const int lane = threadIdx.x & 31;
-  uint32_t most = 0;
-#pragma unroll 4
-  for (int i = lane; i < n; i += 32) most = max(most, keys[i]);
-  int above = 0;
-#pragma unroll
+// The `want` (up to 64) largest of n > want values, of equal ones the first, with their places as indices and in order, to `to`; false, if there are too many candidates.  Values, which lie on 16 bytes
+// with room up to the next multiple of 128, become keys where they are.  At least `want` keys reach the want-th largest of the maxima of 32 or 64 sets, and hardly more than twice as many if keys
+// are in no order.  One warp does this alone, so that its time is that of what waits for what: it takes four keys at a time.
+template <typename T>
+__device__ __forceinline__ bool choose_few(uint32_t* keys, int n, int want, Entry* list, Entry* to) {
+  const int lane = threadIdx.x & 31, groups = (n + 127) / 128;
+  uint4* fours = reinterpret_cast<uint4*>(keys) + lane;
+  uint32_t most[2] = {0, 0};
+#pragma unroll 1
+  for (int g = 0; g < groups; ++g) {
+    uint4 k = fours[g * 32];
+    const int left = n - g * 128 - lane * 4;
+    k.x = left > 0 ? key_of<T>(__uint_as_float(k.x)) : 0u, k.y = left > 1 ? key_of<T>(__uint_as_float(k.y)) : 0u;
+    k.z = left > 2 ? key_of<T>(__uint_as_float(k.z)) : 0u, k.w = left > 3 ? key_of<T>(__uint_as_float(k.w)) : 0u;
+    fours[g * 32] = k;
+    most[0] = max(most[0], max(k.x, k.y)), most[1] = max(most[1], max(k.z, k.w));
+  }
+  const bool two = want > 12;  // 64 sets leave fewer candidates than 32; to rank them takes twice as long
+  if (!two) most[0] = max(most[0], most[1]);
+  int above[2] = {0, 0};
+#pragma unroll 8
   for (int x = 0; x < 32; ++x) {
-    const uint32_t other = __shfl_sync(0xffffffffu, most, x);
-    above += (other > most) | ((other == most) & (x < lane));
+    const uint32_t other = __shfl_sync(0xffffffffu, most[0], x);
+    above[0] += (other > most[0]) | ((other == most[0]) & (x < lane));
+    if (two) {
+      const uint32_t second = __shfl_sync(0xffffffffu, most[1], x);
+      above[0] += second > most[0];
+      above[1] += (other >= most[1]) + ((second > most[1]) | ((second == most[1]) & (x < lane)));
+    }
   }
-  const uint32_t least = __shfl_sync(0xffffffffu, most, __ffs(__ballot_sync(0xffffffffu, above == want - 1)) - 1);
-#pragma unroll 4
-  for (int i = lane; i < n; i += 32) {
-    const uint32_t key = keys[i];
-    if (key >= least) append(list, count, entry_of(key, i));
+  const uint32_t first = __ballot_sync(0xffffffffu, above[0] == want - 1), other = __ballot_sync(0xffffffffu, two && above[1] == want - 1);
+  const uint32_t least = max(1u, __shfl_sync(0xffffffffu, first != 0 ? most[0] : most[1], __ffs(first | other) - 1));  // of few keys, sets may be empty
+  const uint32_t below = (1u << lane) - 1;
+  int found = 0;
+#pragma unroll 1
+  for (int g = 0; g < groups; ++g) {
+    const uint4 four = fours[g * 32];
+    const uint32_t k[4] = {four.x, four.y, four.z, four.w};
+    uint32_t all[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) all[c] = __ballot_sync(0xffffffffu, k[c] >= least);
+    if ((all[0] | all[1] | all[2] | all[3]) == 0) continue;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int at = found + __popc(all[c] & below);
+      if (k[c] >= least && at < kMostCandidates) list[at] = entry_of(k[c], g * 128 + lane * 4 + c);
+      found += __popc(all[c]);
+    }
   }
   __syncwarp();
-  const int found = *static_cast<volatile int*>(count);
-  __syncwarp();
-  if (lane == 0) *count = 0;
   if (found <= kMostCandidates) rank(list, found, want, to);
-  __syncwarp();
   return found <= kMostCandidates;
 }
 
@@ -392,29 +421,91 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
       for (int k = 0; k < 8; ++k) key[k] = j < part.end ? row.key(e + k) : 0u;
     }
   };
+  // The elements of two vectors, the first of which are elements e[0] and e[1], that reach the least; `count`: entries so far, if there is one warp.  Two at a time, since one warp waits for most of
+  // its instructions.
+  [[maybe_unused]] auto gather_from = [&](const typename Row<T>::Vector& raw0, const typename Row<T>::Vector& raw1, const int (&e)[2], float least, int& count) {
+    if constexpr (TOP) {
+    float f[2][8];
+    widen8(raw0, f[0]), widen8(raw1, f[1]);
+    uint32_t mine = 0;
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      uint32_t bit[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) bit[k] = f[y][k] < least ? 0u : 1u << k;  // NaN is among them
+      uint32_t m = ((bit[0] | bit[1]) | (bit[2] | bit[3])) | ((bit[4] | bit[5]) | (bit[6] | bit[7]));
+      if (e[y] < 0) m &= 0xffu << -e[y];
+      if (e[y] > p.vocab - 8) m &= e[y] < p.vocab ? 0xffu >> (e[y] + 8 - p.vocab) : 0u;
+      mine |= m << 8 * y;
+    }
+    for (uint32_t all; (all = __ballot_sync(0xffffffffu, mine != 0)) != 0; mine &= mine - 1) {
+      const int k = __ffs(mine) - 1;
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = k & 8 ? f[1][i] : f[0][i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = k & 4 ? x[i + 4] : x[i];
+      x[0] = k & 2 ? x[2] : x[0], x[1] = k & 2 ? x[3] : x[1];
+      const Entry entry = entry_of(key_of<T>(k & 1 ? x[1] : x[0]), (k & 8 ? e[1] : e[0]) + (k & 7));
+      if (splits > 1) {  // warps share the list
+        count = lane == 0 ? atomicAdd(&sh.count, __popc(all)) : 0;
+        count = __shfl_sync(0xffffffffu, count, 0);
+      }
+      const int at = count + __popc(all & ((1u << lane) - 1));
+      if (mine != 0 && at < kMostCandidates) sh.candidates[at] = entry;
+      count += __popc(all);
+    }
+    }
+  };
   // The elements of the segments that were found which reach the least of their maxima; by one warp, or by all, `member` of which this is
   [[maybe_unused]] auto gather = [&](const Row<T>& row, const Part& part, int member) {
     if constexpr (TOP) {
-    const uint32_t least = key_in(sh.found[p.top - 1]);
-    const int members = splits > 1 ? kWarps + 1 : 1;
-    for (int i0 = member; i0 < p.top; i0 += 4 * members) {
-      uint32_t key[4][8];
+    const float least = value_of<T>(key_in(sh.found[p.top - 1]));
+    int count = 0;
+    if (splits > 1) {
+#pragma unroll 1
+      for (int i0 = member; i0 < p.top; i0 += 2 * (kWarps + 1)) {
+        typename Row<T>::Vector raw[2];
+        int e[2];
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (i0 + x * members < p.top) keys_of(row, part, part.first + index_in(sh.found[i0 + x * members]) * 32 + lane, key[x]);
+        for (int y = 0; y < 2; ++y) {
+          const int i = i0 + y * (kWarps + 1), j = i < p.top ? part.first + index_in(sh.found[i]) * 32 + lane : part.end;
+          e[y] = j < part.end ? j * 8 - row.off : p.vocab;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        if (i0 + x * members >= p.top) break;
-        const int e = (part.first + index_in(sh.found[i0 + x * members]) * 32 + lane) * 8 - row.off;
-        uint32_t most = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) most = max(most, key[x][k]);
-        if (most >= least) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (key[x][k] >= least) append(sh.candidates, &sh.count, entry_of(key[x][k], e + k));
+          for (int k = 0; k < 8; ++k) raw[y].v[k] = narrowed<T>(-INFINITY);
+          if (j < part.end) raw[y] = row.load(j);
         }
+        gather_from(raw[0], raw[1], e, least, count);
       }
+    } else {
+      // a ring of pairs of segments: every lane copies its vectors and reads them, so that no other lane has to be waited for
+      constexpr int kPairs = 4, kVectorBytes = 8 * sizeof(T);
+      static_assert(kPairs * 64 * kVectorBytes <= sizeof(sh.lanes), "the ring lies where lanes do");
+      uint8_t* ring = reinterpret_cast<uint8_t*>(sh.lanes) + lane * kVectorBytes;
+      const int pairs = (p.top + 1) / 2;
+      auto first_of = [&](int i) { return i < p.top ? (part.first + index_in(sh.found[i]) * 32 + lane) * 8 - row.off : p.vocab; };  // element; vocabularies with alternatives are below 2^21
+#pragma unroll 1
+      for (int i = 0; i < pairs + kPairs - 1; ++i) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int e = i < pairs ? first_of(2 * i + y) : p.vocab;
+          uint8_t* to = ring + ((i % kPairs) * 2 + y) * 32 * kVectorBytes;
+          if (e >= 0 && e <= p.vocab - 8) {
+#pragma unroll
+            for (int x = 0; x < kVectorBytes / 16; ++x) copy16(smem_u32(to) + x * 16, reinterpret_cast<const uint4*>(row.x + e) + x);
+          } else if (e < p.vocab) {
+#pragma unroll 1
+            for (int k = 0; k < 8; ++k) reinterpret_cast<T*>(to)[k] = e + k >= 0 && e + k < p.vocab ? row.x[e + k] : narrowed<T>(-INFINITY);
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (i < kPairs - 1) continue;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kPairs - 1) : "memory");
+        const int at = i - (kPairs - 1), e[2] = {first_of(2 * at), first_of(2 * at + 1)};
+        const auto* from = reinterpret_cast<const typename Row<T>::Vector*>(ring + (at % kPairs) * 64 * kVectorBytes);
+        gather_from(Row<T>::whole(from), Row<T>::whole(from + 32), e, least, count);
+      }
+      if (lane == 0) sh.count = count;
     }
     __syncwarp();
     }
@@ -560,9 +651,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
   // ------------------------------------------------------------------------------------------------ the warp that ends rows
   auto choose_segments = [&](const Part& part, uint32_t* segments) {  // sh.few: whether it went without a search
     if constexpr (TOP) {
-    for (int i = lane; i < part.segments; i += 32) segments[i] = key_of<T>(__uint_as_float(segments[i]));
+    const bool few = part.segments > p.top && choose_few<T>(segments, part.segments, p.top, sh.candidates, sh.found);
+    if (part.segments <= p.top)
+      for (int i = lane; i < part.segments; i += 32) segments[i] = key_of<T>(__uint_as_float(segments[i]));
     __syncwarp();
-    const bool few = p.top <= 32 && part.segments > p.top && choose_few(segments, part.segments, p.top, sh.candidates, &sh.count, sh.found);
     if (lane == 0) sh.few = few;
     __syncwarp();
     }
@@ -625,11 +717,15 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
   };
   if (splits == 1) {
     int buffer = 0;
+    auto logit_of = [&](uint32_t r, long long token) { return token >= 0 && token < p.vocab ? widened(row_of(r).x[token]) : 0.f; };
+    long long next_token = p.tokens[blockIdx.x];  // a row ahead
+    float next_logit = logit_of(blockIdx.x, next_token);
     for (uint32_t r = blockIdx.x; r < rows; r += step, buffer ^= 1) {
       const Row<T> row = row_of(r);
-      const long long token = p.tokens[r];
-      const float logit = token >= 0 && token < p.vocab ? widened(row.x[token]) : 0.f;
+      const long long token = next_token;
+      const float logit = next_logit;
       wait_at(1 + buffer);
+      if (r + step < rows) next_token = p.tokens[r + step];
       const Sums sum = sum_of(buffer);
       if constexpr (TOP) {
         const Part part = part_of(row);
@@ -639,6 +735,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
       }
       __syncwarp();
       if (r + 2 * step < rows) arrive_at(3 + buffer);
+      if (r + step < rows) next_logit = logit_of(r + step, next_token);
       finish(r, token, logit, sum);
     }
     return;
@@ -666,12 +763,11 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
   if constexpr (TOP) {
     uint32_t least = 1;  // a part with as many entries has nothing lower to give
     for (int i = 0; i < splits; ++i) least = max(least, key_in(sh.entries[i][p.top - 1]));
-    for (int i = lane; i < splits * kMaxTop; i += 32) {
+    int count = 0;
+    for (int i = lane; i < splits * kMaxTop; i += 32) {  // kMaxTop is a multiple of 32
       const Entry e = i % kMaxTop < p.top ? sh.entries[i / kMaxTop][i % kMaxTop] : 0;
-      if (key_in(e) >= least) append(sh.candidates, &sh.count, e);
+      append(sh.candidates, count, key_in(e) >= least, e);
     }
-    __syncwarp();
-    const int count = *static_cast<volatile int*>(&sh.count);
     __syncwarp();
     rank(sh.candidates, count, p.top, sh.entries[0]);
   }
