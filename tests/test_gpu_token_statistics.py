@@ -80,6 +80,37 @@ def test_alternatives_whatever_the_order(order):
         assert s.top_tokens[0].tolist() == torch.sort(x, descending=True, stable=True).indices[:64].tolist()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,v,top", [(3, 700, 7), (700, 1, 1), (700, 33, 32), (700, 255, 0), (700, 1026, 12), (700, 2049, 64), (700, 8200, 33), (611, 8001, 20), (2000, 32003, 5), (4736 + 13, 900, 3)])
+def test_many_short_rows(rows, v, top, dtype):
+    logits, tokens = _logits(rows, v, dtype=dtype), torch.randint(0, v, (rows,), device=DEV)
+    tokens[::7] = -100
+    _check(logits, tokens, 0.8, top)
+
+
+@pytest.mark.parametrize("order", ["up", "down", "equal", "blocks"])
+def test_alternatives_of_many_short_rows_whatever_the_order(order):
+    for v in (200, 3000, 9000):
+        x = torch.arange(v, device=DEV, dtype=torch.float32) / 1000
+        x = {"up": x, "down": x.flip(0), "equal": torch.zeros_like(x), "blocks": (torch.arange(v, device=DEV) // 300 % 7).float()}[order]
+        for top in (3, 32, 64):
+            s = _check(x.expand(400, v).contiguous(), torch.zeros(400, dtype=torch.int64, device=DEV), top=top, grads=False)
+            assert torch.equal(s.top_tokens, torch.sort(x, descending=True, stable=True).indices[:top].expand(400, top))
+
+
+def test_short_rows_that_are_not_finite():
+    x = _logits(640, 3000, dtype=torch.float32)
+    x[0, 3:], x[1], x[2, 17], x[3, 2001], x[4, ::2] = -INF, -INF, float("nan"), INF, -INF
+    x[5] = torch.finfo(torch.float32).min
+    tokens = torch.ones(640, dtype=torch.int64, device=DEV)
+    for top in (5, 40):
+        s = ops.token_statistics(x, tokens, top=top)
+        want = reference.token_statistics(x.double(), tokens, 1.0, top, -100)
+        assert torch.equal(s.top_tokens, want[3])
+        for a, b in zip(s[:3], want[:3]):
+            torch.testing.assert_close(a.double(), b, rtol=2e-5, atol=2e-5, equal_nan=True)
+
+
 def test_masked_and_non_finite_logits():
     v, low = 5000, torch.finfo(torch.float32).min
     x = _logits(8, v, dtype=torch.float32)

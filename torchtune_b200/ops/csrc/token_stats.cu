@@ -202,6 +202,56 @@ __device__ __forceinline__ float most_of_vector(const Vector& raw) {
 struct Sums {
   float base, s, t;
 };
+// The sums of a thread as it goes along its part.
+struct Running {
+  float c;
+  float most_allowed = -1.f, base = 0.f;  // there is no base until there is a logit above the infinitely low ones
+  uint64_t s2 = 0, t2 = 0;
+  __device__ __forceinline__ Sums sums() const {
+    float s0, s1, t0, t1;
+    unpack_f32x2(s2, s0, s1), unpack_f32x2(t2, t0, t1);
+    return {base, s0 + s1, t0 + t1};
+  }
+  __device__ __forceinline__ void careful(const float (&f)[8]) {  // moves the base, and takes what is infinitely low to have no share (0 * -inf)
+    const float most = most_of(f);
+    if (!(most <= (most_allowed < 0.f ? -INFINITY : base))) {  // NaN too
+      const float d = fminf(fmaxf((base - most) * c, kLowest), 0.f), g = fast_exp2(d);
+      const Sums now = sums();
+      s2 = pack_f32x2(now.s * g, 0.f), t2 = pack_f32x2((now.t + now.s * d) * g, 0.f);
+      base = most, most_allowed = kMostAllowed;
+    }
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float d = (f[i] - base) * c, e = fast_exp2(d);
+      s += e, t += e * (d < kLowest ? kLowest : d);
+    }
+    s2 = add_f32x2(s2, pack_f32x2(s, 0.f)), t2 = add_f32x2(t2, pack_f32x2(t, 0.f));
+  }
+  template <typename T, typename Vector>
+  __device__ __forceinline__ void take(const Vector& raw, uint64_t c2) {  // c2: c twice
+    uint64_t sv = 0, tv = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const uint64_t d = mul_f32x2(minus<T>(raw, i, base), c2);
+      float d0, d1;
+      unpack_f32x2(d, d0, d1);
+      const uint64_t e = pack_f32x2(fast_exp2(d0), fast_exp2(d1));
+      sv = i == 0 ? e : add_f32x2(sv, e);
+      tv = i == 0 ? mul_f32x2(e, d) : fma_f32x2(e, d, tv);
+    }
+    float s0, s1, t0, t1;
+    unpack_f32x2(sv, s0, s1), unpack_f32x2(tv, t0, t1);
+    const float sum = s0 + s1, t = t0 + t1;
+    if (!(sum <= most_allowed) || t != t) {
+      float f[8];
+      widen8(raw, f);
+      careful(f);
+    } else {
+      s2 = add_f32x2(s2, sv), t2 = add_f32x2(t2, tv);
+    }
+  }
+};
 // The sums of all lanes of a warp, over the highest of their bases; one without a finite logit (s = 0) has none.  NaN goes on.
 __device__ __forceinline__ Sums joined_lanes(const Sums& mine, float c) {
   float s = mine.s, t = mine.t;
@@ -318,7 +368,7 @@ __device__ __forceinline__ void append(Entry* list, int& count, bool mine, Entry
 // with room up to the next multiple of 128, become keys where they are.  At least `want` keys reach the want-th largest of the maxima of 32 or 64 sets, and hardly more than twice as many if keys
 // are in no order.  One warp does this alone, so that its time is that of what waits for what: it takes four keys at a time.
 template <typename T>
-__device__ __forceinline__ bool choose_few(uint32_t* keys, int n, int want, Entry* list, Entry* to) {
+__device__ __forceinline__ bool choose_few(uint32_t* keys, int n, int want, Entry* list, int room, Entry* to) {
   const int lane = threadIdx.x & 31, groups = (n + 127) / 128;
   uint4* fours = reinterpret_cast<uint4*>(keys) + lane;
   uint32_t most[2] = {0, 0};
@@ -359,13 +409,74 @@ __device__ __forceinline__ bool choose_few(uint32_t* keys, int n, int want, Entr
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int at = found + __popc(all[c] & below);
-      if (k[c] >= least && at < kMostCandidates) list[at] = entry_of(k[c], g * 128 + lane * 4 + c);
+      if (k[c] >= least && at < room) list[at] = entry_of(k[c], g * 128 + lane * 4 + c);
       found += __popc(all[c]);
     }
   }
   __syncwarp();
-  if (found <= kMostCandidates) rank(list, found, want, to);
-  return found <= kMostCandidates;
+  if (found <= room) rank(list, found, want, to);
+  return found <= room;
+}
+
+// The elements of two vectors, the first of which are elements e[0] and e[1], that reach the least; by one warp.  `count`: entries so far, which lie in
+// `shared_count` where warps share the list.  Two at a time, since one warp waits for most of its instructions.
+template <typename T>
+__device__ __forceinline__ void gather_from(const typename Row<T>::Vector& raw0, const typename Row<T>::Vector& raw1, const int (&e)[2], int vocab, float least, Entry* list, int room, int& count,
+                                          int* shared_count) {
+  const int lane = threadIdx.x & 31;
+  float f[2][8];
+  widen8(raw0, f[0]), widen8(raw1, f[1]);
+  uint32_t mine = 0;
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    uint32_t bit[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) bit[k] = f[y][k] < least ? 0u : 1u << k;  // NaN is among them
+    uint32_t m = ((bit[0] | bit[1]) | (bit[2] | bit[3])) | ((bit[4] | bit[5]) | (bit[6] | bit[7]));
+    if (e[y] < 0) m &= 0xffu << -e[y];
+    if (e[y] > vocab - 8) m &= e[y] < vocab ? 0xffu >> (e[y] + 8 - vocab) : 0u;
+    mine |= m << 8 * y;
+  }
+  for (uint32_t all; (all = __ballot_sync(0xffffffffu, mine != 0)) != 0; mine &= mine - 1) {
+    const int k = __ffs(mine) - 1;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = k & 8 ? f[1][i] : f[0][i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = k & 4 ? x[i + 4] : x[i];
+    x[0] = k & 2 ? x[2] : x[0], x[1] = k & 2 ? x[3] : x[1];
+    const Entry entry = entry_of(key_of<T>(k & 1 ? x[1] : x[0]), (k & 8 ? e[1] : e[0]) + (k & 7));
+    if (shared_count != nullptr) {
+      count = lane == 0 ? atomicAdd(shared_count, __popc(all)) : 0;
+      count = __shfl_sync(0xffffffffu, count, 0);
+    }
+    const int at = count + __popc(all & ((1u << lane) - 1));
+    if (mine != 0 && at < room) list[at] = entry;
+    count += __popc(all);
+  }
+}
+
+// The results of a row, by one warp, with its alternatives in order.
+template <typename T, bool TOP>
+__device__ __forceinline__ void finish(const Params& p, long long r, long long token, float logit, const Sums& sum, const Entry* entries) {
+  const int lane = threadIdx.x & 31;
+  const float log_s = log2f(sum.s);
+  if constexpr (TOP) {
+    for (int x = lane; x < p.top; x += 32) {
+      const Entry e = entries[x];
+      p.top_tokens[r * p.top + x] = index_in(e);
+      p.top_logprobs[r * p.top + x] = (value_of<T>(key_in(e)) - sum.base) * p.rate - log_s * kLn2;
+    }
+    __syncwarp();
+  }
+  if (lane == 0) {
+    float lp = 0.f;
+    if (token >= 0 && token < p.vocab) lp = (logit - sum.base) * p.rate - log_s * kLn2;
+    else if (token != p.ignore) TTB_NOTE_VIOLATION(token_stats);  // as a row that is ignored
+    p.logprobs[r] = token == p.ignore ? 0.f : lp;
+    p.entropy[r] = (log_s - sum.t / sum.s) * kLn2;
+    if (p.stats != nullptr) p.stats[2 * r] = sum.base, p.stats[2 * r + 1] = log_s;
+  }
 }
 
 struct Shared {
@@ -387,6 +498,184 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm vola
 __device__ __forceinline__ void wait_at(int barrier) { asm volatile("barrier.cta.sync %0, %1;" ::"r"(barrier), "n"(kThreads) : "memory"); }
 __device__ __forceinline__ void wait_for_all() { asm volatile("barrier.cta.sync 5, %0;" ::"n"(kThreads) : "memory"); }
 __device__ __forceinline__ void arrive_at(int barrier) { asm volatile("barrier.cta.arrive %0, %1;" ::"r"(barrier), "n"(kThreads) : "memory"); }
+
+// Many rows that are not long: a warp streams and ends rows of its own, so that the ends of some lie beside the streams of others.
+static constexpr int kOwnSegments = 256;  // of a row at most
+static constexpr int kOwnCandidates = 256;
+template <bool TOP>
+static constexpr int kOwnWarps = TOP ? 12 : 16;  // of a CTA; what the ends of rows take in shared memory leaves room for twelve
+struct OwnTop {
+  alignas(16) uint32_t segments[kOwnSegments];
+  Entry candidates[kOwnCandidates], found[kMaxTop], entries[kMaxTop];
+  uint16_t chosen[kMaxTop];
+};
+template <typename T, bool TOP>
+static constexpr int kOwnSlots = kSlots * kRun<T, TOP> * 8 * sizeof(T);
+template <typename T, bool TOP>
+static constexpr int kOwnBytes = kOwnSlots<T, TOP> + (TOP ? (sizeof(OwnTop) + 15) / 16 * 16 : 0);
+
+// The want-th largest (want <= 32) of the lanes' keys, at least 1.
+__device__ __forceinline__ uint32_t nth_of_lanes(uint32_t key, int want) {
+  const int lane = threadIdx.x & 31;
+  int above = 0;
+#pragma unroll 8
+  for (int x = 0; x < 32; ++x) {
+    const uint32_t other = __shfl_sync(0xffffffffu, key, x);
+    above += (other > key) | ((other == key) & (x < lane));
+  }
+  return max(1u, __shfl_sync(0xffffffffu, key, __ffs(__ballot_sync(0xffffffffu, above == want - 1)) - 1));
+}
+
+// The alternatives of a row, in order, from the maxima of its segments and of the lanes' elements; by one warp.
+template <typename T>
+__device__ __forceinline__ void choose_alone(const Row<T>& row, int want, float lane_most, OwnTop& sh) {
+  const int lane = threadIdx.x & 31, segments = (row.vectors() + 31) / 32;
+  const bool by_segments = segments > want;
+  bool few = true;
+  uint32_t least = 1;
+  if (by_segments) {
+    few = choose_few<T>(sh.segments, segments, want, sh.candidates, kOwnCandidates, sh.found);
+    if (few) least = key_in(sh.found[want - 1]);
+  } else {
+    for (int i = lane; i < segments; i += 32) sh.segments[i] = key_of<T>(__uint_as_float(sh.segments[i]));
+    if (want <= 32) least = nth_of_lanes(key_of<T>(lane_most), want);  // as many elements at least reach it
+    else few = row.vocab <= kOwnCandidates;
+  }
+  __syncwarp();
+  if (few) {
+    const int n = by_segments ? want : segments;
+    const float limit = least == 1 ? -INFINITY : value_of<T>(least);  // that of the lowest key is none
+    int count = 0;
+#pragma unroll 1
+    for (int i = 0; i < n; i += 2) {
+      typename Row<T>::Vector raw[2];
+      int e[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int segment = i + y >= n ? segments : by_segments ? index_in(sh.found[i + y]) : i + y;
+        e[y] = (segment * 32 + lane) * 8 - row.off;
+        raw[y] = row.load(segment * 32 + lane);
+      }
+      gather_from<T>(raw[0], raw[1], e, row.vocab, limit, sh.candidates, kOwnCandidates, count, nullptr);
+    }
+    __syncwarp();
+    if (count <= kOwnCandidates) {
+      rank(sh.candidates, count, want, sh.entries);
+      return;
+    }
+  }
+  // many equal or ordered logits: one alternative after the other
+  const int n = choose(sh.segments, segments, want, sh.chosen);
+  Entry last = ~0ull;
+  for (int x = 0; x < want; ++x) {
+    Entry best = 0;
+    for (int i = 0; i < n; ++i) {
+      const int j = sh.chosen[i] * 32 + lane;
+      const typename Row<T>::Vector raw = row.load(j);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int e = j * 8 - row.off + k;
+        const Entry entry = e >= 0 && e < row.vocab ? entry_of(key_of<T>(widened(raw.v[k])), e) : 0;
+        if (entry < last && entry > best) best = entry;
+      }
+    }
+    const uint32_t high = __reduce_max_sync(0xffffffffu, key_in(best));
+    const uint32_t low = __reduce_max_sync(0xffffffffu, key_in(best) == high ? static_cast<uint32_t>(best) : 0u);
+    last = static_cast<Entry>(high) << 32 | low;
+    if (lane == 0) sh.entries[x] = last;
+  }
+  __syncwarp();
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kOwnWarps<TOP> * 32, kCtas) row_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(16) uint8_t slots[];
+  using Vector = typename Row<T>::Vector;
+  constexpr int kMine = kEach<T, TOP>, kVectors = kRun<T, TOP>, kPieces = sizeof(T) / 2, kPieceBytes = kVectors * 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* my_slots = slots + warp * kOwnBytes<T, TOP> + lane * 16;
+  [[maybe_unused]] OwnTop& sh = *reinterpret_cast<OwnTop*>(slots + warp * kOwnBytes<T, TOP> + kOwnSlots<T, TOP>);
+  const uint32_t rows = p.rows, step = gridDim.x * kOwnWarps<TOP>, first = warp * gridDim.x + blockIdx.x;
+  auto row_of = [&](uint32_t r) {
+    const uint32_t outer = p.step_outer == 0 ? 0u : r / p.inner;
+    return Row<T>(static_cast<const T*>(p.x) + outer * p.step_outer + static_cast<long long>(r - outer * p.inner) * p.step_inner, p.vocab);
+  };
+  if (first >= rows) return;
+  uint32_t ahead_r = first;
+  Row<T> ahead_row = row_of(first);
+  int ahead_j = 0, ahead_slot = 0;
+  auto whole = [](const Row<T>& row, int j0) { return j0 >= row.whole_from() && j0 + kVectors <= row.whole_to(); };  // the same for a warp
+  auto copy_ahead = [&]() {
+    if (ahead_r < rows) {
+      if (whole(ahead_row, ahead_j)) {
+        const uint4* from = reinterpret_cast<const uint4*>(ahead_row.vector(ahead_j)) + lane;
+        const uint32_t to = smem_u32(my_slots) + ahead_slot * kPieces * kPieceBytes;
+#pragma unroll
+        for (int a = 0; a < kMine; ++a)
+#pragma unroll
+          for (int x = 0; x < kPieces; ++x) copy16(to + x * kPieceBytes + a * 512, from + (a * kPieces + x) * 32);
+      }
+      ahead_slot = ahead_slot + 1 == kSlots ? 0 : ahead_slot + 1;
+      ahead_j += kVectors;
+      if (ahead_j >= ahead_row.vectors()) {
+        ahead_r += step, ahead_j = 0;
+        if (ahead_r < rows) ahead_row = row_of(ahead_r);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  copy_ahead(), copy_ahead();
+  const uint64_t c2 = pack_f32x2(p.c, p.c);
+  int slot = 0;
+  for (uint32_t r = first; r < rows; r += step) {
+    const Row<T> row = row_of(r);
+    const int vectors = row.vectors();
+    const long long token = p.tokens[r];
+    Running run{p.c};
+    float lane_most = -INFINITY;
+    auto note = [&](int j, float most) {  // the maximum of a segment
+      if constexpr (TOP) {
+        lane_most = max_nan(lane_most, most);
+        const float m = warp_max_nan(most);
+        if (lane == 0) sh.segments[j >> 5] = __float_as_uint(m);
+      }
+    };
+    for (int j0 = 0; j0 < vectors; j0 += kVectors) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      copy_ahead();  // to the slot before this one
+      if (whole(row, j0)) {
+        const uint8_t* at = my_slots + slot * kPieces * kPieceBytes;
+#pragma unroll
+        for (int a = 0; a < kMine; ++a) {
+          Vector raw;
+#pragma unroll
+          for (int x = 0; x < kPieces; ++x) reinterpret_cast<uint4*>(raw.v)[x] = *reinterpret_cast<const uint4*>(at + x * kPieceBytes + a * 512);
+          if constexpr (TOP) note(j0 + a * 32, most_of_vector<T>(raw));
+          run.take<T>(raw, c2);
+        }
+      } else {
+#pragma unroll 1
+        for (int a = 0; a < kMine && j0 + a * 32 < vectors; ++a) {
+          float f[8];
+          widen8(row.load(j0 + a * 32 + lane), f);
+          note(j0 + a * 32, most_of(f));
+          run.careful(f);
+        }
+      }
+      slot = slot + 1 == kSlots ? 0 : slot + 1;
+    }
+    const T logit = token >= 0 && token < p.vocab ? row.x[token] : T();
+    const Sums sum = joined_lanes(run.sums(), p.c);
+    __syncwarp();
+    if constexpr (TOP) {
+      choose_alone<T>(row, p.top, lane_most, sh);
+      finish<T, TOP>(p, r, token, widened(logit), sum, sh.entries);
+    } else {
+      finish<T, TOP>(p, r, token, widened(logit), sum, nullptr);
+    }
+    __syncwarp();
+  }
+}
 
 // grid: CTAs that take rows in turn, or for few rows a cluster for each
 template <typename T, bool TOP>
@@ -421,42 +710,6 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
       for (int k = 0; k < 8; ++k) key[k] = j < part.end ? row.key(e + k) : 0u;
     }
   };
-  // The elements of two vectors, the first of which are elements e[0] and e[1], that reach the least; `count`: entries so far, if there is one warp.  Two at a time, since one warp waits for most of
-  // its instructions.
-  [[maybe_unused]] auto gather_from = [&](const typename Row<T>::Vector& raw0, const typename Row<T>::Vector& raw1, const int (&e)[2], float least, int& count) {
-    if constexpr (TOP) {
-    float f[2][8];
-    widen8(raw0, f[0]), widen8(raw1, f[1]);
-    uint32_t mine = 0;
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      uint32_t bit[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) bit[k] = f[y][k] < least ? 0u : 1u << k;  // NaN is among them
-      uint32_t m = ((bit[0] | bit[1]) | (bit[2] | bit[3])) | ((bit[4] | bit[5]) | (bit[6] | bit[7]));
-      if (e[y] < 0) m &= 0xffu << -e[y];
-      if (e[y] > p.vocab - 8) m &= e[y] < p.vocab ? 0xffu >> (e[y] + 8 - p.vocab) : 0u;
-      mine |= m << 8 * y;
-    }
-    for (uint32_t all; (all = __ballot_sync(0xffffffffu, mine != 0)) != 0; mine &= mine - 1) {
-      const int k = __ffs(mine) - 1;
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = k & 8 ? f[1][i] : f[0][i];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = k & 4 ? x[i + 4] : x[i];
-      x[0] = k & 2 ? x[2] : x[0], x[1] = k & 2 ? x[3] : x[1];
-      const Entry entry = entry_of(key_of<T>(k & 1 ? x[1] : x[0]), (k & 8 ? e[1] : e[0]) + (k & 7));
-      if (splits > 1) {  // warps share the list
-        count = lane == 0 ? atomicAdd(&sh.count, __popc(all)) : 0;
-        count = __shfl_sync(0xffffffffu, count, 0);
-      }
-      const int at = count + __popc(all & ((1u << lane) - 1));
-      if (mine != 0 && at < kMostCandidates) sh.candidates[at] = entry;
-      count += __popc(all);
-    }
-    }
-  };
   // The elements of the segments that were found which reach the least of their maxima; by one warp, or by all, `member` of which this is
   [[maybe_unused]] auto gather = [&](const Row<T>& row, const Part& part, int member) {
     if constexpr (TOP) {
@@ -475,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
           for (int k = 0; k < 8; ++k) raw[y].v[k] = narrowed<T>(-INFINITY);
           if (j < part.end) raw[y] = row.load(j);
         }
-        gather_from(raw[0], raw[1], e, least, count);
+        gather_from<T>(raw[0], raw[1], e, p.vocab, least, sh.candidates, kMostCandidates, count, &sh.count);
       }
     } else {
       // a ring of pairs of segments: every lane copies its vectors and reads them, so that no other lane has to be waited for
@@ -503,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
         asm volatile("cp.async.wait_group %0;" ::"n"(kPairs - 1) : "memory");
         const int at = i - (kPairs - 1), e[2] = {first_of(2 * at), first_of(2 * at + 1)};
         const auto* from = reinterpret_cast<const typename Row<T>::Vector*>(ring + (at % kPairs) * 64 * kVectorBytes);
-        gather_from(Row<T>::whole(from), Row<T>::whole(from + 32), e, least, count);
+        gather_from<T>(Row<T>::whole(from), Row<T>::whole(from + 32), e, p.vocab, least, sh.candidates, kMostCandidates, count, nullptr);
       }
       if (lane == 0) sh.count = count;
     }
@@ -516,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
 
   if (warp < kWarps) {
     const uint64_t c2 = pack_f32x2(p.c, p.c);
-    constexpr int kMine = kEach<T, TOP>, kPieces = sizeof(T) / 2;  // 16-byte pieces of a vector
+    constexpr int kMine = kEach<T, TOP>, kPieces = sizeof(T) / 2;  // 16-byte pieces of a vector; a lane's are 512 bytes apart, since a copy that leaves out every other piece costs as much as all
     using Vector = typename Row<T>::Vector;
     uint8_t* my_slots = slots + (warp * kRun<T, TOP> + lane) * 16;  // piece x of vector a of slot s: (s * kPieces + x) slots' pieces and a * 32 vectors further on
     constexpr int kPieceBytes = kWarps * kRun<T, TOP> * 16;
@@ -533,12 +786,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
       }
       if (ahead_r < rows) {
         if (whole(ahead_row, ahead_part, ahead_j)) {
-          const Vector* from = ahead_row.vector(ahead_j + lane);
+          const uint4* from = reinterpret_cast<const uint4*>(ahead_row.vector(ahead_j)) + lane;
           const uint32_t to = smem_u32(my_slots) + ahead_slot * kPieces * kPieceBytes;
 #pragma unroll
           for (int a = 0; a < kMine; ++a)
 #pragma unroll
-            for (int x = 0; x < kPieces; ++x) copy16(to + x * kPieceBytes + a * 512, reinterpret_cast<const uint4*>(from + a * 32) + x);
+            for (int x = 0; x < kPieces; ++x) copy16(to + x * kPieceBytes + a * 512, from + (a * kPieces + x) * 32);
         }
         ahead_j += kWarps * kRun<T, TOP>;
         ahead_slot = ahead_slot + 1 == kSlots ? 0 : ahead_slot + 1;
@@ -551,48 +804,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
       const Row<T> row = row_of(r);
       const Part part = part_of(row);
       if (turn > 1) wait_at(3 + buffer);  // what lies in this buffer has been used
-      float most_allowed = -1.f, base = 0.f;  // there is no base until there is a logit above the infinitely low ones
-      uint64_t s2 = 0, t2 = 0;
-      auto careful = [&](const float (&f)[8]) {  // moves the base, and takes what is infinitely low to have no share (0 * -inf)
-        const float most = most_of(f);
-        if (!(most <= (most_allowed < 0.f ? -INFINITY : base))) {  // NaN too
-          const float d = fminf(fmaxf((base - most) * p.c, kLowest), 0.f), g = fast_exp2(d);
-          float s0, s1, t0, t1;
-          unpack_f32x2(s2, s0, s1), unpack_f32x2(t2, t0, t1);
-          const float s = s0 + s1, t = t0 + t1;
-          s2 = pack_f32x2(s * g, 0.f), t2 = pack_f32x2((t + s * d) * g, 0.f);
-          base = most, most_allowed = kMostAllowed;
-        }
-        float s = 0.f, t = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float d = (f[i] - base) * p.c, e = fast_exp2(d);
-          s += e, t += e * (d < kLowest ? kLowest : d);
-        }
-        s2 = add_f32x2(s2, pack_f32x2(s, 0.f)), t2 = add_f32x2(t2, pack_f32x2(t, 0.f));
-      };
-      auto take = [&](const Vector& raw) {
-        uint64_t sv = 0, tv = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const uint64_t d = mul_f32x2(minus<T>(raw, i, base), c2);
-          float d0, d1;
-          unpack_f32x2(d, d0, d1);
-          const uint64_t e = pack_f32x2(fast_exp2(d0), fast_exp2(d1));
-          sv = i == 0 ? e : add_f32x2(sv, e);
-          tv = i == 0 ? mul_f32x2(e, d) : fma_f32x2(e, d, tv);
-        }
-        float s0, s1, t0, t1;
-        unpack_f32x2(sv, s0, s1), unpack_f32x2(tv, t0, t1);
-        const float sum = s0 + s1, t = t0 + t1;
-        if (!(sum <= most_allowed) || t != t) {
-          float f[8];
-          widen8(raw, f);
-          careful(f);
-        } else {
-          s2 = add_f32x2(s2, sv), t2 = add_f32x2(t2, tv);
-        }
-      };
+      Running run{p.c};
       auto note = [&](int j, float most) {  // the maximum of a segment
         if constexpr (TOP) {
           const float m = warp_max_nan(most);
@@ -610,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
 #pragma unroll
             for (int x = 0; x < kPieces; ++x) reinterpret_cast<uint4*>(raw.v)[x] = *reinterpret_cast<const uint4*>(at + x * kPieceBytes + a * 512);
             if constexpr (TOP) note(j0 + a * 32, most_of_vector<T>(raw));
-            take(raw);
+            run.take<T>(raw, c2);
           }
         } else {
 #pragma unroll 1
@@ -624,14 +836,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
               for (int i = 0; i < 8; ++i) f[i] = -INFINITY;
             }
             note(j0 + a * 32, most_of(f));
-            careful(f);
+            run.careful(f);
           }
         }
         slot = slot + 1 == kSlots ? 0 : slot + 1;
       }
-      float s0, s1, t0, t1;
-      unpack_f32x2(s2, s0, s1), unpack_f32x2(t2, t0, t1);
-      const Sums mine = joined_lanes({base, s0 + s1, t0 + t1}, p.c);
+      const Sums mine = joined_lanes(run.sums(), p.c);
       if (lane == 0) sh.warp[buffer][warp] = mine;
       __syncwarp();
       arrive_at(1 + buffer);
@@ -651,7 +861,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
   // ------------------------------------------------------------------------------------------------ the warp that ends rows
   auto choose_segments = [&](const Part& part, uint32_t* segments) {  // sh.few: whether it went without a search
     if constexpr (TOP) {
-    const bool few = part.segments > p.top && choose_few<T>(segments, part.segments, p.top, sh.candidates, sh.found);
+    const bool few = part.segments > p.top && choose_few<T>(segments, part.segments, p.top, sh.candidates, kMostCandidates, sh.found);
     if (part.segments <= p.top)
       for (int i = lane; i < part.segments; i += 32) segments[i] = key_of<T>(__uint_as_float(segments[i]));
     __syncwarp();
@@ -693,37 +903,22 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
     rank(sh.candidates, n, p.top, to);
     }
   };
-  auto finish = [&](long long r, long long token, float logit, const Sums& sum) {  // with the alternatives in entries[0]
-    const float log_s = log2f(sum.s);
-    if constexpr (TOP) {
-      for (int x = lane; x < p.top; x += 32) {
-        const Entry e = sh.entries[0][x];
-        p.top_tokens[r * p.top + x] = index_in(e);
-        p.top_logprobs[r * p.top + x] = (value_of<T>(key_in(e)) - sum.base) * p.rate - log_s * kLn2;
-      }
-      __syncwarp();
-    }
-    if (lane == 0) {
-      float lp = 0.f;
-      if (token >= 0 && token < p.vocab) lp = (logit - sum.base) * p.rate - log_s * kLn2;
-      else if (token != p.ignore) TTB_NOTE_VIOLATION(token_stats);  // as a row that is ignored
-      p.logprobs[r] = token == p.ignore ? 0.f : lp;
-      p.entropy[r] = (log_s - sum.t / sum.s) * kLn2;
-      if (p.stats != nullptr) p.stats[2 * r] = sum.base, p.stats[2 * r + 1] = log_s;
-    }
+  auto first_entries = [&]() -> const Entry* {
+    if constexpr (TOP) return sh.entries[0];
+    else return nullptr;
   };
   auto sum_of = [&](int buffer) {  // of the warps
     return joined_lanes(lane < kWarps ? sh.warp[buffer][lane] : Sums{0.f, 0.f, 0.f}, p.c);
   };
   if (splits == 1) {
     int buffer = 0;
-    auto logit_of = [&](uint32_t r, long long token) { return token >= 0 && token < p.vocab ? widened(row_of(r).x[token]) : 0.f; };
+    auto logit_of = [&](uint32_t r, long long token) { return token >= 0 && token < p.vocab ? row_of(r).x[token] : T(); };
     long long next_token = p.tokens[blockIdx.x];  // a row ahead
-    float next_logit = logit_of(blockIdx.x, next_token);
+    T next_logit = logit_of(blockIdx.x, next_token);
     for (uint32_t r = blockIdx.x; r < rows; r += step, buffer ^= 1) {
       const Row<T> row = row_of(r);
       const long long token = next_token;
-      const float logit = next_logit;
+      const T logit = next_logit;
       wait_at(1 + buffer);
       if (r + step < rows) next_token = p.tokens[r + step];
       const Sums sum = sum_of(buffer);
@@ -736,14 +931,14 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
       __syncwarp();
       if (r + 2 * step < rows) arrive_at(3 + buffer);
       if (r + step < rows) next_logit = logit_of(r + step, next_token);
-      finish(r, token, logit, sum);
+      finish<T, TOP>(p, r, token, widened(logit), sum, first_entries());
     }
     return;
   }
   const uint32_t r = blockIdx.x / splits;
   const Row<T> row = row_of(r);
   const long long token = p.tokens[r];
-  const float logit = token >= 0 && token < p.vocab ? widened(row.x[token]) : 0.f;
+  const T logit = token >= 0 && token < p.vocab ? row.x[token] : T();
   wait_at(1);
   if constexpr (TOP) {
     const Part part = part_of(row);
@@ -771,7 +966,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
     __syncwarp();
     rank(sh.candidates, count, p.top, sh.entries[0]);
   }
-  finish(r, token, logit, sum);
+  finish<T, TOP>(p, r, token, widened(logit), sum, first_entries());
 }
 
 static constexpr int kGradVectors = 4;  // of a thread
@@ -786,12 +981,14 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const __grid_cons
   const int vectors = row.vectors(), j0 = part * kBlock;
   const bool whole = same && j0 >= row.whole_from() && j0 + kBlock <= row.whole_to();
   typename Row<T>::Vector raw[kGradVectors];
+  constexpr int kPieces = sizeof(T) / 2;
+  const int mine = (threadIdx.x & ~31) * kPieces + (threadIdx.x & 31);  // first of 16-byte pieces that lie 512 bytes apart: a warp's loads and stores leave no gaps
   if (whole) {
-    const typename Row<T>::Vector* at = row.vector(j0 + threadIdx.x);
+    const uint4* at = reinterpret_cast<const uint4*>(row.vector(j0)) + mine;
 #pragma unroll
     for (int a = 0; a < kGradVectors; ++a)
 #pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4*>(raw[a].v)[i] = __ldcs(reinterpret_cast<const uint4*>(at + a * kGradThreads) + i);
+      for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4*>(raw[a].v)[i] = __ldcs(at + a * kGradThreads * kPieces + i * 32);
   }
   const long long token = p.tokens[r];
   const bool counts = token != p.ignore && token >= 0 && token < p.vocab;
@@ -831,12 +1028,12 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const __grid_cons
     return d;
   };
   if (whole) {
-    typename Row<T>::Vector* to = reinterpret_cast<typename Row<T>::Vector*>(out - row.off) + j0 + threadIdx.x;
+    uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<typename Row<T>::Vector*>(out - row.off) + j0) + mine;
 #pragma unroll
     for (int a = 0; a < kGradVectors; ++a) {
       const typename Row<T>::Vector d = eight(raw[a]);
 #pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) __stcs(reinterpret_cast<uint4*>(to + a * kGradThreads) + i, reinterpret_cast<const uint4*>(d.v)[i]);
+      for (int i = 0; i < kPieces; ++i) __stcs(to + a * kGradThreads * kPieces + i * 32, reinterpret_cast<const uint4*>(d.v)[i]);
     }
   } else {
 #pragma unroll 1
@@ -892,11 +1089,28 @@ static int launch(const Call& c, float log2_rate, float rate, cudaStream_t st) {
   p.top_logprobs = reinterpret_cast<float*>(c.top_logprobs), p.top_tokens = reinterpret_cast<long long*>(c.top_tokens);
   p.ignore = c.ignore, p.rows = c.rows, p.inner = static_cast<int>(c.inner), p.vocab = static_cast<int>(c.vocab), p.top = static_cast<int>(c.top), p.c = log2_rate, p.rate = rate;
   const long long segments = (c.vocab + 7 + 255) / 256;
+  // A warp for a row, where there are rows for a good part of all warps.  us with CTAs for rows -> with warps, without / with 20 alternatives: bf16 600 x 2000 18 -> 12 / 51 -> 16, 8192 x 8000
+  // 121 -> 43 / 317 -> 96, 8192 x 32000 141 -> 117 / 352 -> 180, fp32 8192 x 32000 184 -> 184 / 377 -> 240; on the other side bf16 600 x 32000 19 -> 29 / 47 -> 45, 333 x 50257 25 -> 41 / 39 -> 59,
+  // fp32 1200 x 32000 43 -> 47 / 76 -> 68.
+  const bool own = segments <= kOwnSegments && (segments <= 4 || c.rows * (32 / static_cast<int>(sizeof(T))) >= segments * sm_count());
   // few rows: a cluster to a row, while each of its CTAs has a run for every warp, as long as all are on an SM at once
   const long long at_once = static_cast<long long>(kCtas) * sm_count();
   int splits = 1;
   while (splits < kMaxCluster && ((c.rows * splits * 2 <= at_once && segments >= splits * 2 * kWarps) || (TOP && segments > static_cast<long long>(splits) * kMaxSegments))) splits *= 2;
   if ((TOP && segments > static_cast<long long>(splits) * kMaxSegments) || c.rows * splits > 0x7fffffffll) return kErrTooLarge;
+  if (own) {
+    constexpr int own_bytes = kOwnWarps<TOP> * kOwnBytes<T, TOP>;
+    static bool own_attr[64] = {};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return kErrDriver;
+    if (!own_attr[device]) {
+      if (cudaFuncSetAttribute(row_kernel<T, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, own_bytes) != cudaSuccess) return kErrDriver;
+      own_attr[device] = true;
+    }
+    TTB_COUNT_LAUNCH(1);
+    row_kernel<T, TOP><<<static_cast<unsigned>(c.rows < at_once ? c.rows : at_once), kOwnWarps<TOP> * 32, own_bytes, st>>>(p);
+    return cudaGetLastError() == cudaSuccess ? kOk : kErrDriver;
+  }
   constexpr int bytes = kSlots * kSlotBytes<T, TOP>;
   static bool attr[64] = {};  // an attribute of the kernel on one device
   int device = 0;
