@@ -482,25 +482,29 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
   if (warp == 5) tmem_dealloc(tO, L::kColumns);
 }
 
-// Joins the pieces of a token and query head, those of the prefix and then its own.  A warp of `wide` (a power of two up to 8) takes every wide-th run of 32 pieces or, of fewer, its part of them: a lane
-// per piece finds where it lies, its maximum and sum, and the weights go around, so that all loads but the first two are independent.  Warps meet in shared memory, in their order.
+// Joins the pieces of Q query rows of one row and key head, those of the prefix and then their own.  Where Q is 1, a warp of `wide` (a power of two up to 8) takes every wide-th run of 32 pieces or, of
+// fewer, its part of them; warps meet in shared memory, in their order.  A lane per piece finds where it lies, its maxima and sums, and the weights go around, so that all loads but the first two are
+// independent.  With many results it is the finding that takes the time, so that four of them share it (59 136 results of 3 to 4 pieces, 64 channels: 48 -> 27 us after the last piece).
 static constexpr int kJoinWarps = 8;
-template <int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ Params p, int wide) {
-  __shared__ float outputs[kJoinWarps][D];
+template <int D, int Q>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ Params p, int wide, int chunks) {
+  __shared__ float outputs[kJoinWarps][Q == 1 ? D : 1];
   __shared__ float2 sums[kJoinWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, member = warp & (wide - 1);
-  const uint32_t w = (blockIdx.x * kJoinWarps + warp) / wide;
-  const uint32_t token = w / p.hq;
-  const bool live = token < static_cast<uint32_t>(p.rows) * p.s;
-  const int h = static_cast<int>(w - token * p.hq), head = h / p.group, a = h - head * p.group;
-  const int row = static_cast<int>(token / p.s), i = static_cast<int>(token - static_cast<uint32_t>(row) * p.s);
-  const int per = p.rows / p.prompts, prompt = row / per;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, member = Q == 1 ? warp & (wide - 1) : 0;
+  const uint32_t w = Q == 1 ? (blockIdx.x * kJoinWarps + warp) / wide : blockIdx.x * kJoinWarps + warp;  // of rows, key heads and chunks of query rows
+  const uint32_t owner = w / chunks;
+  const int row = static_cast<int>(owner / p.hkv), head = static_cast<int>(owner - row * static_cast<uint32_t>(p.hkv)), q0 = static_cast<int>(w - owner * chunks) * Q;
+  const bool live = row < p.rows;
+  const int per = p.rows / p.prompts, prompt = row / per, mine = min(Q, p.rows_o - q0);  // query rows
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the pieces are written
   constexpr int kMine = D / 32;
-  float m = -INFINITY, l = 0.f, o[kMine];
+  float m[Q], l[Q], o[Q][kMine];
 #pragma unroll
-  for (int x = 0; x < kMine; ++x) o[x] = 0.f;
+  for (int y = 0; y < Q; ++y) {
+    m[y] = -INFINITY, l[y] = 0.f;
+#pragma unroll
+    for (int x = 0; x < kMine; ++x) o[y][x] = 0.f;
+  }
   if (live) {
     // pieces of the prompt's head, then of the row's own: those of all groups of CTAs with a tile of it
     const int* before_p = p.shared_out + 2;
@@ -519,66 +523,88 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
     for (int first_piece = member * run; first_piece < pieces; first_piece += wide * run) {
       const int piece = first_piece + lane, n = min(run, pieces - first_piece);
       long long place = 0;
-      float2 t = make_float2(-INFINITY, 0.f);
+      float2 t[Q];
+#pragma unroll
+      for (int y = 0; y < Q; ++y) t[y] = make_float2(-INFINITY, 0.f);
       if (lane < n) {
-        place = piece < count[0] ? (static_cast<long long>(owners[0]) * p.hkv + head + from[0] + piece) * p.rows_p + ((row - prompt * per) * p.s + i) * p.group + a
-                                 : static_cast<long long>(p.pieces_p) * p.rows_p + (static_cast<long long>(owners[1]) * p.hkv + head + from[1] + piece - count[0]) * p.rows_o + i * p.group + a;
-        t = p.ml[place];
+        place = piece < count[0] ? (static_cast<long long>(owners[0]) * p.hkv + head + from[0] + piece) * p.rows_p + (row - prompt * per) * p.rows_o + q0
+                                 : static_cast<long long>(p.pieces_p) * p.rows_p + (static_cast<long long>(owners[1]) * p.hkv + head + from[1] + piece - count[0]) * p.rows_o + q0;
+#pragma unroll
+        for (int y = 0; y < Q; ++y)
+          if (y < mine) t[y] = p.ml[place + y];
       }
-      float top = fmaxf(m, t.x);
+      float weight[Q];
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const float base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), weight = exp2f(t.x - base);
-      float sum = t.y * weight;
+      for (int y = 0; y < Q; ++y) {
+        float top = fmaxf(m[y], t[y].x);
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      l = l * f + sum;
-      m = top;
+        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float base = top == -INFINITY ? 0.f : top, f = exp2f(m[y] - base);
+        weight[y] = exp2f(t[y].x - base);
+        float sum = t[y].y * weight[y];
 #pragma unroll
-      for (int y = 0; y < kMine; ++y) o[y] *= f;
-      for (int x0 = 0; x0 < n; x0 += 4) {
-        float v[4][kMine], g[4];
+        for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        l[y] = l[y] * f + sum;
+        m[y] = top;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          g[x] = __shfl_sync(0xffffffffu, weight, x0 + x);  // 0 where no key is seen
+        for (int c = 0; c < kMine; ++c) o[y][c] *= f;
+      }
+      constexpr int kAtOnce = Q == 1 ? 4 : 2;
+      for (int x0 = 0; x0 < n; x0 += kAtOnce) {
+        float v[kAtOnce][Q][kMine], g[kAtOnce][Q];
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x) {
           const float* of = p.part + __shfl_sync(0xffffffffu, place, x0 + x) * D + lane * kMine;
-          if (g[x] != 0.f) {
-            if constexpr (kMine == 4) *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(of);
-            else *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(of);
+#pragma unroll
+          for (int y = 0; y < Q; ++y) {
+            g[x][y] = __shfl_sync(0xffffffffu, weight[y], x0 + x);  // 0 where no key is seen
+            if (g[x][y] != 0.f) {
+              if constexpr (kMine == 4) *reinterpret_cast<float4*>(v[x][y]) = *reinterpret_cast<const float4*>(of + y * D);
+              else *reinterpret_cast<float2*>(v[x][y]) = *reinterpret_cast<const float2*>(of + y * D);
+            }
           }
         }
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          if (g[x] != 0.f) {
+        for (int x = 0; x < kAtOnce; ++x)
 #pragma unroll
-            for (int y = 0; y < kMine; ++y) o[y] += v[x][y] * g[x];
-          }
+          for (int y = 0; y < Q; ++y)
+            if (g[x][y] != 0.f) {
+#pragma unroll
+              for (int c = 0; c < kMine; ++c) o[y][c] += v[x][y][c] * g[x][y];
+            }
       }
     }
   }
-  if (wide > 1) {
-    if (lane == 0) sums[warp] = make_float2(m, l);
+  if constexpr (Q == 1) {
+    if (wide > 1) {
+      if (lane == 0) sums[warp] = make_float2(m[0], l[0]);
 #pragma unroll
-    for (int y = 0; y < kMine; ++y) outputs[warp][lane * kMine + y] = o[y];
-    __syncthreads();
-    if (member != 0) return;
-    for (int x = 1; x < wide; ++x) {
-      const float2 t = sums[warp + x];
-      const float top = fmaxf(m, t.x), base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), g = exp2f(t.x - base);
-      l = l * f + t.y * g;
-      m = top;
+      for (int y = 0; y < kMine; ++y) outputs[warp][lane * kMine + y] = o[0][y];
+      __syncthreads();
+      if (member != 0) return;
+      for (int x = 1; x < wide; ++x) {
+        const float2 t = sums[warp + x];
+        const float top = fmaxf(m[0], t.x), base = top == -INFINITY ? 0.f : top, f = exp2f(m[0] - base), g = exp2f(t.x - base);
+        l[0] = l[0] * f + t.y * g;
+        m[0] = top;
 #pragma unroll
-      for (int y = 0; y < kMine; ++y) o[y] = o[y] * f + outputs[warp + x][lane * kMine + y] * g;
+        for (int y = 0; y < kMine; ++y) o[0][y] = o[0][y] * f + outputs[warp + x][lane * kMine + y] * g;
+      }
     }
   }
   if (!live) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // a query without a key gives 0
-  uint32_t out[kMine / 2];
 #pragma unroll
-  for (int y = 0; y < kMine / 2; ++y) out[y] = pack_bf16x2(o[2 * y] * inv, o[2 * y + 1] * inv);
-  __nv_bfloat16* to = p.o + (static_cast<long long>(token) * p.hq + h) * D + lane * kMine;
-  if constexpr (kMine == 4) *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[1]);
-  else *reinterpret_cast<uint32_t*>(to) = out[0];
+  for (int x = 0; x < Q; ++x) {
+    if (x >= mine) break;
+    const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];  // a query without a key gives 0
+    uint32_t out[kMine / 2];
+#pragma unroll
+    for (int y = 0; y < kMine / 2; ++y) out[y] = pack_bf16x2(o[x][2 * y] * inv, o[x][2 * y + 1] * inv);
+    const int i = token_of(p, q0 + x);
+    __nv_bfloat16* to = p.o + ((static_cast<long long>(row) * p.s + i) * p.hq + head * p.group + q0 + x - i * p.group) * D + lane * kMine;
+    if constexpr (kMine == 4) *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[1]);
+    else *reinterpret_cast<uint32_t*>(to) = out[0];
+  }
 }
 
 // What a call brings, packed by the host language in this order.
@@ -637,9 +663,12 @@ static int launch(const Call& c, Params& p, int ctas, cudaStream_t st) {
   TTB_COUNT_LAUNCH(2);
   piece_kernel<D><<<ctas, kThreads, L::kBytes, st>>>(maps[0], maps[1], maps[2], maps[3], p);
   if (cudaGetLastError() != cudaSuccess) return kErrDriver;
-  const long long warps = static_cast<long long>(p.rows) * p.s * p.hq;
+  const long long results = static_cast<long long>(p.rows) * p.s * p.hq;
+  const bool four = p.rows_o > 2 && results >= 64ll * sm_count();  // to a warp, where that leaves sixteen to an SM
+  const int chunks = four ? (p.rows_o + 3) / 4 : p.rows_o;
+  const long long warps = static_cast<long long>(p.rows) * p.hkv * chunks;
   int wide = 1;  // few results are joined by more warps each, until there are sixteen to an SM
-  while (wide < kJoinWarps && warps * wide * 2 <= 16ll * sm_count()) wide *= 2;
+  while (!four && wide < kJoinWarps && warps * wide * 2 <= 16ll * sm_count()) wide *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((warps * wide + kJoinWarps - 1) / kJoinWarps));
   cfg.blockDim = dim3(kJoinWarps * 32);
@@ -648,7 +677,7 @@ static int launch(const Call& c, Params& p, int ctas, cudaStream_t st) {
   early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = early, cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel<D>, p, wide) == cudaSuccess ? kOk : kErrDriver;
+  return (four ? cudaLaunchKernelEx(&cfg, join_kernel<D, 4>, p, wide, chunks) : cudaLaunchKernelEx(&cfg, join_kernel<D, 1>, p, wide, chunks)) == cudaSuccess ? kOk : kErrDriver;
 }
 
 }  // namespace sprefix
