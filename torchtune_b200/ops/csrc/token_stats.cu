@@ -81,8 +81,8 @@ struct GradParams {
   const long long* top_tokens;
   const float *g, *h, *k;  // gradients of log-probabilities, entropy and alternatives; nullptr: none
   void* dx;                // [rows, vocab]
-  long long ignore;
-  int inner, vocab, top, parts;  // parts: CTAs of a row
+  long long ignore, rows;
+  int inner, vocab, top, parts;  // parts: of a row
   float c, rate;           // rate = 1 / T
 };
 
@@ -970,11 +970,17 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
 }
 
 static constexpr int kGradVectors = 4;  // of a thread
-// grid: rows * parts
+// Vectors of a row, up to which a warp takes a part: a CTA's part is filled badly by short rows, and its threads wait for the row's numbers together.  us with CTAs -> warps of 8192 rows: bf16 x 800
+// 44 -> 12, x 8000 78 -> 51, x 32003 220 -> 186 (with 21 alternatives 259 -> 256), fp32 x 4000 57 -> 44 (73 -> 61); on the other side fp32 x 8000 87 -> 83 (100 -> 115), bf16 2048 x 151936 203 -> 205.
 template <typename T>
+static constexpr int kGradByWarp = sizeof(T) == 2 ? 4096 : 512;
+// G threads, those of a CTA or of a warp, take a part of a row.
+template <typename T, int G>
 __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const __grid_constant__ GradParams p) {
-  constexpr int kBlock = kGradThreads * kGradVectors;
-  const int r = blockIdx.x / p.parts, part = blockIdx.x - r * p.parts;
+  constexpr int kBlock = G * kGradVectors;
+  const int thread = G == kGradThreads ? threadIdx.x : threadIdx.x % G, unit = G == kGradThreads ? blockIdx.x : blockIdx.x * (kGradThreads / G) + threadIdx.x / G;  // units are below 2^31 - 8
+  const int r = unit / p.parts, part = unit - r * p.parts;
+  if (G != kGradThreads && r >= p.rows) return;
   const Row<T> row(static_cast<const T*>(p.x) + r / p.inner * p.step_outer + r % p.inner * p.step_inner, p.vocab);
   T* out = static_cast<T*>(p.dx) + static_cast<long long>(r) * p.vocab;
   const bool same = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(row.x)) & 15) == 0;  // whole vectors of the row are such of the gradient
@@ -982,24 +988,31 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const __grid_cons
   const bool whole = same && j0 >= row.whole_from() && j0 + kBlock <= row.whole_to();
   typename Row<T>::Vector raw[kGradVectors];
   constexpr int kPieces = sizeof(T) / 2;
-  const int mine = (threadIdx.x & ~31) * kPieces + (threadIdx.x & 31);  // first of 16-byte pieces that lie 512 bytes apart: a warp's loads and stores leave no gaps
+  const int mine = (thread & ~31) * kPieces + (thread & 31);  // first of 16-byte pieces that lie 512 bytes apart: a warp's loads and stores leave no gaps
   if (whole) {
     const uint4* at = reinterpret_cast<const uint4*>(row.vector(j0)) + mine;
 #pragma unroll
     for (int a = 0; a < kGradVectors; ++a)
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4*>(raw[a].v)[i] = __ldcs(at + a * kGradThreads * kPieces + i * 32);
+      for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4*>(raw[a].v)[i] = __ldcs(at + a * G * kPieces + i * 32);
+  } else if constexpr (G == 32) {  // rows that are all ends, as a rule
+#pragma unroll
+    for (int a = 0; a < kGradVectors; ++a) raw[a] = row.load(j0 + a * G + thread);
   }
   const long long token = p.tokens[r];
   const bool counts = token != p.ignore && token >= 0 && token < p.vocab;
   const float base = p.stats[2ll * r], log_s = p.stats[2ll * r + 1];
   const float g = p.g != nullptr && counts ? p.g[r] : 0.f, h = p.h != nullptr ? p.h[r] : 0.f;
-  float all = g, any = fabsf(g) + fabsf(h);
-  if (p.k != nullptr)
-    for (int i = 0; i < p.top; ++i) {
+  float all = 0.f, any = 0.f;
+  if (p.k != nullptr) {  // a lane for each
+    for (int i = threadIdx.x & 31; i < p.top; i += 32) {
       const float k = p.k[static_cast<long long>(r) * p.top + i];
       all += k, any += fabsf(k);
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o), any += __shfl_xor_sync(0xffffffffu, any, o);
+  }
+  all += g, any += fabsf(g) + fabsf(h);
   const bool none = any == 0.f;  // zeros then, whatever the logits are; else what is NaN in a row reaches its gradient
   // -p (all + h (H + ln2 q)) / T with q = log2 p
   const float offset = -(all + (h != 0.f ? h * p.entropy[r] : 0.f)) * p.rate, slope = -h * kLn2 * p.rate;
@@ -1033,14 +1046,17 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const __grid_cons
     for (int a = 0; a < kGradVectors; ++a) {
       const typename Row<T>::Vector d = eight(raw[a]);
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) __stcs(to + a * kGradThreads * kPieces + i * 32, reinterpret_cast<const uint4*>(d.v)[i]);
+      for (int i = 0; i < kPieces; ++i) __stcs(to + a * G * kPieces + i * 32, reinterpret_cast<const uint4*>(d.v)[i]);
     }
   } else {
-#pragma unroll 1
+#pragma unroll G == 32 ? kGradVectors : 1
     for (int a = 0; a < kGradVectors; ++a) {
-      const int j = j0 + a * kGradThreads + threadIdx.x;
+      const int j = j0 + a * G + thread;
       if (j >= vectors) break;
-      const typename Row<T>::Vector d = eight(row.load(j));
+      typename Row<T>::Vector at_j;
+      if constexpr (G == 32) at_j = raw[a];
+      else at_j = row.load(j);
+      const typename Row<T>::Vector d = eight(at_j);
       const long long e = j * 8ll - row.off;
       if (same && j >= row.whole_from() && j < row.whole_to()) {
 #pragma unroll
@@ -1054,17 +1070,23 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const __grid_cons
   }
   // the token and the alternatives again, with what is theirs; of two equal ones both write the same
   const int targets = (p.k != nullptr ? p.top : 0) + 1;
-  __syncthreads();
-  if (!none && static_cast<int>(threadIdx.x) < targets) {
-    const long long* best = p.top_tokens + static_cast<long long>(r) * p.top;
-    const float* of_best = p.k + static_cast<long long>(r) * p.top;
-    const long long mine = threadIdx.x == 0 ? (counts ? token : -1) : best[threadIdx.x - 1];
-    if (mine >= 0 && (mine + row.off) / 8 / kBlock == part) {
-      float extra = counts && token == mine ? g : 0.f, d, unused;
-      for (int i = 0; i + 1 < targets; ++i) extra += best[i] == mine ? of_best[i] : 0.f;
-      two(widened(row.x[mine]), 0.f, d, unused);
-      out[mine] = narrowed<T>(fmaf(extra, p.rate, d));
+  if constexpr (G == kGradThreads) __syncthreads();
+  else __syncwarp();
+  const long long* best = p.top_tokens + static_cast<long long>(r) * p.top;
+  const float* of_best = p.k + static_cast<long long>(r) * p.top;
+  auto put = [&](int x) {
+    const long long target = x == 0 ? (counts ? token : -1) : best[x - 1];
+    if (target >= 0 && (target + row.off) / 8 / kBlock == part) {
+      float extra = counts && token == target ? g : 0.f, d, unused;
+      for (int i = 0; i + 1 < targets; ++i) extra += best[i] == target ? of_best[i] : 0.f;
+      two(widened(row.x[target]), 0.f, d, unused);
+      out[target] = narrowed<T>(fmaf(extra, p.rate, d));
     }
+  };
+  if constexpr (G == kGradThreads) {
+    if (!none && thread < targets) put(thread);
+  } else {
+    for (int x = none ? targets : thread; x < targets; x += G) put(x);
   }
 }
 
@@ -1092,7 +1114,7 @@ static int launch(const Call& c, float log2_rate, float rate, cudaStream_t st) {
   // A warp for a row, where there are rows for a good part of all warps.  us with CTAs for rows -> with warps, without / with 20 alternatives: bf16 600 x 2000 18 -> 12 / 51 -> 16, 8192 x 8000
   // 121 -> 43 / 317 -> 96, 8192 x 32000 141 -> 117 / 352 -> 180, fp32 8192 x 32000 184 -> 184 / 377 -> 240; on the other side bf16 600 x 32000 19 -> 29 / 47 -> 45, 333 x 50257 25 -> 41 / 39 -> 59,
   // fp32 1200 x 32000 43 -> 47 / 76 -> 68.
-  const bool own = segments <= kOwnSegments && (segments <= 4 || c.rows * (32 / static_cast<int>(sizeof(T))) >= segments * sm_count());
+  const bool own = segments <= kOwnSegments && (segments <= (c.top > 4 ? c.top : 4) || c.rows * (32 / static_cast<int>(sizeof(T))) >= segments * sm_count());
   // few rows: a cluster to a row, while each of its CTAs has a run for every warp, as long as all are on an SM at once
   const long long at_once = static_cast<long long>(kCtas) * sm_count();
   int splits = 1;
@@ -1137,12 +1159,15 @@ static int launch_grad(const Call& c, float log2_rate, float rate, cudaStream_t 
   p.x = reinterpret_cast<const void*>(c.x), p.step_outer = c.step_outer, p.step_inner = c.step_inner, p.tokens = reinterpret_cast<const long long*>(c.tokens);
   p.stats = reinterpret_cast<const float*>(c.stats), p.entropy = reinterpret_cast<const float*>(c.entropy), p.top_tokens = reinterpret_cast<const long long*>(c.top_tokens);
   p.g = reinterpret_cast<const float*>(c.g), p.h = reinterpret_cast<const float*>(c.h), p.k = reinterpret_cast<const float*>(c.k), p.dx = reinterpret_cast<void*>(c.dx);
-  p.ignore = c.ignore, p.inner = static_cast<int>(c.inner), p.vocab = static_cast<int>(c.vocab), p.top = static_cast<int>(c.top), p.c = log2_rate, p.rate = rate;
+  p.ignore = c.ignore, p.rows = c.rows, p.inner = static_cast<int>(c.inner), p.vocab = static_cast<int>(c.vocab), p.top = static_cast<int>(c.top), p.c = log2_rate, p.rate = rate;
   const long long vectors = (c.vocab + 7 + 7) / 8;
-  p.parts = static_cast<int>((vectors + kGradThreads * kGradVectors - 1) / (kGradThreads * kGradVectors));
-  if (c.rows * p.parts > 0x7fffffffll) return kErrTooLarge;
+  const bool by_warp = vectors <= kGradByWarp<T>;
+  const int each = (by_warp ? 32 : kGradThreads) * kGradVectors;
+  p.parts = static_cast<int>((vectors + each - 1) / each);
+  if (c.rows * p.parts > 0x7ffffff0ll) return kErrTooLarge;
   TTB_COUNT_LAUNCH(1);
-  grad_kernel<T><<<static_cast<unsigned>(c.rows * p.parts), kGradThreads, 0, st>>>(p);
+  if (by_warp) grad_kernel<T, 32><<<static_cast<unsigned>((c.rows * p.parts * 32 + kGradThreads - 1) / kGradThreads), kGradThreads, 0, st>>>(p);
+  else grad_kernel<T, kGradThreads><<<static_cast<unsigned>(c.rows * p.parts), kGradThreads, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrDriver;
 }
 
