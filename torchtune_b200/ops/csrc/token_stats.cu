@@ -1118,7 +1118,9 @@ static int launch(const Call& c, float log2_rate, float rate, cudaStream_t st) {
   // few rows: a cluster to a row, while each of its CTAs has a run for every warp, as long as all are on an SM at once
   const long long at_once = static_cast<long long>(kCtas) * sm_count();
   int splits = 1;
-  while (splits < kMaxCluster && ((c.rows * splits * 2 <= at_once && segments >= splits * 2 * kWarps) || (TOP && segments > static_cast<long long>(splits) * kMaxSegments))) splits *= 2;
+  // and, with alternatives, has more segments than those (the last one too): their choice needs a search otherwise, 20 -> 45 us of 4 rows of 50257 with 29
+  auto enough = [&](long long n) { return segments >= n * kWarps && (!TOP || segments - (n - 1) * ((segments + n - 1) / n) > c.top); };
+  while (splits < kMaxCluster && ((c.rows * splits * 2 <= at_once && enough(splits * 2)) || (TOP && segments > static_cast<long long>(splits) * kMaxSegments))) splits *= 2;
   if ((TOP && segments > static_cast<long long>(splits) * kMaxSegments) || c.rows * splits > 0x7fffffffll) return kErrTooLarge;
   if (own) {
     constexpr int own_bytes = kOwnWarps<TOP> * kOwnBytes<T, TOP>;
