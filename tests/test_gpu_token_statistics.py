@@ -83,6 +83,7 @@ def test_alternatives_whatever_the_order(order):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,v,top", [(3, 700, 7), (700, 1, 1), (700, 33, 32), (700, 255, 0), (700, 1026, 12), (700, 2049, 64), (700, 8200, 33), (611, 8001, 20), (2000, 32003, 5), (4736 + 13, 900, 3)])
 def test_many_short_rows(rows, v, top, dtype):
+    """Rows of one warp each: a lane adds up v / 256 <= 126 vectors, and there are 13 steps more, which stays below the 140 steps of _check."""
     logits, tokens = _logits(rows, v, dtype=dtype), torch.randint(0, v, (rows,), device=DEV)
     tokens[::7] = -100
     _check(logits, tokens, 0.8, top)

@@ -14,6 +14,10 @@
 //
 // What lies behind the last visible key may be anything: scores are masked by selection, and the values of a piece's last tile that nobody sees are overwritten with zeros before they are
 // multiplied.  Every wait is bounded and reports through the error word.
+//
+// Bound by bytes on long rows, else by what a piece does one after the other (products, softmax, products, output: 3 to 5 us, which the two CTAs of an SM hide from each other in part) and by the
+// start (finding the shares, first loads: 5 us) and the joining launch.  Measured (32 query on 8 key heads of 128 channels, kernels behind one another in a graph): 16 rows on 32003 shared keys and
+// 300 of their own 42 us (3.5 TB/s); 64 rows of 4 prompts of 613 and 391 own 32 us; 256 rows of three tokens, 8 prompts of 4096 and 1001 own 209 us (4.4 TB/s); one prompt of 61 11 us.
 #include "common/attn_math.cuh"
 #include "common/ptx.cuh"
 #include "common/tmap.h"
@@ -549,21 +553,24 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
 #pragma unroll
         for (int c = 0; c < kMine; ++c) o[y][c] *= f;
       }
-      constexpr int kAtOnce = Q == 1 ? 4 : 2;
+      constexpr int kAtOnce = Q == 1 ? 8 : 2;
       for (int x0 = 0; x0 < n; x0 += kAtOnce) {
         float v[kAtOnce][Q][kMine], g[kAtOnce][Q];
+        const float* of[kAtOnce];
 #pragma unroll
         for (int x = 0; x < kAtOnce; ++x) {
-          const float* of = p.part + __shfl_sync(0xffffffffu, place, x0 + x) * D + lane * kMine;
+          of[x] = p.part + __shfl_sync(0xffffffffu, place, x0 + x) * D + lane * kMine;
 #pragma unroll
-          for (int y = 0; y < Q; ++y) {
-            g[x][y] = __shfl_sync(0xffffffffu, weight[y], x0 + x);  // 0 where no key is seen
-            if (g[x][y] != 0.f) {
-              if constexpr (kMine == 4) *reinterpret_cast<float4*>(v[x][y]) = *reinterpret_cast<const float4*>(of + y * D);
-              else *reinterpret_cast<float2*>(v[x][y]) = *reinterpret_cast<const float2*>(of + y * D);
-            }
-          }
+          for (int y = 0; y < Q; ++y) g[x][y] = __shfl_sync(0xffffffffu, weight[y], x0 + x);  // 0 where no key is seen
         }
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x)
+#pragma unroll
+          for (int y = 0; y < Q; ++y)
+            if (g[x][y] != 0.f) {
+              if constexpr (kMine == 4) *reinterpret_cast<float4*>(v[x][y]) = *reinterpret_cast<const float4*>(of[x] + y * D);
+              else *reinterpret_cast<float2*>(v[x][y]) = *reinterpret_cast<const float2*>(of[x] + y * D);
+            }
 #pragma unroll
         for (int x = 0; x < kAtOnce; ++x)
 #pragma unroll
