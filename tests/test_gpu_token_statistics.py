@@ -139,6 +139,24 @@ def test_masked_and_non_finite_logits():
     assert g.isfinite().all() and not g[0, 3:].any() and not g[4, :4096].any()
 
 
+@pytest.mark.parametrize("v", [1000, 70001])
+def test_batches_that_share_their_logits(v):
+    """Expanded along the batch, along the rows or both: every row its own token, and the results of a copy (whose rows of an odd width begin elsewhere, so that sums run in another order)."""
+    for shape in ((1, 5, v), (60, 1, v), (1, 1, v)):
+        leaf = _logits(*shape).requires_grad_()
+        shared = leaf.expand(60, 5, v)
+        tokens = torch.randint(0, v, (60, 5), device=DEV)
+        s, want = ops.token_statistics(shared, tokens, top=3), _check(shared.detach().contiguous(), tokens, top=3, grads=False)
+        assert torch.equal(s.top_tokens, want.top_tokens)
+        for a, b in zip(s[:3], want[:3]):
+            assert ((a - b).abs() <= 4 * STEP * (180 + 4 * b.abs()) * (1 + b.abs())).all()
+        (g,) = torch.autograd.grad(s.logprobs.sum(), leaf)
+        assert g.shape == leaf.shape and g.isfinite().all()
+        if v % 8 == 0:
+            (same,) = torch.autograd.grad(ops.token_statistics(shared.contiguous(), tokens, top=3).logprobs.sum(), leaf)
+            assert torch.equal(g, same)
+
+
 def test_gradients_of_rows_that_are_not_finite():
     """NaN reaches the gradient of a row with any weight; a row without weight (padding, say) has zeros."""
     x = _logits(6, 3000)

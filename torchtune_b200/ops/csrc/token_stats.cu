@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(kOwnWarps<TOP> * 32, kCtas) row_kernel(const _
   [[maybe_unused]] OwnTop& sh = *reinterpret_cast<OwnTop*>(slots + warp * kOwnBytes<T, TOP> + kOwnSlots<T, TOP>);
   const uint32_t rows = p.rows, step = gridDim.x * kOwnWarps<TOP>, first = warp * gridDim.x + blockIdx.x;
   auto row_of = [&](uint32_t r) {
-    const uint32_t outer = p.step_outer == 0 ? 0u : r / p.inner;
+    const uint32_t outer = static_cast<uint32_t>(p.inner) >= rows ? 0u : r / p.inner;
     return Row<T>(static_cast<const T*>(p.x) + outer * p.step_outer + static_cast<long long>(r - outer * p.inner) * p.step_inner, p.vocab);
   };
   if (first >= rows) return;
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t step = gridDim.x / splits, rows = p.rows;  // below 2^31
   auto row_of = [&](uint32_t r) {
-    const uint32_t outer = p.step_outer == 0 ? 0u : r / p.inner;
+    const uint32_t outer = static_cast<uint32_t>(p.inner) >= rows ? 0u : r / p.inner;
     return Row<T>(static_cast<const T*>(p.x) + outer * p.step_outer + static_cast<long long>(r - outer * p.inner) * p.step_inner, p.vocab);
   };
   struct Part {  // of a row, in vectors and segments of 32 of them
