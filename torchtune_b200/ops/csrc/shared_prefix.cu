@@ -17,7 +17,7 @@
 //
 // Bound by bytes on long rows, else by what a piece does one after the other (products, softmax, products, output: 3 to 5 us, which the two CTAs of an SM hide from each other in part) and by the
 // start (finding the shares, first loads: 5 us) and the joining launch.  Measured (32 query on 8 key heads of 128 channels, kernels behind one another in a graph): 16 rows on 32003 shared keys and
-// 300 of their own 42 us (3.5 TB/s); 64 rows of 4 prompts of 613 and 391 own 32 us; 256 rows of three tokens, 8 prompts of 4096 and 1001 own 209 us (4.4 TB/s); one prompt of 61 11 us.
+// 300 of their own 40 us (3.7 TB/s); 64 rows of 4 prompts of 613 and 391 own 29 us; 256 rows of three tokens, 8 prompts of 4096 and 1001 own 197 us (4.7 TB/s); one prompt of 61 11 us.
 #include "common/attn_math.cuh"
 #include "common/ptx.cuh"
 #include "common/tmap.h"
@@ -429,18 +429,18 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
             }
           }
           tmem_st_wait();
-          if (last - k0 < kKeys) {  // the last tile: values that nobody sees may be anything, and 0 * NaN is NaN
-            const uint32_t slot = (2 * done + 1) % L::kSlots;
-            if (!(ok = mbar_wait(&full[slot], ((2 * done + 1) / L::kSlots) & 1))) break;
-            uint8_t* v = ring + slot * L::kSlot;
-            const int dead = kKeys - (last - k0);
-            for (int x = threadIdx.x; x < dead * L::kPanels * 8; x += live_warps * 32) {
-              const int key = kKeys - dead + x / (L::kPanels * 8), y = x % (L::kPanels * 8);
-              *reinterpret_cast<uint4*>(v + (y >> 3) * kPanel + key * 128 + (y & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-          }
           tc_fence_before();
+        }
+        if (last - k0 < kKeys && (warp >= live_warps || live_warps == 4)) {  // the last tile: values that nobody sees may be anything, and 0 * NaN is NaN; warps without rows see to it, if there are any
+          const uint32_t slot = (2 * done + 1) % L::kSlots;
+          if (!(ok = mbar_wait(&full[slot], ((2 * done + 1) / L::kSlots) & 1))) break;
+          uint8_t* v = ring + slot * L::kSlot;
+          const int dead = kKeys - (last - k0), from = live_warps == 4 ? 0 : live_warps * 32;
+          for (int x = threadIdx.x - from; x < dead * L::kPanels * 8; x += 128 - from) {
+            const int key = kKeys - dead + x / (L::kPanels * 8), y = x % (L::kPanels * 8);
+            *reinterpret_cast<uint4*>(v + (y >> 3) * kPanel + key * 128 + (y & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[done & 1]);
@@ -461,6 +461,14 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
           uint32_t v[32];
           tmem_ld_32x32(tO + lanes + ch * 32, v);
           tmem_ld_wait();
+          if (count <= 16) {  // few rows: straight from the registers (12 rows to a piece: 205 -> 197 us in all; where pieces have 128, the same from there 50 -> 54)
+            if (lane < count) {
+              float4* at = reinterpret_cast<float4*>(p.part + (base + r) * D + ch * 32);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) at[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+            }
+            continue;
+          }
 #pragma unroll
           for (int i = 0; i < 8; ++i) stage[lane * 8 + (i ^ (lane & 7))] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
           __syncwarp();
