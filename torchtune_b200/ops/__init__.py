@@ -591,8 +591,8 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     belongs to prompt ``r // (rows // prompts)``, whose slots ``prefix_start[prompt]`` ... ``prefix_stop[prompt] - 1`` it sees (int32, by default all ``n``), and of its own the first ``lengths[row]``
     (int32, by default all slots), of which its ``s`` queries are the last ones and see none behind their own.  Numbers out of range are cut off at it.  A query that sees no key gives 0, and what
     lies in slots that no query of a row sees has no influence; one that only later tokens of the same call see should be finite.  The prefix is read once for all rows of a prompt.  bf16 CUDA
-    tensors with 64 or 128 channels outside autograd take the kernels (for keys and values in strides that are multiples of 16 bytes, where they lie); everything else takes the plain statement,
-    which has gradients."""
+    tensors with 64 or 128 channels and up to 256 key heads outside autograd take the kernels (for keys and values in strides that are multiples of 16 bytes, where they lie); everything else takes
+    the plain statement, which has gradients.  The kernels are made for few queries per row: pieces of the softmax wait in fp32 for their join, with many query rows up to some 40 of them per key head."""
     shared_prefix.check_arguments(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, lengths)
     if q.numel() == 0:
         return torch.empty_like(q)
