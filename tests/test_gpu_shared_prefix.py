@@ -173,3 +173,17 @@ def test_same_as_attention_over_joined_keys():
     size = ops.attention(q, keys, values.abs(), ops.AttentionMask(causal=True)).float()
     # both are within the bound of _check
     assert ((ops.shared_prefix_attention(q, kp, vp, k, v).float() - want.float()).abs() <= 2.0**-7 * want.float().abs() + 2 * (2.0**-8 + 2.0**-12) * 1.01 * size).all()
+
+
+@pytest.mark.parametrize("d,hq,hkv,n,m", [(64, 8, 2, 3, 2), (128, 8, 8, 40, 25), (64, 64, 1, 100, 0), (128, 16, 4, 0, 70)])
+def test_probabilities_are_not_rounded_to_16_bits(d, hq, hkv, n, m):
+    """Values that cancel: outputs are far smaller than what they are sums of, whose roundings would show."""
+    q, kp, vp, k, v = _inputs(2, 40, 1, n, m, hq, hkv, d)
+    q.mul_(0.25), vp.sign_(), v.sign_()
+    out = ops.shared_prefix_attention(q, kp, vp, k, v).double()
+    want = reference.shared_prefix_attention(*(t.double() for t in (q, kp, vp, k, v)), None, None, None, None)
+    # the output's rounding; 2^-16 of a probability as two bf16 numbers; scores, sums of d <= 128 products whose sizes add up to less than 4 with the scale: 128 * 4 * 2^-24 = 2^-15; exponentials, sums and
+    # joins: some 50 roundings of 2^-24.  Sizes of values are 1.
+    far = (out - want).abs() - (2.0**-8 * want.abs() + 2.0**-16 + 2.0**-15 + 2.0**-18)
+    assert (far <= 0).all(), float(far.max())
+    _lib.check_device_errors()

@@ -5,7 +5,8 @@
 // A softmax over pieces: each piece leaves m = max, l = sum 2^(x - m) and O = sum 2^(x - m) v, and o = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i.  A piece is a run of keys of one key head with up
 // to 128 query rows: those of all rows of a prompt (answers x tokens x query heads that share the key head) on a run of the prefix, or those of one row on a run of its own keys.  Both are the
 // same work: scores of 128 rows and 64 keys on tcgen05 tensor cores, a thread per row for the softmax, probabilities in the scores' place in tensor memory as the A operand of the second
-// product, its accumulator next to them.  A tile of 64 keys and values is 32 KB: an SM's share of the memory's rate brings it in 1400 cycles, and 128 rows keep the tensor cores busy for 260 of them and the
+// product, its accumulator next to them.  They are two bf16 numbers each, a rounded one and the rest, which take the 32 bits of a score: rounded once, they would be the one rounding beside the output's that
+// shows (outputs 0.0023 from exact ones, of which the output's is 0.0017; now it is all there is), for up to 8 % of the time (256 rows of three tokens: 198 -> 214 us; one token of 16 and 64 rows: the same).  A tile of 64 keys and values is 32 KB: an SM's share of the memory's rate brings it in 1400 cycles, and 128 rows keep the tensor cores busy for 770 of them and the
 // exponentials' unit for 512, so that padding a single token's four rows to 128 costs nothing that is not idle; warps without rows have no part in the softmax.
 // Two CTAs to an SM share the tiles of all key heads out evenly, as they are: tiles of the prefixes in their order are one line, those of the rows another, CTAs get a stretch of one of them each
 // (with more than 128 query rows to a head, as many CTAs next to each other as there are tiles of rows, so that all but one find the keys in L2), and a piece ends where a head or a
@@ -206,6 +207,13 @@ __device__ __forceinline__ bool any_of_four(bool mine) {
   return any != 0;
 }
 
+// What two values' rounding to bf16 leaves over, rounded itself; the widening of the former is part of the difference.
+__device__ __forceinline__ uint32_t rest_of(float a, float b, uint32_t rounded) {
+  float x, y;
+  asm("{\n\t.reg .b16 lo, hi, one;\n\tmov.b32 {lo, hi}, %2;\n\tmov.b16 one, 0xbf80;\n\tfma.rn.f32.bf16 %0, lo, one, %3;\n\tfma.rn.f32.bf16 %1, hi, one, %4;\n\t}" : "=f"(x), "=f"(y) : "r"(rounded), "f"(a), "f"(b));
+  return pack_bf16x2(x, y);
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 2)
 piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ CUtensorMap tm_vp, const __grid_constant__ CUtensorMap tm_ko, const __grid_constant__ CUtensorMap tm_vo,
@@ -305,6 +313,8 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
           const uint32_t v_base = aR + slot * L::kSlot, from = tS + (done & 1) * kKeys;
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k) umma_f16_ts(tO, from + k * 8, make_smem_desc_sw128(v_base + k * 2048, kPanel, 1024), idesc_o, (j | k) != 0);
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k) umma_f16_ts(tO, from + kKeys / 2 + k * 8, make_smem_desc_sw128(v_base + k * 2048, kPanel, 1024), idesc_o, 1);
           umma_commit(&empty[slot]);
           umma_commit(&pv_done[done & 1]);
         }
@@ -400,21 +410,26 @@ piece_kernel(const __grid_constant__ CUtensorMap tm_kp, const __grid_constant__ 
           const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
           const uint64_t nm2 = pack_f32x2(neg_m, neg_m);
           uint64_t sum2[2] = {0ull, 0ull};
-          uint32_t pk[32];
 #pragma unroll
-          for (int i = 0; i < 64; i += 2) {
-            const uint64_t t = fma_f32x2(pack_u32x2(sv[i >> 5][i & 31], sv[i >> 5][(i & 31) + 1]), c2, nm2);
-            float t0, t1;
-            unpack_f32x2(t, t0, t1);
-            const float e0 = fast_exp2(t0), e1 = fast_exp2(t1);
-            sum2[(i >> 1) & 1] = add_f32x2(sum2[(i >> 1) & 1], pack_f32x2(e0, e1));
-            pk[i >> 1] = pack_bf16x2(e0, e1);  // the second product's operand; the sum keeps 32 bits
+          for (int half = 0; half < 2; ++half) {
+            uint32_t hi[16], lo[16];  // the second product's operand: probabilities rounded to 8 bits, and what that leaves over, so that it has 16
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const uint64_t t = fma_f32x2(pack_u32x2(sv[half][i], sv[half][i + 1]), c2, nm2);
+              float t0, t1;
+              unpack_f32x2(t, t0, t1);
+              const float e0 = fast_exp2(t0), e1 = fast_exp2(t1);
+              sum2[(i >> 1) & 1] = add_f32x2(sum2[(i >> 1) & 1], pack_f32x2(e0, e1));
+              hi[i >> 1] = pack_bf16x2(e0, e1);
+              lo[i >> 1] = rest_of(e0, e1, hi[i >> 1]);
+            }
+            tmem_st_32x16(tile + half * 16, hi);
+            tmem_st_32x16(tile + 32 + half * 16, lo);
           }
           float s0, s1, s2, s3;
           unpack_f32x2(sum2[0], s0, s1);
           unpack_f32x2(sum2[1], s2, s3);
           l = l * alpha + (s0 + s1) + (s2 + s3);
-          tmem_st_32x32(tile, pk);
           if (j > 0 && __any_sync(0xffffffffu, rescale)) {
             if (!(ok = mbar_wait(&pv_done[(done - 1) & 1], ((done - 1) >> 1) & 1))) break;  // the second product before this one has left the output
             tc_fence_after();
