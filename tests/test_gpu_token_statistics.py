@@ -264,3 +264,15 @@ def test_rows_beyond_32_bits():
     assert torch.equal(s.top_tokens[-1:], want[3])
     torch.testing.assert_close(s.logprobs[-1:].double(), want[0], rtol=1e-5, atol=1e-5)
     torch.testing.assert_close(s.entropy[-1:].double(), want[1], rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,v,top", [(640, 1000, 5), (640, 3000, 40), (640, 12000, 64), (3, 50000, 7)])
+def test_rows_of_nan_keep_the_first_index(rows, v, top, dtype):
+    """All of them equal and above all numbers: the choice of one alternative after the other, too, begins at index 0."""
+    x = _logits(rows, v, dtype=dtype)
+    x[::2] = float("nan")
+    x[1::4, 0] = float("nan")
+    s = ops.token_statistics(x, torch.zeros(rows, dtype=torch.int64, device=DEV), top=top)
+    assert torch.equal(s.top_tokens, torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :top])
+    assert s.top_logprobs[::2].isnan().all()

@@ -571,7 +571,7 @@ __device__ __forceinline__ void choose_alone(const Row<T>& row, int want, float 
   }
   // many equal or ordered logits: one alternative after the other
   const int n = choose(sh.segments, segments, want, sh.chosen);
-  Entry last = ~0ull;
+  Entry last = 0;
   for (int x = 0; x < want; ++x) {
     Entry best = 0;
     for (int i = 0; i < n; ++i) {
@@ -581,7 +581,7 @@ __device__ __forceinline__ void choose_alone(const Row<T>& row, int want, float 
       for (int k = 0; k < 8; ++k) {
         const int e = j * 8 - row.off + k;
         const Entry entry = e >= 0 && e < row.vocab ? entry_of(key_of<T>(widened(raw.v[k])), e) : 0;
-        if (entry < last && entry > best) best = entry;
+        if ((x == 0 || entry < last) && entry > best) best = entry;  // nothing bounds the first: a NaN of 32 bits at index 0 is the largest number
       }
     }
     const uint32_t high = __reduce_max_sync(0xffffffffu, key_in(best));
