@@ -276,3 +276,22 @@ def test_rows_of_nan_keep_the_first_index(rows, v, top, dtype):
     s = ops.token_statistics(x, torch.zeros(rows, dtype=torch.int64, device=DEV), top=top)
     assert torch.equal(s.top_tokens, torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :top])
     assert s.top_logprobs[::2].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,v", [(700, 600), (700, 9001), (300, 70000), (3, 128256)])
+def test_sure_tokens(rows, v, dtype):
+    """One token far above another one, and nothing else: probabilities do not go above 1 nor entropies below 0."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.full((rows, v), -80.0, device=DEV)
+    first, sure = torch.randint(0, 8, (rows,), generator=g, device=DEV), 256 + torch.randint(0, 8, (rows,), generator=g, device=DEV)  # the same lane's elements
+    x.scatter_(1, first[:, None], 0.0)
+    x.scatter_(1, sure[:, None], 12 + 5 * torch.rand(rows, 1, generator=g, device=DEV))
+    x = x.to(dtype)
+    s = ops.token_statistics(x, sure, top=2)
+    want = reference.token_statistics(x.double(), sure, 1.0, 2, -100)
+    assert (s.logprobs <= 0).all() and (s.top_logprobs <= 0).all() and (s.entropy >= 0).all()
+    # sums of 1 + 2^-17 and less: a rounding for each of some 12 joins of lanes and warps; t is below 2^-12 and its roundings nothing; the logarithm is one step off, the product with ln 2 half of one
+    assert (s.logprobs.double() - want[0]).abs().max() <= 16 * STEP
+    assert (s.top_logprobs[:, 0].double() - want[2][:, 0]).abs().max() <= 16 * STEP
+    assert (s.entropy.double() - want[1]).abs().max() <= 16 * STEP

@@ -1,10 +1,12 @@
 // Log-probabilities of given tokens with the entropy and the likeliest alternatives, from one pass over the logits, and their gradient in one more.
 //
-// Of z = x / T, in units of log2 (c = log2(e) / T):  d = (x - base) c,  s = sum 2^d,  t = sum 2^d d,  base so that 2^d stays below 2^24, so that
-//   log p = ln2 (d - log2 s)        H = -sum p log p = ln2 (log2 s - t / s),
-// where both terms stay below some 40: little cancels.  When the base moves up by a / c, s' = s 2^-a and t' = (t - a s) 2^-a.  A base that followed every new maximum would move in nearly all
-// steps of a warp, since one of its 32 lanes has a new one; so it hardly ever moves after a thread's first elements.  Differences are taken before they are scaled: a row of a type's lowest values is
-// one of equal logits.
+// Of z = x / T, in units of log2 (c = log2(e) / T):  d = (x - base) c,  s = sum 2^d,  t = sum 2^d d,  with a base less than some four powers of two from the maximum, so that
+//   log p = ln2 (d - log2 s)        H = -sum p log p = ln2 (log2 s - t / s)
+// are differences of numbers that are small where the results are.  Near certainty what is left of them is their roundings: some 5e-7 of log p and 2e-6 of H (400 x 128256 with one token 14 above the
+// others' maximum; with a base up to 2^24 away 2e-6 and 1e-5), neither of which crosses 0.  When the base moves up by a / c, s' = s 2^-a and t' = (t - a s) 2^-a.  A base that followed every new
+// maximum would move in nearly all steps of a warp, since one of its 32 lanes has a new one; so it begins four powers of two above the maximum of the warp's first 256 elements, and a lane whose elements
+// go four above it moves its own.  Rows in rising order, whose lanes move it all the time, take 1.1 to 1.35 times as long (8192 x 8000 bf16 41 -> 55 us).  Differences are taken before they are
+// scaled: a row of a type's lowest values is one of equal logits.
 // With g, h and k_j the gradients of the token's log-probability, of the entropy and of the alternatives' log-probabilities:
 //   dx_v = ([v = token] g + sum_j [v = alternative j] k_j - p_v (g + sum_j k_j + h (log p_v + H))) / T.
 //
@@ -63,7 +65,8 @@ static constexpr int kMaxSegments = 1024;  // of a CTA
 static constexpr int kMaxCluster = 8;
 static constexpr float kLn2 = 0.6931471805599453f;
 static constexpr float kLowest = -200.f;  // 2^kLowest is 0 in fp32
-static constexpr float kMostAllowed = 0x1p24f;  // sum of the exponentials of eight elements
+static constexpr float kMostAllowed = 16.f;  // sum of the exponentials of eight elements: eight equal to the base leave as much room again
+static constexpr float kLift = 4.f;         // powers of two from a warp's first maximum up to its first base
 
 struct Params {
   const void* x;  // row r at x + (r / inner) * step_outer + (r % inner) * step_inner, in elements
@@ -76,7 +79,7 @@ struct Params {
   long long* top_tokens;
   long long ignore, rows;
   int inner, vocab, top;
-  float c, rate;  // log2(e) / T and 1 / T
+  float c, rate, lift;  // log2(e) / T, 1 / T and kLift / c
 };
 struct GradParams {
   const void* x;
@@ -212,6 +215,9 @@ struct Running {
   float c;
   float most_allowed = -1.f, base = 0.f;  // there is no base until there is a logit above the infinitely low ones
   uint64_t s2 = 0, t2 = 0;
+  __device__ __forceinline__ void begin(float most) {  // of the whole warp; a row that begins with NaN or infinitely low logits leaves its lanes to themselves
+    if (most > -INFINITY) base = most, most_allowed = kMostAllowed;
+  }
   __device__ __forceinline__ Sums sums() const {
     float s0, s1, t0, t1;
     unpack_f32x2(s2, s0, s1), unpack_f32x2(t2, t0, t1);
@@ -461,6 +467,8 @@ __device__ __forceinline__ void gather_from(const typename Row<T>::Vector& raw0,
   }
 }
 
+// What cannot be above 0 but for roundings; NaN stays.
+__device__ __forceinline__ float at_most_0(float x) { return x > 0.f ? 0.f : x; }
 // The results of a row, by one warp, with its alternatives in order.
 template <typename T, bool TOP>
 __device__ __forceinline__ void finish(const Params& p, long long r, long long token, float logit, const Sums& sum, const Entry* entries) {
@@ -470,16 +478,17 @@ __device__ __forceinline__ void finish(const Params& p, long long r, long long t
     for (int x = lane; x < p.top; x += 32) {
       const Entry e = entries[x];
       p.top_tokens[r * p.top + x] = index_in(e);
-      p.top_logprobs[r * p.top + x] = (value_of<T>(key_in(e)) - sum.base) * p.rate - log_s * kLn2;
+      p.top_logprobs[r * p.top + x] = at_most_0((value_of<T>(key_in(e)) - sum.base) * p.rate - log_s * kLn2);
     }
     __syncwarp();
   }
   if (lane == 0) {
     float lp = 0.f;
-    if (token >= 0 && token < p.vocab) lp = (logit - sum.base) * p.rate - log_s * kLn2;
+    if (token >= 0 && token < p.vocab) lp = at_most_0((logit - sum.base) * p.rate - log_s * kLn2);
     else if (token != p.ignore) TTB_NOTE_VIOLATION(token_stats);  // as a row that is ignored
     p.logprobs[r] = token == p.ignore ? 0.f : lp;
-    p.entropy[r] = (log_s - sum.t / sum.s) * kLn2;
+    const float entropy = (log_s - sum.t / sum.s) * kLn2;
+    p.entropy[r] = entropy < 0.f ? 0.f : entropy;
     if (p.stats != nullptr) p.stats[2 * r] = sum.base, p.stats[2 * r + 1] = log_s;
   }
 }
@@ -656,6 +665,7 @@ __global__ void __launch_bounds__(kOwnWarps<TOP> * 32, kCtas) row_kernel(const _
 #pragma unroll
           for (int x = 0; x < kPieces; ++x) reinterpret_cast<uint4*>(raw.v)[x] = *reinterpret_cast<const uint4*>(at + x * kPieceBytes + a * 512);
           if constexpr (TOP) note(j0 + a * 32, most_of_vector<T>(raw));
+          if (a == 0 && j0 == 0) run.begin(warp_max_nan(most_of_vector<T>(raw)) + p.lift);
           run.take<T>(raw, c2);
         }
       } else {
@@ -664,6 +674,7 @@ __global__ void __launch_bounds__(kOwnWarps<TOP> * 32, kCtas) row_kernel(const _
           float f[8];
           widen8(row.load(j0 + a * 32 + lane), f);
           note(j0 + a * 32, most_of(f));
+          if (a == 0 && j0 == 0) run.begin(warp_max_nan(most_of(f)) + p.lift);
           run.careful(f);
         }
       }
@@ -816,7 +827,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
           if (lane == 0) sh.segments[buffer][(j - part.first) >> 5] = __float_as_uint(m);  // the warp that ends the row makes a key of it
         }
       };
-      for (int j0 = part.first + warp * kRun<T, TOP>; j0 < part.end; j0 += kWarps * kRun<T, TOP>) {
+      const int first = part.first + warp * kRun<T, TOP>;
+      for (int j0 = first; j0 < part.end; j0 += kWarps * kRun<T, TOP>) {
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         copy_ahead();  // to the slot before this one
         if (whole(row, part, j0)) {
@@ -827,6 +839,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
 #pragma unroll
             for (int x = 0; x < kPieces; ++x) reinterpret_cast<uint4*>(raw.v)[x] = *reinterpret_cast<const uint4*>(at + x * kPieceBytes + a * 512);
             if constexpr (TOP) note(j0 + a * 32, most_of_vector<T>(raw));
+            if (a == 0 && j0 == first) run.begin(warp_max_nan(most_of_vector<T>(raw)) + p.lift);
             run.take<T>(raw, c2);
           }
         } else {
@@ -841,6 +854,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) stats_kernel(const __grid_con
               for (int i = 0; i < 8; ++i) f[i] = -INFINITY;
             }
             note(j0 + a * 32, most_of(f));
+            if (a == 0 && j0 == first) run.begin(warp_max_nan(most_of(f)) + p.lift);
             run.careful(f);
           }
         }
@@ -1114,7 +1128,7 @@ static int launch(const Call& c, float log2_rate, float rate, cudaStream_t st) {
   p.x = reinterpret_cast<const void*>(c.x), p.step_outer = c.step_outer, p.step_inner = c.step_inner, p.tokens = reinterpret_cast<const long long*>(c.tokens);
   p.logprobs = reinterpret_cast<float*>(c.logprobs), p.entropy = reinterpret_cast<float*>(c.entropy), p.stats = reinterpret_cast<float*>(c.stats);
   p.top_logprobs = reinterpret_cast<float*>(c.top_logprobs), p.top_tokens = reinterpret_cast<long long*>(c.top_tokens);
-  p.ignore = c.ignore, p.rows = c.rows, p.inner = static_cast<int>(c.inner), p.vocab = static_cast<int>(c.vocab), p.top = static_cast<int>(c.top), p.c = log2_rate, p.rate = rate;
+  p.ignore = c.ignore, p.rows = c.rows, p.inner = static_cast<int>(c.inner), p.vocab = static_cast<int>(c.vocab), p.top = static_cast<int>(c.top), p.c = log2_rate, p.rate = rate, p.lift = kLift / log2_rate;
   const long long segments = (c.vocab + 7 + 255) / 256;
   // A warp for a row, where there are rows for a good part of all warps.  us with CTAs for rows -> with warps, without / with 20 alternatives: bf16 600 x 2000 18 -> 12 / 51 -> 16, 8192 x 8000
   // 121 -> 43 / 317 -> 96, 8192 x 32000 141 -> 117 / 352 -> 180, fp32 8192 x 32000 184 -> 184 / 377 -> 240; on the other side bf16 600 x 32000 19 -> 29 / 47 -> 45, 333 x 50257 25 -> 41 / 39 -> 59,
