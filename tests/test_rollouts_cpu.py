@@ -160,3 +160,42 @@ def test_grpo_recipe_with_shared_prompts_and_entropy(tmp_path, tune_path, monkey
     for k in ("rewards", "response_lengths"):
         assert logs["plain"][k] == logs["shared"][k]
     assert logs["bonus"]["loss"][0] == pytest.approx(logs["plain"]["loss"][0] - 0.5 * logs["bonus"]["entropy"][0], abs=1e-3)
+
+
+def test_entropy_bonus_does_not_depend_on_the_size_of_the_pieces():
+    """Answers of 1 to 6 tokens: gradients and the logged entropy of one pass over all of them and of pieces."""
+    from torchtune_b200.dev.grpo import GRPOSimpleLoss, GRPOTrajectory
+    from torchtune_b200.engine.grpo import GRPOTrainer
+
+    n, ctx, m = 5, 4, 6
+    g = torch.Generator().manual_seed(4)
+    tokens = torch.randint(1, 90, (n, ctx + m), generator=g)
+    pad = torch.arange(m) >= torch.tensor([1, 6, 3, 2, 5])[:, None]
+    ones = torch.ones(n, ctx + m, dtype=torch.bool)
+    traj = GRPOTrajectory(query_responses=tokens, logprobs=torch.randn(n, m, generator=g) - 4, ref_logprobs=torch.randn(n, m, generator=g) - 4, advantages=torch.randn(n, generator=g),
+                          masks=generation.get_causal_mask_from_padding_mask(ones), position_ids=generation.get_position_ids_from_padding_mask(ones), response_padding_masks=pad, seq_lens=None, answers=None)
+    seen = []
+    for size in (5, 1, 2):
+        trainer = GRPOTrainer.__new__(GRPOTrainer)
+        trainer._model = _llama()
+        trainer._device, trainer.parallel, trainer._lr_scheduler, trainer._clip_grad_norm, trainer.global_step = torch.device("cpu"), None, None, None, 0
+        trainer._forward_batch_size, trainer._temperature, trainer._log_entropy, trainer._entropy_coeff, trainer._loss_fn = size, 0.9, True, 0.7, GRPOSimpleLoss(kl_coeff=0.1)
+        grads = []
+
+        class Keep:
+            def step(self, of=trainer._model):
+                grads.extend(p.grad.clone() for p in of.parameters())
+
+            def zero_grad(self, set_to_none):
+                pass
+
+        trainer._optimizer = Keep()
+        stats = trainer.grpo_step(traj, ctx)
+        seen.append((stats.metadata["entropy"], stats.loss, *grads))
+    logits = _llama()(tokens)[:, ctx - 1 : -1] / 0.9
+    h = -(torch.softmax(logits, -1) * torch.log_softmax(logits, -1)).sum(-1)
+    want = torch.stack([row[~p].mean() for row, p in zip(h, pad)]).mean()
+    torch.testing.assert_close(seen[0][0], want.detach(), rtol=1e-5, atol=1e-5)
+    for other in seen[1:]:
+        for a, b in zip(seen[0], other):
+            torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-6)

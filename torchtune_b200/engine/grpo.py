@@ -113,7 +113,7 @@ class GRPOTrainer:
         self._temperature = cfg.get("temperature", 1.0)
         self._top_k = cfg.get("top_k")
         self._share_prompts = cfg.get("share_prompts", False)  # a prompt's answers read its keys and values from one place (generation.generate_group)
-        self._entropy_coeff = cfg.get("entropy_coeff", 0.0)  # weight of the policy's mean entropy, which the loss is lowered by
+        self._entropy_coeff = cfg.get("entropy_coeff", 0.0)  # weight of the policy's entropy (mean over responses of the mean over their tokens), which the loss is lowered by
         self._log_entropy = cfg.get("log_entropy", False) or self._entropy_coeff != 0.0
         self._total_steps = cfg.num_steps
         self._total_epochs = cfg.get("epochs", 1)
@@ -189,7 +189,7 @@ class GRPOTrainer:
             pad, entropy = traj.response_padding_masks[idx], None
             if self._log_entropy:
                 pi, entropy = self._response_statistics(self._model, traj.query_responses[idx], traj.masks[idx], traj.position_ids[idx], ctx)
-                entropy = rlhf.masked_mean(entropy, ~pad)
+                entropy = rlhf.masked_mean(entropy, ~pad, dim=1).mean()  # of responses, as the loss is, so that it does not depend on the size of the pieces
             else:
                 pi = self._response_logprobs(self._model, traj.query_responses[idx], traj.masks[idx], traj.position_ids[idx], ctx)
             pi = pi.masked_fill(pad, 1.0)
