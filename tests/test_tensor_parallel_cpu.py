@@ -273,3 +273,55 @@ def test_tp_generation_model_of_an_early_fusion_model_is_built_layer_by_layer():
         assert not r["meta_left"]
         assert r["expert_cols"] == 48 // world  # the experts' columns are split, the vision tower is whole
         torch.testing.assert_close(r["logits"].float(), want.float(), rtol=1e-4, atol=1e-4)
+
+
+# ----------------------------------------------------------------------------- norms and rotation of queries and keys as one operator
+QK_ARCH = dict(vocab_size=64, num_layers=2, num_heads=4, num_kv_heads=2, embed_dim=32, head_dim=16, max_seq_len=32, intermediate_dim=48, norm_eps=1e-6, q_proj_bias=False, k_proj_bias=False,
+               v_proj_bias=False, q_norm=True, k_norm=True, fuse_qk_norm=True)
+
+
+def _qk_model():
+    from torchtune_b200.models.qwen3 import qwen3
+
+    model = qwen3(**QK_ARCH)
+    fixed_init_(model, std=0.1)
+    return model
+
+
+def _qk_worker(rank, world, port, results):
+    from torchtune_b200 import ops
+
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        calls, fused = [], ops.qk_norm_rope
+        ops.qk_norm_rope = lambda *a, **how: calls.append(1) or fused(*a, **how)
+        tpm = tensor_parallelize(_qk_model(), TensorParallelContext(torch.device("cpu"), max_rows_per_rank=8, max_width=64))
+        tokens, labels = _data()
+        loss = F.cross_entropy(tpm(tokens).reshape(-1, 64), tpm.shard_rows(labels).reshape(-1), ignore_index=-100, reduction="sum")
+        loss.backward()
+        tpm.sync_replicated_grads()
+        trained = len(calls)
+        with torch.no_grad():
+            got = tpm.forward_inference(tokens)
+        attn = tpm.layers[1].attn
+        results[rank] = dict(trained=trained, inferred=len(calls) - trained, logits=got, wqkv=attn.wqkv.grad.clone())
+    finally:
+        dist.destroy_process_group()
+
+
+def test_tp_decoder_keeps_the_fused_norms_and_rotation():
+    world = 2
+    results = mp.Manager().dict()
+    mp.spawn(_qk_worker, args=(world, 29567, results), nprocs=world, join=True)
+    model = _qk_model()
+    tokens, labels = _data()
+    logits = model(tokens)
+    F.cross_entropy(logits.reshape(-1, 64), labels.reshape(-1), ignore_index=-100, reduction="sum").backward()
+    attn = model.layers[1].attn
+    for rank in range(world):
+        r = results[rank]
+        assert r["trained"] == r["inferred"] == QK_ARCH["num_layers"]
+        torch.testing.assert_close(r["logits"], logits.detach(), rtol=1e-4, atol=1e-4)
+        q, k, v = (getattr(attn, f"{x}_proj").weight.grad.chunk(world)[rank] for x in "qkv")
+        torch.testing.assert_close(r["wqkv"], torch.cat([q, k, v]), rtol=1e-4, atol=1e-5)

@@ -27,6 +27,14 @@ def _as_mask(mask: MaskLike, default_causal: bool) -> AttentionMask:
     return AttentionMask(causal=False, bool_mask=mask)
 
 
+def norms_and_rotates(attn: nn.Module) -> bool:
+    """Whether norms and rotation of an attention's queries and keys are one operator (its ``fuse_qk_norm``)."""
+    pe, norms = attn.pos_embeddings, (attn.q_norm, attn.k_norm)
+    if not attn.fuse_qk_norm or any(type(m) is not RMSNorm or has_hooks(m) for m in norms) or norms[0].eps != norms[1].eps:
+        return False
+    return isinstance(pe, RotaryPositionalEmbeddings) and type(pe).forward is RotaryPositionalEmbeddings.forward and not has_hooks(pe)
+
+
 class MultiHeadAttention(nn.Module):
     """Attention with ``num_kv_heads <= num_heads`` key/value heads.
 
@@ -128,13 +136,6 @@ class MultiHeadAttention(nn.Module):
             cache.advance(s)
         return out
 
-    def _norms_and_rotates(self) -> bool:
-        """Whether norms and rotation of queries and keys may be one operator."""
-        pe, norms = self.pos_embeddings, (self.q_norm, self.k_norm)
-        if not self.fuse_qk_norm or any(type(m) is not RMSNorm or has_hooks(m) for m in norms) or norms[0].eps != norms[1].eps:
-            return False
-        return isinstance(pe, RotaryPositionalEmbeddings) and type(pe).forward is RotaryPositionalEmbeddings.forward and not has_hooks(pe)
-
     def _norm_and_rotate(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, input_pos: Optional[torch.Tensor]) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         """Queries and keys; ``None`` for the keys if they and the values have gone to the cache."""
         pe, cache, gains = self.pos_embeddings, self.kv_cache, (self.q_norm.scale, self.k_norm.scale)
@@ -174,7 +175,7 @@ class MultiHeadAttention(nn.Module):
         if k is not None:
             k, v = (t.view(b, s_x, self.num_kv_heads, self.head_dim) for t in (k, v))
             rotated = self._rotate_into_cache(q, k, v, input_pos)
-        fused = rotated is None and y is x and self._norms_and_rotates()
+        fused = rotated is None and y is x and norms_and_rotates(self)
         if rotated is not None:
             q, k, v = rotated, None, None
         elif fused:

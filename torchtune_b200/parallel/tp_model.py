@@ -17,7 +17,7 @@ checkpoint layout (``layers.N.attn.q_proj.weight`` …).
 """
 from __future__ import annotations
 
-from typing import Any, Dict, List, Optional
+from typing import Any, Dict, List, Optional, Tuple
 
 import torch
 import torch.distributed as dist
@@ -25,7 +25,7 @@ from torch import nn
 
 from .. import ops
 from ..modules import TransformerDecoder, TransformerSelfAttentionLayer
-from ..modules.attention import _as_mask
+from ..modules.attention import _as_mask, norms_and_rotates
 from .tp import TensorParallelContext, column_parallel_linear, row_parallel_linear
 
 
@@ -91,7 +91,7 @@ class TPAttention(nn.Module):
         in_per = attn.output_proj.weight.shape[1] // w
         self.wo = nn.Parameter(attn.output_proj.weight.data[:, r * in_per : (r + 1) * in_per].contiguous())
         self.pos_embeddings, self.q_norm, self.k_norm = attn.pos_embeddings, attn.q_norm, attn.k_norm
-        self.qk_norm_before_rope = getattr(attn, "qk_norm_before_rope", False)
+        self.qk_norm_before_rope, self.fuse_qk_norm = getattr(attn, "qk_norm_before_rope", False), getattr(attn, "fuse_qk_norm", False)
         self.is_causal, self.scale, self.softcap = attn.is_causal, attn.scale, attn.softcap
 
     def _pos(self, t: torch.Tensor, norm: Optional[nn.Module], input_pos) -> torch.Tensor:
@@ -103,12 +103,18 @@ class TPAttention(nn.Module):
             t = norm(t)
         return t
 
+    def _placed(self, q: torch.Tensor, k: torch.Tensor, input_pos) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Queries and keys of the local heads behind their norms and the rotation."""
+        if norms_and_rotates(self):
+            return ops.qk_norm_rope(q, k, self.q_norm.scale, self.k_norm.scale, self.pos_embeddings.cache, input_pos, eps=self.q_norm.eps, interleaved=self.pos_embeddings.interleaved,
+                                    norm_first=self.qk_norm_before_rope)
+        return self._pos(q, self.q_norm, input_pos), self._pos(k, self.k_norm, input_pos)
+
     def forward(self, hn: torch.Tensor, residual: torch.Tensor, b: int, s: int, mask, input_pos) -> torch.Tensor:
         hd = self.head_dim
         qkv = _column(hn, self.wqkv, self.tp, self.fp8)  # [b·s, (h + 2·h_kv)·hd] for the local heads
         nq, nk = self.heads * hd, self.kv_heads * hd
-        q = self._pos(qkv[:, :nq].reshape(b, s, self.heads, hd), self.q_norm, input_pos)
-        k = self._pos(qkv[:, nq : nq + nk].reshape(b, s, self.kv_heads, hd), self.k_norm, input_pos)
+        q, k = self._placed(qkv[:, :nq].reshape(b, s, self.heads, hd), qkv[:, nq : nq + nk].reshape(b, s, self.kv_heads, hd), input_pos)
         v = qkv[:, nq + nk :].reshape(b, s, self.kv_heads, hd)
         out = ops.attention(q.contiguous(), k.contiguous(), v.contiguous(), _as_mask(mask, default_causal=self.is_causal and mask is None), scale=self.scale, softcap=self.softcap)
         return _row(out.reshape(b * s, nq), self.wo, self.tp, residual, self.fp8)
@@ -126,8 +132,7 @@ class TPAttention(nn.Module):
         hd = self.head_dim
         qkv = ops.linear(hn, self.wqkv)
         nq, nk = self.heads * hd, self.kv_heads * hd
-        q = self._pos(qkv[..., :nq].reshape(b, s, self.heads, hd), self.q_norm, input_pos)
-        k = self._pos(qkv[..., nq : nq + nk].reshape(b, s, self.kv_heads, hd), self.k_norm, input_pos)
+        q, k = self._placed(qkv[..., :nq].reshape(b, s, self.heads, hd), qkv[..., nq : nq + nk].reshape(b, s, self.kv_heads, hd), input_pos)
         v = qkv[..., nq + nk :].reshape(b, s, self.kv_heads, hd)
         cache = getattr(self, "kv_cache", None)
         if cache is not None:
