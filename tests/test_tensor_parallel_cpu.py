@@ -2,6 +2,7 @@
 re-assembled checkpoint must equal the single-process model."""
 import os
 
+import pytest
 import torch
 import torch.distributed as dist
 import torch.multiprocessing as mp
@@ -280,10 +281,10 @@ QK_ARCH = dict(vocab_size=64, num_layers=2, num_heads=4, num_kv_heads=2, embed_d
                v_proj_bias=False, q_norm=True, k_norm=True, fuse_qk_norm=True)
 
 
-def _qk_model():
+def _qk_model(fuse=True):
     from torchtune_b200.models.qwen3 import qwen3
 
-    model = qwen3(**QK_ARCH)
+    model = qwen3(**{**QK_ARCH, "fuse_qk_norm": fuse})
     fixed_init_(model, std=0.1)
     return model
 
@@ -325,3 +326,31 @@ def test_tp_decoder_keeps_the_fused_norms_and_rotation():
         torch.testing.assert_close(r["logits"], logits.detach(), rtol=1e-4, atol=1e-4)
         q, k, v = (getattr(attn, f"{x}_proj").weight.grad.chunk(world)[rank] for x in "qkv")
         torch.testing.assert_close(r["wqkv"], torch.cat([q, k, v]), rtol=1e-4, atol=1e-5)
+
+
+def _qk_grad_worker(rank, world, port, fuse, results):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        tpm = tensor_parallelize(_qk_model(fuse), TensorParallelContext(torch.device("cpu"), max_rows_per_rank=8, max_width=64))
+        tokens, labels = _data()
+        F.cross_entropy(tpm(tokens).reshape(-1, 64), tpm.shard_rows(labels).reshape(-1), ignore_index=-100, reduction="sum").backward()
+        tpm.sync_replicated_grads()
+        results[rank] = [getattr(layer.attn, name).scale.grad.clone() for layer in tpm.layers for name in ("q_norm", "k_norm")]
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("fuse", [False, True])
+def test_tp_decoder_sums_the_gains_of_queries_and_keys(fuse):
+    """Every rank has the gradients of its own heads: the gains, which all heads share, are replicated parameters."""
+    world = 2
+    results = mp.Manager().dict()
+    mp.spawn(_qk_grad_worker, args=(world, 29569 + 2 * fuse, fuse, results), nprocs=world, join=True)
+    model = _qk_model(fuse)
+    tokens, labels = _data()
+    F.cross_entropy(model(tokens).reshape(-1, 64), labels.reshape(-1), ignore_index=-100, reduction="sum").backward()
+    want = [getattr(layer.attn, name).scale.grad for layer in model.layers for name in ("q_norm", "k_norm")]
+    for rank in range(world):
+        for got, exact in zip(results[rank], want):
+            torch.testing.assert_close(got, exact, rtol=1e-4, atol=1e-5)

@@ -320,6 +320,9 @@ class TPDecoder(nn.Module):
         self._replicated = [p for m in (self.tok_embeddings, self.norm, self.output) for p in m.parameters()]
         for layer in self.layers:
             self._replicated += list(layer.sa_norm.parameters()) + list(layer.mlp_norm.parameters())
+            for norm in (layer.attn.q_norm, layer.attn.k_norm):  # shared by all heads, of which a rank has its own
+                if isinstance(norm, nn.Module):
+                    self._replicated += list(norm.parameters())
             if isinstance(layer.mlp, TPMoE):
                 self._replicated += layer.mlp.replicated_parameters()
         seen = set()
