@@ -92,3 +92,25 @@ def test_refusals():
         with pytest.raises(ValueError):
             call(**how)
     assert ops.shared_prefix_attention(q[:0], kp[:0], vp[:0], k[:0], v[:0]).shape == (0, 1, 4, 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_statement_does_not_repeat_the_prefix(dtype):
+    """Nothing of the size of every row's own copy of its prompt's keys is made, forward or backward."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Largest(TorchDispatchMode):
+        size = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            for t in out if isinstance(out, (tuple, list)) else (out,):
+                if isinstance(t, torch.Tensor):
+                    self.size = max(self.size, t.numel() if t._base is None else 0)
+            return out
+
+    prompts, rows, n, d = 2, 48, 160, 64
+    t = [x.requires_grad_() for x in _inputs(prompts, rows, 1, n, 3, 4, 2, d, dtype)]
+    with Largest() as seen:
+        ops.shared_prefix_attention(*t, prefix_start=_int(3, 0)).square().sum().backward()
+    assert seen.size <= 2 * rows * 4 * (n + 3) < rows * n * 2 * d / 4

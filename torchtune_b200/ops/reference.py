@@ -176,24 +176,32 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     rows, s, hq, d = q.shape
     prompts, n, hkv, _ = k_prefix.shape
     m, dev, wide = k.shape[1], q.device, torch.promote_types(q.dtype, torch.float32)
+    per, group = rows // prompts, hq // hkv
     at = torch.arange(n, device=dev)
     shared = torch.ones(prompts, n, dtype=torch.bool, device=dev)
     if prefix_start is not None:
         shared &= at >= prefix_start[:, None]
     if prefix_stop is not None:
         shared &= at < prefix_stop[:, None]
-    shared = shared.repeat_interleave(rows // prompts, 0)
     length = torch.full((rows,), m, device=dev) if lengths is None else lengths.clamp(0, m).long()
     last = length[:, None] - s + torch.arange(s, device=dev)
-    seen = torch.cat([shared[:, None].expand(rows, s, n), torch.arange(m, device=dev) <= last[..., None]], -1)  # [rows, s, n + m]
-    any_seen = torch.cat([shared, torch.arange(m, device=dev) < length[:, None]], -1)[..., None, None]
-    keys, values = (torch.cat([a.repeat_interleave(rows // prompts, 0), b], 1).to(wide).masked_fill(~any_seen, 0.0) for a, b in ((k_prefix, k), (v_prefix, v)))
-    qh = q.to(wide).view(rows, s, hkv, hq // hkv, d).permute(0, 2, 3, 1, 4)
-    score = (qh @ keys.permute(0, 2, 3, 1).unsqueeze(2)) * (d**-0.5 if scale is None else scale)
-    score = score.masked_fill(~seen[:, None, None], float("-inf"))
+    seen = torch.cat([shared.repeat_interleave(per, 0)[:, None].expand(rows, s, n), torch.arange(m, device=dev) <= last[..., None]], -1)  # [rows, s, n + m]
+    # [prompts or rows, h_kv, slots, d]; a prompt's keys meet the queries of all its rows in one product, so that they are not repeated
+    (kp, vp), (ko, vo) = ([t.to(wide).masked_fill(~visible[..., None, None], 0.0).transpose(1, 2) for t in pair]
+                          for pair, visible in (((k_prefix, v_prefix), shared), ((k, v), torch.arange(m, device=dev) < length[:, None])))
+
+    def of_prompts(t: torch.Tensor) -> torch.Tensor:  # [rows, h_kv, group, s, x] -> [prompts, h_kv, per * group * s, x]
+        return t.reshape(prompts, per, hkv, group * s, t.shape[-1]).transpose(1, 2).reshape(prompts, hkv, per * group * s, t.shape[-1])
+
+    def of_rows(t: torch.Tensor) -> torch.Tensor:  # and back
+        return t.view(prompts, hkv, per, group, s, t.shape[-1]).transpose(1, 2).reshape(rows, hkv, group, s, t.shape[-1])
+
+    qh = q.to(wide).view(rows, s, hkv, group, d).permute(0, 2, 3, 1, 4)
+    score = torch.cat([of_rows(of_prompts(qh) @ kp.transpose(-1, -2)), (qh.reshape(rows, hkv, group * s, d) @ ko.transpose(-1, -2)).view(rows, hkv, group, s, m)], -1)
+    score = (score * (d**-0.5 if scale is None else scale)).masked_fill(~seen[:, None, None], float("-inf"))
     nothing = ~seen.any(-1)[:, None, None, :, None]
     p = torch.softmax(score.masked_fill(nothing, 0.0), -1).masked_fill(nothing, 0.0)
-    out = p @ values.permute(0, 2, 1, 3).unsqueeze(2)
+    out = of_rows(of_prompts(p[..., :n]) @ vp) + (p[..., n:].reshape(rows, hkv, group * s, m) @ vo).view(rows, hkv, group, s, d)
     return out.permute(0, 3, 1, 2, 4).reshape(rows, s, hq, d).to(q.dtype)
 
 
