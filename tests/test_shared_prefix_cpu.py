@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from torchtune_b200 import ops
+from torchtune_b200.ops import _lib
 
 
 def _inputs(prompts, rows, s, n, m, hq, hkv, d, dtype=torch.float64, seed=0):
@@ -114,3 +115,16 @@ def test_statement_does_not_repeat_the_prefix(dtype):
     with Largest() as seen:
         ops.shared_prefix_attention(*t, prefix_start=_int(3, 0)).square().sum().backward()
     assert seen.size <= 2 * rows * 4 * (n + 3) < rows * n * 2 * d / 4
+
+
+@pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="the kernel library is not built")
+def test_kernels_refuse_more_tiles_than_they_count():
+    """Tiles of 64 keys of all heads are numbered in 32 bits."""
+    from torchtune_b200.ops import shared_prefix
+
+    def floats(prompts, rows, hkv, prefix, own):
+        return _lib.lib().ttb_shared_prefix_floats(shared_prefix._pack(*shared_prefix._WITHOUT, prompts, rows, 1, hkv, hkv, 64, prefix, own), None)
+
+    assert floats(1, 4, 8, 100, 100) > 0 and floats(1, 1, 256, 2**23 * 64 - 64, 64) > 0
+    for sizes in ((1, 1, 256, 2**23 * 64, 64), (2**20, 2**20, 256, 32000, 64), (1, 2**21, 128, 64, 6400), (1, 1, 256, 64, 2**29)):
+        assert floats(*sizes) == -3

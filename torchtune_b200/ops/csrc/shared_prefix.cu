@@ -72,8 +72,8 @@ __device__ __forceinline__ int key_tiles(const Params& p, bool prefix, int owner
   return lo < hi ? (hi - lo + kKeys - 1) / kKeys : 0;
 }
 
-// n tiles over g groups: group i has [i n / g, (i + 1) n / g).  Quotients of whole numbers below 2^40 by such below 2^31: those that are no whole number are further from one than a double's
-// rounding, and the others are exact; a division of doubles is a tenth of one of 64-bit integers.
+// n tiles over g groups: group i has [i n / g, (i + 1) n / g).  The check of sizes keeps n below 2^31, and g is a number of CTAs, below 2^11: quotients are below 2^31 and those that are no whole number
+// at least 2^-11 from one (border), or below 2^11 and 2^-31 (group_of), further than a double's rounding of 2^-53 of them, and the others are exact; a division of doubles is a tenth of one of 64-bit integers.
 __device__ __forceinline__ long long border(long long n, int g, int i) { return static_cast<long long>(static_cast<double>(n * i) / g); }
 __device__ __forceinline__ int group_of(long long n, int g, long long tile) { return static_cast<int>(static_cast<double>((tile + 1) * g - 1) / static_cast<double>(n)); }
 
@@ -180,7 +180,7 @@ __device__ __forceinline__ void find_share(const Params& p, const int (&mine)[2]
       int owner = t * (which ? run_o : run_p), tiles = key_tiles(p, share.prefix, owner);
       const int owners = which ? p.rows : p.prompts;
       while (owner + 1 < owners && from >= at_owner + static_cast<long long>(tiles) * p.hkv) at_owner += static_cast<long long>(tiles) * p.hkv, tiles = key_tiles(p, share.prefix, ++owner);
-      const int in = static_cast<int>(from - at_owner);  // below 2^24 tiles times 256 heads, at most 2^31 - 1 by the check of sizes
+      const int in = static_cast<int>(from - at_owner);  // of all tiles, below 2^31
       found[0] = owner, found[1] = in / tiles, found[2] = in % tiles;
     }
   }
@@ -648,14 +648,15 @@ struct Call {
 static int plan_of(const Call& c, Params& p, long long& rows, long long& head_floats, int& ctas) {
   if (c.prompts <= 0 || c.rows <= 0 || c.rows % c.prompts || c.s <= 0 || c.hkv <= 0 || c.hq <= 0 || c.hq % c.hkv || (c.d != 64 && c.d != 128) || c.prefix < 0 || c.own < 0) return kErrBadShape;
   if (c.rows > 0x3fffffff || c.prefix > 0x3fffffff || c.own > 0x3fffffff || c.rows * c.s > 0x7fffffff / c.hq || c.hkv > 256 || c.rows * (c.own / kKeys + 1) > 0x3fffffff ||
-      c.prompts * (c.prefix / kKeys + 1) > 0x3fffffff || (c.prefix / kKeys + 1) * c.hkv > 0x3fffffff || (c.own / kKeys + 1) * c.hkv > 0x3fffffff)
+      c.prompts * (c.prefix / kKeys + 1) > 0x3fffffff)
     return kErrTooLarge;
+  const long long np = (c.prefix + kKeys - 1) / kKeys, no = (c.own + kKeys - 1) / kKeys;  // tiles of keys
+  if (c.prompts * np * c.hkv > 0x7fffffff || c.rows * no * c.hkv > 0x7fffffff) return kErrTooLarge;  // those of all heads are counted in 32 bits
   p.prompts = static_cast<int>(c.prompts), p.rows = static_cast<int>(c.rows), p.s = static_cast<int>(c.s), p.hq = static_cast<int>(c.hq), p.hkv = static_cast<int>(c.hkv);
   p.group = p.hq / p.hkv, p.prefix = static_cast<int>(c.prefix), p.own = static_cast<int>(c.own);
   p.per_group = p.group == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + p.group - 1) / p.group);
   if (c.rows / c.prompts * c.s * p.group * p.group > 0xffffffffll) return kErrTooLarge;
   p.rows_p = static_cast<int>(c.rows / c.prompts * c.s * p.group), p.rows_o = static_cast<int>(c.s * p.group);
-  const long long np = (c.prefix + kKeys - 1) / kKeys, no = (c.own + kKeys - 1) / kKeys;  // tiles of keys
   const long long most = c.prompts * c.hkv * np * tiles_of(p.rows_p) + c.rows * c.hkv * no * tiles_of(p.rows_o);
   const int all = 2 * sm_count();
   ctas = most < 2 * kSide ? 2 * kSide : most < all ? static_cast<int>(most) : all;
