@@ -185,3 +185,17 @@ def test_streams_and_recordings():
     torch.cuda.synchronize()
     for _, out in graphs:
         assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_plain_writes_leave_out_slots_that_a_cache_does_not_have():
+    """Head sizes and types without a kernel: as the kernel does."""
+    for d, dtype in ((24, torch.float32), (16, torch.float64)):
+        q, k, v = (torch.randn(2, 4, h, d, device=DEV, dtype=dtype) for h in (4, 2, 2))
+        table = torch.randn(20, d // 2, 2, device=DEV)
+        caches = [torch.randn(2, 9, 2, d, device=DEV, dtype=dtype) for _ in range(2)]
+        want = [c.clone() for c in caches]
+        out_q, out_k = ops.qk_norm_rope(q, k, None, None, table)
+        for c, new in zip(want, (out_k, v)):
+            c[:, 8], c[:, 2] = new[:, 0], new[:, 3]
+        got = ops.qk_norm_rope_append(q, k, v, None, None, table, None, *caches, torch.tensor([8, 9, -1, 2], device=DEV))
+        assert torch.equal(got, out_q) and all(torch.equal(a, b) for a, b in zip(caches, want))

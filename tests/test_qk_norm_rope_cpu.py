@@ -144,3 +144,18 @@ def test_zeros_and_non_finite_rows_stay_apart():
     out = reference.norm_rope(q, gq, _table(4, 16), None, 1e-6, True, True)
     assert not out[0, 0, 0].any() and out[0, 1, 0].isnan().any() and out[0, 2, 0].isnan().all()
     assert out[0, :, 1].isfinite().all() and out[0, 3].isfinite().all()
+
+
+def test_plain_writes_leave_out_slots_that_a_cache_does_not_have():
+    """What stands in for the kernel on a device must not reach outside of the cache."""
+    cache, values = torch.randn(2, 5, 3, 4), torch.randn(2, 4, 3, 4)
+    want = cache.clone()
+    want[:, 3], want[:, 0] = values[:, 0], values[:, 3]
+    reference.write_known_slots(cache, torch.tensor([3, 5, -1, 0]), values)
+    assert torch.equal(cache, want)
+    reference.write_known_slots(cache, torch.tensor([2**40, -(2**40), 7, 9]), values)
+    assert torch.equal(cache, want)
+    empty = cache[:, :0].clone()
+    reference.write_known_slots(empty, torch.tensor([0, 1, 2, 3]), values)
+    with pytest.raises((IndexError, RuntimeError)):
+        reference.write_slots(cache, torch.tensor([3, 5, 1, 0]), values)

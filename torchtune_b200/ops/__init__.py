@@ -398,8 +398,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gain: Optional[torch.Tensor
                  eps: float = 1e-6, interleaved: bool = True, norm_first: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
     """RMS norm of every head of ``q`` and ``k`` ``[b, s, heads, d]``, times a gain ``[d]`` each (``None``: none), and :func:`rope`, in that order or (``norm_first=False``) the other way round, with
     one rounding at the end where the two operators of their own make two.  ``cache``: fp32 (angles in 16 bits are widened by a copy, per call).  One launch forward for CUDA tensors in bf16, fp16 or fp32 with ``d`` a multiple of 16 up to 512, and one backward (two
-    with gains' gradients).  ``input_pos``: ``[b, s]``, ``[s]``, or ``[b]`` for one token per row; the angles are constants.  On a CUDA device a position that the table does not have counts as
-    an index violation and position 0 stands in; elsewhere it is an error."""
+    with gains' gradients).  ``input_pos``: ``[b, s]``, ``[s]``, or ``[b]`` for one token per row; the angles are constants.  On a CUDA device position 0 stands in
+    for one that the table does not have, which the kernel counts as an index violation; elsewhere it is an error."""
     qk_norm.check_arguments(q, k, (q_gain, k_gain), cache)
     if cache.dtype in (torch.bfloat16, torch.float16):  # of a model that was converted as a whole
         cache = cache.float()
@@ -419,8 +419,8 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_gai
                         input_pos: Optional[torch.Tensor], k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, *, eps: float = 1e-6, interleaved: bool = True,
                         norm_first: bool = True) -> torch.Tensor:
     """:func:`qk_norm_rope` of ``q`` (returned) and of ``k``, the latter and ``v`` written to ``k_cache`` / ``v_cache`` ``[b, max_seq, heads, d]`` at ``slots`` (int64 ``[s]``, no two the same), in one
-    launch.  No gradient flows through a cache: calls that would be differentiated are refused.  On a CUDA device a slot outside the cache counts as an index violation and nothing is written
-    for it; elsewhere it is an error."""
+    launch.  No gradient flows through a cache: calls that would be differentiated are refused.  On a CUDA device nothing is written for a slot outside the cache, which the kernel counts as an index
+    violation; elsewhere it is an error."""
     qk_norm.check_arguments(q, k, (q_gain, k_gain), cache)
     if cache.dtype in (torch.bfloat16, torch.float16):  # of a model that was converted as a whole
         cache = cache.float()
@@ -443,8 +443,8 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_gai
             and _has_memory(q, k, v, cache, k_cache, v_cache, slots, *(t for t in (q_gain, k_gain, pos) if t is not None))):
         return qk_norm.norm_rope_append(q, k, v, q_gain, k_gain, cache, pos, k_cache, v_cache, slots, float(eps), bool(interleaved), bool(norm_first))
     _fallback("qk_norm_rope_append", f"head dimension {q.shape[-1]}, angles in {cache.dtype} or caches whose rows do not start on 16 bytes", q)
-    k_cache.index_copy_(1, slots, reference.norm_rope(k, k_gain, cache, pos, eps, interleaved, norm_first))
-    v_cache.index_copy_(1, slots, v)
+    reference.write_slots(k_cache, slots, reference.norm_rope(k, k_gain, cache, pos, eps, interleaved, norm_first))
+    reference.write_slots(v_cache, slots, v)
     return reference.norm_rope(q, q_gain, cache, pos, eps, interleaved, norm_first)
 
 

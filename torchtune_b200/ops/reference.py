@@ -169,6 +169,24 @@ def norm_rope(x: torch.Tensor, gain: Optional[torch.Tensor], cache: torch.Tensor
     return (turn(y) if norm_first else y).to(x.dtype)
 
 
+def write_slots(cache: torch.Tensor, slots: torch.Tensor, values: torch.Tensor) -> None:
+    """``cache[:, slots] = values`` for ``cache`` ``[b, n, ...]`` and ``values`` ``[b, s, ...]``.  A slot that the cache does not have is an error on the CPU; on a device, where nobody can be asked
+    without waiting, nothing is written for it."""
+    if cache.device.type == "cpu":
+        cache.index_copy_(1, slots, values)
+    else:
+        write_known_slots(cache, slots, values)
+
+
+def write_known_slots(cache: torch.Tensor, slots: torch.Tensor, values: torch.Tensor) -> None:
+    n = cache.shape[1]
+    source = slots.new_full((n + 1,), -1)  # of every slot of the cache; the last one takes what belongs nowhere
+    source[torch.where((slots >= 0) & (slots < n), slots, n)] = torch.arange(slots.shape[0], device=slots.device)
+    source = source[:n]
+    written = (source >= 0).view(1, n, *(1,) * (cache.dim() - 2))
+    cache.copy_(torch.where(written, values.index_select(1, source.clamp(min=0)), cache))
+
+
 def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_start: Optional[torch.Tensor],
                             prefix_stop: Optional[torch.Tensor], lengths: Optional[torch.Tensor], scale: Optional[float]) -> torch.Tensor:
     """``q`` ``[rows, s, h, d]`` over the visible slots of the row's prompt ``[prompts, n, h_kv, d]`` and of its own ``[rows, slots, h_kv, d]``, in fp32 (fp64 for fp64 inputs); a query that sees no key
