@@ -137,3 +137,27 @@ def test_fused_norms_in_training_and_in_cached_steps():
         outs.append(torch.cat([first, *rest], 1).float())
     assert (outs[0] - outs[1]).norm() / outs[0].norm() < 0.03 and (outs[1] - grads[1][0]).norm() / grads[1][0].norm() < 0.03
     assert _lib.index_violations() == 0
+
+
+def test_recorded_steps_run_count_and_end_with_their_caches(monkeypatch):
+    """A generation of this length records a step and replays it; the host's count is the device's, and a step too many is refused."""
+    model, prompts, replays = _qwen(fuse_qk_norm=True), _prompts(), []
+    replay = torch.cuda.CUDAGraph.replay
+    monkeypatch.setattr(torch.cuda.CUDAGraph, "replay", lambda self: replays.append(1) or replay(self))
+    generation.generate_group(model, prompts, samples=2, max_generated_tokens=9)
+    assert len(replays) == 7  # eight steps, of which the first runs as it is
+    real, device = prompts != 0, prompts.device
+    with torch.no_grad(), generation.shared_prompts(model, 70 - real.sum(1), 6, 70, 5) as groups:
+        model(prompts, input_pos=generation.get_position_ids_from_padding_mask(real), mask=generation.get_causal_mask_from_padding_mask(real))
+        groups.begin()
+        tokens = torch.ones(6, 1, dtype=torch.long, device=device)
+        step = _group._Steps(model, groups, torch.full((6, 1), 70, dtype=torch.int32, device=device), tokens.clone(), True)
+        for i in range(5):
+            step(tokens)
+            assert groups.steps == i + 1 == int(groups.slot)
+        assert step.graph is not None
+        with pytest.raises(AssertionError, match="full"):
+            step(tokens)
+        assert groups.steps == 5 == int(groups.slot)
+        del step
+    _lib.check_device_errors()

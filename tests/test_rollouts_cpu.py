@@ -199,3 +199,22 @@ def test_entropy_bonus_does_not_depend_on_the_size_of_the_pieces():
     for other in seen[1:]:
         for a, b in zip(seen[0], other):
             torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-6)
+
+
+@pytest.mark.parametrize("build", [_llama, lambda: _qwen(fuse_qk_norm=True)])
+def test_a_shared_cache_that_is_full_says_so(build):
+    """More steps than it was made for: as of any cache, before anything is written."""
+    model, prompts = build(), _prompts(False)
+    step = lambda pos: model(torch.ones(6, 1, dtype=torch.long), input_pos=torch.full((6, 1), pos), mask=ops.AttentionMask(causal=True))  # noqa: E731
+    with torch.no_grad(), generation.shared_prompts(model, torch.zeros(3, dtype=torch.int64), 6, 7, 2) as groups:
+        model(prompts, input_pos=torch.arange(7), mask=torch.tril(torch.ones(1, 7, 7, dtype=torch.bool)))
+        for _ in range(2):  # the same caches may answer anew
+            groups.begin()
+            for i in range(2):
+                step(7 + i)
+                groups.advance()
+            assert groups.steps == int(groups.slot) == 2
+            held = [layer.attn.kv_cache.own_k.clone() for layer in model.layers]
+            with pytest.raises(AssertionError, match="full"):
+                step(9)
+            assert all(torch.equal(a, layer.attn.kv_cache.own_k) for a, layer in zip(held, model.layers))

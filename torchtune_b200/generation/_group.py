@@ -83,7 +83,10 @@ class _Steps:
                 finally:
                     graph.capture_end()
             torch.cuda.current_stream(device).wait_stream(stream)
-            self.graph = graph
+            self.graph = graph  # and this step is counted
+        else:
+            self.model.layers[0].attn.kv_cache.reserve(self.groups.rows, 1)  # raises when the cache is full
+            self.groups.steps += 1
         self.graph.replay()
         return self.logits.clone()
 

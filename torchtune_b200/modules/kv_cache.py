@@ -149,16 +149,19 @@ class PromptGroups:
         self.lengths = torch.zeros(rows, dtype=torch.int32, device=starts.device)  # tokens of a row, the one of the step at hand included
         self.slot = torch.zeros(1, dtype=torch.int64, device=starts.device)  # of the step at hand
         self.answering = False  # False while the prompts are read
+        self.steps = 0  # the number in ``slot``, as the host counts it: whoever replays a recorded step counts it himself
 
     def begin(self) -> None:
         """The prompts are read; the rows' first token comes next."""
         self.answering = True
         self.lengths.fill_(1)
         self.slot.zero_()
+        self.steps = 0
 
     def advance(self) -> None:
         self.lengths.add_(1)
         self.slot.add_(1)
+        self.steps += 1
 
 
 class SharedPrefixKVCache(nn.Module):
@@ -190,6 +193,8 @@ class SharedPrefixKVCache(nn.Module):
             return torch.arange(seq_len, device=groups.slot.device)
         if bsz != groups.rows or seq_len != 1:
             raise ValueError(f"{groups.rows} rows answer one token at a time, not {bsz} rows of {seq_len}")
+        if groups.steps >= self.max_seq_len:
+            raise AssertionError("KV cache is full: cannot write past max_seq_len")
         return groups.slot
 
     def advance(self, seq_len: int) -> None:
