@@ -159,3 +159,15 @@ def test_plain_writes_leave_out_slots_that_a_cache_does_not_have():
     reference.write_known_slots(empty, torch.tensor([0, 1, 2, 3]), values)
     with pytest.raises((IndexError, RuntimeError)):
         reference.write_slots(cache, torch.tensor([3, 5, 1, 0]), values)
+
+
+@pytest.mark.parametrize("shape", [(2, 0), (0, 3), (0, 0)])
+def test_nothing_is_differentiated_too(shape):
+    """No rows or no tokens: outputs are part of the graph as others are, and gains have gradients of zeros."""
+    q, k = (torch.randn(*shape, h, 16, requires_grad=True) for h in (4, 2))
+    gains = [torch.ones(16, requires_grad=True) for _ in range(2)]
+    for pos in (None, torch.zeros(shape, dtype=torch.int32)):
+        a, b = ops.qk_norm_rope(q, k, *gains, _table(8, 16), pos)
+        assert a.shape == q.shape and b.shape == k.shape
+        grads = torch.autograd.grad(a.sum() + b.sum(), (q, k, *gains))
+        assert [g.shape for g in grads] == [q.shape, k.shape, (16,), (16,)] and not any(g.any() for g in grads)

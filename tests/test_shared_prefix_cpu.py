@@ -128,3 +128,13 @@ def test_kernels_refuse_more_tiles_than_they_count():
     assert floats(1, 4, 8, 100, 100) > 0 and floats(1, 1, 256, 2**23 * 64 - 64, 64) > 0
     for sizes in ((1, 1, 256, 2**23 * 64, 64), (2**20, 2**20, 256, 32000, 64), (1, 2**21, 128, 64, 6400), (1, 1, 256, 64, 2**29)):
         assert floats(*sizes) == -3
+
+
+@pytest.mark.parametrize("prompts,rows,s", [(2, 4, 0), (0, 0, 1), (0, 0, 0)])
+def test_nothing_is_differentiated_too(prompts, rows, s):
+    """No rows or no tokens: the output is part of the graph as others are."""
+    t = [x.requires_grad_() for x in _inputs(prompts, rows, s, 5, 3, 4, 2, 8, torch.float32)]
+    out = ops.shared_prefix_attention(*t, prefix_start=torch.zeros(prompts, dtype=torch.int32), lengths=torch.zeros(rows, dtype=torch.int32))
+    assert out.shape == t[0].shape
+    grads = torch.autograd.grad(out.sum(), t)
+    assert not any(g.any() for g in grads)

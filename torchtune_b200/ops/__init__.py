@@ -407,11 +407,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gain: Optional[torch.Tensor
     pos = qk_norm.positions(input_pos, b, s, cache.shape[0])
     if pos is not None and pos.device != q.device:
         pos = pos.to(q.device)
-    if q.numel() == 0:
-        return torch.empty_like(q), torch.empty_like(k)
-    if cuda_ops_enabled(q) and qk_norm.suits(q, k, cache) and _has_memory(q, k, cache, *(t for t in (q_gain, k_gain, pos) if t is not None)) and torch.autograd.forward_ad._current_level < 0:
+    if q.numel() > 0 and cuda_ops_enabled(q) and qk_norm.suits(q, k, cache) and _has_memory(q, k, cache, *(t for t in (q_gain, k_gain, pos) if t is not None)) and torch.autograd.forward_ad._current_level < 0:
         return qk_norm.norm_rope(q, k, q_gain, k_gain, cache, pos, float(eps), bool(interleaved), bool(norm_first), _differentiated(q, k, q_gain, k_gain))
-    _fallback("qk_norm_rope", f"head dimension {q.shape[-1]} or angles in {cache.dtype}", q)
+    if q.numel() > 0:
+        _fallback("qk_norm_rope", f"head dimension {q.shape[-1]} or angles in {cache.dtype}", q)
     return tuple(reference.norm_rope(x, gain, cache, pos, eps, interleaved, norm_first) for x, gain in ((q, q_gain), (k, k_gain)))
 
 
@@ -594,9 +593,7 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     tensors with 64 or 128 channels and up to 256 key heads outside autograd take the kernels (for keys and values in strides that are multiples of 16 bytes, where they lie); everything else takes
     the plain statement, which has gradients.  The kernels are made for few queries per row: pieces of the softmax wait in fp32 for their join, with many query rows up to some 40 of them per key head."""
     shared_prefix.check_arguments(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, lengths)
-    if q.numel() == 0:
-        return torch.empty_like(q)
-    if _native(q):
+    if _native(q) and q.numel() > 0:
         index = tuple(t for t in (prefix_start, prefix_stop, lengths) if t is not None)
         if not shared_prefix.suits(q, k, k_prefix.shape[0]):
             _fallback("shared_prefix_attention", f"{q.shape[2]} query and {k.shape[2]} key heads of {q.shape[3]} channels", q)

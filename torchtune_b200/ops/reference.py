@@ -194,7 +194,7 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     rows, s, hq, d = q.shape
     prompts, n, hkv, _ = k_prefix.shape
     m, dev, wide = k.shape[1], q.device, torch.promote_types(q.dtype, torch.float32)
-    per, group = rows // prompts, hq // hkv
+    per, group = rows // max(prompts, 1), hq // hkv
     at = torch.arange(n, device=dev)
     shared = torch.ones(prompts, n, dtype=torch.bool, device=dev)
     if prefix_start is not None:
@@ -216,7 +216,7 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
 
     qh = q.to(wide).view(rows, s, hkv, group, d).permute(0, 2, 3, 1, 4)
     score = torch.cat([of_rows(of_prompts(qh) @ kp.transpose(-1, -2)), (qh.reshape(rows, hkv, group * s, d) @ ko.transpose(-1, -2)).view(rows, hkv, group, s, m)], -1)
-    score = (score * (d**-0.5 if scale is None else scale)).masked_fill(~seen[:, None, None], float("-inf"))
+    score = (score * (max(d, 1) ** -0.5 if scale is None else scale)).masked_fill(~seen[:, None, None], float("-inf"))
     nothing = ~seen.any(-1)[:, None, None, :, None]
     p = torch.softmax(score.masked_fill(nothing, 0.0), -1).masked_fill(nothing, 0.0)
     out = of_rows(of_prompts(p[..., :n]) @ vp) + (p[..., n:].reshape(rows, hkv, group * s, m) @ vo).view(rows, hkv, group, s, d)
