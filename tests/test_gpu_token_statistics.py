@@ -295,3 +295,32 @@ def test_sure_tokens(rows, v, dtype):
     assert (s.logprobs.double() - want[0]).abs().max() <= 16 * STEP
     assert (s.top_logprobs[:, 0].double() - want[2][:, 0]).abs().max() <= 16 * STEP
     assert (s.entropy.double() - want[1]).abs().max() <= 16 * STEP
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("copies", [1, 100])
+@pytest.mark.parametrize("skip", [1, 3, 7])
+def test_masked_and_non_finite_logits_at_odd_addresses(skip, copies, dtype):
+    """Rows that do not begin on 16 bytes and end anywhere, few and many: their first and last elements are read one by one."""
+    v, low = 5001, torch.finfo(dtype).min
+    x = _logits(8 * copies, v + skip, dtype=dtype).view(copies, 8, v + skip)
+    x[:, 0, skip + 3 :] = -INF  # three tokens are left
+    x[:, 1] = -INF
+    x[:, 2] = low
+    x[:, 3, skip + 1 : -1] = low
+    x[:, 4, skip] = float("nan")
+    x[:, 5, -1] = INF
+    x[:, 6, ::2] = -INF
+    x[:, 7, : 4096 + skip] = -INF  # whole segments
+    x[:, :, :skip] = float("nan")  # in front of the rows
+    case = x.view(8 * copies, v + skip)[:, skip:]
+    tokens = torch.tensor([2, 0, 9, 0, 1, 1, 1 - skip % 2 + 1, v - 1], device=DEV).repeat(copies)
+    leaf = case.detach().requires_grad_()
+    s = ops.token_statistics(leaf, tokens, top=5)
+    want = reference.token_statistics(case.double(), tokens, 1.0, 5, -100)
+    assert torch.equal(s.top_tokens, want[3])
+    for a, b in zip(s[:3], want[:3]):
+        torch.testing.assert_close(a.detach().double(), b, rtol=2e-5, atol=2e-5, equal_nan=True)
+    (g,) = torch.autograd.grad(s.logprobs.sum() + s.entropy.sum(), leaf)
+    g = g.view(copies, 8, v)
+    assert g[:, [1, 4, 5]].isnan().all() and g[:, [0, 2, 3, 7]].isfinite().all() and not g[:, 0, 3:].any() and not g[:, 7, :4096].any() and g[:, 7, 4096:].any(-1).all()
