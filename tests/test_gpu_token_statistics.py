@@ -324,3 +324,15 @@ def test_masked_and_non_finite_logits_at_odd_addresses(skip, copies, dtype):
     (g,) = torch.autograd.grad(s.logprobs.sum() + s.entropy.sum(), leaf)
     g = g.view(copies, 8, v)
     assert g[:, [1, 4, 5]].isnan().all() and g[:, [0, 2, 3, 7]].isfinite().all() and not g[:, 0, 3:].any() and not g[:, 7, :4096].any() and g[:, 7, 4096:].any(-1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_one_logit_is_certain(dtype):
+    """And so is one beside infinitely low ones: nothing is left to round."""
+    one = _logits(900, 1, dtype=dtype)
+    few = torch.cat([one, torch.full((900, 30), -INF, device=DEV, dtype=dtype)], 1)
+    for x in (one, few):
+        leaf = x.requires_grad_()
+        s = ops.token_statistics(leaf, torch.zeros(900, dtype=torch.int64, device=DEV), temperature=0.7, top=1)
+        (g,) = torch.autograd.grad(s.logprobs.sum() + 3 * s.entropy.sum(), leaf)
+        assert not s.logprobs.any() and not s.entropy.any() and not s.top_logprobs.any() and not g.any()

@@ -646,6 +646,7 @@ __global__ void __launch_bounds__(kOwnWarps<TOP> * 32, kCtas) row_kernel(const _
     const int vectors = row.vectors();
     const long long token = p.tokens[r];
     Running run{p.c};
+    const float lift = vectors > 32 ? p.lift : 0.f;  // the first vectors are the row: their maximum is the base
     float lane_most = -INFINITY;
     auto note = [&](int j, float most) {  // the maximum of a segment
       if constexpr (TOP) {
@@ -665,7 +666,7 @@ __global__ void __launch_bounds__(kOwnWarps<TOP> * 32, kCtas) row_kernel(const _
 #pragma unroll
           for (int x = 0; x < kPieces; ++x) reinterpret_cast<uint4*>(raw.v)[x] = *reinterpret_cast<const uint4*>(at + x * kPieceBytes + a * 512);
           if constexpr (TOP) note(j0 + a * 32, most_of_vector<T>(raw));
-          if (a == 0 && j0 == 0) run.begin(warp_max_nan(most_of_vector<T>(raw)) + p.lift);
+          if (a == 0 && j0 == 0) run.begin(warp_max_nan(most_of_vector<T>(raw)) + lift);
           run.take<T>(raw, c2);
         }
       } else {
@@ -674,7 +675,7 @@ __global__ void __launch_bounds__(kOwnWarps<TOP> * 32, kCtas) row_kernel(const _
           float f[8];
           widen8(row.load(j0 + a * 32 + lane), f);
           note(j0 + a * 32, most_of(f));
-          if (a == 0 && j0 == 0) run.begin(warp_max_nan(most_of(f)) + p.lift);
+          if (a == 0 && j0 == 0) run.begin(warp_max_nan(most_of(f)) + lift);
           run.careful(f);
         }
       }
