@@ -397,8 +397,9 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: torch.
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: Optional[torch.Tensor], cache: torch.Tensor, input_pos: Optional[torch.Tensor] = None, *,
                  eps: float = 1e-6, interleaved: bool = True, norm_first: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
     """RMS norm of every head of ``q`` and ``k`` ``[b, s, heads, d]``, times a gain ``[d]`` each (``None``: none), and :func:`rope`, in that order or (``norm_first=False``) the other way round, with
-    one rounding at the end where the two operators of their own make two.  ``cache``: fp32 (angles in 16 bits are widened by a copy, per call).  One launch forward for CUDA tensors in bf16, fp16 or fp32 with ``d`` a multiple of 16 up to 512, and one backward (two
-    with gains' gradients).  ``input_pos``: ``[b, s]``, ``[s]``, or ``[b]`` for one token per row; the angles are constants.  On a CUDA device position 0 stands in
+    one rounding at the end where the two operators of their own make two.  ``cache``: fp32 (angles in 16 bits are widened, the whole table in every call: 16 MB written for 32 768 positions of 128 channels).
+    One launch forward for CUDA tensors in bf16, fp16 or fp32 with ``d`` a multiple of 16 up to 512, and one backward (two with gains' gradients); positions in int64 are converted in front of it by
+    two more, tensors whose heads do not lie on 16 bytes copied.  ``input_pos``: ``[b, s]``, ``[s]``, or ``[b]`` for one token per row; the angles are constants.  On a CUDA device position 0 stands in
     for one that the table does not have, which the kernel counts as an index violation; elsewhere it is an error."""
     qk_norm.check_arguments(q, k, (q_gain, k_gain), cache)
     if cache.dtype in (torch.bfloat16, torch.float16):  # of a model that was converted as a whole
@@ -665,7 +666,8 @@ def logits_logprobs(logits: torch.Tensor, tokens: torch.Tensor, temperature: flo
 
 def token_statistics(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0, top: int = 0, ignore_index: int = -100) -> TokenStatistics:
     """Of ``softmax(logits / temperature)`` over the last dimension: the log-probability of ``tokens`` (int64, the shape of ``logits`` without it), the entropy, and the ``top`` (up to 64)
-    likeliest tokens with their log-probabilities, the largest logits first and of equal ones those of the lower index (NaN counts as largest).  CUDA logits in bf16, fp16 or fp32, of any width and
+    likeliest tokens with their log-probabilities, the largest logits first and of equal ones those of the lower index (NaN counts as largest).  More than some 30 of them take many times as long in
+    rows of fewer than 256 logits for each, where they are searched for one after the other.  CUDA logits in bf16, fp16 or fp32, of any width and
     row pitch, are read once, and once more for the gradient of all three.  A token equal to ``ignore_index`` has log-probability 0 without a gradient (its row's entropy and alternatives are
     still those of the row); so, counted as an index violation, has one outside the vocabulary on a CUDA device; elsewhere that is an error.  Infinitely low logits have probability 0 and no share
     in the entropy; a row of nothing else, or one with a NaN or an infinitely high logit, has NaN for both and, on a CUDA device unless all its gradients are 0, in its logits' gradient."""

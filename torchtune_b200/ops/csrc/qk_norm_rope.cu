@@ -11,7 +11,8 @@
 // pairs lie within the N, so that no value crosses lanes but the sums.  A group of lanes takes up to HEADS heads of one token, whose angles it keeps.
 // The gains' gradients are sums in registers over all that a CTA does, then rows of a workspace that a second launch adds up, both in an order that depends on sizes alone.
 //
-// Bound by bytes once there are enough of them, and otherwise by latency: a value costs some 18 instructions, conversions, two products of the turn, the square, the gain and its part of the sums.
+// Bound by no one unit: with a third of the warps' places taken (registers) 64 % of the cycles issue and 4.3 TB/s flow; a value costs 18 instructions forward and 29 backward, conversions, two products of
+// the turn, the square, the gain and its part of the sums.  Few tokens: by latency.
 // Measured (bf16, 32 query and 8 key heads of 128 channels, cold L2, out of a graph): one token of 16 rows with the write to the cache 3.1 us; 4 x 1999 tokens with it 47 us (196 MB: 4.2 TB/s); 4 x 2048
 // tokens forward 39 us (168 MB: 4.3 TB/s), backward 58 us (252 MB: 4.3 TB/s) and 3 us for the gains.
 #include <cuda_bf16.h>

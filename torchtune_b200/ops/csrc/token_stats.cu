@@ -13,17 +13,18 @@
 // The alternatives are the `top` largest logits, of equal ones those with the lower index.  The pass leaves the largest value of every segment of 256 elements (what a warp reads at once) in shared
 // memory; the `top` segments with the largest ones (of equal ones the first) hold all alternatives, since an element outside is beaten by `top` maxima.  Of their elements those count that reach the
 // least of these maxima: hardly more than `top` as a rule, whose ranks one warp finds by comparing each with each.  Rows of no more segments than alternatives take the maxima of the lanes' elements
-// instead.  Where candidates are too many (logits in order, ties), the choice is a search: for the `top`-th largest key bit by bit among the segments, their lanes and the lanes' elements, or for one
-// alternative after the other.
+// instead, of which there are 32.  Where candidates are too many (logits in order, ties), the choice is a search: for the `top`-th largest key bit by bit among the segments, their lanes and the lanes'
+// elements, or, where a warp has a row of its own, for one alternative after the other.  So it is there for ordinary logits too, where more than 32 alternatives come from no more segments than that, or
+// some 30 from few lanes' maxima: 8192 x 8000 bf16 94 us with 20, 770 with 32, 3000 with 33, 5800 with 64; 8192 x 16000 123, 147, 152 and 12 200; 8192 x 20000 133, 160, 164 and 254.
 //
 // Three ways through the rows.  Long ones: CTAs go from row to row; warps that stream take runs of a row and go on to the next one without waiting for each other, and a warp of its own ends the row
 // before, from sums and segments that lie in shared memory twice.  Many that are not long: a warp streams and ends rows of its own, since the end of a row, some 5 us of instructions that wait for one
 // another, takes longer than its stream, and there it lies beside the streams of 23 other warps.  Few rows: split over clusters of up to eight CTAs, which meet in the shared memory of the first.
 // In all of them a lane copies its vectors two runs ahead, over the ends of rows too, to slots of its own.
 //
-// Bound by bytes in 32 bits, in 16 bits by issue and the exponentials' unit (16 a cycle and SM: 60 % busy), and with alternatives by the maxima beside them.
-// Measured (cold L2, out of a graph): 4096 x 151936 bf16 forward 250 us (5.0 TB/s), gradient 446 us (5.6 TB/s); 4136 x 128256 bf16 with 5 alternatives 262 us (4.1 TB/s); 8192 x 32000 fp32 184 us
-// (5.7 TB/s), its gradient 309 us; 8192 x 8000 bf16 43 us; 16 x 128256 fp32 with 20 alternatives 17 us (kernels behind one another).
+// Bound by bytes in 32 bits, in 16 bits by issue and the exponentials' unit (16 a cycle and SM: 64 % busy, and 66 % of the cycles issue), and with alternatives by the maxima beside them.
+// Measured (cold L2, out of a graph): 4096 x 151936 bf16 forward 248 us (5.0 TB/s), gradient 446 us (5.6 TB/s); 4136 x 128256 bf16 with 5 alternatives 262 us (4.1 TB/s); 8192 x 32000 fp32 184 us
+// (5.7 TB/s), its gradient 309 us; 8192 x 8000 bf16 41 us; 16 x 128256 fp32 with 20 alternatives 17 us (kernels behind one another).
 //
 // Rows begin at any address: vectors lie on 16 bytes, and the first and last of a row are read element by element.
 #include <cooperative_groups.h>
