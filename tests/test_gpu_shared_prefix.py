@@ -187,3 +187,18 @@ def test_probabilities_are_not_rounded_to_16_bits(d, hq, hkv, n, m):
     far = (out - want).abs() - (2.0**-8 * want.abs() + 2.0**-16 + 2.0**-15 + 2.0**-18)
     assert (far <= 0).all(), float(far.max())
     _lib.check_device_errors()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_non_finite_values_that_are_seen(bad):
+    """They reach the channel of the queries that see them and nothing else."""
+    q, kp, vp, k, v = _inputs(2, 6, 1, 100, 70, 4, 2, 64)
+    lengths = _int([70, 21, 20, 70, 70, 0])
+    want = ops.shared_prefix_attention(q, kp, vp, k, v, lengths=lengths)
+    v[:3, 20, 1, 5] = bad  # rows 0 and 1 see it, row 2 ends in front of it
+    vp[1, 3, 0, 7] = bad  # rows 3 to 5
+    out = ops.shared_prefix_attention(q, kp, vp, k, v, lengths=lengths)
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[:2, :, 2:, 5] = True
+    hit[3:, :, :2, 7] = True
+    assert not out[hit].isfinite().any() and torch.equal(out[~hit], want[~hit])

@@ -590,7 +590,7 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     """Attention of ``q`` ``[rows, s, h, d]`` over the keys and values of a prompt that several rows share, ``[prompts, n, h_kv, d]``, and over each row's own, ``[rows, slots, h_kv, d]``: row ``r``
     belongs to prompt ``r // (rows // prompts)``, whose slots ``prefix_start[prompt]`` ... ``prefix_stop[prompt] - 1`` it sees (int32, by default all ``n``), and of its own the first ``lengths[row]``
     (int32, by default all slots), of which its ``s`` queries are the last ones and see none behind their own.  Numbers out of range are cut off at it.  A query that sees no key gives 0, and what
-    lies in slots that no query of a row sees has no influence; one that only later tokens of the same call see should be finite.  The prefix is read once for all rows of a prompt.  bf16 CUDA
+    lies in slots that no query of a row sees has no influence; one that only later tokens of the same call see should be finite.  An infinite value that is seen gives an infinity or, on the kernels, NaN.  The prefix is read once for all rows of a prompt.  bf16 CUDA
     tensors with 64 or 128 channels and up to 256 key heads outside autograd take the kernels (for keys and values in strides that are multiples of 16 bytes, where they lie); everything else takes
     the plain statement, which has gradients.  The kernels are made for few queries per row: pieces of the softmax wait in fp32 for their join, with many query rows up to some 40 of them per key head."""
     shared_prefix.check_arguments(q, k_prefix, v_prefix, k, v, prefix_start, prefix_stop, lengths)
@@ -667,7 +667,7 @@ def logits_logprobs(logits: torch.Tensor, tokens: torch.Tensor, temperature: flo
 def token_statistics(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0, top: int = 0, ignore_index: int = -100) -> TokenStatistics:
     """Of ``softmax(logits / temperature)`` over the last dimension: the log-probability of ``tokens`` (int64, the shape of ``logits`` without it), the entropy, and the ``top`` (up to 64)
     likeliest tokens with their log-probabilities, the largest logits first and of equal ones those of the lower index (NaN counts as largest).  More than some 30 of them take many times as long in
-    rows of fewer than 256 logits for each, where they are searched for one after the other.  CUDA logits in bf16, fp16 or fp32, of any width and
+    rows of fewer than some 300 logits for each, where they are searched for one after the other.  CUDA logits in bf16, fp16 or fp32, of any width and
     row pitch, are read once, and once more for the gradient of all three.  A token equal to ``ignore_index`` has log-probability 0 without a gradient (its row's entropy and alternatives are
     still those of the row); so, counted as an index violation, has one outside the vocabulary on a CUDA device; elsewhere that is an error.  Infinitely low logits have probability 0 and no share
     in the entropy; a row of nothing else, or one with a NaN or an infinitely high logit, has NaN for both and, on a CUDA device unless all its gradients are 0, in its logits' gradient."""

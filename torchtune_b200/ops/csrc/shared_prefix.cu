@@ -16,7 +16,7 @@
 // arrive while the output of the last is written; the scores of a tile are computed while the softmax of the one before is.  Pieces lie in a workspace that a second launch joins in a fixed order.
 //
 // What lies behind the last visible key may be anything: scores are masked by selection, and the values of a piece's last tile that nobody sees are overwritten with zeros before they are
-// multiplied.  Every wait is bounded and reports through the error word.
+// multiplied.  A value that is seen and infinite times a rest of 0 is NaN, as it is times a probability of 0.  Every wait is bounded and reports through the error word.
 //
 // Bound by bytes on long rows, else by what a piece does one after the other (products, softmax, products, output: 3 to 5 us, which the two CTAs of an SM hide from each other in part) and by the
 // start (finding the shares, first loads: 5 us) and the joining launch.  Measured (32 query on 8 key heads of 128 channels, kernels behind one another in a graph): 16 rows on 32003 shared keys and

@@ -14,8 +14,8 @@
 // memory; the `top` segments with the largest ones (of equal ones the first) hold all alternatives, since an element outside is beaten by `top` maxima.  Of their elements those count that reach the
 // least of these maxima: hardly more than `top` as a rule, whose ranks one warp finds by comparing each with each.  Rows of no more segments than alternatives take the maxima of the lanes' elements
 // instead, of which there are 32.  Where candidates are too many (logits in order, ties), the choice is a search: for the `top`-th largest key bit by bit among the segments, their lanes and the lanes'
-// elements, or, where a warp has a row of its own, for one alternative after the other.  So it is there for ordinary logits too, where more than 32 alternatives come from no more segments than that, or
-// some 30 from few lanes' maxima: 8192 x 8000 bf16 94 us with 20, 770 with 32, 3000 with 33, 5800 with 64; 8192 x 16000 123, 147, 152 and 12 200; 8192 x 20000 133, 160, 164 and 254.
+// elements, or, where a warp has a row of its own, for one alternative after the other.  So it is there for ordinary logits too, where more than 32 alternatives come from hardly more segments than that, or
+// some 30 from as many: 8192 x 8000 bf16 94 us with 20, 770 with 32, 3000 with 33, 5800 with 64; 8192 x 16000 123, 147, 152 and 12 200; 8192 x 20000 133, 160, 164 and 254.
 //
 // Three ways through the rows.  Long ones: CTAs go from row to row; warps that stream take runs of a row and go on to the next one without waiting for each other, and a warp of its own ends the row
 // before, from sums and segments that lie in shared memory twice.  Many that are not long: a warp streams and ends rows of its own, since the end of a row, some 5 us of instructions that wait for one
