@@ -7,7 +7,7 @@
 // same work: scores of 128 rows and 64 keys on tcgen05 tensor cores, a thread per row for the softmax, probabilities in the scores' place in tensor memory as the A operand of the second
 // product, its accumulator next to them.  They are two bf16 numbers each, a rounded one and the rest, which take the 32 bits of a score: rounded once, they are off
 // by more than the output's own rounding (outputs 0.0023 from exact ones, of which the latter is 0.0017; now it is all there is).  The second product takes twice as long, which shows where several
-// tiles of rows meet the same keys and the tensor cores bound (256 rows of three tokens: 197 -> 223 us; one token of 4 to 64 rows: 1 % at most).
+// tiles of rows meet the same keys and the tensor cores bound (256 rows of three tokens: 200 -> 216 us; one token of 4 to 64 rows: 1 % at most).
 // A tile of 64 keys and values is 32 KB: an SM's share of the memory's rate brings it in 1400 cycles, and 128 rows keep the tensor cores busy for 770 of them and the
 // exponentials' unit for 512, so that padding a single token's four rows to 128 costs nothing that is not idle; warps without rows have no part in the softmax.
 // Two CTAs to an SM share the tiles of all key heads out evenly, as they are: tiles of the prefixes in their order are one line, those of the rows another, CTAs get a stretch of one of them each
@@ -20,7 +20,7 @@
 //
 // Bound by bytes on long rows, else by what a piece does one after the other (products, softmax, products, output: 3 to 5 us, which the two CTAs of an SM hide from each other in part) and by the
 // start (finding the shares, first loads: 5 us) and the joining launch.  Measured (32 query on 8 key heads of 128 channels, kernels behind one another in a graph): 16 rows on 32003 shared keys and
-// 300 of their own 39 us (3.7 TB/s); 64 rows of 4 prompts of 613 and 391 own 30 us; 256 rows of three tokens, 8 prompts of 4096 and 1001 own 223 us (4.2 TB/s; tensor cores 63 % busy); one prompt of 61
+// 300 of their own 39 us (3.7 TB/s); 64 rows of 4 prompts of 613 and 391 own 30 us; 256 rows of three tokens, 8 prompts of 4096 and 1001 own 216 us (4.3 TB/s; tensor cores 63 % busy); one prompt of 61
 // 11 us.
 #include "common/attn_math.cuh"
 #include "common/ptx.cuh"
