@@ -2,7 +2,7 @@
 //
 // Of z = x / T, in units of log2 (c = log2(e) / T):  d = (x - base) c,  s = sum 2^d,  t = sum 2^d d,  with a base less than some four powers of two from the maximum, so that
 //   log p = ln2 (d - log2 s)        H = -sum p log p = ln2 (log2 s - t / s)
-// are differences of numbers that are small where the results are.  Near certainty what is left of them is their roundings: some 5e-7 of log p and 2e-6 of H (400 x 128256 with one token 14 above the
+// are differences of numbers that are small where the results are.  Near certainty what is left of them is their roundings: up to 1e-6 of log p and 3e-6 of H (400 x 128256 with one token 14 above the
 // others' maximum; with a base up to 2^24 away 2e-6 and 1e-5), neither of which crosses 0.  When the base moves up by a / c, s' = s 2^-a and t' = (t - a s) 2^-a.  A base that followed every new
 // maximum would move in nearly all steps of a warp, since one of its 32 lanes has a new one; so it begins four powers of two above the maximum of the warp's first 256 elements, and a lane whose elements
 // go four above it moves its own.  Rows in rising order, whose lanes move it all the time, take 1.1 to 1.35 times as long (8192 x 8000 bf16 41 -> 55 us).  Differences are taken before they are
